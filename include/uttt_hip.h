@@ -681,6 +681,90 @@ int uttt_dense_wgrad_pair_layers(const void* dy0_dy2_tok, const void* const* k_l
  * y [b*H, l, d] bf16 -> out [b, l, H*d] bf16; d % 8 == 0, 16-byte aligned. */
 int uttt_dense_scatter_heads(const void* y, int b, int l, int H, int d, void* out, void* stream);
 
+/* ---- The gated delta rule ------------------------------------------------
+ * Per value head, with a state S [Dk, Dv] fp32:
+ *   S_t = e^{g_t} S_{t-1} + k_t u_t^T,  u_t = beta_t (v_t - e^{g_t} S_{t-1}^T k_t),
+ *   o_t = scale S_t^T q_t
+ * q, k [B, T, Hk, Dk] and v [B, T, Hv, Dv] bf16, Hv a multiple of Hk (value
+ * head h reads key head h / (Hv / Hk)), each with three element strides
+ * {batch, token, head} (multiples of 8; features contiguous, 16-byte aligned);
+ * g, beta [B, T, Hv] contiguous in any dtype code; Dk a multiple of 8 up to
+ * 256, Dv a multiple of 8.  cu_seqlens NULL: B sequences of T tokens, nseq =
+ * B.  Else B = 1 and sequence n is tokens cu_seqlens[n] .. cu_seqlens[n + 1]
+ * (nseq + 1 offsets on the device, int32 or int64; clamped to ascending
+ * offsets in [0, T]); outputs and gradients of tokens of no sequence are
+ * zeros.  States are [nseq, Hv, Dk, Dv] fp32 contiguous.
+ *
+ * fwd: out [B, T, Hv, Dv] bf16; initial_state NULL: zeros; final_state NULL:
+ * not wanted.  u_saved [2, B, T, Hv, Dv] and s_saved [chunks, Hv, 2, Dk, Dv]
+ * bf16 (uttt_gated_delta_chunks slots; fp32 values as two parts each) are what
+ * the backward reads; both NULL without one.  bwd: dout [B, T, Hv, Dv] bf16 with strides, dfinal_state NULL:
+ * zeros, dinitial_state NULL: not wanted; dq, dk, dv bf16 contiguous, dg and
+ * dbeta in g's and beta's dtypes.  The reference's gated delta layers
+ * (gated_deltanet_swa/, uttt_nvs/models/gated_deltanet_block.py) call an
+ * external package. */
+size_t uttt_gated_delta_workspace_bytes(int B, int T, int nseq, int Hk, int Hv, int Dk, int Dv,
+                                        int packed, int backward);
+int uttt_gated_delta_chunks(int B, int T, int nseq, int packed);
+int uttt_gated_delta_fwd(const void* q, const int64_t* q_strides, const void* k,
+                         const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                         const void* g, int g_dtype, const void* beta, int beta_dtype,
+                         const void* cu_seqlens, int cu_is_int64, int B, int T, int nseq, int Hk,
+                         int Hv, int Dk, int Dv, float scale, const float* initial_state, void* out,
+                         float* final_state, void* u_saved, void* s_saved, void* workspace,
+                         size_t workspace_bytes, void* stream);
+int uttt_gated_delta_bwd(const void* q, const int64_t* q_strides, const void* k,
+                         const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                         const void* g, int g_dtype, const void* beta, int beta_dtype,
+                         const void* cu_seqlens, int cu_is_int64, int B, int T, int nseq, int Hk,
+                         int Hv, int Dk, int Dv, float scale, const void* u_saved,
+                         const void* s_saved, const void* dout, const int64_t* do_strides,
+                         const float* dfinal_state, void* dq, void* dk, void* dv, void* dg,
+                         void* dbeta, float* dinitial_state, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* The same rule token by token, T tokens per row, against states in place:
+ * state [slots, Hv, Dk, Dv] fp32, slots state_stride elements apart (16-byte
+ * aligned).  q, k, v, out of one dtype code, strides as above but of any size;
+ * Dk up to 256, Dv a multiple of 4.  indices [B] (int32 or int64 on the
+ * device; NULL: row b has slot b): a row whose index is no slot changes no
+ * state and gets zeros; rows of one slot follow one another in row order. */
+int uttt_gated_delta_step(const void* q, const int64_t* q_strides, const void* k,
+                          const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                          int dtype, const void* g, int g_dtype, const void* beta, int beta_dtype,
+                          int B, int T, int Hk, int Hv, int Dk, int Dv, float scale, float* state,
+                          int64_t state_stride, int slots, const void* indices, int indices_int64,
+                          void* out, void* stream);
+
+/* ---- Layer norm ----------------------------------------------------------
+ * y = (x - mean) / sqrt(var + eps) * weight + bias over rows of N elements,
+ * in fp32, rounded once.  x [rows, N] with a row stride, out contiguous;
+ * weight and bias [N], each NULL or in its own dtype code.  stats [2, rows]
+ * fp32 (mean, 1 / deviation), NULL where no backward follows.  bwd: dy with a
+ * row stride, dx contiguous, dweight / dbias NULL where not wanted (else [N]
+ * in weight's / bias' dtype, and the workspace); summed in a fixed order. */
+int uttt_layer_norm_fwd(const void* x, int dtype, int64_t x_stride, int64_t rows, int N,
+                        const void* weight, int weight_dtype, const void* bias, int bias_dtype,
+                        float eps, void* out, float* stats, void* stream);
+size_t uttt_layer_norm_bwd_workspace_bytes(int64_t rows, int N);
+int uttt_layer_norm_bwd(const void* x, int dtype, int64_t x_stride, const void* dy,
+                        int64_t dy_stride, int64_t rows, int N, const void* weight,
+                        int weight_dtype, const float* stats, void* dx, void* dweight, void* dbias,
+                        int bias_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- Rotary embedding over several position axes --------------------------
+ * x [B, L, H, D] (element strides {batch, token, head}, features contiguous)
+ * -> out contiguous: pair j of R = sum(sections) turns by positions[b, l,
+ * axis(j)] * inv_freq[j], axis(j) the section that holds j (sections: host
+ * array, 1 to 8 axes).  Pairs are features (j, j + R), or (2j, 2j + 1)
+ * interleaved; features from 2R on are copied.  positions int32 or int64 with
+ * element strides {batch, token, axis}.  inverse: the turn back (the
+ * backward). */
+int uttt_rotary_axes(const void* x, int dtype, const int64_t* x_strides, int B, int L, int H, int D,
+                     const void* positions, int positions_int64, const int64_t* position_strides,
+                     const float* inv_freq, const int* sections, int axes, int interleaved,
+                     int inverse, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

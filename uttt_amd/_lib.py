@@ -197,6 +197,39 @@ SIGNATURES = {
         [c_p, c_int, c_int, c_int, c_p, c_p, c_int, c_int, c_p, c_int, c_i64, c_i64, c_i64,
          c_p, c_i64, c_i64, c_i64, c_int, c_p, c_p],
     ),
+    "uttt_gated_delta_workspace_bytes": (c_sz, [c_int] * 9),
+    "uttt_gated_delta_chunks": (c_int, [c_int] * 4),
+    "uttt_gated_delta_fwd": (
+        c_int,
+        [c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_int, c_p, c_int, c_p, c_int, c_int, c_int, c_int,
+         c_int, c_int, c_int, c_int, ctypes.c_float, c_p, c_p, c_p, c_p, c_p, c_p, c_sz, c_p],
+    ),
+    "uttt_gated_delta_bwd": (
+        c_int,
+        [c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_int, c_p, c_int, c_p, c_int, c_int, c_int, c_int,
+         c_int, c_int, c_int, c_int, ctypes.c_float, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p,
+         c_p, c_p, c_p, c_sz, c_p],
+    ),
+    "uttt_gated_delta_step": (
+        c_int,
+        [c_p, c_p, c_p, c_p, c_p, c_p, c_int, c_p, c_int, c_p, c_int, c_int, c_int, c_int, c_int,
+         c_int, c_int, ctypes.c_float, c_p, c_i64, c_int, c_p, c_int, c_p, c_p],
+    ),
+    "uttt_layer_norm_fwd": (
+        c_int,
+        [c_p, c_int, c_i64, c_i64, c_int, c_p, c_int, c_p, c_int, ctypes.c_float, c_p, c_p, c_p],
+    ),
+    "uttt_layer_norm_bwd_workspace_bytes": (c_sz, [c_i64, c_int]),
+    "uttt_layer_norm_bwd": (
+        c_int,
+        [c_p, c_int, c_i64, c_p, c_i64, c_i64, c_int, c_p, c_int, c_p, c_p, c_p, c_p, c_int, c_p,
+         c_sz, c_p],
+    ),
+    "uttt_rotary_axes": (
+        c_int,
+        [c_p, c_int, c_p, c_int, c_int, c_int, c_int, c_p, c_int, c_p, c_p, c_p, c_int, c_int,
+         c_int, c_p, c_p],
+    ),
 }
 
 _lib = None
@@ -237,6 +270,16 @@ def call(name: str, *args) -> None:
     if rc != 0:
         msg = lib().uttt_last_error().decode(errors="replace")
         raise RuntimeError(f"{name} failed ({rc}): {msg}")
+
+
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """call() with t's device current: a launch goes to the current device,
+    which need not be the one of its stream."""
+    if t.get_device() == torch.cuda.current_device():
+        call(name, *args)
+    else:
+        with torch.cuda.device(t.device):
+            call(name, *args)
 
 
 def dtype_code(dt: torch.dtype) -> int:

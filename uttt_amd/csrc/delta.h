@@ -1,0 +1,286 @@
+// Shared pieces of the gated delta rule's chunked kernels (delta_fwd.hip,
+// delta_bwd.hip): the call's geometry, the chunk table of packed sequences,
+// operand fragments and the split of fp32 values into bf16 parts.
+//
+// The rule, per value head, with a state S [Dk, Dv]:
+//   S_t = e^{g_t} S_{t-1} + k_t u_t^T,  u_t = b_t (v_t - e^{g_t} S_{t-1}^T k_t),
+//   o_t = s S_t^T q_t
+// Over a chunk of C = 64 tokens that starts from S0, with G = cumsum(g),
+// gam = e^G, E_ij = e^{G_i - G_j}:
+//   A_ij = b_i E_ij k_i.k_j (j < i),  T = (I + A)^-1,  P_ij = s E_ij q_i.k_j (j <= i)
+//   R = b (V - gam K S0),  U = T R
+//   O = s gam Q S0 + P U
+//   S' = gam_C S0 + (e^{G_C - G} K)^T U
+// and for gradients dO and dS' of a chunk's outputs
+//   dU = P^T dO + e^{G_C - G} K dS',  dR = T^T dU,  dV = b dR
+//   dS0 = gam_C dS' + (s gam Q)^T dO - (b gam K)^T dR
+//
+// Precision.  The state and its gradient are fp32 and stay exact to fp32's
+// order: a product with one of them, with U, T, P, R or their gradients takes
+// that fp32 operand as the sum of two bf16 values (hi = bf16(x), lo = bf16(x -
+// hi); at most 2^-16 of x is left out) and adds both products in fp32; q, k, v
+// and do are bf16 as given.  What a backward keeps or exchanges (U, S0, dR,
+// dS') is stored as the two parts too, planes hi and lo.
+//
+// Fragments.  v_mfma_f32_16x16x32_bf16 takes from lane (r = lane % 16, q =
+// lane / 16) eight consecutive values 8q..8q+7 of the contracted axis for row
+// (column) r, and gives it rows 4q..4q+3 of column r.
+#pragma once
+
+#include "common.h"
+
+namespace uttt {
+namespace delta {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kC = 64;           // tokens of a chunk
+constexpr int kTFrags = 6;       // nonzero 16 x 32 fragments of a triangular 64 x 64 operand
+constexpr int kTriBytes = 4 * kTFrags * 1024;   // T hi, T lo, P hi, P lo
+constexpr int kScal = 5 * kC;    // gam, e^{G_C - G}, beta and G in two parts, per token
+
+struct Args {
+  const uint16_t *q, *k, *v;
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+  const void *g, *beta;          // [B, T, Hv]
+  int g_dtype, beta_dtype;
+  int B, T, Hk, Hv, Dk, Dv, nseq, nchunks;   // nchunks: slots of the chunk table
+  int cps;                       // chunks per sequence where there is no table
+  float scale;
+  const int4* table;             // [nchunks] sequence, first token, tokens; packed sequences only
+  const int4* seqs;              // [nseq] first chunk, chunks
+  uint8_t* tri;                  // [nchunks, Hv] kTriBytes
+  float* scal;                   // [nchunks, Hv, kScal]
+  uint8_t* kt;                   // [nchunks, Hk, 4 KS] KiB: K^T fragments
+  uint8_t* qt;                   // the same of Q (backward)
+  const float* h0;               // [nseq, Hv, Dk, Dv] or null
+  uint16_t* o;                   // [B, T, Hv, Dv]
+  float* hT;                     // final states or null
+  uint16_t* u;                   // [2, B, T, Hv, Dv] parts of U, or null
+  uint16_t* s0;                  // [nchunks, Hv, 2, Dk, Dv] parts of S0, or null
+  // backward
+  const uint16_t* dout;          // [B, T, Hv, Dv]
+  int64_t do_sb, do_st, do_sh;
+  const float* dhT;              // or null
+  float* dh0;                    // or null
+  uint16_t* ds;                  // [nchunks, Hv, 2, Dk, Dv] parts of dS'
+  uint16_t* dr;                  // [2, B, T, Hv, Dv] parts of dR
+  uint16_t *dq, *dk;             // [B, T, Hk, Dk]
+  uint16_t* dv;                  // [B, T, Hv, Dv]
+  void *dg, *dbeta;              // [B, T, Hv] in their inputs' types
+};
+
+struct Chunk {
+  int seq;        // -1: tokens of no sequence, -2: nothing
+  int b, t0, n;   // batch row, first token, tokens
+};
+
+__device__ __forceinline__ Chunk chunk_of(const Args& a, int c) {
+  if (a.table == nullptr) {
+    const int seq = c / a.cps, t0 = (c - seq * a.cps) * kC;
+    return {seq, seq, t0, min(kC, a.T - t0)};
+  }
+  const int4 e = a.table[c];
+  return {e.x, 0, e.y, e.z};
+}
+
+// Index of fragment (16-row tile, 32-column step) of a lower triangular
+// operand, its row tiles 0, 1 having step 0 alone; of an upper one (its
+// transpose) tiles 2, 3 have step 1 alone.
+__device__ __forceinline__ constexpr int lower_frag(int rt, int ks) {
+  return rt < 2 ? rt : 2 + 2 * (rt - 2) + ks;
+}
+__device__ __forceinline__ constexpr int upper_frag(int rt, int ks) {
+  return rt < 2 ? 2 * rt + ks : 2 + rt;
+}
+
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// x[0..3] = a, x[4..7] = b as bf16 parts hi + lo.
+__device__ __forceinline__ void split8(f32x4 a, f32x4 b, bf16x8& hi, bf16x8& lo) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    hi[i] = (__bf16)a[i];
+    hi[4 + i] = (__bf16)b[i];
+    lo[i] = (__bf16)(a[i] - (float)hi[i]);
+    lo[4 + i] = (__bf16)(b[i] - (float)hi[4 + i]);
+  }
+}
+
+// Raw buffers: a lane whose offset is kNoRow (past any record count) reads
+// zeros and writes nothing, without a branch.
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+constexpr uint32_t kNoRow = 0x80000000u;
+__device__ __forceinline__ Rsrc buffer_at(const void* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, 0x7fffffff, 0x00020000);
+}
+__device__ __forceinline__ bf16x8 load_frag(Rsrc r, uint32_t off) {
+  return __builtin_bit_cast(bf16x8, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+}
+
+// NT adjacent bf16 columns of one row, held as raw words.
+template <int NT>
+struct Cols {
+  uint32_t w[(NT + 1) / 2];
+  __device__ __forceinline__ void load(Rsrc r, uint32_t off) {
+    if constexpr (NT == 1) w[0] = __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+    else if constexpr (NT == 2) w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+    else {
+      const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
+      w[0] = x[0];
+      w[1] = x[1];
+    }
+  }
+  __device__ __forceinline__ float get(int c) const {
+    return __uint_as_float(c & 1 ? w[c / 2] & 0xffff0000u : w[c / 2] << 16);
+  }
+};
+// x[0..NT) as bf16, and as the parts hi + lo, to one or two rows.
+template <int NT>
+__device__ __forceinline__ void store_cols(Rsrc r, uint32_t off, const __bf16 (&x)[NT]) {
+  if constexpr (NT == 1)
+    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, x[0]), r, off, 0, 0);
+  else if constexpr (NT == 2)
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), r, off, 0, 0);
+  else
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), r, off, 0, 0);
+}
+
+// Four fp32 values of one column as bf16 parts.
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void split4(f32x4 x, bf16x4& hi, bf16x4& lo) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    hi[i] = (__bf16)x[i];
+    lo[i] = (__bf16)(x[i] - (float)hi[i]);
+  }
+}
+
+__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
+  if (dtype == UTTT_F32) return static_cast<const float*>(p)[i];
+  const uint16_t h = static_cast<const uint16_t*>(p)[i];
+  return dtype == UTTT_BF16 ? bf16_to_f32(h) : f16_to_f32(h);
+}
+__device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float x) {
+  if (dtype == UTTT_F32) static_cast<float*>(p)[i] = x;
+  else static_cast<uint16_t*>(p)[i] = dtype == UTTT_BF16 ? f32_to_bf16(x) : f32_to_f16(x);
+}
+
+// The part of a call that a scan's workgroup walks over: one sequence, one
+// value head, `width` columns.  Column blocks of one head are eight workgroups
+// apart: on one XCD, whose L2 the head's fragments then pass once.
+struct Scan {
+  int head, seq, hv, hk, b, c0, nc, tok0, len, col0;
+  __device__ __forceinline__ bool init(const Args& a, int width) {
+    const int ncb = (a.Dv + width - 1) / width;
+    const int grp = blockIdx.x / (8 * ncb), in = blockIdx.x % (8 * ncb);
+    head = grp * 8 + (in & 7);
+    if (head >= a.nseq * a.Hv) return false;
+    col0 = (in >> 3) * width;
+    seq = head / a.Hv;
+    hv = head % a.Hv;
+    hk = hv / (a.Hv / a.Hk);
+    b = a.table ? 0 : seq;
+    if (a.table) {
+      const int4 s = a.seqs[seq];
+      c0 = s.x; nc = s.y; tok0 = s.z; len = s.w;
+    } else {
+      c0 = seq * a.cps; nc = a.cps; tok0 = 0; len = a.T;
+    }
+    return true;
+  }
+};
+inline unsigned scan_blocks(const Args& a, int width) {
+  return (unsigned)(((int64_t)a.nseq * a.Hv + 7) / 8 * 8 * ((a.Dv + width - 1) / width));
+}
+// 16-column tiles of a scan's workgroup: as wide as leaves every CU one (an
+// operand fragment then serves more columns), at most 4.
+inline int scan_tiles(const Args& a) {
+  const int64_t heads = (int64_t)a.nseq * a.Hv;
+  return heads * ((a.Dv + 63) / 64) >= 256 ? 4 : heads * ((a.Dv + 31) / 32) >= 256 ? 2 : 1;
+}
+
+// Features up to which a kernel instance goes, in steps of 32: the next of 2,
+// 3, 4, 6, 8 (K, Q past Dk are zeros in LDS).
+inline int steps_of(int Dk) {
+  const int ks = (Dk + 31) / 32;
+  return ks <= 2 ? 2 : ks <= 4 ? ks : ks <= 6 ? 6 : 8;
+}
+
+#define UTTT_DELTA_STEPS(ks, KS, ...)                       \
+  switch (ks) {                                             \
+    case 2: { constexpr int KS = 2; __VA_ARGS__; } break;   \
+    case 3: { constexpr int KS = 3; __VA_ARGS__; } break;   \
+    case 4: { constexpr int KS = 4; __VA_ARGS__; } break;   \
+    case 6: { constexpr int KS = 6; __VA_ARGS__; } break;   \
+    default: { constexpr int KS = 8; __VA_ARGS__; } break;  \
+  }
+
+// delta_prep.hip: the chunk table of packed sequences (cu [nseq + 1], clamped
+// to ascending offsets within T) and the per-chunk operands.  `transposed`:
+// T^T, P^T and Q^T for the backward, else T and P.
+int launch_table(const void* cu, int cu64, int nseq, int T, int nchunks, int4* table, int4* seqs,
+                 hipStream_t st);
+int launch_prep(const Args& a, bool transposed, hipStream_t st);
+
+// The parts of a call's workspace, in order.
+struct Workspace {
+  size_t table, seqs, scal, kt, tri, qt, ds, dr, total;
+};
+inline int chunk_slots(int64_t B, int64_t T, int nseq, bool packed) {
+  const int64_t n = packed ? T / kC + nseq + 2 : B * ((T + kC - 1) / kC);
+  return n > 0x7fffffff ? -1 : (int)n;
+}
+inline Workspace workspace_of(int64_t B, int64_t T, int nseq, int Hk, int Hv, int Dk, int Dv,
+                              bool packed, bool backward) {
+  Workspace w{};
+  const size_t n = (size_t)chunk_slots(B, T, nseq, packed);
+  const size_t frags = n * Hk * 4 * steps_of(Dk) * 1024;
+  size_t at = 0;
+  const auto take = [&at](size_t bytes) {
+    const size_t p = at;
+    at += (bytes + 255) & ~(size_t)255;
+    return p;
+  };
+  w.table = take(packed ? n * 16 : 0);
+  w.seqs = take(packed ? (size_t)nseq * 16 : 0);
+  w.scal = take(n * Hv * kScal * 4);
+  w.kt = take(frags);
+  w.tri = take(n * Hv * kTriBytes);
+  w.qt = take(backward ? frags : 0);
+  w.ds = take(backward ? n * Hv * Dk * Dv * 4 : 0);
+  w.dr = take(backward ? (size_t)B * T * Hv * Dv * 4 : 0);
+  w.total = at;
+  return w;
+}
+// Fills the fields of `a` that point into the workspace.
+inline void bind_workspace(Args& a, const Workspace& w, uint8_t* ws, bool packed, bool backward) {
+  a.table = packed ? reinterpret_cast<const int4*>(ws + w.table) : nullptr;
+  a.seqs = packed ? reinterpret_cast<const int4*>(ws + w.seqs) : nullptr;
+  a.scal = reinterpret_cast<float*>(ws + w.scal);
+  a.kt = ws + w.kt;
+  a.tri = ws + w.tri;
+  if (backward) {
+    a.qt = ws + w.qt;
+    a.ds = reinterpret_cast<uint16_t*>(ws + w.ds);
+    a.dr = reinterpret_cast<uint16_t*>(ws + w.dr);
+  }
+}
+
+// delta_fwd.hip: the argument checks of both directions.
+int check_args(const Args& a, int B, bool packed, const char* what);
+
+}  // namespace delta
+}  // namespace uttt
