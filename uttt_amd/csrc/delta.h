@@ -118,25 +118,35 @@ __device__ __forceinline__ void split8(f32x4 a, f32x4 b, bf16x8& hi, bf16x8& lo)
   }
 }
 
-// Raw buffers: a lane whose offset is kNoRow (past any record count) reads
-// zeros and writes nothing, without a branch.
+// Raw buffers: a lane whose offset has bit 31 (past any record count) reads
+// zeros and writes nothing, without a branch.  The bit is set by arithmetic:
+// of two offsets chosen between by a condition the compiler makes two branches
+// with a load in each.
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr uint32_t kNoRow = 0x80000000u;
 __device__ __forceinline__ Rsrc buffer_at(const void* p) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, 0x7fffffff, 0x00020000);
 }
-__device__ __forceinline__ bf16x8 load_frag(Rsrc r, uint32_t off) {
-  return __builtin_bit_cast(bf16x8, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+__device__ __forceinline__ uint32_t miss_from(int i, int n) {   // kNoRow where i >= n
+  return (uint32_t)(n - 1 - i) & kNoRow;
+}
+__device__ __forceinline__ bf16x8 load_frag(Rsrc r, uint32_t off, uint32_t uniform = 0) {
+  return __builtin_bit_cast(bf16x8, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(r, off, uniform, 0));
+}
+__device__ __forceinline__ f32x4 load_f4(Rsrc r, uint32_t off, uint32_t uniform = 0) {
+  return __builtin_bit_cast(f32x4, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(r, off, uniform, 0));
+}
+__device__ __forceinline__ float load_f1(Rsrc r, uint32_t off) {
+  return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
 }
 
 // NT adjacent bf16 columns of one row, held as raw words.
 template <int NT>
 struct Cols {
-  uint32_t w[(NT + 1) / 2];
+  uint32_t w[NT / 2];
   __device__ __forceinline__ void load(Rsrc r, uint32_t off) {
-    if constexpr (NT == 1) w[0] = __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
-    else if constexpr (NT == 2) w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+    if constexpr (NT == 2) w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
     else {
       const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
       w[0] = x[0];
@@ -146,25 +156,58 @@ struct Cols {
   __device__ __forceinline__ float get(int c) const {
     return __uint_as_float(c & 1 ? w[c / 2] & 0xffff0000u : w[c / 2] << 16);
   }
+  __device__ __forceinline__ uint32_t half(int c) const { return c & 1 ? w[c / 2] >> 16 : w[c / 2] & 0xffffu; }
 };
-// x[0..NT) as bf16, and as the parts hi + lo, to one or two rows.
-template <int NT>
-__device__ __forceinline__ void store_cols(Rsrc r, uint32_t off, const __bf16 (&x)[NT]) {
-  if constexpr (NT == 1)
-    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, x[0]), r, off, 0, 0);
-  else if constexpr (NT == 2)
-    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), r, off, 0, 0);
-  else
-    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), r, off, 0, 0);
-}
 
-// Four fp32 values of one column as bf16 parts.
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ void split4(f32x4 x, bf16x4& hi, bf16x4& lo) {
+template <>
+struct Cols<1> {
+  uint16_t w;   // widened where it is used, not where it is loaded
+  __device__ __forceinline__ void load(Rsrc r, uint32_t off) {
+    w = __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+  }
+  __device__ __forceinline__ float get(int) const { return bf16_to_f32(w); }
+  __device__ __forceinline__ uint32_t half(int) const { return w; }
+};
+
+// Every load that is under way done.  Before a pipelined loop: the compiler's
+// wait counts at the loop's head allow for both ways into it, and loads in
+// another order in front of it made each turn wait for its own last loads.
+__device__ __forceinline__ void settle() { __builtin_amdgcn_s_waitcnt(0); }
+
+// Four fp32 rows of one column as bf16 parts, two rows a word.
+struct Parts {
+  u32x2 hi, lo;
+};
+__device__ __forceinline__ Parts parts_of(f32x4 x) {
+  Parts p;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    hi[i] = (__bf16)x[i];
-    lo[i] = (__bf16)(x[i] - (float)hi[i]);
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t h = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+    p.hi[i] = h;
+    p.lo[i] = pack_bf16x2(x[2 * i] - __uint_as_float(h << 16), x[2 * i + 1] - __uint_as_float(h & 0xffff0000u));
+  }
+  return p;
+}
+__device__ __forceinline__ u32x2 round_of(f32x4 x) {
+  u32x2 p;
+  p[0] = pack_bf16x2(x[0], x[1]);
+  p[1] = pack_bf16x2(x[2], x[3]);
+  return p;
+}
+// Row i of NT columns' words to memory as adjacent bf16.
+template <int NT>
+__device__ __forceinline__ void store_row(Rsrc r, uint32_t off, const u32x2 (&x)[NT], int i, uint32_t uniform = 0) {
+  const auto pair = [&](int n) -> uint32_t {
+    const uint32_t a = x[n][i >> 1], b = x[n + 1][i >> 1];
+    return i & 1 ? (a >> 16) | (b & 0xffff0000u) : (a & 0xffffu) | (b << 16);
+  };
+  if constexpr (NT == 1)
+    __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(i & 1 ? x[0][i >> 1] >> 16 : x[0][i >> 1]), r, off, uniform, 0);
+  else if constexpr (NT == 2)
+    __builtin_amdgcn_raw_buffer_store_b32(pair(0), r, off, uniform, 0);
+  else {
+    const u32x2 w = {pair(0), pair(2)};
+    __builtin_amdgcn_raw_buffer_store_b64(w, r, off, uniform, 0);
   }
 }
 

@@ -35,13 +35,12 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
   const int r = lane & 15, q = lane >> 4;
   const int col = s.col0 + NT * r;
   const bool live = col < a.Dv;
+  const uint32_t dead = miss_from(col, a.Dv);
   const uint32_t put = (r + 16 * (q >> 1)) * 16 + (q & 1) * 8;
-  const auto put_tile = [&](uint8_t (*buf)[2 * NT * 1024], int n, f32x4 x) {
-    bf16x4 hi, lo;
-    split4(x, hi, lo);
-    const uint32_t at = ((wave >> 1) * NT + n) * 1024 + (wave & 1) * 512 + put;
-    *reinterpret_cast<bf16x4*>(buf[0] + at) = hi;
-    *reinterpret_cast<bf16x4*>(buf[1] + at) = lo;
+  const uint32_t put_tok = (wave >> 1) * NT * 1024 + (wave & 1) * 512 + put;
+  const auto put_tile = [&](uint8_t (*buf)[2 * NT * 1024], int n, const Parts& p) {
+    *reinterpret_cast<u32x2*>(buf[0] + put_tok + n * 1024) = p.hi;
+    *reinterpret_cast<u32x2*>(buf[1] + put_tok + n * 1024) = p.lo;
   };
   const auto get = [&](const uint8_t* buf, int f) {
     return *reinterpret_cast<const bf16x8*>(buf + f * 1024 + lane * 16);
@@ -63,105 +62,114 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
   f32x4 gam, ge, bt;
   float gc;
   Cols<NT> gr[4];
-  // Loads of chunk c's operands; before the first chunk they repeat it.
-  const auto load_k = [&](int c) {
-    c = max(c, 0);
-    const int n = min(kC, s.len - c * kC), t = 16 * wave + r;
-    const Rsrc kp = buffer_at(a.k + s.b * a.k_sb + s.hk * a.k_sh + (s.tok0 + (int64_t)c * kC) * a.k_st);
+  // Operands of the chunk before: pointers that go along, at first those of the last chunk.
+  const int lastc = s.nc - 1;
+  const int64_t crow = (int64_t)s.b * a.T + s.tok0 + (int64_t)lastc * kC;
+  const uint16_t* kp = a.k + s.b * a.k_sb + s.hk * a.k_sh + (s.tok0 + (int64_t)lastc * kC) * a.k_st;
+  const uint16_t* gp = a.dout + s.b * a.do_sb + s.hv * a.do_sh + (s.tok0 + (int64_t)lastc * kC) * a.do_st;
+  const uint8_t* trip = a.tri + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kTriBytes;
+  const int64_t trans_at = ((int64_t)(s.c0 + lastc) * a.Hk + s.hk) * (4 * KS * 1024);
+  const uint8_t *ktp = a.kt + trans_at, *qtp = a.qt + trans_at;
+  const float* scp = a.scal + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kScal;
+  const uint32_t krow = 2 * ((16 * wave + r) * (uint32_t)a.k_st + 8 * q);
+  const uint32_t grow = 2 * ((16 * wave + 4 * q) * (uint32_t)a.do_st + col);
+  const uint32_t orow = 2 * ((16 * wave + 4 * q) * (uint32_t)(a.Hv * a.Dv) + col);
+  const uint32_t last_half = miss_from(32 * (KS - 1) + 8 * q, a.Dk), before_half = miss_from(32 * (KS - 2) + 8 * q, a.Dk);
+  // `left`: tokens from the chunk on to the sequence's end; 0 before its first chunk
+  const auto load_k = [&](int left) {
+    const uint32_t miss = miss_from(16 * wave + r, left);
+    const Rsrc kr = buffer_at(kp);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int e = 32 * ks + 8 * q;
-      kf[ks] = load_frag(kp, t < n && e < a.Dk ? 2 * (t * (uint32_t)a.k_st + e) : kNoRow);
-    }
+    for (int ks = 0; ks < KS; ++ks)
+      kf[ks] = load_frag(kr, (krow + 64 * ks) | miss | (ks == KS - 1 ? last_half : ks == KS - 2 ? before_half : 0));
+    ge = load_f4(buffer_at(scp), 4 * (16 * wave + 4 * q) | miss_from(0, left), 4 * kC);
+    kp -= kC * a.k_st;
   };
-  const auto load_do = [&](int c) {
-    c = max(c, 0);
-    const int n = min(kC, s.len - c * kC);
-    const Rsrc gp = buffer_at(a.dout + s.b * a.do_sb + s.hv * a.do_sh + (s.tok0 + (int64_t)c * kC) * a.do_st);
+  const auto load_do = [&](int left) {
+    const Rsrc gr_ = buffer_at(gp);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = 16 * wave + 4 * q + i;
-      gr[i].load(gp, t < n && live ? 2 * (t * (uint32_t)a.do_st + col) : kNoRow);
-    }
+    for (int i = 0; i < 4; ++i)
+      gr[i].load(gr_, (grow + 2 * i * (uint32_t)a.do_st) | dead | miss_from(16 * wave + 4 * q + i, left));
+    gp -= kC * a.do_st;
   };
-  const auto load_scal = [&](int c) {
-    const float* sc = a.scal + ((size_t)(s.c0 + max(c, 0)) * a.Hv + s.hv) * kScal;
-    const int t = 16 * wave + 4 * q;
-    gam = *reinterpret_cast<const f32x4*>(sc + t);
-    ge = *reinterpret_cast<const f32x4*>(sc + kC + t);
-    bt = *reinterpret_cast<const f32x4*>(sc + 2 * kC + t);
-    gc = sc[kC - 1];
-  };
-  const auto load_tri = [&](int c, int which, bf16x8 (&x)[2][2]) {
-    const uint8_t* p = a.tri + ((size_t)(s.c0 + max(c, 0)) * a.Hv + s.hv) * kTriBytes +
-                       which * 2 * kTFrags * 1024 + lane * 16;
+  const auto load_tri = [&](int left, int which, bf16x8 (&x)[2][2]) {
+    const Rsrc tr = buffer_at(trip);
+    const uint32_t at = lane * 16 | miss_from(0, left);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       // step 0 of the lower tiles is zero and not stored: step 1 again, unused
-      const int f = upper_frag(wave, wave < 2 ? ks : 1);
-      x[ks][0] = *reinterpret_cast<const bf16x8*>(p + f * 1024);
-      x[ks][1] = *reinterpret_cast<const bf16x8*>(p + (kTFrags + f) * 1024);
+      const int f = 2 * which * kTFrags + upper_frag(wave, wave < 2 ? ks : 1);
+      x[ks][0] = load_frag(tr, at, f * 1024);
+      x[ks][1] = load_frag(tr, at, (kTFrags + f) * 1024);
+    }
+    if (!which) {
+      const Rsrc sr = buffer_at(scp);
+      const uint32_t s_at = 4 * (16 * wave + 4 * q) | miss_from(0, left);
+      gam = load_f4(sr, s_at);
+      bt = load_f4(sr, s_at, 8 * kC);
+      gc = load_f1(sr, 4 * (kC - 1) | miss_from(0, left));
+      scp -= a.Hv * kScal;
+      trip -= (int64_t)a.Hv * kTriBytes;
     }
   };
-  const auto load_trans = [&](int c, const uint8_t* base, bf16x8 (&x)[FT][2]) {
-    const uint8_t* p = base + ((size_t)(s.c0 + max(c, 0)) * a.Hk + s.hk) * (4 * KS) * 1024 + lane * 16;
+  const auto load_trans = [&](int left, const uint8_t*& p, bf16x8 (&x)[FT][2]) {
+    const Rsrc tr = buffer_at(p);
+    const uint32_t at = lane * 16 | miss_from(0, left);
 #pragma unroll
     for (int f = 0; f < FT; ++f)
 #pragma unroll
       for (int t = 0; t < 2; ++t)
-        if (wave * FT + f < 2 * KS)
-          x[f][t] = *reinterpret_cast<const bf16x8*>(p + (2 * (wave * FT + f) + t) * 1024);
+        if (wave * FT + f < 2 * KS) x[f][t] = load_frag(tr, at, (2 * (wave * FT + f) + t) * 1024);
+    p -= (int64_t)a.Hk * (4 * KS * 1024);
   };
   // dS' to LDS and memory, dO to LDS
-  const auto put_state = [&](int c) {
-    const Rsrc sp = buffer_at(a.ds + ((int64_t)(s.c0 + c) * a.Hv + s.hv) * 2 * a.Dk * a.Dv);
+  uint16_t* dsp = a.ds + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * 2 * a.Dk * a.Dv;
+  const auto put_state = [&]() {
+    const Rsrc sr = buffer_at(dsp);
 #pragma unroll
     for (int f = 0; f < FT; ++f) {
       const int tile = wave * FT + f;
       if (tile < 2 * KS) {
-        bf16x4 hi[NT], lo[NT];
+        u32x2 hi[NT], lo[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          split4(S[f][n], hi[n], lo[n]);
+          const Parts p = parts_of(S[f][n]);
           const uint32_t at = ((tile >> 1) * NT + n) * 1024 + (tile & 1) * 512 + put;
-          *reinterpret_cast<bf16x4*>(Sb[0] + at) = hi[n];
-          *reinterpret_cast<bf16x4*>(Sb[1] + at) = lo[n];
+          *reinterpret_cast<u32x2*>(Sb[0] + at) = hi[n] = p.hi;
+          *reinterpret_cast<u32x2*>(Sb[1] + at) = lo[n] = p.lo;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int feat = 16 * tile + 4 * q + i;
-          const uint32_t at = live && feat < a.Dk ? 2 * (feat * a.Dv + col) : kNoRow;
-          __bf16 h[NT], l[NT];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            h[n] = hi[n][i];
-            l[n] = lo[n][i];
-          }
-          store_cols<NT>(sp, at, h);
-          store_cols<NT>(sp, at + 2 * (uint32_t)(a.Dk * a.Dv), l);
+          const uint32_t at = 2 * (feat * a.Dv + col) | dead | miss_from(feat, a.Dk);
+          store_row<NT>(sr, at, hi, i);
+          store_row<NT>(sr, at, lo, i, 2 * (uint32_t)(a.Dk * a.Dv));
         }
       }
     }
+    dsp -= (int64_t)a.Hv * 2 * a.Dk * a.Dv;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      bf16x4 g;   // bf16 as given: exact
-#pragma unroll
-      for (int i = 0; i < 4; ++i) g[i] = (__bf16)gr[i].get(n);
-      *reinterpret_cast<bf16x4*>(Gb + ((wave >> 1) * NT + n) * 1024 + (wave & 1) * 512 + put) = g;
+      const u32x2 g = {gr[0].half(n) | (gr[1].half(n) << 16), gr[2].half(n) | (gr[3].half(n) << 16)};
+      *reinterpret_cast<u32x2*>(Gb + put_tok + n * 1024) = g;
     }
   };
 
-  if (s.nc > 0) {
-    load_do(s.nc - 1);
-    load_k(s.nc - 1);
-    load_scal(s.nc - 1);
-    load_tri(s.nc - 1, 1, pf);
-    load_tri(s.nc - 1, 0, tf);
-    load_trans(s.nc - 1, a.qt, qtf);
-    load_trans(s.nc - 1, a.kt, ktf);
-    put_state(s.nc - 1);
+  const int first_left = s.len - lastc * kC;
+  if (lastc >= 0) {
+    load_do(first_left);
+    load_k(first_left);
+    load_tri(first_left, 1, pf);
+    load_tri(first_left, 0, tf);
+    load_trans(first_left, qtp, qtf);
+    load_trans(first_left, ktp, ktf);
+    put_state();
+    settle();
   }
-  for (int c = s.nc - 1; c >= 0; --c) {
+  const int64_t plane = (int64_t)a.B * a.T * a.Hv * a.Dv;
+  int64_t out_at = (crow * a.Hv + s.hv) * a.Dv;
+  for (int c = lastc; c >= 0; --c) {
+    const int left = s.len - c * kC, next = c > 0 ? kC : 0;
     lds_barrier();   // dS' and dO are in LDS
     // dU = e^{G_C - G} K dS' + P^T dO
     {
@@ -189,31 +197,35 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
           }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        put_tile(Ub, n, X[n] + X2[n]);
+        put_tile(Ub, n, parts_of(X[n] + X2[n]));
         f32x4 g;
 #pragma unroll
         for (int i = 0; i < 4; ++i) g[i] = gr[i].get(n);
-        put_tile(Hb, n, g * (gam * a.scale));
+        put_tile(Hb, n, parts_of(g * (gam * a.scale)));
       }
     }
-    load_do(c - 1);
-    load_k(c - 1);
-    load_tri(c - 1, 1, pf);
+    load_do(next);
+    load_k(next);
+    load_tri(next, 1, pf);
     lds_barrier();   // dU and s gam dO are in LDS
     f32x4 R[NT] = {};   // dR = T^T dU
+    {
+      f32x4 R2[NT] = {};
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-      if (ks >= wave >> 1)
+      for (int ks = 0; ks < 2; ++ks)
+        if (ks >= wave >> 1)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const bf16x8 hi = get(Ub[0], ks * NT + n), lo = get(Ub[1], ks * NT + n);
-          R[n] = mfma(tf[ks][0], hi, R[n]);
-          R[n] = mfma(tf[ks][1], hi, R[n]);
-          R[n] = mfma(tf[ks][0], lo, R[n]);
-        }
-    load_tri(c - 1, 0, tf);
+          for (int n = 0; n < NT; ++n) {
+            const bf16x8 hi = get(Ub[0], ks * NT + n), lo = get(Ub[1], ks * NT + n);
+            R[n] = mfma(tf[ks][0], hi, R[n]);
+            R2[n] = mfma(tf[ks][1], hi, R2[n]);
+            R2[n] = mfma(tf[ks][0], lo, R2[n]);
+          }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) put_tile(Eb, n, -(bt * gam) * R[n]);
+      for (int n = 0; n < NT; ++n) R[n] += R2[n];
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) put_tile(Eb, n, parts_of(-(bt * gam) * R[n]));
     // dS0 = gam_C dS' + Q^T (s gam dO) - K^T (b gam dR): the first product here
 #pragma unroll
     for (int f = 0; f < FT; ++f)
@@ -231,29 +243,27 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
             S[f][n] = mfma(qtf[f][t], lo, S[f][n]);
           }
       }
-    load_trans(c - 1, a.qt, qtf);
+    load_trans(next, qtp, qtf);
     {
-      const int left = s.len - c * kC;
-      const int64_t at = (((int64_t)s.b * a.T + s.tok0 + (int64_t)c * kC) * a.Hv + s.hv) * a.Dv;
-      const Rsrc vp = buffer_at(a.dv + at), hp = buffer_at(a.dr + at),
-                 lp = buffer_at(a.dr + (int64_t)a.B * a.T * a.Hv * a.Dv + at);
+      const Rsrc vr = buffer_at(a.dv + out_at), hr = buffer_at(a.dr + out_at), lr = buffer_at(a.dr + plane + out_at);
+      u32x2 v[NT], hi[NT], lo[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const Parts p = parts_of(R[n]);
+        hi[n] = p.hi;
+        lo[n] = p.lo;
+        v[n] = round_of(bt * R[n]);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int t = 16 * wave + 4 * q + i;
-        const uint32_t off = live && t < left ? 2 * (t * (uint32_t)(a.Hv * a.Dv) + col) : kNoRow;
-        __bf16 v[NT], h[NT], l[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          v[n] = (__bf16)(bt[i] * R[n][i]);
-          h[n] = (__bf16)R[n][i];
-          l[n] = (__bf16)(R[n][i] - (float)h[n]);
-        }
-        store_cols<NT>(vp, off, v);
-        store_cols<NT>(hp, off, h);
-        store_cols<NT>(lp, off, l);
+        const uint32_t at = (orow + 2 * i * (uint32_t)(a.Hv * a.Dv)) | dead | miss_from(16 * wave + 4 * q + i, left);
+        store_row<NT>(vr, at, v, i);
+        store_row<NT>(hr, at, hi, i);
+        store_row<NT>(lr, at, lo, i);
       }
+      out_at -= (int64_t)kC * a.Hv * a.Dv;
     }
-    load_scal(c - 1);
+    load_tri(next, 0, tf);
     lds_barrier();   // b gam dR is in LDS
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -267,8 +277,8 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
             S[f][n] = mfma(ktf[f][t], lo, S[f][n]);
           }
       }
-    load_trans(c - 1, a.kt, ktf);
-    if (c > 0) put_state(c - 1);
+    load_trans(next, ktp, ktf);
+    if (c > 0) put_state();
   }
   if (a.dh0 && live) {
 #pragma unroll
@@ -316,9 +326,9 @@ __global__ __launch_bounds__(64 * NW) void delta_grads_kernel(Args a) {
     const Rsrc qp = buffer_at(a.q + ch.b * a.q_sb + ch.t0 * a.q_st + hk * a.q_sh);
     for (int p = tid; p < kC * 4 * KS; p += kThreads) {
       const int t = p / (4 * KS), e = 8 * (p % (4 * KS));
-      const bool ok = t < ch.n && e < a.Dk;
-      *reinterpret_cast<bf16x8*>(Kl + t * LD + e) = load_frag(kp, ok ? 2 * (t * (uint32_t)a.k_st + e) : kNoRow);
-      *reinterpret_cast<bf16x8*>(Ql + t * LD + e) = load_frag(qp, ok ? 2 * (t * (uint32_t)a.q_st + e) : kNoRow);
+      const uint32_t miss = miss_from(t, ch.n) | miss_from(e, a.Dk);
+      *reinterpret_cast<bf16x8*>(Kl + t * LD + e) = load_frag(kp, 2 * (t * (uint32_t)a.k_st + e) | miss);
+      *reinterpret_cast<bf16x8*>(Ql + t * LD + e) = load_frag(qp, 2 * (t * (uint32_t)a.q_st + e) | miss);
     }
   }
   __syncthreads();
@@ -360,21 +370,21 @@ __global__ __launch_bounds__(64 * NW) void delta_grads_kernel(Args a) {
           const int t = 16 * (f & 3) + r;
           const uint32_t ld = f < 4 ? (uint32_t)a.do_st : (uint32_t)orow;
           const Rsrc p = f < 4 ? src[0] : f < 8 ? src[1] : f < 12 ? src[2] : f < 16 ? src[3] : src[4];
-          st[i] = load_frag(p, t < ch.n && e < a.Dv ? 2 * (t * ld + e) : kNoRow);
+          st[i] = load_frag(p, 2 * (t * ld + e) | miss_from(t, ch.n) | miss_from(e, a.Dv));
         }
       }
 #pragma unroll
       for (int x = 0; x < FT; ++x) {
         const int feat = 16 * (wave * FT + x) + r;
-        const uint32_t at = feat < a.Dk && e < a.Dv ? 2 * (feat * a.Dv + e) : kNoRow;
+        const uint32_t at = 2 * (feat * a.Dv + e) | miss_from(feat, a.Dk) | miss_from(e, a.Dv);
         sh[x] = load_frag(sp, at);
-        sl[x] = load_frag(sp, at + lo_at);
+        sl[x] = load_frag(sp, at, lo_at);
         dh[x] = load_frag(dp, at);
-        dl[x] = load_frag(dp, at + lo_at);
+        dl[x] = load_frag(dp, at, lo_at);
       }
       if (wave < 4) {
         const int t = 16 * rw + r;
-        vf = load_frag(vp, t < ch.n && e < a.Dv ? 2 * (t * (uint32_t)a.v_st + e) : kNoRow);
+        vf = load_frag(vp, 2 * (t * (uint32_t)a.v_st + e) | miss_from(t, ch.n) | miss_from(e, a.Dv));
       }
     };
     f32x4 EQ[4][FT] = {}, ER[4][FT] = {}, EU[4][FT] = {}, dP[CT] = {}, dA[CT] = {};

@@ -1,44 +1,50 @@
 // Forward of the chunked gated delta rule: the scan over each sequence's
 // chunks (formulas, precision and fragment layout in delta.h).
 //
-// A workgroup of four waves owns 16 NT value columns of one head of one
-// sequence and walks its chunks in order.  Each wave has a quarter of every
-// product's rows: 16 tokens of X = K S0, of U = T R and of O, and a quarter of
-// the state's features, which stay in its registers from the first chunk to
-// the last.  So an operand fragment (K, Q, T, P, K^T) is read by one wave,
-// straight into its registers and a chunk ahead, and only S, R and U pass
-// through LDS, from the wave that made them to all four: three barriers a
-// chunk.  With one wave for all rows of 16 columns instead, and the fragments
-// in LDS for four such waves, a chunk took 4.9 us (79 chunks of 128 x 128).
+// A workgroup owns 16 NT value columns of one head of one sequence and walks
+// its chunks in order, with two kinds of waves.  Four carry the state: each has
+// 16 tokens of X = K S0 and of U = T R, and a quarter of the state's features,
+// which stay in its registers from the first chunk to the last.  Four make the
+// outputs, 16 tokens each, from the same S0 and U, off the chain that bounds a
+// chunk.  An operand fragment (K, Q, T, P, K^T) is read by one wave, straight
+// into its registers and a chunk ahead; S, R and U pass through LDS, from the
+// wave that made them to all: three barriers a chunk.
 #include "delta.h"
 
 namespace uttt {
 namespace delta {
 namespace {
 
+// LDS of a scan's workgroup: operand fragments (32 contracted rows x 16
+// columns, 1 KiB), in two bf16 parts.
+template <int KS, int NT>
+struct ScanLds {
+  uint8_t S[2][KS * NT * 1024];
+  uint8_t R[2][2 * NT * 1024];
+  uint8_t U[2][2 * NT * 1024];
+  uint8_t E[2][2 * NT * 1024];   // e^{G_C - G} U
+};
+
+// What both kinds of waves know of their place.
+struct Lane {
+  int wave, lane, r, q, col;   // wave: its row tile; col: the lane's first column
+  uint32_t dead;               // kNoRow where the column is none
+  uint32_t last_half, before_half;   // kNoRow where the last two steps' features are none
+};
+
 template <int KS, int NT, bool SAVE>
-__global__ __launch_bounds__(256) void delta_scan_kernel(Args a) {
+__device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const Lane& l, ScanLds<KS, NT>& lds) {
   constexpr int FT = (2 * KS + 3) / 4;   // 16-feature tiles of a wave
-  __shared__ __attribute__((aligned(16))) uint8_t Sb[2][KS * NT * 1024];
-  __shared__ __attribute__((aligned(16))) uint8_t Rb[2][2 * NT * 1024];
-  __shared__ __attribute__((aligned(16))) uint8_t Ub[2][2 * NT * 1024];   // U
-  __shared__ __attribute__((aligned(16))) uint8_t Eb[2][2 * NT * 1024];   // e^{G_C - G} U
-  Scan s;
-  if (!s.init(a, 16 * NT)) return;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int r = lane & 15, q = lane >> 4;
-  const int col = s.col0 + NT * r;   // the lane's first column
-  const bool live = col < a.Dv;
+  const int wave = l.wave, r = l.r, q = l.q, col = l.col;
+  const uint32_t dead = l.dead;
   const uint32_t put = (r + 16 * (q >> 1)) * 16 + (q & 1) * 8;   // 4 rows of a tile in a fragment
-  const auto put_tile = [&](uint8_t (*buf)[2 * NT * 1024], int n, f32x4 x) {
-    bf16x4 hi, lo;
-    split4(x, hi, lo);
-    const uint32_t at = ((wave >> 1) * NT + n) * 1024 + (wave & 1) * 512 + put;
-    *reinterpret_cast<bf16x4*>(buf[0] + at) = hi;
-    *reinterpret_cast<bf16x4*>(buf[1] + at) = lo;
+  const uint32_t put_tok = (wave >> 1) * NT * 1024 + (wave & 1) * 512 + put;
+  const auto put_tile = [&](uint8_t (*buf)[2 * NT * 1024], int n, const Parts& p) {
+    *reinterpret_cast<u32x2*>(buf[0] + put_tok + n * 1024) = p.hi;
+    *reinterpret_cast<u32x2*>(buf[1] + put_tok + n * 1024) = p.lo;
   };
   const auto get = [&](const uint8_t* buf, int f) {
-    return *reinterpret_cast<const bf16x8*>(buf + f * 1024 + lane * 16);
+    return *reinterpret_cast<const bf16x8*>(buf + f * 1024 + l.lane * 16);
   };
 
   f32x4 S[FT][NT];
@@ -49,119 +55,123 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(Args a) {
       const int feat = 16 * (wave * FT + f) + 4 * q + i;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
-        S[f][n][i] = a.h0 && live && feat < a.Dk
+        S[f][n][i] = a.h0 && col < a.Dv && feat < a.Dk
                          ? a.h0[((int64_t)s.head * a.Dk + feat) * a.Dv + col + n] : 0.0f;
     }
 
-  bf16x8 kf[KS], qf[KS], tf[2][2], pf[2][2], ktf[FT][2];
+  bf16x8 kf[KS], tf[2][2], ktf[FT][2];
   f32x4 gam, ge, bt;
   float gc;
   Cols<NT> vr[4];
-  // The loads of chunk c's operands; past the last chunk they repeat it.
-  const auto load_rows = [&](int c) {
-    c = min(c, s.nc - 1);
-    const int n = min(kC, s.len - c * kC), t = 16 * wave + r;
-    const Rsrc kp = buffer_at(a.k + s.b * a.k_sb + s.hk * a.k_sh + (s.tok0 + (int64_t)c * kC) * a.k_st);
-    const Rsrc qp = buffer_at(a.q + s.b * a.q_sb + s.hk * a.q_sh + (s.tok0 + (int64_t)c * kC) * a.q_st);
-    const Rsrc vp = buffer_at(a.v + s.b * a.v_sb + s.hv * a.v_sh + (s.tok0 + (int64_t)c * kC) * a.v_st);
+  // Operands of the next chunk: pointers that go along, per-lane offsets that
+  // stay, and the bit that masks rows past the sequence.  Each is loaded where
+  // its last value was used, in the order of use, which is the order in which
+  // loads are waited for.
+  const uint16_t* kp = a.k + s.b * a.k_sb + s.hk * a.k_sh + s.tok0 * a.k_st;
+  const uint16_t* vp = a.v + s.b * a.v_sb + s.hv * a.v_sh + s.tok0 * a.v_st;
+  const uint8_t* trip = a.tri + ((size_t)s.c0 * a.Hv + s.hv) * kTriBytes;
+  const uint8_t* ktp = a.kt + ((size_t)s.c0 * a.Hk + s.hk) * (4 * KS * 1024);
+  const float* scp = a.scal + ((size_t)s.c0 * a.Hv + s.hv) * kScal;
+  const uint32_t krow = 2 * ((16 * wave + r) * (uint32_t)a.k_st + 8 * q);
+  const uint32_t vrow = 2 * ((16 * wave + 4 * q) * (uint32_t)a.v_st + col);
+  const uint32_t urow = 2 * ((16 * wave + 4 * q) * (uint32_t)(a.Hv * a.Dv) + col);
+  const auto load_rows = [&](int left) {
+    const uint32_t miss = miss_from(16 * wave + r, left), at = 4 * (16 * wave + 4 * q) | miss_from(0, left);
+    const Rsrc kr = buffer_at(kp), vr_ = buffer_at(vp), sr = buffer_at(scp);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int e = 32 * ks + 8 * q;
-      const bool ok = t < n && e < a.Dk;
-      kf[ks] = load_frag(kp, ok ? 2 * (t * (uint32_t)a.k_st + e) : kNoRow);
-      qf[ks] = load_frag(qp, ok ? 2 * (t * (uint32_t)a.q_st + e) : kNoRow);
-    }
+    for (int ks = 0; ks < KS; ++ks)
+      kf[ks] = load_frag(kr, (krow + 64 * ks) | miss | (ks == KS - 1 ? l.last_half : ks == KS - 2 ? l.before_half : 0));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int tv = 16 * wave + 4 * q + i;
-      vr[i].load(vp, tv < n && live ? 2 * (tv * (uint32_t)a.v_st + col) : kNoRow);
-    }
+    for (int i = 0; i < 4; ++i)
+      vr[i].load(vr_, (vrow + 2 * i * (uint32_t)a.v_st) | dead | miss_from(16 * wave + 4 * q + i, left));
+    gam = load_f4(sr, at);
+    bt = load_f4(sr, at, 8 * kC);
+    kp += kC * a.k_st;
+    vp += kC * a.v_st;
   };
-  const auto load_scal = [&](int c) {
-    const float* sc = a.scal + ((size_t)(s.c0 + min(c, s.nc - 1)) * a.Hv + s.hv) * kScal;
-    const int t = 16 * wave + 4 * q;
-    gam = *reinterpret_cast<const f32x4*>(sc + t);
-    ge = *reinterpret_cast<const f32x4*>(sc + kC + t);
-    bt = *reinterpret_cast<const f32x4*>(sc + 2 * kC + t);
-    gc = sc[kC - 1];
-  };
-  const auto load_tri = [&](int c, int which, bf16x8 (&x)[2][2]) {
-    const uint8_t* p = a.tri + ((size_t)(s.c0 + min(c, s.nc - 1)) * a.Hv + s.hv) * kTriBytes +
-                       which * 2 * kTFrags * 1024 + lane * 16;
+  const auto load_t = [&](int left) {
+    const Rsrc tr = buffer_at(trip);
+    const uint32_t at = l.lane * 16 | miss_from(0, left);
+    ge = load_f4(buffer_at(scp), 4 * (16 * wave + 4 * q) | miss_from(0, left), 4 * kC);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       // step 1 of the upper tiles is zero and not stored: step 0 again, unused
       const int f = lower_frag(wave, wave < 2 ? 0 : ks);
-      x[ks][0] = *reinterpret_cast<const bf16x8*>(p + f * 1024);
-      x[ks][1] = *reinterpret_cast<const bf16x8*>(p + (kTFrags + f) * 1024);
+      tf[ks][0] = load_frag(tr, at, f * 1024);
+      tf[ks][1] = load_frag(tr, at, (kTFrags + f) * 1024);
     }
+    trip += (size_t)a.Hv * kTriBytes;
   };
-  const auto load_kt = [&](int c) {
-    const uint8_t* p = a.kt + ((size_t)(s.c0 + min(c, s.nc - 1)) * a.Hk + s.hk) * (4 * KS) * 1024 + lane * 16;
+  const auto load_kt = [&](int left) {
+    const Rsrc tr = buffer_at(ktp);
+    const uint32_t at = l.lane * 16 | miss_from(0, left);
 #pragma unroll
     for (int f = 0; f < FT; ++f)
 #pragma unroll
       for (int t = 0; t < 2; ++t)
-        if (wave * FT + f < 2 * KS)
-          ktf[f][t] = *reinterpret_cast<const bf16x8*>(p + (2 * (wave * FT + f) + t) * 1024);
+        if (wave * FT + f < 2 * KS) ktf[f][t] = load_frag(tr, at, (2 * (wave * FT + f) + t) * 1024);
+    gc = load_f1(buffer_at(scp), 4 * (kC - 1) | miss_from(0, left));
+    ktp += (size_t)a.Hk * (4 * KS * 1024);
+    scp += a.Hv * kScal;
   };
   // the state's parts to LDS, and of a chunk that a backward will read to memory
-  const auto put_state = [&](int c) {
-    Rsrc sp;
-    if constexpr (SAVE) sp = buffer_at(a.s0 + ((int64_t)(s.c0 + c) * a.Hv + s.hv) * 2 * a.Dk * a.Dv);
+  uint16_t* s0p = SAVE ? a.s0 + ((int64_t)s.c0 * a.Hv + s.hv) * 2 * a.Dk * a.Dv : nullptr;
+  Parts sw[FT][NT];
+  const auto put_state = [&]() {
 #pragma unroll
     for (int f = 0; f < FT; ++f) {
       const int tile = wave * FT + f;
-      if (tile < 2 * KS) {
-        bf16x4 hi[NT], lo[NT];
+      if (tile < 2 * KS)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          split4(S[f][n], hi[n], lo[n]);
+          sw[f][n] = parts_of(S[f][n]);
           const uint32_t at = ((tile >> 1) * NT + n) * 1024 + (tile & 1) * 512 + put;
-          *reinterpret_cast<bf16x4*>(Sb[0] + at) = hi[n];
-          *reinterpret_cast<bf16x4*>(Sb[1] + at) = lo[n];
+          *reinterpret_cast<u32x2*>(lds.S[0] + at) = sw[f][n].hi;
+          *reinterpret_cast<u32x2*>(lds.S[1] + at) = sw[f][n].lo;
         }
-        if constexpr (SAVE) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int feat = 16 * tile + 4 * q + i;
-            const uint32_t at = live && feat < a.Dk ? 2 * (feat * a.Dv + col) : kNoRow;
-            __bf16 h[NT], l[NT];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              h[n] = hi[n][i];
-              l[n] = lo[n][i];
-            }
-            store_cols<NT>(sp, at, h);
-            store_cols<NT>(sp, at + 2 * (uint32_t)(a.Dk * a.Dv), l);
-          }
-        }
-      }
     }
   };
+  const auto save_state = [&]() {
+    const Rsrc sr = buffer_at(s0p);
+#pragma unroll
+    for (int f = 0; f < FT; ++f)
+      if (wave * FT + f < 2 * KS) {
+        u32x2 hi[NT], lo[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          hi[n] = sw[f][n].hi;
+          lo[n] = sw[f][n].lo;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int feat = 16 * (wave * FT + f) + 4 * q + i;
+          const uint32_t at = 2 * (feat * a.Dv + col) | dead | miss_from(feat, a.Dk);
+          store_row<NT>(sr, at, hi, i);
+          store_row<NT>(sr, at, lo, i, 2 * (uint32_t)(a.Dk * a.Dv));
+        }
+      }
+    s0p += (int64_t)a.Hv * 2 * a.Dk * a.Dv;
+  };
 
-  if (s.nc > 0) {
-    load_rows(0);
-    load_scal(0);
-    load_tri(0, 0, tf);
-    load_tri(0, 1, pf);
-    load_kt(0);
-    put_state(0);
+  if (s.len > 0) {
+    load_rows(s.len);
+    load_t(s.len);
+    load_kt(s.len);
+    put_state();
+    settle();
   }
-  for (int c = 0; c < s.nc; ++c) {
+  uint16_t* up = SAVE ? a.u + (((int64_t)s.b * a.T + s.tok0) * a.Hv + s.hv) * a.Dv : nullptr;
+  const int64_t plane = (int64_t)a.B * a.T * a.Hv * a.Dv;
+  for (int left = s.len; left > 0; left -= kC) {
     lds_barrier();   // S0 is in LDS
-    f32x4 X[NT] = {}, O[NT] = {};
     {
-      f32x4 X2[NT] = {}, O2[NT] = {};
+      f32x4 X[NT] = {}, X2[NT] = {};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const bf16x8 hi = get(Sb[0], ks * NT + n), lo = get(Sb[1], ks * NT + n);
-          X[n] = mfma(kf[ks], hi, X[n]);
-          O[n] = mfma(qf[ks], hi, O[n]);
-          X2[n] = mfma(kf[ks], lo, X2[n]);
-          O2[n] = mfma(qf[ks], lo, O2[n]);
+          X[n] = mfma(kf[ks], get(lds.S[0], ks * NT + n), X[n]);
+          X2[n] = mfma(kf[ks], get(lds.S[1], ks * NT + n), X2[n]);
         }
       // R = b (V - gam X); rows behind the sequence's end have b = 0 and V = 0
 #pragma unroll
@@ -169,48 +179,37 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(Args a) {
         f32x4 v;
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = vr[i].get(n);
-        put_tile(Rb, n, bt * (v - gam * (X[n] + X2[n])));
-        O[n] = (O[n] + O2[n]) * (gam * a.scale);
+        put_tile(lds.R, n, parts_of(bt * (v - gam * (X[n] + X2[n]))));
       }
     }
-    load_rows(c + 1);
+    load_rows(left - kC);
     lds_barrier();   // R is in LDS
     f32x4 U[NT] = {};
+    {
+      f32x4 U2[NT] = {};
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-      if (ks <= wave >> 1)
+      for (int ks = 0; ks < 2; ++ks)
+        if (ks <= wave >> 1)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const bf16x8 hi = get(Rb[0], ks * NT + n), lo = get(Rb[1], ks * NT + n);
-          U[n] = mfma(tf[ks][0], hi, U[n]);
-          U[n] = mfma(tf[ks][1], hi, U[n]);
-          U[n] = mfma(tf[ks][0], lo, U[n]);
-        }
-    load_tri(c + 1, 0, tf);
+          for (int n = 0; n < NT; ++n) {
+            const bf16x8 hi = get(lds.R[0], ks * NT + n), lo = get(lds.R[1], ks * NT + n);
+            U[n] = mfma(tf[ks][0], hi, U[n]);
+            U2[n] = mfma(tf[ks][1], hi, U2[n]);
+            U2[n] = mfma(tf[ks][0], lo, U2[n]);
+          }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) U[n] += U2[n];
+    }
+    u32x2 uh[NT], ul[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      put_tile(Eb, n, ge * U[n]);
-      put_tile(Ub, n, U[n]);
+      put_tile(lds.E, n, parts_of(ge * U[n]));
+      const Parts p = parts_of(U[n]);
+      put_tile(lds.U, n, p);
+      uh[n] = p.hi;
+      ul[n] = p.lo;
     }
-    const int left = s.len - c * kC;
-    const int64_t row0 = (int64_t)s.b * a.T + s.tok0 + (int64_t)c * kC;
-    if constexpr (SAVE) {
-      const int64_t at = (row0 * a.Hv + s.hv) * a.Dv;
-      const Rsrc hp = buffer_at(a.u + at), lp = buffer_at(a.u + (int64_t)a.B * a.T * a.Hv * a.Dv + at);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = 16 * wave + 4 * q + i;
-        const uint32_t off = live && t < left ? 2 * (t * (uint32_t)(a.Hv * a.Dv) + col) : kNoRow;
-        __bf16 h[NT], l[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          h[n] = (__bf16)U[n][i];
-          l[n] = (__bf16)(U[n][i] - (float)h[n]);
-        }
-        store_cols<NT>(hp, off, h);
-        store_cols<NT>(lp, off, l);
-      }
-    }
+    load_t(left - kC);
     lds_barrier();   // U is in LDS
     // S' = gam_C S0 + K^T (e^{G_C - G} U)
 #pragma unroll
@@ -221,7 +220,7 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(Args a) {
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const bf16x8 hi = get(Eb[0], t * NT + n), lo = get(Eb[1], t * NT + n);
+        const bf16x8 hi = get(lds.E[0], t * NT + n), lo = get(lds.E[1], t * NT + n);
 #pragma unroll
         for (int f = 0; f < FT; ++f)
           if (wave * FT + f < 2 * KS) {
@@ -229,32 +228,21 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(Args a) {
             S[f][n] = mfma(ktf[f][t], lo, S[f][n]);
           }
       }
-    load_kt(c + 1);
-    load_scal(c + 1);
-    // O += P U
+    load_kt(left - kC);
+    if constexpr (SAVE) {
+      const Rsrc hr = buffer_at(up), lr = buffer_at(up + plane);
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-      if (ks <= wave >> 1)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const bf16x8 hi = get(Ub[0], ks * NT + n), lo = get(Ub[1], ks * NT + n);
-          O[n] = mfma(pf[ks][0], hi, O[n]);
-          O[n] = mfma(pf[ks][1], hi, O[n]);
-          O[n] = mfma(pf[ks][0], lo, O[n]);
-        }
-    load_tri(c + 1, 1, pf);
-    if (c + 1 < s.nc) put_state(c + 1);
-    const Rsrc op = buffer_at(a.o + (row0 * a.Hv + s.hv) * a.Dv);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = 16 * wave + 4 * q + i;
-      __bf16 h[NT];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) h[n] = (__bf16)O[n][i];
-      store_cols<NT>(op, live && t < left ? 2 * (t * (uint32_t)(a.Hv * a.Dv) + col) : kNoRow, h);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t at = (urow + 2 * i * (uint32_t)(a.Hv * a.Dv)) | dead | miss_from(16 * wave + 4 * q + i, left);
+        store_row<NT>(hr, at, uh, i);
+        store_row<NT>(lr, at, ul, i);
+      }
+      up += (int64_t)kC * a.Hv * a.Dv;
+      save_state();   // S0, whose parts the last put_state left
     }
+    if (left > kC) put_state();
   }
-  if (a.hT && live) {
+  if (a.hT && col < a.Dv) {
 #pragma unroll
     for (int f = 0; f < FT; ++f)
 #pragma unroll
@@ -268,10 +256,103 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(Args a) {
 }
 
 template <int KS, int NT>
+__device__ __forceinline__ void scan_outputs(const Args& a, const Scan& s, const Lane& l, ScanLds<KS, NT>& lds) {
+  const int wave = l.wave, q = l.q;
+  const auto get = [&](const uint8_t* buf, int f) {
+    return *reinterpret_cast<const bf16x8*>(buf + f * 1024 + l.lane * 16);
+  };
+  bf16x8 qf[KS], pf[2][2];
+  f32x4 gam;
+  const uint16_t* qp = a.q + s.b * a.q_sb + s.hk * a.q_sh + s.tok0 * a.q_st;
+  const uint8_t* trip = a.tri + ((size_t)s.c0 * a.Hv + s.hv) * kTriBytes;
+  const float* scp = a.scal + ((size_t)s.c0 * a.Hv + s.hv) * kScal;
+  uint16_t* op = a.o + (((int64_t)s.b * a.T + s.tok0) * a.Hv + s.hv) * a.Dv;
+  const uint32_t qrow = 2 * ((16 * wave + l.r) * (uint32_t)a.q_st + 8 * q);
+  const uint32_t orow = 2 * ((16 * wave + 4 * q) * (uint32_t)(a.Hv * a.Dv) + l.col);
+  const auto load_rows = [&](int left) {
+    const uint32_t miss = miss_from(16 * wave + l.r, left);
+    const Rsrc qr = buffer_at(qp), sr = buffer_at(scp);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      qf[ks] = load_frag(qr, (qrow + 64 * ks) | miss | (ks == KS - 1 ? l.last_half : ks == KS - 2 ? l.before_half : 0));
+    gam = load_f4(sr, 4 * (16 * wave + 4 * q) | miss_from(0, left));
+    qp += kC * a.q_st;
+    scp += a.Hv * kScal;
+  };
+  const auto load_p = [&](int left) {
+    const Rsrc tr = buffer_at(trip);
+    const uint32_t at = l.lane * 16 | miss_from(0, left);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const int f = 2 * kTFrags + lower_frag(wave, wave < 2 ? 0 : ks);
+      pf[ks][0] = load_frag(tr, at, f * 1024);
+      pf[ks][1] = load_frag(tr, at, (kTFrags + f) * 1024);
+    }
+    trip += (size_t)a.Hv * kTriBytes;
+  };
+  if (s.len > 0) {
+    load_rows(s.len);
+    load_p(s.len);
+    settle();
+  }
+  for (int left = s.len; left > 0; left -= kC) {
+    lds_barrier();   // S0 is in LDS
+    f32x4 O[NT] = {}, O2[NT] = {};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        O[n] = mfma(qf[ks], get(lds.S[0], ks * NT + n), O[n]);
+        O2[n] = mfma(qf[ks], get(lds.S[1], ks * NT + n), O2[n]);
+      }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      O[n] = (O[n] + O2[n]) * (gam * a.scale);
+      O2[n] = f32x4{};
+    }
+    load_rows(left - kC);
+    lds_barrier();   // R is in LDS
+    lds_barrier();   // U is in LDS
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+      if (ks <= wave >> 1)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const bf16x8 hi = get(lds.U[0], ks * NT + n), lo = get(lds.U[1], ks * NT + n);
+          O[n] = mfma(pf[ks][0], hi, O[n]);
+          O2[n] = mfma(pf[ks][1], hi, O2[n]);
+          O2[n] = mfma(pf[ks][0], lo, O2[n]);
+        }
+    load_p(left - kC);
+    const Rsrc orsrc = buffer_at(op);
+    u32x2 ow[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) ow[n] = round_of(O[n] + O2[n]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      store_row<NT>(orsrc, (orow + 2 * i * (uint32_t)(a.Hv * a.Dv)) | l.dead | miss_from(16 * wave + 4 * q + i, left), ow, i);
+    op += (int64_t)kC * a.Hv * a.Dv;
+  }
+}
+
+template <int KS, int NT, bool SAVE>
+__global__ __launch_bounds__(512) void delta_scan_kernel(Args a) {
+  __shared__ __attribute__((aligned(16))) ScanLds<KS, NT> lds;
+  Scan s;
+  if (!s.init(a, 16 * NT)) return;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int r = lane & 15, q = lane >> 4, col = s.col0 + NT * r;
+  const Lane l{wave & 3, lane, r, q, col, miss_from(col, a.Dv), miss_from(32 * (KS - 1) + 8 * q, a.Dk),
+               miss_from(32 * (KS - 2) + 8 * q, a.Dk)};
+  if (wave < 4) scan_state<KS, NT, SAVE>(a, s, l, lds);
+  else scan_outputs<KS, NT>(a, s, l, lds);
+}
+
+template <int KS, int NT>
 void launch_scan_as(const Args& a, hipStream_t st) {
   const dim3 grid(scan_blocks(a, 16 * NT));
-  if (a.s0) hipLaunchKernelGGL((delta_scan_kernel<KS, NT, true>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((delta_scan_kernel<KS, NT, false>), grid, dim3(256), 0, st, a);
+  if (a.s0) hipLaunchKernelGGL((delta_scan_kernel<KS, NT, true>), grid, dim3(512), 0, st, a);
+  else hipLaunchKernelGGL((delta_scan_kernel<KS, NT, false>), grid, dim3(512), 0, st, a);
 }
 
 int launch_scan(const Args& a, hipStream_t st) {

@@ -139,11 +139,12 @@ __device__ __forceinline__ void write_transposed(const uint16_t* lds, uint8_t* o
 
 constexpr int kLT = kC + 4;   // fp32 row stride of the 64 x 64 matrices
 
-// hi and lo fragments of a triangular matrix (or its transpose) in LDS.
+// hi and lo fragments first, first + step, .. of a triangular matrix (or its
+// transpose) in LDS.
 template <bool TRANS>
-__device__ __forceinline__ void write_tri(const float* m, uint8_t* out) {
+__device__ __forceinline__ void write_tri(const float* m, uint8_t* out, int first, int step) {
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  for (int f = threadIdx.x >> 6; f < kTFrags; f += 4) {
+  for (int f = first; f < kTFrags; f += step) {
     const int rt = TRANS ? (f < 4 ? f >> 1 : f - 2) : (f < 2 ? f : 2 + (f - 2) / 2);
     const int ks = TRANS ? (f < 4 ? f & 1 : 1) : (f < 2 ? 0 : f & 1);
     const int row = 16 * rt + r, c0 = 32 * ks + 8 * q;
@@ -165,12 +166,11 @@ __device__ __forceinline__ void write_tri(const float* m, uint8_t* out) {
 // stable for any keys, where a product of powers of A is not), then pairs of
 // blocks joined by T21 = -T22 A21 T11 in fp32 matrix instructions.
 template <int KS, bool BWD>
-__global__ __launch_bounds__(256) void delta_prep_kernel(Args a) {
+__global__ __launch_bounds__(256, KS <= 4 ? 4 : 2) void delta_prep_kernel(Args a) {
   constexpr int LD = 32 * KS + 8;
   constexpr int kRows = 2 * kC * LD * 2;                 // K and Q, bytes
   constexpr int kMats = 2 * kC * kLT * 4;                // A and P
   __shared__ __attribute__((aligned(16))) uint8_t buf[kRows > kMats ? kRows : kMats];
-  __shared__ __attribute__((aligned(16))) float Tm[kC * kLT];
   __shared__ double Gd[kC];
   __shared__ float bet[kC];
   const int c = blockIdx.x / a.Hk, hk = blockIdx.x % a.Hk;
@@ -204,6 +204,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Args a) {
   __syncthreads();
   float* Am = reinterpret_cast<float*>(buf);
   float* Pm = Am + kC * kLT;
+  float* Tm = Pm;   // T takes P's place once P's fragments are written
   const int group = a.Hv / a.Hk;
   for (int hv = hk * group; hv < (hk + 1) * group; ++hv) {
     if (wave == 0) {
@@ -247,10 +248,10 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Args a) {
     }
     __syncthreads();
     uint8_t* tri = a.tri + ((size_t)c * a.Hv + hv) * kTriBytes;
+    // wave 0: column r of diagonal block q, top to bottom; the others: P's fragments
+    float t[16];
     if (wave == 0) {
-      // column r of diagonal block q, top to bottom
       const float* A0 = Am + 16 * q * kLT + 16 * q;
-      float t[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float x = i == r ? 1.0f : 0.0f;
@@ -258,6 +259,11 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Args a) {
         for (int j = 0; j < i; ++j) x = __builtin_fmaf(-A0[i * kLT + j], t[j], x);
         t[i] = x;
       }
+    } else {
+      write_tri<BWD>(Pm, tri + 2 * kTFrags * 1024, wave - 1, 3);
+    }
+    __syncthreads();
+    if (wave == 0) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) Tm[(16 * q + i) * kLT + 16 * q + r] = t[i];
     } else if (wave == 1) {
@@ -268,7 +274,6 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Args a) {
         Tm[(32 + 4 * q + i) * kLT + 48 + r] = 0.0f;
       }
     }
-    write_tri<BWD>(Pm, tri + 2 * kTFrags * 1024);
     __syncthreads();
     if (wave < 2) {   // blocks 2w, 2w + 1 joined
       const int b0 = 32 * wave, b1 = b0 + 16;
@@ -301,7 +306,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Args a) {
       for (int i = 0; i < 4; ++i) Tm[(32 + 16 * rt + 4 * q + i) * kLT + 16 * ct + r] = -z[i];
     }
     __syncthreads();
-    write_tri<BWD>(Tm, tri);
+    write_tri<BWD>(Tm, tri, wave, 4);
     __syncthreads();
   }
 }

@@ -38,7 +38,7 @@ struct LnArgs {
 template <class TT, int V>
 __device__ __forceinline__ void load_piece(const typename TT::S* p, float (&v)[V]) {
   typename TT::S w[V];
-  __builtin_memcpy(w, __builtin_assume_aligned(p, sizeof w), sizeof w);
+  __builtin_memcpy(w, __builtin_assume_aligned(p, sizeof w > 16 ? 16 : sizeof w), sizeof w);
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i] = TT::load(w[i]);
 }
@@ -48,6 +48,20 @@ __device__ __forceinline__ void store_piece(typename TT::S* p, const float (&v)[
 #pragma unroll
   for (int i = 0; i < V; ++i) w[i] = TT::store(v[i]);
   __builtin_memcpy(__builtin_assume_aligned(p, sizeof w), w, sizeof w);
+}
+// V weights from element e, `none` where there is no weight tensor.
+template <int V>
+__device__ __forceinline__ void load_weights(const void* p, int dtype, int e, float none, float (&v)[V]) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = none;
+  } else if (dtype == UTTT_F32) {
+    load_piece<F32T, V>(static_cast<const float*>(p) + e, v);
+  } else if (dtype == UTTT_BF16) {
+    load_piece<BF16T, V>(static_cast<const uint16_t*>(p) + e, v);
+  } else {
+    load_piece<F16T, V>(static_cast<const uint16_t*>(p) + e, v);
+  }
 }
 __device__ __forceinline__ float load_w(const void* p, int dtype, int i) {
   if (dtype == UTTT_F32) return static_cast<const float*>(p)[i];
@@ -80,52 +94,60 @@ __device__ __forceinline__ void row_sums(float& a, float& b, float* red) {
 template <class TT, int V, int LPR, int NI>
 __global__ __launch_bounds__(kLnThreads) void ln_fwd_kernel(LnArgs a) {
   using S = typename TT::S;
+  constexpr int RPB = kLnThreads / LPR;
   __shared__ float red[8];
-  const int64_t row0 = (int64_t)blockIdx.x * (kLnThreads / LPR) + threadIdx.x / LPR;
-  const bool live = row0 < a.rows;
-  const int64_t row = live ? row0 : a.rows - 1;
-  const int lane = threadIdx.x % LPR;
-  const S* x = static_cast<const S*>(a.x) + row * a.x_st;
-  float v[NI][V];
-  float sum = 0.0f, dummy = 0.0f;
+  const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR;
+  float w[NI][V], b[NI][V];   // for all the rows that the workgroup walks over
 #pragma unroll
   for (int c = 0; c < NI; ++c) {
     const int e = (lane + LPR * c) * V;
-    if (e < a.N) load_piece<TT, V>(x + e, v[c]);
-    else
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[c][i] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) sum += v[c][i];
-  }
-  row_sums<LPR>(sum, dummy, red);
-  const float mean = sum / (float)a.N;
-  float sq = 0.0f;
-#pragma unroll
-  for (int c = 0; c < NI; ++c)
-    if ((lane + LPR * c) * V < a.N)
-#pragma unroll
-      for (int i = 0; i < V; ++i) sq = __builtin_fmaf(v[c][i] - mean, v[c][i] - mean, sq);
-  row_sums<LPR>(sq, dummy, red);
-  const float rstd = 1.0f / sqrtf(sq / (float)a.N + a.eps);
-  if (!live) return;
-  if (a.stats && lane == 0) {
-    a.stats[row] = mean;
-    a.stats[a.rows + row] = rstd;
-  }
-  S* y = static_cast<S*>(a.y) + row * a.N;
-#pragma unroll
-  for (int c = 0; c < NI; ++c) {
-    const int e = (lane + LPR * c) * V;
-    if (e >= a.N) continue;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float h = (v[c][i] - mean) * rstd;
-      if (a.w) h *= load_w(a.w, a.w_dtype, e + i);
-      if (a.b) h += load_w(a.b, a.b_dtype, e + i);
-      v[c][i] = h;
+    if (e < a.N) {
+      load_weights<V>(a.w, a.w_dtype, e, 1.0f, w[c]);
+      load_weights<V>(a.b, a.b_dtype, e, 0.0f, b[c]);
     }
-    store_piece<TT, V>(y + e, v[c]);
+  }
+  for (int64_t base = (int64_t)blockIdx.x * RPB; base < a.rows; base += (int64_t)gridDim.x * RPB) {
+    const bool live = base + slot < a.rows;
+    const int64_t row = live ? base + slot : a.rows - 1;
+    const S* x = static_cast<const S*>(a.x) + row * a.x_st;
+    float v[NI][V];
+    float sum = 0.0f, dummy = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NI; ++c) {
+      const int e = (lane + LPR * c) * V;
+      if (e < a.N) load_piece<TT, V>(x + e, v[c]);
+      else
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[c][i] = 0.0f;
+    }
+#pragma unroll
+    for (int c = 0; c < NI; ++c)
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum += v[c][i];
+    row_sums<LPR>(sum, dummy, red);
+    const float mean = sum / (float)a.N;
+    float sq = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NI; ++c)
+      if ((lane + LPR * c) * V < a.N)
+#pragma unroll
+        for (int i = 0; i < V; ++i) sq = __builtin_fmaf(v[c][i] - mean, v[c][i] - mean, sq);
+    row_sums<LPR>(sq, dummy, red);
+    const float rstd = 1.0f / sqrtf(sq / (float)a.N + a.eps);
+    if (!live) continue;   // whole rows: no later exchange in this turn
+    if (a.stats && lane == 0) {
+      a.stats[row] = mean;
+      a.stats[a.rows + row] = rstd;
+    }
+    S* y = static_cast<S*>(a.y) + row * a.N;
+#pragma unroll
+    for (int c = 0; c < NI; ++c) {
+      const int e = (lane + LPR * c) * V;
+      if (e >= a.N) continue;
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[c][i] = __builtin_fmaf((v[c][i] - mean) * rstd, w[c][i], b[c][i]);
+      store_piece<TT, V>(y + e, v[c]);
+    }
   }
 }
 
@@ -138,13 +160,12 @@ __global__ __launch_bounds__(kLnThreads) void ln_bwd_kernel(LnArgs a) {
   const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR;
   float w[NI][V], dw[NI][V], db[NI][V];
 #pragma unroll
-  for (int c = 0; c < NI; ++c)
+  for (int c = 0; c < NI; ++c) {
+    const int e = (lane + LPR * c) * V;
+    if (e < a.N) load_weights<V>(a.w, a.w_dtype, e, 1.0f, w[c]);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = (lane + LPR * c) * V + i;
-      w[c][i] = e < a.N ? (a.w ? load_w(a.w, a.w_dtype, e) : 1.0f) : 0.0f;
-      dw[c][i] = db[c][i] = 0.0f;
-    }
+    for (int i = 0; i < V; ++i) dw[c][i] = db[c][i] = 0.0f;
+  }
   const float inv_n = 1.0f / (float)a.N;
   for (int64_t base = (int64_t)blockIdx.x * RPB; base < a.rows; base += (int64_t)gridDim.x * RPB) {
     const bool live = base + slot < a.rows;
@@ -287,21 +308,27 @@ __global__ __launch_bounds__(kLnThreads) void ln_cols_kernel(LnArgs a, int64_t r
   out[a.N + e] = (float)db;
 }
 
-// The workgroups' totals added: 16 columns by 16 slices of the workgroups, in
+// The workgroups' totals added: 16 columns by 64 slices of the workgroups, in
 // a fixed order.
-__global__ __launch_bounds__(kLnThreads) void ln_sum_kernel(const float* __restrict__ part, int n, int N,
-                                                            void* dw, int w_dtype, void* db, int b_dtype) {
-  __shared__ float red[16][17];
+constexpr int kSumSlices = 64;
+__global__ __launch_bounds__(16 * kSumSlices) void ln_sum_kernel(const float* __restrict__ part, int n, int N,
+                                                                 void* dw, int w_dtype, void* db, int b_dtype) {
+  __shared__ float red[kSumSlices][17];
   const int c = threadIdx.x & 15, s = threadIdx.x >> 4;
   const int64_t e = (int64_t)blockIdx.x * 16 + c;   // over dw then db
   float sum = 0.0f;
   if (e < 2 * (int64_t)N)
-    for (int i = s; i < n; i += 16) sum += part[(int64_t)i * 2 * N + e];
+#pragma unroll 8
+    for (int i = s; i < n; i += kSumSlices) sum += part[(int64_t)i * 2 * N + e];
   red[s][c] = sum;
   __syncthreads();
-  if (s != 0 || e >= 2 * (int64_t)N) return;
 #pragma unroll
-  for (int i = 1; i < 16; ++i) sum += red[i][c];
+  for (int d = kSumSlices / 2; d > 0; d >>= 1) {
+    if (s < d) red[s][c] += red[s + d][c];
+    __syncthreads();
+  }
+  if (s != 0 || e >= 2 * (int64_t)N) return;
+  sum = red[0][c];
   const bool second = e >= N;
   void* out = second ? db : dw;
   const int dt = second ? b_dtype : w_dtype;
@@ -316,22 +343,25 @@ constexpr int kLnPieces = 2048, kLnOddMost = 8192;   // longest rows held in reg
 bool whole_pieces(const LnArgs& a, int size) {
   return ((int64_t)a.N * size) % 16 == 0 && (a.x_st * size) % 16 == 0 && (a.dy_st * size) % 16 == 0 &&
          ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) |
-           reinterpret_cast<uintptr_t>(a.dy)) & 15u) == 0;
+           reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.w) |
+           reinterpret_cast<uintptr_t>(a.b)) & 15u) == 0;
 }
 
-// Workgroups of the backward; a function of the sizes alone, so that its sums
-// come out the same on every run.
+// Workgroups of the backward: each writes 8 bytes per column, so that it has
+// 4 rows or more to walk over (4099 rows of 1537 fp32: 256 workgroups 55 us,
+// 1024 23 us).  A function of the sizes alone, so that its sums come out the
+// same on every run.
 int64_t bwd_blocks(int64_t rows, int N) {
-  const int64_t most = N <= 2048 ? 1024 : 512;
-  const int64_t per = N <= 64 ? 16 : 4;   // rows that a workgroup holds at once
-  const int64_t want = (rows + per - 1) / per;
-  return want < 1 ? 1 : want > most ? most : want;
+  const int64_t per = N <= 64 ? 16 : 4;
+  const int64_t n = (rows + per - 1) / per;
+  return n < 1024 ? n : 1024;
 }
 
 template <class TT, int V, int LPR, int NI>
 void ln_launch(const LnArgs& a, bool bwd, hipStream_t st) {
   constexpr int RPB = kLnThreads / LPR;
-  const int64_t blocks = (a.rows + RPB - 1) / RPB;
+  int64_t blocks = (a.rows + RPB - 1) / RPB;
+  if (blocks > 2048) blocks = 2048;   // 8 workgroups a CU: the weights are read once for many rows
   if (bwd)
     hipLaunchKernelGGL((ln_bwd_kernel<TT, V, LPR, NI>), dim3((unsigned)bwd_blocks(a.rows, a.N)),
                        dim3(kLnThreads), 0, st, a);
@@ -433,7 +463,7 @@ extern "C" int uttt_layer_norm_bwd(const void* x, int dtype, int64_t x_stride, c
     default: rc = ln_rows<F16T>(a, true, st); break;
   }
   if (rc || !sums) return rc;
-  hipLaunchKernelGGL(ln_sum_kernel, dim3((unsigned)((2 * (int64_t)N + 15) / 16)), dim3(kLnThreads), 0, st,
-                     a.part, (int)bwd_blocks(rows, N), N, dweight, weight_dtype, dbias, bias_dtype);
+  hipLaunchKernelGGL(ln_sum_kernel, dim3((unsigned)((2 * (int64_t)N + 15) / 16)), dim3(16 * kSumSlices), 0,
+                     st, a.part, (int)bwd_blocks(rows, N), N, dweight, weight_dtype, dbias, bias_dtype);
   return check_launch("layer_norm_sum");
 }
