@@ -211,6 +211,19 @@ __device__ __forceinline__ void store_row(Rsrc r, uint32_t off, const u32x2 (&x)
   }
 }
 
+// Sum over the 16 lanes of equal lane / 16, in all of them: four additions
+// with a lane permutation each, where a shuffle goes through LDS.
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float x) {
+  return x + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float sum16(float x) {
+  x = dpp_add<0xb1>(x);    // lane ^ 1
+  x = dpp_add<0x4e>(x);    // lane ^ 2
+  x = dpp_add<0x141>(x);   // 7 - lane % 8: the other four of eight
+  return dpp_add<0x140>(x);   // 15 - lane % 16
+}
+
 __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
   if (dtype == UTTT_F32) return static_cast<const float*>(p)[i];
   const uint16_t h = static_cast<const uint16_t*>(p)[i];

@@ -294,291 +294,352 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
 }
 
 // One chunk of one key head, its value heads one after another so that the
-// shared gradients of q and k are added in registers, in a fixed order.  NW
-// waves: each has FT 16-feature tiles of the [64, Dk] products, and a 16-token
-// row tile with CT column tiles of the [64, 64] ones.  The rows of dO, dR and U
-// pass through LDS 32 columns at a time (every wave reads all of them), loaded
-// a step ahead; S0 and dS' go straight to the wave that has their features.
-template <int KS, int NW>
-__global__ __launch_bounds__(64 * NW) void delta_grads_kernel(Args a) {
-  constexpr int LD = 32 * KS + 8, FT = (2 * KS + NW - 1) / NW, CT = 16 / NW, LX = kC + 4, LM = kC + 8;
+// shared gradients of q and k are added in registers, in a fixed order.  Each
+// of the 2 KS waves has one 16-feature tile of the [64, Dk] products; the
+// first PW also have a 16-token row tile and CT column tiles of the [64, 64]
+// ones.  The rows of dO, dR and U pass through LDS 32 columns at a time (every
+// wave reads all of them), loaded a step ahead; S0 and dS' go straight to the
+// wave that has their features.  It is bound by memory (S0, dS', U and dR are
+// 4 bytes an element) and its latency, so that registers (128) and LDS are
+// kept to what lets two workgroups of eight waves share a CU: the products
+// with dS' come in a second pass, when those with S0 and the [64, 64] ones are
+// done, which reads U and S0 (for <S0, dS'>) once more from cache.  With all
+// of them in one pass and one workgroup a CU 6144 chunks of 128 x 128 took 745
+// us, with two workgroups and the registers spilled 1129.
+constexpr int grads_waves(int KS, bool shared) {   // per SIMD, at least
+  return KS == 8 ? 4 : KS == 6 ? 3 : shared ? 2 : 4;
+}
+
+template <int KS, bool SHARED>
+__global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads_kernel(Args a) {
+  constexpr int NW = 2 * KS, PW = NW >= 16 ? 16 : NW >= 8 ? 8 : 4, CT = 16 / PW;
+  constexpr int LX = kC + 4, LM = kC + 8, LO = 32 * KS + 8;
   constexpr int kThreads = 64 * NW, kStage = 5 * 4 * 1024;   // dO, dR hi, lo, U hi, lo: 4 fragments each
-  constexpr int kMats = kC * LX * 4 + 3 * kC * LM * 2;
-  __shared__ __attribute__((aligned(16))) uint16_t Kl[kC * LD];
-  __shared__ __attribute__((aligned(16))) uint16_t Ql[kC * LD];
-  __shared__ __attribute__((aligned(16))) uint8_t buf[kMats > 2 * kStage ? kMats : 2 * kStage];
+  constexpr int kMats = 3 * kC * LM * 2;                      // D, D^T, M + M^T; before them X
+  constexpr int kRows = 3 * NW * kC * 4, kOut = kC * LO * 2;
+  constexpr int kPair = 8 * KS * 1024;                         // K and Q fragments
+  constexpr int kBig = 2 * kStage > kMats + kRows ? 2 * kStage : kMats + kRows;
+  constexpr int kBuf = kBig > kPair ? kBig : kPair;
+  __shared__ __attribute__((aligned(16))) uint8_t trans[NW][4 * 1024];   // a wave's K^T and Q^T fragments
+  __shared__ __attribute__((aligned(16))) uint8_t buf[kBuf > kOut ? kBuf : kOut];
   __shared__ __attribute__((aligned(16))) float Sc[kScal];
-  __shared__ float rows[3][NW][kC];   // per wave: q.(S0 dO), k.(S0 dR), k.(dS' U)
-  __shared__ float bsum[NW][16], zsum[NW][kC], rvs[kC], dots[NW];
+  __shared__ float bsum[PW][16], zsum[PW][kC], rvs[kC], dots[NW];
   float* Xl = reinterpret_cast<float*>(buf);
-  __bf16* Dl = reinterpret_cast<__bf16*>(buf + kC * LX * 4);   // D, D^T, M + M^T
+  __bf16* Dl = reinterpret_cast<__bf16*>(buf);
   __bf16* DTl = Dl + kC * LM;
   __bf16* Nl = DTl + kC * LM;
+  float* rows = reinterpret_cast<float*>(buf + kMats);   // [3][NW][kC]: q.(S0 dO), k.(S0 dR), k.(dS' U)
   const int c = blockIdx.x / a.Hk, hk = blockIdx.x % a.Hk;
   const Chunk ch = chunk_of(a, c);
   if (ch.seq < 0) return;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int r = lane & 15, q = lane >> 4;
+  const int r0 = lane & 15, q0 = lane >> 4;
   const int rw = wave & 3, cw = (wave >> 2) * CT;   // the wave's row tile, first column tile
   const int group = a.Hv / a.Hk;
+  const uint16_t* kp = a.k + ch.b * a.k_sb + ch.t0 * a.k_st + hk * a.k_sh;
+  const uint16_t* qp = a.q + ch.b * a.q_sb + ch.t0 * a.q_st + hk * a.q_sh;
   {
-    const Rsrc kp = buffer_at(a.k + ch.b * a.k_sb + ch.t0 * a.k_st + hk * a.k_sh);
-    const Rsrc qp = buffer_at(a.q + ch.b * a.q_sb + ch.t0 * a.q_st + hk * a.q_sh);
-    for (int p = tid; p < kC * 4 * KS; p += kThreads) {
-      const int t = p / (4 * KS), e = 8 * (p % (4 * KS));
-      const uint32_t miss = miss_from(t, ch.n) | miss_from(e, a.Dk);
-      *reinterpret_cast<bf16x8*>(Kl + t * LD + e) = load_frag(kp, 2 * (t * (uint32_t)a.k_st + e) | miss);
-      *reinterpret_cast<bf16x8*>(Ql + t * LD + e) = load_frag(qp, 2 * (t * (uint32_t)a.q_st + e) | miss);
+    const int64_t at = ((int64_t)c * a.Hk + hk) * (4 * KS * 1024) + wave * 2048 + lane * 16;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      *reinterpret_cast<bf16x8*>(trans[wave] + i * 1024 + lane * 16) =
+          *reinterpret_cast<const bf16x8*>(a.kt + at + i * 1024);
+      *reinterpret_cast<bf16x8*>(trans[wave] + (2 + i) * 1024 + lane * 16) =
+          *reinterpret_cast<const bf16x8*>(a.qt + at + i * 1024);
     }
   }
-  __syncthreads();
-  f32x4 kk[CT] = {}, qk[CT] = {};
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) {
-    const int e = 32 * ks + 8 * q;
-    const bf16x8 ka = *reinterpret_cast<const bf16x8*>(Kl + (16 * rw + r) * LD + e);
-    const bf16x8 qa = *reinterpret_cast<const bf16x8*>(Ql + (16 * rw + r) * LD + e);
-#pragma unroll
-    for (int x = 0; x < CT; ++x) {
-      const bf16x8 kb = *reinterpret_cast<const bf16x8*>(Kl + (16 * (cw + x) + r) * LD + e);
-      kk[x] = mfma(ka, kb, kk[x]);
-      qk[x] = mfma(qa, kb, qk[x]);
-    }
-  }
-  f32x4 dQ[4][FT] = {}, dK[4][FT] = {};
+  f32x4 dQ[4] = {}, dK[4] = {};
   const int64_t orow = (int64_t)a.Hv * a.Dv, tok = (int64_t)ch.b * a.T + ch.t0;
   const int64_t plane = (int64_t)a.B * a.T * orow;
-  for (int hv = hk * group; hv < (hk + 1) * group; ++hv) {
+  const int hv_end = SHARED ? (hk + 1) * group : hk + 1;
+  for (int hv = SHARED ? hk * group : hk; hv < hv_end; ++hv) {
+    // Behind this the compiler takes r and q for new values in every turn: the
+    // some 60 offsets and masks made of them, kept over the loop, would be
+    // spilled for the products' registers.
+    int r = r0, q = q0;
+    asm volatile("" : "+v"(r), "+v"(q));
+    const int feat = 16 * wave + r;
     for (int i = tid; i < kScal; i += kThreads) Sc[i] = a.scal[((size_t)c * a.Hv + hv) * kScal + i];
     const int64_t oat = tok * orow + (int64_t)hv * a.Dv;
-    const Rsrc src[5] = {buffer_at(a.dout + ch.b * a.do_sb + ch.t0 * a.do_st + hv * a.do_sh),
-                         buffer_at(a.dr + oat), buffer_at(a.dr + plane + oat),
-                         buffer_at(a.u + oat), buffer_at(a.u + plane + oat)};
+    const uint16_t* gp = a.dout + ch.b * a.do_sb + ch.t0 * a.do_st + hv * a.do_sh;
     const Rsrc vp = buffer_at(a.v + ch.b * a.v_sb + ch.t0 * a.v_st + hv * a.v_sh);
     const int64_t sat = ((int64_t)c * a.Hv + hv) * 2 * a.Dk * a.Dv;
     const Rsrc sp = buffer_at(a.s0 + sat), dp = buffer_at(a.ds + sat);
     const uint32_t lo_at = 2 * (uint32_t)(a.Dk * a.Dv);
-    // wave w stages fragments w, w + NW, ... of the 20 of a step
-    constexpr int kMine = (20 + NW - 1) / NW;
-    bf16x8 st[kMine], sh[FT], sl[FT], dh[FT], dl[FT], vf;
-    const auto load_step = [&](int e0) {
-      const int e = e0 + 8 * q;
+    const uint32_t srow = 2 * (feat * a.Dv + 8 * q) | miss_from(feat, a.Dk);
+    bf16x8 st[(20 + NW - 1) / NW], sh, sl;
+    // Rows of 16 tokens by 32 columns to LDS: wave w has fragments w, w + NW, ..
+    // of `count`, four of each tensor, the first of them tensor `from` of dO, dR
+    // hi, lo, U hi, lo.
+    const auto load_rows = [&](int e0, int from, int count) {
+      const uint32_t miss = miss_from(e0 + 8 * q, a.Dv);
 #pragma unroll
-      for (int i = 0; i < kMine; ++i) {
+      for (int i = 0; i < (20 + NW - 1) / NW; ++i) {
         const int f = i * NW + wave;
-        if (f < 20) {
-          const int t = 16 * (f & 3) + r;
-          const uint32_t ld = f < 4 ? (uint32_t)a.do_st : (uint32_t)orow;
-          const Rsrc p = f < 4 ? src[0] : f < 8 ? src[1] : f < 12 ? src[2] : f < 16 ? src[3] : src[4];
-          st[i] = load_frag(p, 2 * (t * ld + e) | miss_from(t, ch.n) | miss_from(e, a.Dv));
+        if (f < count) {
+          const int t = 16 * (f & 3) + r, which = from + (f >> 2);
+          const uint32_t ld = which == 0 ? (uint32_t)a.do_st : (uint32_t)orow;
+          const uint16_t* p = which == 0 ? gp : (which < 3 ? a.dr : a.u) + oat + (which & 1 ? 0 : plane);
+          st[i] = load_frag(buffer_at(p), 2 * (t * ld + e0 + 8 * q) | miss_from(t, ch.n) | miss);
         }
-      }
-#pragma unroll
-      for (int x = 0; x < FT; ++x) {
-        const int feat = 16 * (wave * FT + x) + r;
-        const uint32_t at = 2 * (feat * a.Dv + e) | miss_from(feat, a.Dk) | miss_from(e, a.Dv);
-        sh[x] = load_frag(sp, at);
-        sl[x] = load_frag(sp, at, lo_at);
-        dh[x] = load_frag(dp, at);
-        dl[x] = load_frag(dp, at, lo_at);
-      }
-      if (wave < 4) {
-        const int t = 16 * rw + r;
-        vf = load_frag(vp, 2 * (t * (uint32_t)a.v_st + e) | miss_from(t, ch.n) | miss_from(e, a.Dv));
       }
     };
-    f32x4 EQ[4][FT] = {}, ER[4][FT] = {}, EU[4][FT] = {}, dP[CT] = {}, dA[CT] = {};
-    float dot = 0.0f, rv = 0.0f;
-    load_step(0);
-    int half = 0;
-    for (int e0 = 0; e0 < a.Dv; e0 += 32, half ^= 1) {
-      uint8_t* stage = buf + half * kStage;
+    const auto put_rows = [&](uint8_t* stage, int count) {
 #pragma unroll
-      for (int i = 0; i < kMine; ++i)
-        if (i * NW + wave < 20)
+      for (int i = 0; i < (20 + NW - 1) / NW; ++i)
+        if (i * NW + wave < count)
           *reinterpret_cast<bf16x8*>(stage + (i * NW + wave) * 1024 + lane * 16) = st[i];
-      bf16x8 s0h[FT], s0l[FT], dsh[FT], dsl[FT];
+    };
+    const auto load_state = [&](Rsrc p, int e0, bf16x8& hi, bf16x8& lo) {
+      const uint32_t at = (srow + 2 * e0) | miss_from(e0 + 8 * q, a.Dv);
+      hi = load_frag(p, at);
+      lo = load_frag(p, at, lo_at);
+    };
+    // a wave's own 16 x 16 products, of which the diagonal is wanted
+    const auto diagonal = [&](f32x4 x) {
+      float d = 0.0f;
 #pragma unroll
-      for (int x = 0; x < FT; ++x) {
-        s0h[x] = sh[x];
-        s0l[x] = sl[x];
-        dsh[x] = dh[x];
-        dsl[x] = dl[x];
-      }
-      const bf16x8 vv = vf;
-      load_step(e0 + 32);   // past Dv: nothing is read
-      lds_barrier();        // the step's rows are in LDS; the other half is free after the next one
-      const auto row = [&](int which, int rt) {
-        return *reinterpret_cast<const bf16x8*>(stage + (4 * which + rt) * 1024 + lane * 16);
+      for (int i = 0; i < 4; ++i) d += 4 * q + i == r ? x[i] : 0.0f;
+      return d;
+    };
+    f32x4 EQ[4] = {}, ER[4] = {}, dP[CT] = {}, dA[CT] = {}, rv = {};
+    {
+      bf16x8 vf;
+      const auto load_v = [&](int e0) {
+        const int t = 16 * rw + r;
+        vf = load_frag(vp, 2 * (t * (uint32_t)a.v_st + e0 + 8 * q) | miss_from(t, ch.n) | miss_from(e0 + 8 * q, a.Dv));
       };
+      load_rows(0, 0, 20);
+      load_state(sp, 0, sh, sl);
+      if (wave < 4) load_v(0);
+      int half = 0;
+      for (int e0 = 0; e0 < a.Dv; e0 += 32, half ^= 1) {
+        uint8_t* stage = buf + half * kStage;
+        put_rows(stage, 20);
+        load_rows(e0 + 32, 0, 20);   // past Dv: nothing is read
+        lds_barrier();               // the step's rows are in LDS; the other half is free after the next one
+        const auto row = [&](int which, int rt) {
+          return *reinterpret_cast<const bf16x8*>(stage + (4 * which + rt) * 1024 + lane * 16);
+        };
 #pragma unroll
-      for (int x = 0; x < FT; ++x)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          dot = __builtin_fmaf((float)s0h[x][i] + (float)s0l[x][i], (float)dsh[x][i] + (float)dsl[x][i], dot);
-#pragma unroll
-      for (int rt = 0; rt < 4; ++rt) {
-        const bf16x8 g = row(0, rt), rh = row(1, rt), rl = row(2, rt), uh = row(3, rt), ul = row(4, rt);
-#pragma unroll
-        for (int x = 0; x < FT; ++x) {
-          EQ[rt][x] = mfma(g, s0h[x], EQ[rt][x]);
-          ER[rt][x] = mfma(rh, s0h[x], ER[rt][x]);
-          EU[rt][x] = mfma(uh, dsh[x], EU[rt][x]);
-          EQ[rt][x] = mfma(g, s0l[x], EQ[rt][x]);
-          ER[rt][x] = mfma(rh, s0l[x], ER[rt][x]);
-          EU[rt][x] = mfma(uh, dsl[x], EU[rt][x]);
-          ER[rt][x] = mfma(rl, s0h[x], ER[rt][x]);
-          EU[rt][x] = mfma(ul, dsh[x], EU[rt][x]);
+        for (int rt = 0; rt < 4; ++rt) {
+          const bf16x8 g = row(0, rt), rh = row(1, rt), rl = row(2, rt);
+          EQ[rt] = mfma(g, sh, EQ[rt]);
+          ER[rt] = mfma(rh, sh, ER[rt]);
+          EQ[rt] = mfma(g, sl, EQ[rt]);
+          ER[rt] = mfma(rh, sl, ER[rt]);
+          ER[rt] = mfma(rl, sh, ER[rt]);
         }
-      }
-      const bf16x8 gw = row(0, rw), rh = row(1, rw), rl = row(2, rw);
-      if (wave < 4)
+        load_state(sp, e0 + 32, sh, sl);
+        if (wave < PW) {
+          const bf16x8 gw = row(0, rw), rh = row(1, rw), rl = row(2, rw);
+          if (wave < 4) {   // dR.v
+            rv = mfma(rh, vf, rv);
+            rv = mfma(rl, vf, rv);
+            load_v(e0 + 32);
+          }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) rv = __builtin_fmaf((float)rh[i] + (float)rl[i], (float)vv[i], rv);
-#pragma unroll
-      for (int x = 0; x < CT; ++x) {
-        const bf16x8 uh = row(3, cw + x), ul = row(4, cw + x);
-        dP[x] = mfma(gw, uh, dP[x]);
-        dA[x] = mfma(rh, uh, dA[x]);
-        dP[x] = mfma(gw, ul, dP[x]);
-        dA[x] = mfma(rh, ul, dA[x]);
-        dA[x] = mfma(rl, uh, dA[x]);
+          for (int x = 0; x < CT; ++x) {
+            const bf16x8 uh = row(3, cw + x), ul = row(4, cw + x);
+            dP[x] = mfma(gw, uh, dP[x]);
+            dA[x] = mfma(rh, uh, dA[x]);
+            dP[x] = mfma(gw, ul, dP[x]);
+            dA[x] = mfma(rh, ul, dA[x]);
+            dA[x] = mfma(rl, uh, dA[x]);
+          }
+        }
       }
     }
     lds_barrier();   // every wave is done with the staged rows
-    rv += __shfl_xor(rv, 16);
-    rv += __shfl_xor(rv, 32);
-    if (wave < 4 && q == 0) rvs[16 * rw + r] = rv;   // dR.v
+    asm volatile("" : "+v"(r), "+v"(q));
+    // kk = K K^T and qk = Q K^T, the chunk's rows through LDS
+    f32x4 kk[CT] = {}, qk[CT] = {};
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) dot += __shfl_xor(dot, d);
-    if (lane == 0) dots[wave] = dot;
-    // the 64 x 64 matrices
-    f32x4 bs = {};
+    for (int i = 0; i < 4; ++i) {
+      const int f = i * NW + wave, ks = f >> 3, t = 16 * (f & 3) + r, e = 32 * ks + 8 * q;
+      const uint32_t st = (uint32_t)(f & 4 ? a.q_st : a.k_st);
+      *reinterpret_cast<bf16x8*>(buf + f * 1024 + lane * 16) =
+          load_frag(buffer_at(f & 4 ? qp : kp), 2 * (t * st + e) | miss_from(t, ch.n) | miss_from(e, a.Dk));
+    }
+    lds_barrier();
+    if (wave < PW) {
 #pragma unroll
-    for (int x = 0; x < CT; ++x) {
-      const int j = 16 * (cw + x) + r;
+      for (int ks = 0; ks < KS; ++ks) {
+        const auto row = [&](int f) { return *reinterpret_cast<const bf16x8*>(buf + (8 * ks + f) * 1024 + lane * 16); };
+        const bf16x8 ka = row(rw), qa = row(4 + rw);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * rw + 4 * q + i;
-        const float E = row >= j ? __expf((Sc[3 * kC + row] - Sc[3 * kC + j]) +
-                                          (Sc[4 * kC + row] - Sc[4 * kC + j])) : 0.0f;
-        const float D = a.scale * E * dP[x][i];
-        const float m = row > j ? -E * dA[x][i] : 0.0f;
-        const float M = Sc[2 * kC + row] * m;
-        bs[i] = __builtin_fmaf(m, kk[x][i], bs[i]);
-        Xl[row * LX + j] = D * qk[x][i] + M * kk[x][i];
-        Dl[row * LM + j] = (__bf16)D;
-        DTl[j * LM + row] = (__bf16)D;
-        if (row > j) {
-          Nl[row * LM + j] = (__bf16)M;
-          Nl[j * LM + row] = (__bf16)M;
-        } else if (row == j) {
-          Nl[row * LM + j] = (__bf16)0.0f;
+        for (int x = 0; x < CT; ++x) {
+          const bf16x8 kb = row(cw + x);
+          kk[x] = mfma(ka, kb, kk[x]);
+          qk[x] = mfma(qa, kb, qk[x]);
         }
       }
     }
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) bs[i] += __shfl_xor(bs[i], d);
-    if (r == 0)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) bsum[wave][4 * q + i] = bs[i];
-    // the [64, Dk] products, and their rows' products with q and k
-#pragma unroll
-    for (int rt = 0; rt < 4; ++rt) {
-      const int t0 = 16 * rt + 4 * q;
-      const f32x4 gam = *reinterpret_cast<const f32x4*>(Sc + t0);
-      const f32x4 ge = *reinterpret_cast<const f32x4*>(Sc + kC + t0);
-      const f32x4 bt = *reinterpret_cast<const f32x4*>(Sc + 2 * kC + t0);
-      f32x4 s1 = {}, s2 = {}, s3 = {};
-#pragma unroll
-      for (int x = 0; x < FT; ++x) {
-        const int f = wave * FT + x, feat = 16 * f + r;
-        if (f < 2 * KS)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float kv = bf16_to_f32(Kl[(t0 + i) * LD + feat]);
-            const float qv = bf16_to_f32(Ql[(t0 + i) * LD + feat]);
-            s1[i] = __builtin_fmaf(EQ[rt][x][i], qv, s1[i]);
-            s2[i] = __builtin_fmaf(ER[rt][x][i], kv, s2[i]);
-            s3[i] = __builtin_fmaf(EU[rt][x][i], kv, s3[i]);
-          }
-        dQ[rt][x] += a.scale * gam * EQ[rt][x];
-        dK[rt][x] += ge * EU[rt][x] - bt * gam * ER[rt][x];
+    lds_barrier();
+    asm volatile("" : "+v"(r), "+v"(q));
+    // X; dP and dA become D and M
+    if (wave < PW) {
+      if (wave < 4) {
+        const float d = diagonal(rv);   // of column r, in one of the four lanes that have it
+        if (r >> 2 == q) rvs[16 * rw + r] = d;
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) {
-          s1[i] += __shfl_xor(s1[i], d);
-          s2[i] += __shfl_xor(s2[i], d);
-          s3[i] += __shfl_xor(s3[i], d);
-        }
-        if (r == 0) {
-          rows[0][wave][t0 + i] = s1[i];
-          rows[1][wave][t0 + i] = s2[i];
-          rows[2][wave][t0 + i] = s3[i];
-        }
-      }
-    }
-    __syncthreads();
-    // sum_{j < t} X_ij as a product with the strictly upper ones, X in two bf16 parts
-    f32x4 Z[CT] = {};
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const float* xp = Xl + (16 * rw + r) * LX + 32 * ks + 8 * q;
-      bf16x8 hi, lo;
-      split8(*reinterpret_cast<const f32x4*>(xp), *reinterpret_cast<const f32x4*>(xp + 4), hi, lo);
+      f32x4 bs = {};
 #pragma unroll
       for (int x = 0; x < CT; ++x) {
-        bf16x8 ones;
+        const int j = 16 * (cw + x) + r;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          ones[i] = (__bf16)(32 * ks + 8 * q + i < 16 * (cw + x) + r ? 1.0f : 0.0f);
-        Z[x] = mfma(hi, ones, Z[x]);
-        Z[x] = mfma(lo, ones, Z[x]);
+        for (int i = 0; i < 4; ++i) {
+          const int row = 16 * rw + 4 * q + i;
+          const float E = row >= j ? __expf((Sc[3 * kC + row] - Sc[3 * kC + j]) +
+                                            (Sc[4 * kC + row] - Sc[4 * kC + j])) : 0.0f;
+          const float D = a.scale * E * dP[x][i];
+          const float m = row > j ? -E * dA[x][i] : 0.0f;
+          const float M = Sc[2 * kC + row] * m;
+          bs[i] = __builtin_fmaf(m, kk[x][i], bs[i]);
+          Xl[row * LX + j] = D * qk[x][i] + M * kk[x][i];
+          dP[x][i] = D;
+          dA[x][i] = M;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bs[i] = sum16(bs[i]);
+      if (r == 0)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bsum[wave][4 * q + i] = bs[i];
+    }
+    // Rows' products with q (which = 1) or k (0), a wave's features' share of them
+    const auto row_products = [&](int which, int slot, int rt, f32x4 x) {
+      const uint8_t* tp = trans[wave] + 2048 * which + (rt >> 1) * 1024 +
+                          ((2 * (rt & 1) + (q >> 1)) * 16 + r) * 16 + (q & 1) * 8;
+      const u32x2 w = *reinterpret_cast<const u32x2*>(tp);
+      f32x4 s;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        s[i] = sum16(x[i] * __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16));
+      if (r == 0) *reinterpret_cast<f32x4*>(rows + (slot * NW + wave) * kC + 16 * rt + 4 * q) = s;
+    };
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt) {
+      row_products(1, 0, rt, EQ[rt]);
+      row_products(0, 1, rt, ER[rt]);
+      const f32x4 gam = *reinterpret_cast<const f32x4*>(Sc + 16 * rt + 4 * q);
+      const f32x4 bt = *reinterpret_cast<const f32x4*>(Sc + 2 * kC + 16 * rt + 4 * q);
+      const f32x4 nq = a.scale * gam * EQ[rt], nk = -bt * gam * ER[rt];
+      dQ[rt] = SHARED ? dQ[rt] + nq : nq;
+      dK[rt] = SHARED ? dK[rt] + nk : nk;
+    }
+    lds_barrier();
+    asm volatile("" : "+v"(r), "+v"(q));
+    // sum_{j < t} X_ij as a product with the strictly upper ones, X in two bf16 parts
+    if (wave < PW) {
+      f32x4 Z[CT] = {};
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const float* xp = Xl + (16 * rw + r) * LX + 32 * ks + 8 * q;
+        bf16x8 hi, lo;
+        split8(*reinterpret_cast<const f32x4*>(xp), *reinterpret_cast<const f32x4*>(xp + 4), hi, lo);
+#pragma unroll
+        for (int x = 0; x < CT; ++x) {
+          const int below = 16 * (cw + x) + r - (32 * ks + 8 * q);   // ones in places under it
+          u32x4 ones;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            ones[i] = 2 * i + 1 < below ? 0x3f803f80u : 2 * i < below ? 0x3f80u : 0u;
+          Z[x] = mfma(hi, __builtin_bit_cast(bf16x8, ones), Z[x]);
+          Z[x] = mfma(lo, __builtin_bit_cast(bf16x8, ones), Z[x]);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < CT; ++x) {
+        const int t = 16 * (cw + x) + r;
+        float z = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z += 16 * rw + 4 * q + i >= t ? Z[x][i] : 0.0f;
+        z += __shfl_xor(z, 16);
+        z += __shfl_xor(z, 32);
+        if (q == 0) zsum[wave][t] = z;
       }
     }
+    lds_barrier();   // X is read: D, D^T and M + M^T take its place
+    if (wave < PW) {
 #pragma unroll
-    for (int x = 0; x < CT; ++x) {
-      const int t = 16 * (cw + x) + r;
-      float z = 0.0f;
+      for (int x = 0; x < CT; ++x) {
+        const int j = 16 * (cw + x) + r, row0 = 16 * rw + 4 * q;
+        const u32x2 d = round_of(dP[x]), m = round_of(dA[x]);
+        *reinterpret_cast<u32x2*>(DTl + j * LM + row0) = d;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) z += 16 * rw + 4 * q + i >= t ? Z[x][i] : 0.0f;
-      z += __shfl_xor(z, 16);
-      z += __shfl_xor(z, 32);
-      if (q == 0) zsum[wave][t] = z;
-    }
-    // dQ += D K, dK += D^T Q + (M + M^T) K
-#pragma unroll
-    for (int x = 0; x < FT; ++x) {
-      const int f = wave * FT + x;
-      if (f < 2 * KS) {
-        const size_t at = ((size_t)c * a.Hk + hk) * (4 * KS) * 1024 + (size_t)f * 2048 + lane * 16;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          const bf16x8 kb = *reinterpret_cast<const bf16x8*>(a.kt + at + ks * 1024);
-          const bf16x8 qb = *reinterpret_cast<const bf16x8*>(a.qt + at + ks * 1024);
-#pragma unroll
-          for (int rt = 0; rt < 4; ++rt) {
-            const int o = (16 * rt + r) * LM + 32 * ks + 8 * q;
-            if (ks == 0 || rt >= 2)
-              dQ[rt][x] = mfma(*reinterpret_cast<const bf16x8*>(Dl + o), kb, dQ[rt][x]);
-            if (ks == 1 || rt < 2)
-              dK[rt][x] = mfma(*reinterpret_cast<const bf16x8*>(DTl + o), qb, dK[rt][x]);
-            dK[rt][x] = mfma(*reinterpret_cast<const bf16x8*>(Nl + o), kb, dK[rt][x]);
+        for (int i = 0; i < 4; ++i) {
+          const int row = row0 + i;
+          const uint16_t mw = (uint16_t)(i & 1 ? m[i >> 1] >> 16 : m[i >> 1]);
+          reinterpret_cast<uint16_t*>(Dl)[row * LM + j] = (uint16_t)(i & 1 ? d[i >> 1] >> 16 : d[i >> 1]);
+          if (row >= j) {   // M is zero on the diagonal
+            reinterpret_cast<uint16_t*>(Nl)[row * LM + j] = mw;
+            reinterpret_cast<uint16_t*>(Nl)[j * LM + row] = mw;
           }
         }
       }
     }
-    __syncthreads();
-    if (wave == 0) {   // lane = token
+    lds_barrier();
+    load_rows(0, 3, 8);
+    // dQ += D K, dK += D^T Q + (M + M^T) K
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const bf16x8 kb = *reinterpret_cast<const bf16x8*>(trans[wave] + ks * 1024 + lane * 16);
+      const bf16x8 qb = *reinterpret_cast<const bf16x8*>(trans[wave] + (2 + ks) * 1024 + lane * 16);
+#pragma unroll
+      for (int rt = 0; rt < 4; ++rt) {
+        const int o = (16 * rt + r) * LM + 32 * ks + 8 * q;
+        if (ks == 0 || rt >= 2) dQ[rt] = mfma(*reinterpret_cast<const bf16x8*>(Dl + o), kb, dQ[rt]);
+        if (ks == 1 || rt < 2) dK[rt] = mfma(*reinterpret_cast<const bf16x8*>(DTl + o), qb, dK[rt]);
+        dK[rt] = mfma(*reinterpret_cast<const bf16x8*>(Nl + o), kb, dK[rt]);
+      }
+    }
+    lds_barrier();   // every wave is done with the 64 x 64 matrices
+    // the second pass: U dS'^T and <S0, dS'>
+    f32x4 EU[4] = {}, dot = {};
+    {
+      bf16x8 dh, dl;
+      load_state(sp, 0, sh, sl);
+      load_state(dp, 0, dh, dl);
+      int half = 0;
+      for (int e0 = 0; e0 < a.Dv; e0 += 32, half ^= 1) {
+        uint8_t* stage = buf + half * 8 * 1024;
+        put_rows(stage, 8);
+        load_rows(e0 + 32, 3, 8);
+        lds_barrier();
+#pragma unroll
+        for (int rt = 0; rt < 4; ++rt) {
+          const bf16x8 uh = *reinterpret_cast<const bf16x8*>(stage + rt * 1024 + lane * 16);
+          const bf16x8 ul = *reinterpret_cast<const bf16x8*>(stage + (4 + rt) * 1024 + lane * 16);
+          EU[rt] = mfma(uh, dh, EU[rt]);
+          EU[rt] = mfma(uh, dl, EU[rt]);
+          EU[rt] = mfma(ul, dh, EU[rt]);
+        }
+        dot = mfma(sh, dh, dot);
+        dot = mfma(sh, dl, dot);
+        dot = mfma(sl, dh, dot);
+        load_state(sp, e0 + 32, sh, sl);
+        load_state(dp, e0 + 32, dh, dl);
+      }
+    }
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt) {
+      row_products(0, 2, rt, EU[rt]);
+      dK[rt] += *reinterpret_cast<const f32x4*>(Sc + kC + 16 * rt + 4 * q) * EU[rt];
+    }
+    {
+      float d = sum16(diagonal(dot));
+      d += __shfl_xor(d, 16);
+      d += __shfl_xor(d, 32);
+      if (lane == 0) dots[wave] = d;
+    }
+    lds_barrier();
+    if (wave == NW - 1) {   // lane = token
       float s[3] = {};
 #pragma unroll
       for (int i = 0; i < 3; ++i)
 #pragma unroll
-        for (int w = 0; w < NW; ++w) s[i] += rows[i][w][lane];
+        for (int w = 0; w < NW; ++w) s[i] += rows[(i * NW + w) * kC + lane];
       const float gam = Sc[lane], ge = Sc[kC + lane], bt = Sc[2 * kC + lane];
       const float after = a.scale * gam * s[0] - bt * gam * s[1];   // of tokens t and later
       const float before = ge * s[2];                                // of tokens before t
@@ -598,30 +659,35 @@ __global__ __launch_bounds__(64 * NW) void delta_grads_kernel(Args a) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) z += zsum[w + 4 * ((lane >> 4) / CT)][lane];
 #pragma unroll
-      for (int w = 0; w < NW / 4; ++w) b += bsum[(lane >> 4) + 4 * w][lane & 15];
+      for (int w = 0; w < PW / 4; ++w) b += bsum[(lane >> 4) + 4 * w][lane & 15];
       if (lane < ch.n) {
         const int64_t at = (tok + lane) * a.Hv + hv;
         store_any(a.dg, a.g_dtype, at, z + suf + pre + Sc[kC - 1] * all);
         store_any(a.dbeta, a.beta_dtype, at, rvs[lane] - gam * s[1] + b);
       }
     }
-    __syncthreads();
+    lds_barrier();   // LDS is free for the next head, or for the results
   }
+  // through LDS to whole rows
+  __bf16* Ol = reinterpret_cast<__bf16*>(buf);
 #pragma unroll
-  for (int rt = 0; rt < 4; ++rt)
+  for (int which = 0; which < 2; ++which) {
+    if (which) lds_barrier();
 #pragma unroll
-    for (int x = 0; x < FT; ++x) {
-      const int feat = 16 * (wave * FT + x) + r;
+    for (int rt = 0; rt < 4; ++rt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = 16 * rt + 4 * q + i;
-        if (t < ch.n && feat < a.Dk) {
-          const int64_t at = ((tok + t) * a.Hk + hk) * a.Dk + feat;
-          a.dq[at] = f32_to_bf16(dQ[rt][x][i]);
-          a.dk[at] = f32_to_bf16(dK[rt][x][i]);
-        }
-      }
+      for (int i = 0; i < 4; ++i)
+        Ol[(16 * rt + 4 * q0 + i) * LO + 16 * wave + r0] = (__bf16)(which ? dK[rt][i] : dQ[rt][i]);
+    lds_barrier();
+    uint16_t* out = (which ? a.dk : a.dq) + (tok * a.Hk + hk) * a.Dk;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int p = i * kThreads + tid, t = p / (4 * KS), e = 8 * (p % (4 * KS));
+      if (t < ch.n && e < a.Dk)
+        *reinterpret_cast<u32x4*>(out + (int64_t)t * a.Hk * a.Dk + e) =
+            *reinterpret_cast<const u32x4*>(Ol + t * LO + e);
     }
+  }
 }
 
 template <int KS>
@@ -638,9 +704,9 @@ int launch_bwd(const Args& a, hipStream_t st) {
   }
   if (const int rc = check_launch("delta_scan_bwd")) return rc;
   if (a.nchunks == 0) return UTTT_OK;
-  constexpr int NW = KS == 2 ? 4 : 8;
-  hipLaunchKernelGGL((delta_grads_kernel<KS, NW>), dim3((unsigned)((int64_t)a.nchunks * a.Hk)), dim3(64 * NW),
-                     0, st, a);
+  const dim3 grid((unsigned)((int64_t)a.nchunks * a.Hk));
+  if (a.Hv > a.Hk) hipLaunchKernelGGL((delta_grads_kernel<KS, true>), grid, dim3(128 * KS), 0, st, a);
+  else hipLaunchKernelGGL((delta_grads_kernel<KS, false>), grid, dim3(128 * KS), 0, st, a);
   return check_launch("delta_grads");
 }
 
