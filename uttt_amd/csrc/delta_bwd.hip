@@ -19,25 +19,30 @@ namespace uttt {
 namespace delta {
 namespace {
 
-// The forward scan's division of work (delta_fwd.hip), from the last chunk to
-// the first; a wave has 16 tokens of dU and dR and a quarter of dS's features.
 template <int KS, int NT>
-__global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
+struct ScanBwdLds {
+  uint8_t S[2][KS * NT * 1024];   // dS'
+  uint8_t G[2 * NT * 1024];       // dO
+  uint8_t U[2][2 * NT * 1024];    // dU
+  uint8_t H[2][2 * NT * 1024];    // s gam dO
+  uint8_t E[2][2 * NT * 1024];    // -b gam dR
+  f32x4 Z[4][NT][64];             // P^T dO and dR in fp32, as their waves' lanes hold them
+  f32x4 R[4][NT][64];
+};
+
+template <int NT>
+__device__ __forceinline__ uint32_t put_at(int wave, int r, int q) {
+  return (wave >> 1) * NT * 1024 + (wave & 1) * 512 + (r + 16 * (q >> 1)) * 16 + (q & 1) * 8;
+}
+
+// The state's waves: 16 tokens of dU and dR and a quarter of dS's features each.
+template <int KS, int NT>
+__device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int wave, int lane,
+                                               ScanBwdLds<KS, NT>& lds) {
   constexpr int FT = (2 * KS + 3) / 4;
-  __shared__ __attribute__((aligned(16))) uint8_t Sb[2][KS * NT * 1024];
-  __shared__ __attribute__((aligned(16))) uint8_t Gb[2 * NT * 1024];      // dO
-  __shared__ __attribute__((aligned(16))) uint8_t Ub[2][2 * NT * 1024];   // dU
-  __shared__ __attribute__((aligned(16))) uint8_t Hb[2][2 * NT * 1024];   // s gam dO
-  __shared__ __attribute__((aligned(16))) uint8_t Eb[2][2 * NT * 1024];   // -b gam dR
-  Scan s;
-  if (!s.init(a, 16 * NT)) return;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int r = lane & 15, q = lane >> 4;
-  const int col = s.col0 + NT * r;
-  const bool live = col < a.Dv;
-  const uint32_t dead = miss_from(col, a.Dv);
+  const int r = lane & 15, q = lane >> 4, col = s.col0 + NT * r;
+  const uint32_t dead = miss_from(col, a.Dv), put_tok = put_at<NT>(wave, r, q);
   const uint32_t put = (r + 16 * (q >> 1)) * 16 + (q & 1) * 8;
-  const uint32_t put_tok = (wave >> 1) * NT * 1024 + (wave & 1) * 512 + put;
   const auto put_tile = [&](uint8_t (*buf)[2 * NT * 1024], int n, const Parts& p) {
     *reinterpret_cast<u32x2*>(buf[0] + put_tok + n * 1024) = p.hi;
     *reinterpret_cast<u32x2*>(buf[1] + put_tok + n * 1024) = p.lo;
@@ -54,26 +59,21 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
       const int feat = 16 * (wave * FT + f) + 4 * q + i;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
-        S[f][n][i] = a.dhT && live && feat < a.Dk
+        S[f][n][i] = a.dhT && col < a.Dv && feat < a.Dk
                          ? a.dhT[((int64_t)s.head * a.Dk + feat) * a.Dv + col + n] : 0.0f;
     }
 
-  bf16x8 kf[KS], tf[2][2], pf[2][2], ktf[FT][2], qtf[FT][2];
-  f32x4 gam, ge, bt;
+  bf16x8 kf[KS], tf[2][2], ktf[FT][2], qtf[FT][2];
+  f32x4 ge, bg;
   float gc;
-  Cols<NT> gr[4];
   // Operands of the chunk before: pointers that go along, at first those of the last chunk.
   const int lastc = s.nc - 1;
-  const int64_t crow = (int64_t)s.b * a.T + s.tok0 + (int64_t)lastc * kC;
   const uint16_t* kp = a.k + s.b * a.k_sb + s.hk * a.k_sh + (s.tok0 + (int64_t)lastc * kC) * a.k_st;
-  const uint16_t* gp = a.dout + s.b * a.do_sb + s.hv * a.do_sh + (s.tok0 + (int64_t)lastc * kC) * a.do_st;
   const uint8_t* trip = a.tri + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kTriBytes;
   const int64_t trans_at = ((int64_t)(s.c0 + lastc) * a.Hk + s.hk) * (4 * KS * 1024);
   const uint8_t *ktp = a.kt + trans_at, *qtp = a.qt + trans_at;
   const float* scp = a.scal + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kScal;
   const uint32_t krow = 2 * ((16 * wave + r) * (uint32_t)a.k_st + 8 * q);
-  const uint32_t grow = 2 * ((16 * wave + 4 * q) * (uint32_t)a.do_st + col);
-  const uint32_t orow = 2 * ((16 * wave + 4 * q) * (uint32_t)(a.Hv * a.Dv) + col);
   const uint32_t last_half = miss_from(32 * (KS - 1) + 8 * q, a.Dk), before_half = miss_from(32 * (KS - 2) + 8 * q, a.Dk);
   // `left`: tokens from the chunk on to the sequence's end; 0 before its first chunk
   const auto load_k = [&](int left) {
@@ -85,32 +85,20 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
     ge = load_f4(buffer_at(scp), 4 * (16 * wave + 4 * q) | miss_from(0, left), 4 * kC);
     kp -= kC * a.k_st;
   };
-  const auto load_do = [&](int left) {
-    const Rsrc gr_ = buffer_at(gp);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      gr[i].load(gr_, (grow + 2 * i * (uint32_t)a.do_st) | dead | miss_from(16 * wave + 4 * q + i, left));
-    gp -= kC * a.do_st;
-  };
-  const auto load_tri = [&](int left, int which, bf16x8 (&x)[2][2]) {
-    const Rsrc tr = buffer_at(trip);
-    const uint32_t at = lane * 16 | miss_from(0, left);
+  const auto load_t = [&](int left) {
+    const Rsrc tr = buffer_at(trip), sr = buffer_at(scp);
+    const uint32_t at = lane * 16 | miss_from(0, left), s_at = 4 * (16 * wave + 4 * q) | miss_from(0, left);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       // step 0 of the lower tiles is zero and not stored: step 1 again, unused
-      const int f = 2 * which * kTFrags + upper_frag(wave, wave < 2 ? ks : 1);
-      x[ks][0] = load_frag(tr, at, f * 1024);
-      x[ks][1] = load_frag(tr, at, (kTFrags + f) * 1024);
+      const int f = upper_frag(wave, wave < 2 ? ks : 1);
+      tf[ks][0] = load_frag(tr, at, f * 1024);
+      tf[ks][1] = load_frag(tr, at, (kTFrags + f) * 1024);
     }
-    if (!which) {
-      const Rsrc sr = buffer_at(scp);
-      const uint32_t s_at = 4 * (16 * wave + 4 * q) | miss_from(0, left);
-      gam = load_f4(sr, s_at);
-      bt = load_f4(sr, s_at, 8 * kC);
-      gc = load_f1(sr, 4 * (kC - 1) | miss_from(0, left));
-      scp -= a.Hv * kScal;
-      trip -= (int64_t)a.Hv * kTriBytes;
-    }
+    bg = load_f4(sr, s_at) * load_f4(sr, s_at, 8 * kC);
+    gc = load_f1(sr, 4 * (kC - 1) | miss_from(0, left));
+    scp -= a.Hv * kScal;
+    trip -= (int64_t)a.Hv * kTriBytes;
   };
   const auto load_trans = [&](int left, const uint8_t*& p, bf16x8 (&x)[FT][2]) {
     const Rsrc tr = buffer_at(p);
@@ -122,7 +110,7 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
         if (wave * FT + f < 2 * KS) x[f][t] = load_frag(tr, at, (2 * (wave * FT + f) + t) * 1024);
     p -= (int64_t)a.Hk * (4 * KS * 1024);
   };
-  // dS' to LDS and memory, dO to LDS
+  // dS' to LDS and memory
   uint16_t* dsp = a.ds + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * 2 * a.Dk * a.Dv;
   const auto put_state = [&]() {
     const Rsrc sr = buffer_at(dsp);
@@ -135,8 +123,8 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
         for (int n = 0; n < NT; ++n) {
           const Parts p = parts_of(S[f][n]);
           const uint32_t at = ((tile >> 1) * NT + n) * 1024 + (tile & 1) * 512 + put;
-          *reinterpret_cast<u32x2*>(Sb[0] + at) = hi[n] = p.hi;
-          *reinterpret_cast<u32x2*>(Sb[1] + at) = lo[n] = p.lo;
+          *reinterpret_cast<u32x2*>(lds.S[0] + at) = hi[n] = p.hi;
+          *reinterpret_cast<u32x2*>(lds.S[1] + at) = lo[n] = p.lo;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -148,29 +136,21 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
       }
     }
     dsp -= (int64_t)a.Hv * 2 * a.Dk * a.Dv;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const u32x2 g = {gr[0].half(n) | (gr[1].half(n) << 16), gr[2].half(n) | (gr[3].half(n) << 16)};
-      *reinterpret_cast<u32x2*>(Gb + put_tok + n * 1024) = g;
-    }
   };
 
   const int first_left = s.len - lastc * kC;
   if (lastc >= 0) {
-    load_do(first_left);
     load_k(first_left);
-    load_tri(first_left, 1, pf);
-    load_tri(first_left, 0, tf);
+    load_t(first_left);
     load_trans(first_left, qtp, qtf);
     load_trans(first_left, ktp, ktf);
     put_state();
     settle();
+    lds_barrier();   // dO is in LDS, for the other waves
   }
-  const int64_t plane = (int64_t)a.B * a.T * a.Hv * a.Dv;
-  int64_t out_at = (crow * a.Hv + s.hv) * a.Dv;
   for (int c = lastc; c >= 0; --c) {
-    const int left = s.len - c * kC, next = c > 0 ? kC : 0;
-    lds_barrier();   // dS' and dO are in LDS
+    const int next = c > 0 ? kC : 0;
+    lds_barrier();   // dS', P^T dO and s gam dO are in LDS
     // dU = e^{G_C - G} K dS' + P^T dO
     {
       f32x4 X[NT] = {}, X2[NT] = {};
@@ -178,36 +158,14 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          X[n] = mfma(kf[ks], get(Sb[0], ks * NT + n), X[n]);
-          X2[n] = mfma(kf[ks], get(Sb[1], ks * NT + n), X2[n]);
+          X[n] = mfma(kf[ks], get(lds.S[0], ks * NT + n), X[n]);
+          X2[n] = mfma(kf[ks], get(lds.S[1], ks * NT + n), X2[n]);
         }
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        X[n] = ge * (X[n] + X2[n]);
-        X2[n] = f32x4{};
-      }
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-        if (ks >= wave >> 1)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const bf16x8 g = get(Gb, ks * NT + n);
-            X[n] = mfma(pf[ks][0], g, X[n]);
-            X2[n] = mfma(pf[ks][1], g, X2[n]);
-          }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        put_tile(Ub, n, parts_of(X[n] + X2[n]));
-        f32x4 g;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) g[i] = gr[i].get(n);
-        put_tile(Hb, n, parts_of(g * (gam * a.scale)));
-      }
+      for (int n = 0; n < NT; ++n) put_tile(lds.U, n, parts_of(ge * (X[n] + X2[n]) + lds.Z[wave][n][lane]));
     }
-    load_do(next);
     load_k(next);
-    load_tri(next, 1, pf);
-    lds_barrier();   // dU and s gam dO are in LDS
+    lds_barrier();   // dU is in LDS
     f32x4 R[NT] = {};   // dR = T^T dU
     {
       f32x4 R2[NT] = {};
@@ -216,7 +174,7 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
         if (ks >= wave >> 1)
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const bf16x8 hi = get(Ub[0], ks * NT + n), lo = get(Ub[1], ks * NT + n);
+            const bf16x8 hi = get(lds.U[0], ks * NT + n), lo = get(lds.U[1], ks * NT + n);
             R[n] = mfma(tf[ks][0], hi, R[n]);
             R2[n] = mfma(tf[ks][1], hi, R2[n]);
             R2[n] = mfma(tf[ks][0], lo, R2[n]);
@@ -225,17 +183,21 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
       for (int n = 0; n < NT; ++n) R[n] += R2[n];
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) put_tile(Eb, n, parts_of(-(bt * gam) * R[n]));
+    for (int n = 0; n < NT; ++n) {
+      put_tile(lds.E, n, parts_of(-bg * R[n]));
+      lds.R[wave][n][lane] = R[n];
+    }
     // dS0 = gam_C dS' + Q^T (s gam dO) - K^T (b gam dR): the first product here
 #pragma unroll
     for (int f = 0; f < FT; ++f)
 #pragma unroll
       for (int n = 0; n < NT; ++n) S[f][n] *= gc;
+    load_t(next);
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const bf16x8 hi = get(Hb[0], t * NT + n), lo = get(Hb[1], t * NT + n);
+        const bf16x8 hi = get(lds.H[0], t * NT + n), lo = get(lds.H[1], t * NT + n);
 #pragma unroll
         for (int f = 0; f < FT; ++f)
           if (wave * FT + f < 2 * KS) {
@@ -244,32 +206,12 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
           }
       }
     load_trans(next, qtp, qtf);
-    {
-      const Rsrc vr = buffer_at(a.dv + out_at), hr = buffer_at(a.dr + out_at), lr = buffer_at(a.dr + plane + out_at);
-      u32x2 v[NT], hi[NT], lo[NT];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const Parts p = parts_of(R[n]);
-        hi[n] = p.hi;
-        lo[n] = p.lo;
-        v[n] = round_of(bt * R[n]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t at = (orow + 2 * i * (uint32_t)(a.Hv * a.Dv)) | dead | miss_from(16 * wave + 4 * q + i, left);
-        store_row<NT>(vr, at, v, i);
-        store_row<NT>(hr, at, hi, i);
-        store_row<NT>(lr, at, lo, i);
-      }
-      out_at -= (int64_t)kC * a.Hv * a.Dv;
-    }
-    load_tri(next, 0, tf);
     lds_barrier();   // b gam dR is in LDS
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const bf16x8 hi = get(Eb[0], t * NT + n), lo = get(Eb[1], t * NT + n);
+        const bf16x8 hi = get(lds.E[0], t * NT + n), lo = get(lds.E[1], t * NT + n);
 #pragma unroll
         for (int f = 0; f < FT; ++f)
           if (wave * FT + f < 2 * KS) {
@@ -280,7 +222,7 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
     load_trans(next, ktp, ktf);
     if (c > 0) put_state();
   }
-  if (a.dh0 && live) {
+  if (a.dh0 && col < a.Dv) {
 #pragma unroll
     for (int f = 0; f < FT; ++f)
 #pragma unroll
@@ -291,6 +233,144 @@ __global__ __launch_bounds__(256) void delta_scan_bwd_kernel(Args a) {
           for (int n = 0; n < NT; ++n) a.dh0[((int64_t)s.head * a.Dk + feat) * a.Dv + col + n] = S[f][n][i];
       }
   }
+}
+
+// The other waves: 16 tokens each of P^T dO and s gam dO, a chunk before the
+// state's waves need them, and of dR and dV on their way to memory.
+template <int KS, int NT>
+__device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, int wave, int lane,
+                                                ScanBwdLds<KS, NT>& lds) {
+  const int r = lane & 15, q = lane >> 4, col = s.col0 + NT * r;
+  const uint32_t dead = miss_from(col, a.Dv), put_tok = put_at<NT>(wave, r, q);
+  bf16x8 pf[2][2];
+  f32x4 gam, bt;
+  Cols<NT> gr[4];
+  const int lastc = s.nc - 1;
+  const uint16_t* gp = a.dout + s.b * a.do_sb + s.hv * a.do_sh + (s.tok0 + (int64_t)lastc * kC) * a.do_st;
+  const uint8_t* trip = a.tri + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kTriBytes;
+  const float* gamp = a.scal + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kScal;   // goes with dO
+  const float* betap = gamp;                                                      // with dR
+  const uint32_t grow = 2 * ((16 * wave + 4 * q) * (uint32_t)a.do_st + col);
+  const uint32_t orow = 2 * ((16 * wave + 4 * q) * (uint32_t)(a.Hv * a.Dv) + col);
+  int64_t out_at = (((int64_t)s.b * a.T + s.tok0 + (int64_t)lastc * kC) * a.Hv + s.hv) * a.Dv;
+  const int64_t plane = (int64_t)a.B * a.T * a.Hv * a.Dv;
+  const auto load_do = [&](int left) {
+    const Rsrc gr_ = buffer_at(gp);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      gr[i].load(gr_, (grow + 2 * i * (uint32_t)a.do_st) | dead | miss_from(16 * wave + 4 * q + i, left));
+    gam = load_f4(buffer_at(gamp), 4 * (16 * wave + 4 * q) | miss_from(0, left));
+    gamp -= a.Hv * kScal;
+    gp -= kC * a.do_st;
+  };
+  const auto load_p = [&](int left) {
+    const Rsrc tr = buffer_at(trip);
+    const uint32_t at = lane * 16 | miss_from(0, left);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const int f = 2 * kTFrags + upper_frag(wave, wave < 2 ? ks : 1);
+      pf[ks][0] = load_frag(tr, at, f * 1024);
+      pf[ks][1] = load_frag(tr, at, (kTFrags + f) * 1024);
+    }
+    trip -= (int64_t)a.Hv * kTriBytes;
+  };
+  const auto load_beta = [&](int left) {
+    bt = load_f4(buffer_at(betap), 4 * (16 * wave + 4 * q) | miss_from(0, left), 8 * kC);
+    betap -= a.Hv * kScal;
+  };
+  const auto put_do = [&]() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const u32x2 g = {gr[0].half(n) | (gr[1].half(n) << 16), gr[2].half(n) | (gr[3].half(n) << 16)};
+      *reinterpret_cast<u32x2*>(lds.G + put_tok + n * 1024) = g;
+    }
+  };
+  const auto put_z = [&]() {
+    f32x4 Z[NT] = {}, Z2[NT] = {};
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+      if (ks >= wave >> 1)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const bf16x8 g = *reinterpret_cast<const bf16x8*>(lds.G + (ks * NT + n) * 1024 + lane * 16);
+          Z[n] = mfma(pf[ks][0], g, Z[n]);
+          Z2[n] = mfma(pf[ks][1], g, Z2[n]);
+        }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) lds.Z[wave][n][lane] = Z[n] + Z2[n];
+  };
+  const auto put_h = [&]() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      f32x4 g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) g[i] = gr[i].get(n);
+      const Parts p = parts_of(g * (gam * a.scale));
+      *reinterpret_cast<u32x2*>(lds.H[0] + put_tok + n * 1024) = p.hi;
+      *reinterpret_cast<u32x2*>(lds.H[1] + put_tok + n * 1024) = p.lo;
+    }
+  };
+
+  // beta is a chunk behind dO and P: it is of the chunk whose dR comes out
+  const int first_left = s.len - lastc * kC;
+  if (lastc >= 0) {
+    load_do(first_left);
+    load_p(first_left);
+    load_beta(first_left);
+    settle();
+    put_do();
+    lds_barrier();   // dO is in LDS
+    put_z();
+    put_h();
+    const int next = lastc > 0 ? kC : 0;
+    load_do(next);
+    load_p(next);
+    settle();
+  }
+  for (int c = lastc; c >= 0; --c) {
+    const int left = s.len - c * kC, later = c > 1 ? kC : 0;
+    lds_barrier();   // dS', P^T dO and s gam dO are in LDS
+    put_do();        // of the chunk before, as all that follows
+    lds_barrier();   // dU is in LDS, P^T dO read
+    put_z();
+    load_p(later);
+    lds_barrier();   // b gam dR is in LDS, s gam dO read
+    put_h();
+    load_do(later);
+    {
+      const Rsrc vr = buffer_at(a.dv + out_at), hr = buffer_at(a.dr + out_at), lr = buffer_at(a.dr + plane + out_at);
+      u32x2 v[NT], hi[NT], lo[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const f32x4 R = lds.R[wave][n][lane];
+        const Parts p = parts_of(R);
+        hi[n] = p.hi;
+        lo[n] = p.lo;
+        v[n] = round_of(bt * R);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t at = (orow + 2 * i * (uint32_t)(a.Hv * a.Dv)) | dead | miss_from(16 * wave + 4 * q + i, left);
+        store_row<NT>(vr, at, v, i);
+        store_row<NT>(hr, at, hi, i);
+        store_row<NT>(lr, at, lo, i);
+      }
+      out_at -= (int64_t)kC * a.Hv * a.Dv;
+    }
+    load_beta(c > 0 ? kC : 0);
+  }
+}
+
+// The forward scan's geometry and division of work (delta_fwd.hip), from the
+// last chunk to the first.
+template <int KS, int NT>
+__global__ __launch_bounds__(512) void delta_scan_bwd_kernel(Args a) {
+  __shared__ __attribute__((aligned(16))) ScanBwdLds<KS, NT> lds;
+  Scan s;
+  if (!s.init(a, 16 * NT)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (wave < 4) scan_bwd_state<KS, NT>(a, s, wave, lane, lds);
+  else scan_bwd_tokens<KS, NT>(a, s, wave & 3, lane, lds);
 }
 
 // One chunk of one key head, its value heads one after another so that the
@@ -694,13 +774,13 @@ template <int KS>
 int launch_bwd(const Args& a, hipStream_t st) {
   switch (scan_tiles(a)) {
     case 1:
-      hipLaunchKernelGGL((delta_scan_bwd_kernel<KS, 1>), dim3(scan_blocks(a, 16)), dim3(256), 0, st, a);
+      hipLaunchKernelGGL((delta_scan_bwd_kernel<KS, 1>), dim3(scan_blocks(a, 16)), dim3(512), 0, st, a);
       break;
     case 2:
-      hipLaunchKernelGGL((delta_scan_bwd_kernel<KS, 2>), dim3(scan_blocks(a, 32)), dim3(256), 0, st, a);
+      hipLaunchKernelGGL((delta_scan_bwd_kernel<KS, 2>), dim3(scan_blocks(a, 32)), dim3(512), 0, st, a);
       break;
     default:
-      hipLaunchKernelGGL((delta_scan_bwd_kernel<KS, 4>), dim3(scan_blocks(a, 64)), dim3(256), 0, st, a);
+      hipLaunchKernelGGL((delta_scan_bwd_kernel<KS, 4>), dim3(scan_blocks(a, 64)), dim3(512), 0, st, a);
   }
   if (const int rc = check_launch("delta_scan_bwd")) return rc;
   if (a.nchunks == 0) return UTTT_OK;
