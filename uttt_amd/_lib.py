@@ -275,7 +275,7 @@ def call(name: str, *args) -> None:
 def call_on(t: torch.Tensor, name: str, *args) -> None:
     """call() with t's device current: a launch goes to the current device,
     which need not be the one of its stream."""
-    if t.get_device() == torch.cuda.current_device():
+    if t.get_device() == torch._C._cuda_getDevice():
         call(name, *args)
     else:
         with torch.cuda.device(t.device):

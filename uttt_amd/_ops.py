@@ -44,17 +44,18 @@ class _NoGraph:
         pass
 
 
-def run_function(fn, *args):
+def run_function(fn, *args, graph=True):
     """fn.apply(*args) of a torch.autograd.Function, or its forward alone where
-    nothing could see the difference: gradients are off and neither
-    torch.compile, jit tracing, a functorch transform nor a forward-mode level
-    is active (under which apply records, refuses or transforms the call).
+    nothing could see the difference: gradients are off (or the caller knows
+    that no input requires one: graph=False) and neither torch.compile, jit
+    tracing, a functorch transform nor a forward-mode level is active (under
+    which apply records, refuses or transforms the call).
     A forward that hands an input through returns it as it is, where apply
     returns an alias: its caller makes one (permute_with_expert_mask).
     apply costs 5 to 8 us of host time per call; a routed read without
     gradients, three of them, is paced by its host time (88 us against 61 on
     the GPU for 16 384 tokens of 192 over 48 experts)."""
-    if (torch.is_grad_enabled() or torch.compiler.is_compiling()
+    if (graph and torch.is_grad_enabled() or torch.compiler.is_compiling()
             or torch._C._are_functorch_transforms_active()
             or torch._C._get_tracing_state() is not None or forward_ad._current_level >= 0):
         return fn.apply(*args)

@@ -217,6 +217,23 @@ template <int CTRL>
 __device__ __forceinline__ float dpp_add(float x) {
   return x + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
 }
+// Inclusive sums over the 64 lanes in 64 bits: within rows of 16, then the
+// totals of the rows before.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add64(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xf, true);
+  return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double scan64(double x) {
+  x = dpp_add64<0x111, 0xf>(x);
+  x = dpp_add64<0x112, 0xf>(x);
+  x = dpp_add64<0x114, 0xf>(x);
+  x = dpp_add64<0x118, 0xf>(x);
+  x = dpp_add64<0x142, 0xa>(x);   // lane 15 of rows 0 and 2 to rows 1 and 3
+  return dpp_add64<0x143, 0xc>(x);   // lane 31 to rows 2 and 3
+}
 __device__ __forceinline__ float sum16(float x) {
   x = dpp_add<0xb1>(x);    // lane ^ 1
   x = dpp_add<0x4e>(x);    // lane ^ 2
@@ -261,11 +278,35 @@ struct Scan {
 inline unsigned scan_blocks(const Args& a, int width) {
   return (unsigned)(((int64_t)a.nseq * a.Hv + 7) / 8 * 8 * ((a.Dv + width - 1) / width));
 }
-// 16-column tiles of a scan's workgroup: as wide as leaves every CU one (an
-// operand fragment then serves more columns), at most 4.
+// 16-column tiles of a scan's workgroup.  One workgroup runs on a CU at a
+// time, and its chunk takes about 2.0, 2.3 and 3.0 us for 1, 2 and 4 tiles
+// (128 features): wide ones do more a CU, narrow ones end a long sequence
+// sooner.  What is estimated: rounds of workgroups over the 256 CUs, and of
+// packed sequences, whose lengths the host does not know, the work over the
+// CUs and a longest sequence of three times the mean.  Measured (us for 1, 2,
+// 4): 12 prompts of 1 to 5000 tokens, 16 heads 269, 180, 230; 16 x 2048 tokens,
+// 12 heads, with what a backward reads 631, 420, 353; one of 4096 tokens, 4
+// heads of 192 141, 158, 264.
 inline int scan_tiles(const Args& a) {
-  const int64_t heads = (int64_t)a.nseq * a.Hv;
-  return heads * ((a.Dv + 63) / 64) >= 256 ? 4 : heads * ((a.Dv + 31) / 32) >= 256 ? 2 : 1;
+  const int tiles[3] = {1, 2, 4}, tenths[3] = {20, 23, 30};
+  const int64_t total = a.T / kC + a.nseq, mean = (total + a.nseq - 1) / a.nseq;
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int i = 0; i < 3; ++i) {
+    const int64_t blocks = (a.Dv + 16 * tiles[i] - 1) / (16 * tiles[i]);
+    int64_t cost;
+    if (a.table) {
+      const int64_t longest = 3 * mean < total ? 3 * mean : total, work = total * a.Hv * blocks / 256;
+      cost = (longest > work ? longest : work) * tenths[i];
+    } else {
+      cost = ((int64_t)a.nseq * a.Hv * blocks + 255) / 256 * a.cps * tenths[i];
+    }
+    if (cost < least) {
+      least = cost;
+      best = tiles[i];
+    }
+  }
+  return best;
 }
 
 // Features up to which a kernel instance goes, in steps of 32: the next of 2,

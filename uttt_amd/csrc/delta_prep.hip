@@ -123,11 +123,12 @@ __device__ __forceinline__ void stage_rows(const uint16_t* src, int64_t st, int 
   }
 }
 
-// The transposed fragments of staged rows: 16 features by 32 tokens each.
+// The transposed fragments first, first + step, .. of staged rows: 16 features
+// by 32 tokens each.
 template <int KS, int LD>
-__device__ __forceinline__ void write_transposed(const uint16_t* lds, uint8_t* out) {
+__device__ __forceinline__ void write_transposed(const uint16_t* lds, uint8_t* out, int first, int step) {
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  for (int f = threadIdx.x >> 6; f < 4 * KS; f += 4) {
+  for (int f = first; f < 4 * KS; f += step) {
     const int feat = 16 * (f >> 1) + r, t0 = 32 * (f & 1) + 8 * q;
     uint32_t w[4];
 #pragma unroll
@@ -180,6 +181,31 @@ __global__ __launch_bounds__(256, KS <= 4 ? 4 : 2) void delta_prep_kernel(Args a
     return;
   }
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, q = lane >> 4;
+  const int group = a.Hv / a.Hk;
+  float gv = 0.0f, bv = 0.0f;   // wave 0: the lane's token
+  const auto load_gates = [&](int hv) {
+    if (lane < ch.n) {
+      const int64_t at = ((int64_t)ch.b * a.T + ch.t0 + lane) * a.Hv + hv;
+      gv = load_any(a.g, a.g_dtype, at);
+      bv = load_any(a.beta, a.beta_dtype, at);
+    }
+  };
+  // Cumulative log decays in 64 bits: differences of far tokens' sums keep
+  // fp32's relative order.  A decay below e^-200 is one of zero in fp32 and
+  // would only cost the sums their digits.
+  const auto put_decays = [&](int hv) {
+    const double G = scan64(gv < -200.0f ? -200.0f : gv);
+    const double Gc = __shfl(G, 63);
+    Gd[lane] = G;
+    bet[lane] = bv;
+    float* sc = a.scal + ((size_t)c * a.Hv + hv) * kScal;
+    sc[lane] = exp_diff(G);
+    sc[kC + lane] = exp_diff(Gc - G);
+    sc[2 * kC + lane] = bv;
+    sc[3 * kC + lane] = (float)G;
+    sc[4 * kC + lane] = (float)(G - (double)(float)G);
+  };
+  if (wave == 0) load_gates(hk * group);
   uint16_t* Kl = reinterpret_cast<uint16_t*>(buf);
   uint16_t* Ql = Kl + kC * LD;
   stage_rows<KS, LD>(a.k + ch.b * a.k_sb + ch.t0 * a.k_st + hk * a.k_sh, a.k_st, ch.n, a.Dk, Kl);
@@ -198,42 +224,18 @@ __global__ __launch_bounds__(256, KS <= 4 ? 4 : 2) void delta_prep_kernel(Args a
       qk[ct] = mfma(qa, kb, qk[ct]);
     }
   }
-  const size_t frag = ((size_t)c * a.Hk + hk) * (4 * KS) * 1024;
-  write_transposed<KS, LD>(Kl, a.kt + frag);
-  if constexpr (BWD) write_transposed<KS, LD>(Ql, a.qt + frag);
+  if (wave == 0) {
+    put_decays(hk * group);
+  } else {
+    const size_t frag = ((size_t)c * a.Hk + hk) * (4 * KS) * 1024;
+    write_transposed<KS, LD>(Kl, a.kt + frag, wave - 1, 3);
+    if constexpr (BWD) write_transposed<KS, LD>(Ql, a.qt + frag, wave - 1, 3);
+  }
   __syncthreads();
   float* Am = reinterpret_cast<float*>(buf);
   float* Pm = Am + kC * kLT;
   float* Tm = Pm;   // T takes P's place once P's fragments are written
-  const int group = a.Hv / a.Hk;
   for (int hv = hk * group; hv < (hk + 1) * group; ++hv) {
-    if (wave == 0) {
-      // Cumulative log decays in 64 bits: differences of far tokens' sums keep
-      // fp32's relative order.  A decay below e^-200 is one of zero in fp32
-      // and would only cost the sums their digits.
-      const int64_t at = ((int64_t)ch.b * a.T + ch.t0 + lane) * a.Hv + hv;
-      float gv = 0.0f, bv = 0.0f;
-      if (lane < ch.n) {
-        gv = load_any(a.g, a.g_dtype, at);
-        bv = load_any(a.beta, a.beta_dtype, at);
-      }
-      double G = gv < -200.0f ? -200.0f : gv;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const double x = __shfl_up(G, d);
-        if (lane >= d) G += x;
-      }
-      const double Gc = __shfl(G, 63);
-      Gd[lane] = G;
-      bet[lane] = bv;
-      float* sc = a.scal + ((size_t)c * a.Hv + hv) * kScal;
-      sc[lane] = exp_diff(G);
-      sc[kC + lane] = exp_diff(Gc - G);
-      sc[2 * kC + lane] = bv;
-      sc[3 * kC + lane] = (float)G;
-      sc[4 * kC + lane] = (float)(G - (double)(float)G);
-    }
-    __syncthreads();
 #pragma unroll
     for (int ct = 0; ct < 4; ++ct) {
       const int j = 16 * ct + r;
@@ -306,7 +308,12 @@ __global__ __launch_bounds__(256, KS <= 4 ? 4 : 2) void delta_prep_kernel(Args a
       for (int i = 0; i < 4; ++i) Tm[(32 + 16 * rt + 4 * q + i) * kLT + 16 * ct + r] = -z[i];
     }
     __syncthreads();
-    write_tri<BWD>(Tm, tri, wave, 4);
+    const bool more = hv + 1 < (hk + 1) * group;
+    if (wave == 0 && more) {   // the next head's decays meanwhile
+      load_gates(hv + 1);
+      put_decays(hv + 1);
+    }
+    write_tri<BWD>(Tm, tri, more ? (wave == 0 ? kTFrags : wave - 1) : wave, more ? 3 : 4);
     __syncthreads();
   }
 }

@@ -20,46 +20,54 @@ There is no CPU path.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
 
 from . import _lib as L
-from ._ops import none_if_empty, run_function, traced_op
+from ._ops import run_function, traced_op
 
 MAX_KEY_DIM = 256
 
 
+@functools.lru_cache(maxsize=256)
+def _int64s(*values):
+    """Host integers as the C ABI takes them (read during a call, never written)."""
+    return (ctypes.c_int64 * len(values))(*values)
+
+
 def _strides(t: Tensor):
-    """Element strides of [B, T, H, D] with D contiguous, as the C ABI takes them."""
-    return (ctypes.c_int64 * 3)(*t.stride()[:3])
+    """Element strides of [B, T, H, D] with D contiguous."""
+    return _int64s(*t.stride()[:3])
 
 
 def _rows16(t: Tensor) -> Tensor:
     """t itself where its rows can be read 16 bytes at a time, else a copy."""
-    ok = t.stride(3) == 1 and all(s % 8 == 0 for s in t.stride()[:3]) and t.data_ptr() % 16 == 0
-    return t if ok else t.contiguous()
+    sb, st, sh, sd = t.stride()
+    return t if sd == 1 and not (sb | st | sh) % 8 and not t.data_ptr() % 16 else t.contiguous()
+
+
+_GATE_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _check(q, k, v, g, beta, what):
-    tensors = dict(q=q, k=k, v=v, g=g, beta=beta)
-    L.require_device(*tensors.values())
-    for name, t in tensors.items():
-        assert t.device == q.device, f"{what}: {name} is on {t.device}, q on {q.device}"
-    assert q.dim() == 4 and k.dim() == 4 and v.dim() == 4, (
+    L.require_device(q, k, v, g, beta)
+    assert q.get_device() == k.get_device() == v.get_device() == g.get_device() == beta.get_device(), (
+        f"{what}: q, k, v, g and beta must be on one device")
+    assert q.dim() == 4 and v.dim() == 4, (
         f"{what}: q and k must be [B, T, Hk, Dk], v [B, T, Hv, Dv]")
-    B, T, Hk, Dk = q.shape
-    Hv, Dv = v.shape[2:]
-    assert k.shape == q.shape, f"{what}: k {tuple(k.shape)} must have q's shape {tuple(q.shape)}"
-    assert v.shape[:2] == q.shape[:2], f"{what}: v {tuple(v.shape)} must have q's batch and tokens"
+    B, T, Hk, Dk = shape = q.shape
+    Bv, Tv, Hv, Dv = v.shape
+    assert k.shape == shape, f"{what}: k {tuple(k.shape)} must have q's shape {tuple(q.shape)}"
+    assert Bv == B and Tv == T, f"{what}: v {tuple(v.shape)} must have q's batch and tokens"
     assert Hk > 0 and Hv % Hk == 0, f"{what}: {Hv} value heads must be a multiple of {Hk} key heads"
-    assert tuple(g.shape) == (B, T, Hv) and tuple(beta.shape) == (B, T, Hv), (
+    assert g.shape == (B, T, Hv) and beta.shape == (B, T, Hv), (
         f"{what}: g and beta must be [B, T, Hv] = {(B, T, Hv)}")
-    assert k.dtype == q.dtype and v.dtype == q.dtype, f"{what}: q, k and v must have one dtype"
-    for name, t in (("g", g), ("beta", beta)):
-        assert t.dtype in (torch.float32, torch.bfloat16, torch.float16), (
-            f"{what}: {name} must be fp32, bf16 or fp16, got {t.dtype}")
+    assert k.dtype is q.dtype and v.dtype is q.dtype, f"{what}: q, k and v must have one dtype"
+    assert g.dtype in _GATE_TYPES, f"{what}: g must be fp32, bf16 or fp16, got {g.dtype}"
+    assert beta.dtype in _GATE_TYPES, f"{what}: beta must be fp32, bf16 or fp16, got {beta.dtype}"
     return B, T, Hk, Hv, Dk, Dv
 
 
@@ -67,39 +75,59 @@ def _seqs(q, cu_seqlens):
     return q.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1
 
 
-def _fwd_fake(q, k, v, g, beta, initial_state, cu_seqlens, scale, want_state, keep):
-    B, T, Hk, Dk = q.shape
-    Hv, Dv = v.shape[2:]
-    n = _seqs(q, cu_seqlens)
-    o = v.new_empty((B, T, Hv, Dv))
-    state = v.new_empty((n, Hv, Dk, Dv) if want_state else (0,), dtype=torch.float32)
-    slots = T // 64 + n + 2 if cu_seqlens is not None else B * ((T + 63) // 64)
-    u = v.new_empty((2, B, T, Hv, Dv) if keep else (0,))
-    return o, state, u, v.new_empty((slots, Hv, 2, Dk, Dv) if keep else (0,))
-
-
-@traced_op("gated_delta_fwd", _fwd_fake)
-def _fwd(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, initial_state: Optional[Tensor],
-         cu_seqlens: Optional[Tensor], scale: float, want_state: bool,
-         keep: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
-    """(o, final states, U, chunk-start states), the last two as bf16 parts hi
-    and lo; what is not wanted is empty."""
+def _launch_fwd(q, k, v, g, beta, initial_state, cu_seqlens, scale, o, state, u, s0):
     B, T, Hk, Dk = q.shape
     Hv, Dv = v.shape[2:]
     n = _seqs(q, cu_seqlens)
     packed = cu_seqlens is not None
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    o, state, u, s0 = _fwd_fake(q, k, v, g, beta, initial_state, cu_seqlens, scale, want_state, keep)
     g, beta = g.contiguous(), beta.contiguous()
-    lib = L.lib()
-    size = lib.uttt_gated_delta_workspace_bytes(B, T, n, Hk, Hv, Dk, Dv, int(packed), 0)
+    size = L.lib().uttt_gated_delta_workspace_bytes(B, T, n, Hk, Hv, Dk, Dv, int(packed), 0)
     ws = torch.empty(size, dtype=torch.uint8, device=q.device)
     L.call_on(q, "uttt_gated_delta_fwd", L.ptr(q), _strides(q), L.ptr(k), _strides(k), L.ptr(v),
               _strides(v), L.ptr(g), L.dtype_code(g.dtype), L.ptr(beta), L.dtype_code(beta.dtype),
               L.ptr(cu_seqlens), int(packed and cu_seqlens.dtype == torch.int64), B, T, n, Hk, Hv,
-              Dk, Dv, scale, L.ptr(initial_state), L.ptr(o), L.ptr(state) if want_state else None,
-              L.ptr(u) if keep else None, L.ptr(s0) if keep else None, L.ptr(ws), size,
-              L.stream_of(q))
+              Dk, Dv, scale, L.ptr(initial_state), L.ptr(o), L.ptr(state), L.ptr(u), L.ptr(s0),
+              L.ptr(ws), size, L.stream_of(q))
+
+
+def _state_like(v, q, cu_seqlens, wanted):
+    shape = (_seqs(q, cu_seqlens), v.shape[2], q.shape[3], v.shape[3]) if wanted else (0,)
+    return torch.empty(shape, dtype=torch.float32, device=v.device)
+
+
+def _infer_fake(q, k, v, g, beta, initial_state, cu_seqlens, scale, want_state):
+    return (torch.empty(v.shape, dtype=v.dtype, device=v.device),
+            _state_like(v, q, cu_seqlens, want_state))
+
+
+@traced_op("gated_delta_infer", _infer_fake)
+def _infer(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, initial_state: Optional[Tensor],
+           cu_seqlens: Optional[Tensor], scale: float, want_state: bool) -> Tuple[Tensor, Tensor]:
+    """(o, final states, empty where not wanted)."""
+    o, state = _infer_fake(q, k, v, g, beta, initial_state, cu_seqlens, scale, want_state)
+    _launch_fwd(q, k, v, g, beta, initial_state, cu_seqlens, scale, o, state if want_state else None,
+                None, None)
+    return o, state
+
+
+def _fwd_fake(q, k, v, g, beta, initial_state, cu_seqlens, scale, want_state):
+    B, T, Hk, Dk = q.shape
+    Hv, Dv = v.shape[2:]
+    slots = T // 64 + _seqs(q, cu_seqlens) + 2 if cu_seqlens is not None else B * ((T + 63) // 64)
+    return (*_infer_fake(q, k, v, g, beta, initial_state, cu_seqlens, scale, want_state),
+            v.new_empty((2, B, T, Hv, Dv)), v.new_empty((slots, Hv, 2, Dk, Dv)))
+
+
+@traced_op("gated_delta_fwd", _fwd_fake)
+def _fwd(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, initial_state: Optional[Tensor],
+         cu_seqlens: Optional[Tensor], scale: float,
+         want_state: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """_infer, and what the backward reads: U and the states at the chunks'
+    starts, as bf16 parts hi and lo."""
+    o, state, u, s0 = _fwd_fake(q, k, v, g, beta, initial_state, cu_seqlens, scale, want_state)
+    _launch_fwd(q, k, v, g, beta, initial_state, cu_seqlens, scale, o, state if want_state else None,
+                u, s0)
     return o, state, u, s0
 
 
@@ -137,13 +165,15 @@ def _bwd(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, cu_seqlens: O
 class _GatedDeltaRule(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, initial_state, cu_seqlens, scale, want_state, keep):
-        o, state, u, s0 = _fwd(q, k, v, g, beta, initial_state, cu_seqlens, scale, want_state, keep)
-        if keep:
-            ctx.save_for_backward(q, k, v, g, beta, cu_seqlens, u, s0)
-            ctx.scale = scale
-            ctx.want_dh0 = initial_state is not None and initial_state.requires_grad
-            ctx.set_materialize_grads(False)
-        return o, none_if_empty(state) if want_state is False else state
+        args = (q, k, v, g, beta, initial_state, cu_seqlens, scale, want_state)
+        if not keep:
+            return _infer(*args)
+        o, state, u, s0 = _fwd(*args)
+        ctx.save_for_backward(q, k, v, g, beta, cu_seqlens, u, s0)
+        ctx.scale = scale
+        ctx.want_dh0 = initial_state is not None and initial_state.requires_grad
+        ctx.set_materialize_grads(False)
+        return o, state
 
     @staticmethod
     def backward(ctx, do, dstate):
@@ -194,7 +224,7 @@ def gated_delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, *
         cu_seqlens = cu_seqlens.contiguous()
     if initial_state is not None:
         shape = (_seqs(q, cu_seqlens), Hv, Dk, Dv)
-        assert tuple(initial_state.shape) == shape, f"{what}: initial_state must be {shape}"
+        assert initial_state.shape == shape, f"{what}: initial_state must be {shape}"
         assert initial_state.dtype == torch.float32, f"{what}: states are fp32"
         assert initial_state.device == q.device, f"{what}: initial_state is on {initial_state.device}"
         initial_state = initial_state.contiguous()
@@ -202,12 +232,12 @@ def gated_delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, *
     keep = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state))
     o, state = run_function(_GatedDeltaRule, q, k, v, g, beta, initial_state, cu_seqlens, scale,
-                            bool(output_final_state), keep)
+                            bool(output_final_state), keep, graph=keep)
     return o, state if output_final_state else None
 
 
 def _step_fake(q, k, v, g, beta, state, scale, state_indices):
-    return v.new_empty(v.shape)
+    return torch.empty(v.shape, dtype=v.dtype, device=v.device)
 
 
 @traced_op("gated_delta_step", _step_fake, mutates_args=("state",))
@@ -220,7 +250,8 @@ def _step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, state: Tenso
     o = _step_fake(q, k, v, g, beta, state, scale, state_indices)
     L.call_on(q, "uttt_gated_delta_step", L.ptr(q), _strides(q), L.ptr(k), _strides(k), L.ptr(v),
               _strides(v), L.dtype_code(q.dtype), L.ptr(g), L.dtype_code(g.dtype), L.ptr(beta),
-              L.dtype_code(beta.dtype), B, T, Hk, Hv, Dk, Dv, scale, L.ptr(state), state.stride(0),
+              L.dtype_code(beta.dtype), B, T, Hk, Hv, Dk, Dv, scale, L.ptr(state),
+              max(state.stride(0), Hv * Dk * Dv),
               state.shape[0], L.ptr(state_indices),
               int(state_indices is not None and state_indices.dtype == torch.int64), L.ptr(o),
               L.stream_of(q))
@@ -247,14 +278,15 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
     assert q.dtype in (torch.float32, torch.bfloat16, torch.float16), f"{what}: dtype {q.dtype}"
     assert 1 <= Dk <= MAX_KEY_DIM and Dv >= 4 and Dv % 4 == 0, (
         f"{what}: Dk = {Dk} must be at most {MAX_KEY_DIM}, Dv = {Dv} a multiple of 4")
-    assert state.dim() == 4 and tuple(state.shape[1:]) == (Hv, Dk, Dv), (
+    assert state.dim() == 4 and state.shape[1:] == (Hv, Dk, Dv), (
         f"{what}: state must be [slots, {Hv}, {Dk}, {Dv}], got {tuple(state.shape)}")
     assert state.dtype == torch.float32 and state.device == q.device, f"{what}: state must be fp32 on {q.device}"
-    assert state.shape[0] == 0 or (state[0].is_contiguous() and state.stride(0) % 4 == 0
-                                   and (state.shape[0] == 1 or state.stride(0) >= Hv * Dk * Dv)), (
+    ss, sh, sk, sd = state.stride()
+    assert state.is_contiguous() or (sd == 1 and sk == Dv and sh == Dk * Dv and ss % 4 == 0
+                                     and (ss >= Hv * Dk * Dv or state.shape[0] <= 1)), (
         f"{what}: each slot's state must be contiguous and apart from the others")
     if state_indices is not None:
-        assert tuple(state_indices.shape) == (B,), f"{what}: state_indices must be [{B}]"
+        assert state_indices.shape == (B,), f"{what}: state_indices must be [{B}]"
         assert state_indices.dtype in (torch.int32, torch.int64), f"{what}: state_indices must be int32 or int64"
         assert state_indices.device == q.device, f"{what}: state_indices is on {state_indices.device}"
         state_indices = state_indices.contiguous()

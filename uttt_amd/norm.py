@@ -18,18 +18,34 @@ def _code(t: Optional[Tensor]) -> int:
     return L.F32 if t is None else L.dtype_code(t.dtype)
 
 
-def _fwd_fake(x, weight, bias, eps, keep):
-    return x.new_empty(x.shape), x.new_empty((2, x.shape[0]) if keep else (0,), dtype=torch.float32)
+def _launch_fwd(x, weight, bias, eps, y, stats):
+    L.call_on(x, "uttt_layer_norm_fwd", L.ptr(x), L.dtype_code(x.dtype), x.stride(0), x.shape[0],
+              x.shape[1], L.ptr(weight), _code(weight), L.ptr(bias), _code(bias), eps, L.ptr(y),
+              L.ptr(stats), L.stream_of(x))
+
+
+def _infer_fake(x, weight, bias, eps):
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+@traced_op("layer_norm_infer", _infer_fake)
+def _infer(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float) -> Tensor:
+    """y of x [rows, N] with any row stride."""
+    y = _infer_fake(x, weight, bias, eps)
+    _launch_fwd(x, weight, bias, eps, y, None)
+    return y
+
+
+def _fwd_fake(x, weight, bias, eps):
+    return _infer_fake(x, weight, bias, eps), x.new_empty((2, x.shape[0]), dtype=torch.float32)
 
 
 @traced_op("layer_norm_fwd", _fwd_fake)
-def _fwd(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
-         keep: bool) -> Tuple[Tensor, Tensor]:
-    """x [rows, N] with any row stride -> (y, fp32 mean and 1 / deviation of each row)."""
-    y, stats = _fwd_fake(x, weight, bias, eps, keep)
-    L.call_on(x, "uttt_layer_norm_fwd", L.ptr(x), L.dtype_code(x.dtype), x.stride(0), x.shape[0],
-              x.shape[1], L.ptr(weight), _code(weight), L.ptr(bias), _code(bias), eps, L.ptr(y),
-              L.ptr(stats) if keep else None, L.stream_of(x))
+def _fwd(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor],
+         eps: float) -> Tuple[Tensor, Tensor]:
+    """y, and the fp32 mean and 1 / deviation of each row for the backward."""
+    y, stats = _fwd_fake(x, weight, bias, eps)
+    _launch_fwd(x, weight, bias, eps, y, stats)
     return y, stats
 
 
@@ -55,9 +71,10 @@ def _bwd(x: Tensor, dy: Tensor, weight: Optional[Tensor], bias: Optional[Tensor]
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, keep):
-        y, stats = _fwd(x, weight, bias, eps, keep)
-        if keep:
-            ctx.save_for_backward(x, weight, bias, stats)
+        if not keep:
+            return _infer(x, weight, bias, eps)
+        y, stats = _fwd(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, bias, stats)
         return y
 
     @staticmethod
@@ -83,15 +100,17 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
     assert x.dim() >= 1 and x.shape[-1] >= 1, "layer_norm: x must be [..., N] with N of 1 or more"
     assert x.dtype in _TYPES, f"layer_norm: dtype {x.dtype}"
     N = x.shape[-1]
+    keep = x.requires_grad
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None:
-            assert tuple(t.shape) == (N,), f"layer_norm: {name} must be [{N}], got {tuple(t.shape)}"
+            assert t.shape == (N,), f"layer_norm: {name} must be [{N}], got {tuple(t.shape)}"
             assert t.dtype in _TYPES, f"layer_norm: {name} has dtype {t.dtype}"
-            assert t.device == x.device, f"layer_norm: {name} is on {t.device}, x on {x.device}"
-    rows = x.reshape(-1, N)   # a view wherever the rows are evenly spaced
+            assert t.get_device() == x.get_device(), f"layer_norm: {name} is on {t.device}, x on {x.device}"
+            keep = keep or t.requires_grad
+    rows = x if x.dim() == 2 else x.reshape(-1, N)   # a view wherever the rows are evenly spaced
     if (rows.stride(1) != 1 and N > 1) or rows.stride(0) < 0:
         rows = rows.contiguous()
-    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
-    keep = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (x, weight, bias))
-    return run_function(_LayerNorm, rows, weight, bias, float(eps), keep).view(x.shape)
+    keep = keep and torch.is_grad_enabled()
+    y = run_function(_LayerNorm, rows, None if weight is None else weight.contiguous(),
+                     None if bias is None else bias.contiguous(), float(eps), keep, graph=keep)
+    return y if x.dim() == 2 else y.view(x.shape)

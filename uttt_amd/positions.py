@@ -4,6 +4,7 @@ position per token, from tables, is uttt_amd.moe.Rope.  No CPU path."""
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import List, Sequence
 
 import torch
@@ -25,8 +26,14 @@ def axis_frequencies(sections: Sequence[int], base: float = 10000.0, *, per_axis
     return torch.tensor([float(base) ** (-j / m) for j, m in rows], dtype=torch.float32, device=device)
 
 
+@functools.lru_cache(maxsize=256)
+def _host(ctype, *values):
+    """Host integers as the C ABI takes them (read during a call, never written)."""
+    return (ctype * len(values))(*values)
+
+
 def _turn_fake(x, positions, inv_freq, sections, interleaved, inverse):
-    return x.new_empty(x.shape)
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 @traced_op("rotary_axes", _turn_fake)
@@ -37,9 +44,9 @@ def _turn(x: Tensor, positions: Tensor, inv_freq: Tensor, sections: List[int], i
         x = x.contiguous()
     y = _turn_fake(x, positions, inv_freq, sections, interleaved, inverse)
     L.call_on(x, "uttt_rotary_axes", L.ptr(x), L.dtype_code(x.dtype),
-              (ctypes.c_int64 * 3)(*x.stride()[:3]), B, Lx, H, D, L.ptr(positions),
-              int(positions.dtype == torch.int64), (ctypes.c_int64 * 3)(*positions.stride()),
-              L.ptr(inv_freq), (ctypes.c_int * len(sections))(*sections), len(sections),
+              _host(ctypes.c_int64, *x.stride()[:3]), B, Lx, H, D, L.ptr(positions),
+              int(positions.dtype == torch.int64), _host(ctypes.c_int64, *positions.stride()),
+              L.ptr(inv_freq), _host(ctypes.c_int, *sections), len(sections),
               int(interleaved), int(inverse), L.ptr(y), L.stream_of(x))
     return y
 
@@ -82,11 +89,12 @@ def rotary_axes(x: Tensor, positions: Tensor, inv_freq: Tensor, sections: Sequen
     assert 1 <= A <= MAX_AXES and min(sections) >= 0, f"{what}: 1 to {MAX_AXES} sections of 0 or more pairs"
     assert 1 <= R and 2 * R <= D, f"{what}: {R} pairs do not fit {D} features"
     assert positions.dtype in (torch.int32, torch.int64), f"{what}: positions must be int32 or int64"
-    assert tuple(positions.shape) in ((B, Lx, A), (Lx, A)), (
+    assert positions.shape == (B, Lx, A) or positions.shape == (Lx, A), (
         f"{what}: positions must be [{B}, {Lx}, {A}] or [{Lx}, {A}], got {tuple(positions.shape)}")
-    assert tuple(inv_freq.shape) == (R,) and inv_freq.dtype == torch.float32, (
+    assert inv_freq.shape == (R,) and inv_freq.dtype == torch.float32, (
         f"{what}: inv_freq must be [{R}] fp32")
-    assert positions.device == x.device and inv_freq.device == x.device, f"{what}: tensors on several devices"
+    assert positions.get_device() == inv_freq.get_device() == x.get_device(), f"{what}: tensors on several devices"
     if positions.dim() == 2:
         positions = positions.expand(B, Lx, A)
-    return run_function(_RotaryAxes, x, positions, inv_freq.contiguous(), sections, bool(interleaved))
+    return run_function(_RotaryAxes, x, positions, inv_freq.contiguous(), sections, bool(interleaved),
+                        graph=x.requires_grad)
