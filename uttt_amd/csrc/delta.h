@@ -55,6 +55,7 @@ struct Args {
   float* scal;                   // [nchunks, Hv, kScal]
   uint8_t* kt;                   // [nchunks, Hk, 4 KS] KiB: K^T fragments
   uint8_t* qt;                   // the same of Q (backward)
+  uint8_t *kf, *qf;              // [nchunks, Hk, 4 KS] KiB: K and Q fragments, or null: rows are read
   const float* h0;               // [nseq, Hv, Dk, Dv] or null
   uint16_t* o;                   // [B, T, Hv, Dv]
   float* hT;                     // final states or null
@@ -287,19 +288,19 @@ inline unsigned scan_blocks(const Args& a, int width) {
 // 4): 12 prompts of 1 to 5000 tokens, 16 heads 269, 180, 230; 16 x 2048 tokens,
 // 12 heads, with what a backward reads 631, 420, 353; one of 4096 tokens, 4
 // heads of 192 141, 158, 264.
-inline int scan_tiles(const Args& a) {
+inline int scan_tiles(int64_t T, int nseq, int Hv, int Dv, bool packed) {
   const int tiles[3] = {1, 2, 4}, tenths[3] = {20, 23, 30};
-  const int64_t total = a.T / kC + a.nseq, mean = (total + a.nseq - 1) / a.nseq;
+  const int64_t total = T / kC + nseq, mean = (total + nseq - 1) / nseq, cps = (T + kC - 1) / kC;
   int best = 1;
   int64_t least = INT64_MAX;
   for (int i = 0; i < 3; ++i) {
-    const int64_t blocks = (a.Dv + 16 * tiles[i] - 1) / (16 * tiles[i]);
+    const int64_t blocks = (Dv + 16 * tiles[i] - 1) / (16 * tiles[i]);
     int64_t cost;
-    if (a.table) {
-      const int64_t longest = 3 * mean < total ? 3 * mean : total, work = total * a.Hv * blocks / 256;
+    if (packed) {
+      const int64_t longest = 3 * mean < total ? 3 * mean : total, work = total * Hv * blocks / 256;
       cost = (longest > work ? longest : work) * tenths[i];
     } else {
-      cost = ((int64_t)a.nseq * a.Hv * blocks + 255) / 256 * a.cps * tenths[i];
+      cost = ((int64_t)nseq * Hv * blocks + 255) / 256 * cps * tenths[i];
     }
     if (cost < least) {
       least = cost;
@@ -308,6 +309,7 @@ inline int scan_tiles(const Args& a) {
   }
   return best;
 }
+inline int scan_tiles(const Args& a) { return scan_tiles(a.T, a.nseq, a.Hv, a.Dv, a.table != nullptr); }
 
 // Features up to which a kernel instance goes, in steps of 32: the next of 2,
 // 3, 4, 6, 8 (K, Q past Dk are zeros in LDS).
@@ -334,7 +336,7 @@ int launch_prep(const Args& a, bool transposed, hipStream_t st);
 
 // The parts of a call's workspace, in order.
 struct Workspace {
-  size_t table, seqs, scal, kt, tri, qt, ds, dr, total;
+  size_t table, seqs, scal, kt, tri, kf, qf, qt, ds, dr, total;
 };
 inline int chunk_slots(int64_t B, int64_t T, int nseq, bool packed) {
   const int64_t n = packed ? T / kC + nseq + 2 : B * ((T + kC - 1) / kC);
@@ -356,6 +358,15 @@ inline Workspace workspace_of(int64_t B, int64_t T, int nseq, int Hk, int Hv, in
   w.scal = take(n * Hv * kScal * 4);
   w.kt = take(frags);
   w.tri = take(n * Hv * kTriBytes);
+  // Where 16 columns a workgroup are taken, each of them loads all of K and Q:
+  // then from a copy in fragment order, 1 KiB a load, and not 64 bytes of each
+  // of 16 rows (a chunk of 192 features 2.1 -> 1.5 us; with more columns a
+  // workgroup the copy costs more than it saves).
+  const bool copies = scan_tiles(T, nseq, Hv, Dv, packed) == 1;
+  w.kf = take(copies ? frags : 0);
+  w.qf = take(copies && !backward ? frags : 0);
+  if (!copies) w.kf = w.qf = SIZE_MAX;
+  if (backward) w.qf = SIZE_MAX;
   w.qt = take(backward ? frags : 0);
   w.ds = take(backward ? n * Hv * Dk * Dv * 4 : 0);
   w.dr = take(backward ? (size_t)B * T * Hv * Dv * 4 : 0);
@@ -369,6 +380,8 @@ inline void bind_workspace(Args& a, const Workspace& w, uint8_t* ws, bool packed
   a.scal = reinterpret_cast<float*>(ws + w.scal);
   a.kt = ws + w.kt;
   a.tri = ws + w.tri;
+  a.kf = w.kf == SIZE_MAX ? nullptr : ws + w.kf;
+  a.qf = w.qf == SIZE_MAX ? nullptr : ws + w.qf;
   if (backward) {
     a.qt = ws + w.qt;
     a.ds = reinterpret_cast<uint16_t*>(ws + w.ds);

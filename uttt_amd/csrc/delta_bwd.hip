@@ -68,12 +68,18 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
   float gc;
   // Operands of the chunk before: pointers that go along, at first those of the last chunk.
   const int lastc = s.nc - 1;
-  const uint16_t* kp = a.k + s.b * a.k_sb + s.hk * a.k_sh + (s.tok0 + (int64_t)lastc * kC) * a.k_st;
+  const bool copies = a.kf != nullptr;   // K's fragments in place of its rows
+  const int64_t copy_step = (int64_t)a.Hk * (4 * KS * 1024);
+  const uint8_t* kp = copies ? a.kf + (s.c0 + lastc) * copy_step + s.hk * (4 * KS * 1024)
+                             : reinterpret_cast<const uint8_t*>(a.k + s.b * a.k_sb + s.hk * a.k_sh +
+                                                                (s.tok0 + (int64_t)lastc * kC) * a.k_st);
+  const int64_t k_step = copies ? copy_step : 2 * kC * a.k_st;
   const uint8_t* trip = a.tri + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kTriBytes;
   const int64_t trans_at = ((int64_t)(s.c0 + lastc) * a.Hk + s.hk) * (4 * KS * 1024);
   const uint8_t *ktp = a.kt + trans_at, *qtp = a.qt + trans_at;
   const float* scp = a.scal + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kScal;
-  const uint32_t krow = 2 * ((16 * wave + r) * (uint32_t)a.k_st + 8 * q);
+  const uint32_t krow = copies ? wave * KS * 1024 + lane * 16 : 2 * ((16 * wave + r) * (uint32_t)a.k_st + 8 * q);
+  const uint32_t along = copies ? 1024 : 64;
   const uint32_t last_half = miss_from(32 * (KS - 1) + 8 * q, a.Dk), before_half = miss_from(32 * (KS - 2) + 8 * q, a.Dk);
   // `left`: tokens from the chunk on to the sequence's end; 0 before its first chunk
   const auto load_k = [&](int left) {
@@ -81,9 +87,9 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
     const Rsrc kr = buffer_at(kp);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
-      kf[ks] = load_frag(kr, (krow + 64 * ks) | miss | (ks == KS - 1 ? last_half : ks == KS - 2 ? before_half : 0));
+      kf[ks] = load_frag(kr, krow | miss | (ks == KS - 1 ? last_half : ks == KS - 2 ? before_half : 0), along * ks);
     ge = load_f4(buffer_at(scp), 4 * (16 * wave + 4 * q) | miss_from(0, left), 4 * kC);
-    kp -= kC * a.k_st;
+    kp -= k_step;
   };
   const auto load_t = [&](int left) {
     const Rsrc tr = buffer_at(trip), sr = buffer_at(scp);

@@ -2,13 +2,21 @@
 // chunks (formulas, precision and fragment layout in delta.h).
 //
 // A workgroup owns 16 NT value columns of one head of one sequence and walks
-// its chunks in order, with two kinds of waves.  Four carry the state: each has
-// 16 tokens of X = K S0 and of U = T R, and a quarter of the state's features,
-// which stay in its registers from the first chunk to the last.  Four make the
-// outputs, 16 tokens each, from the same S0 and U, off the chain that bounds a
-// chunk.  An operand fragment (K, Q, T, P, K^T) is read by one wave, straight
-// into its registers and a chunk ahead; S, R and U pass through LDS, from the
-// wave that made them to all: three barriers a chunk.
+// its chunks in order, with two kinds of waves.  Four have the tokens, 16 each:
+// X = K S0 and R = b (V - gam X), then O = s gam Q S0 + P U.  Four have the
+// state: U = T R, 16 tokens each, and S' = gam_C S0 + K^T (e^{G_C - G} U), a
+// quarter of the features each, which stay in registers from the first chunk to
+// the last.  The chain R, U, S' bounds a chunk, so what is off it stands where
+// the other kind works on it: the state's waves load the next chunk's operands
+// and store what a backward will read while R is made, the others have Q S0
+// while U is made and P U while S' is.  An operand fragment (K, Q, T, P, K^T) is
+// read by one wave, straight into its registers and a chunk ahead; S, R and U
+// pass through LDS, from the wave that made them to all: three barriers a chunk.
+//
+// Measured: one sequence of 4096 tokens, 4 heads of 192 by 192, 85 us (1.3 us a
+// chunk; with X in the state's waves and K read by rows 140); 16 x 2048 tokens,
+// 12 heads of 128 by 128, with U and S0 stored for a backward, 338 us: 0.7 GB of
+// stores and 0.55 GB of loads at 3.7 TB/s (a copy reaches 5.1).
 #include "delta.h"
 
 namespace uttt {
@@ -32,6 +40,9 @@ struct Lane {
   uint32_t last_half, before_half;   // kNoRow where the last two steps' features are none
 };
 
+// The state's waves: U = T R and S' = gam_C S0 + K^T (e^{G_C - G} U).  While the
+// others work on R they load the next chunk's operands and store what a
+// backward will read.
 template <int KS, int NT, bool SAVE>
 __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const Lane& l, ScanLds<KS, NT>& lds) {
   constexpr int FT = (2 * KS + 3) / 4;   // 16-feature tiles of a wave
@@ -59,64 +70,38 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
                          ? a.h0[((int64_t)s.head * a.Dk + feat) * a.Dv + col + n] : 0.0f;
     }
 
-  bf16x8 kf[KS], tf[2][2], ktf[FT][2];
-  f32x4 gam, ge, bt;
-  float gc;
-  Cols<NT> vr[4];
-  // Operands of the next chunk: pointers that go along, per-lane offsets that
-  // stay, and the bit that masks rows past the sequence.  Each is loaded where
-  // its last value was used, in the order of use, which is the order in which
-  // loads are waited for.
-  const uint16_t* kp = a.k + s.b * a.k_sb + s.hk * a.k_sh + s.tok0 * a.k_st;
-  const uint16_t* vp = a.v + s.b * a.v_sb + s.hv * a.v_sh + s.tok0 * a.v_st;
+  // Operands of this chunk, and of the next on their way.
+  struct Ops {
+    bf16x8 t[2][2], kt[FT][2];
+    f32x4 ge;
+    float gc;
+  };
+  Ops now, coming;
   const uint8_t* trip = a.tri + ((size_t)s.c0 * a.Hv + s.hv) * kTriBytes;
   const uint8_t* ktp = a.kt + ((size_t)s.c0 * a.Hk + s.hk) * (4 * KS * 1024);
   const float* scp = a.scal + ((size_t)s.c0 * a.Hv + s.hv) * kScal;
-  const uint32_t krow = 2 * ((16 * wave + r) * (uint32_t)a.k_st + 8 * q);
-  const uint32_t vrow = 2 * ((16 * wave + 4 * q) * (uint32_t)a.v_st + col);
-  const uint32_t urow = 2 * ((16 * wave + 4 * q) * (uint32_t)(a.Hv * a.Dv) + col);
-  const auto load_rows = [&](int left) {
-    const uint32_t miss = miss_from(16 * wave + r, left), at = 4 * (16 * wave + 4 * q) | miss_from(0, left);
-    const Rsrc kr = buffer_at(kp), vr_ = buffer_at(vp), sr = buffer_at(scp);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-      kf[ks] = load_frag(kr, (krow + 64 * ks) | miss | (ks == KS - 1 ? l.last_half : ks == KS - 2 ? l.before_half : 0));
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      vr[i].load(vr_, (vrow + 2 * i * (uint32_t)a.v_st) | dead | miss_from(16 * wave + 4 * q + i, left));
-    gam = load_f4(sr, at);
-    bt = load_f4(sr, at, 8 * kC);
-    kp += kC * a.k_st;
-    vp += kC * a.v_st;
-  };
-  const auto load_t = [&](int left) {
-    const Rsrc tr = buffer_at(trip);
-    const uint32_t at = l.lane * 16 | miss_from(0, left);
-    ge = load_f4(buffer_at(scp), 4 * (16 * wave + 4 * q) | miss_from(0, left), 4 * kC);
+  const auto load = [&](int left, Ops& o) {
+    const uint32_t none = miss_from(0, left), at = l.lane * 16 | none;
+    const Rsrc tr = buffer_at(trip), kr = buffer_at(ktp), sr = buffer_at(scp);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       // step 1 of the upper tiles is zero and not stored: step 0 again, unused
       const int f = lower_frag(wave, wave < 2 ? 0 : ks);
-      tf[ks][0] = load_frag(tr, at, f * 1024);
-      tf[ks][1] = load_frag(tr, at, (kTFrags + f) * 1024);
+      o.t[ks][0] = load_frag(tr, at, f * 1024);
+      o.t[ks][1] = load_frag(tr, at, (kTFrags + f) * 1024);
     }
-    trip += (size_t)a.Hv * kTriBytes;
-  };
-  const auto load_kt = [&](int left) {
-    const Rsrc tr = buffer_at(ktp);
-    const uint32_t at = l.lane * 16 | miss_from(0, left);
+    o.ge = load_f4(sr, 4 * (16 * wave + 4 * q) | none, 4 * kC);
+    o.gc = load_f1(sr, 4 * (kC - 1) | none);
 #pragma unroll
     for (int f = 0; f < FT; ++f)
 #pragma unroll
       for (int t = 0; t < 2; ++t)
-        if (wave * FT + f < 2 * KS) ktf[f][t] = load_frag(tr, at, (2 * (wave * FT + f) + t) * 1024);
-    gc = load_f1(buffer_at(scp), 4 * (kC - 1) | miss_from(0, left));
+        if (wave * FT + f < 2 * KS) o.kt[f][t] = load_frag(kr, at, (2 * (wave * FT + f) + t) * 1024);
+    trip += (size_t)a.Hv * kTriBytes;
     ktp += (size_t)a.Hk * (4 * KS * 1024);
     scp += a.Hv * kScal;
   };
-  // the state's parts to LDS, and of a chunk that a backward will read to memory
-  uint16_t* s0p = SAVE ? a.s0 + ((int64_t)s.c0 * a.Hv + s.hv) * 2 * a.Dk * a.Dv : nullptr;
-  Parts sw[FT][NT];
+  Parts sw[FT][NT];   // the state's parts
   const auto put_state = [&]() {
 #pragma unroll
     for (int f = 0; f < FT; ++f) {
@@ -131,6 +116,7 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
         }
     }
   };
+  uint16_t* s0p = SAVE ? a.s0 + ((int64_t)s.c0 * a.Hv + s.hv) * 2 * a.Dk * a.Dv : nullptr;
   const auto save_state = [&]() {
     const Rsrc sr = buffer_at(s0p);
 #pragma unroll
@@ -152,37 +138,31 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
       }
     s0p += (int64_t)a.Hv * 2 * a.Dk * a.Dv;
   };
+  uint16_t* up = SAVE ? a.u + (((int64_t)s.b * a.T + s.tok0) * a.Hv + s.hv) * a.Dv : nullptr;
+  const int64_t plane = (int64_t)a.B * a.T * a.Hv * a.Dv;
+  const uint32_t urow = 2 * ((16 * wave + 4 * q) * (uint32_t)(a.Hv * a.Dv) + col);
+  u32x2 uh[NT], ul[NT];
+  const auto save_u = [&](int left) {
+    const Rsrc hr = buffer_at(up), lr = buffer_at(up + plane);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = (urow + 2 * i * (uint32_t)(a.Hv * a.Dv)) | dead | miss_from(16 * wave + 4 * q + i, left);
+      store_row<NT>(hr, at, uh, i);
+      store_row<NT>(lr, at, ul, i);
+    }
+    up += (int64_t)kC * a.Hv * a.Dv;
+  };
 
   if (s.len > 0) {
-    load_rows(s.len);
-    load_t(s.len);
-    load_kt(s.len);
+    load(s.len, coming);
     put_state();
     settle();
   }
-  uint16_t* up = SAVE ? a.u + (((int64_t)s.b * a.T + s.tok0) * a.Hv + s.hv) * a.Dv : nullptr;
-  const int64_t plane = (int64_t)a.B * a.T * a.Hv * a.Dv;
   for (int left = s.len; left > 0; left -= kC) {
     lds_barrier();   // S0 is in LDS
-    {
-      f32x4 X[NT] = {}, X2[NT] = {};
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          X[n] = mfma(kf[ks], get(lds.S[0], ks * NT + n), X[n]);
-          X2[n] = mfma(kf[ks], get(lds.S[1], ks * NT + n), X2[n]);
-        }
-      // R = b (V - gam X); rows behind the sequence's end have b = 0 and V = 0
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        f32x4 v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = vr[i].get(n);
-        put_tile(lds.R, n, parts_of(bt * (v - gam * (X[n] + X2[n]))));
-      }
-    }
-    load_rows(left - kC);
+    now = coming;
+    load(left - kC, coming);
+    if constexpr (SAVE) save_state();
     lds_barrier();   // R is in LDS
     f32x4 U[NT] = {};
     {
@@ -193,29 +173,27 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             const bf16x8 hi = get(lds.R[0], ks * NT + n), lo = get(lds.R[1], ks * NT + n);
-            U[n] = mfma(tf[ks][0], hi, U[n]);
-            U2[n] = mfma(tf[ks][1], hi, U2[n]);
-            U2[n] = mfma(tf[ks][0], lo, U2[n]);
+            U[n] = mfma(now.t[ks][0], hi, U[n]);
+            U2[n] = mfma(now.t[ks][1], hi, U2[n]);
+            U2[n] = mfma(now.t[ks][0], lo, U2[n]);
           }
 #pragma unroll
       for (int n = 0; n < NT; ++n) U[n] += U2[n];
     }
-    u32x2 uh[NT], ul[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      put_tile(lds.E, n, parts_of(ge * U[n]));
+      put_tile(lds.E, n, parts_of(now.ge * U[n]));
       const Parts p = parts_of(U[n]);
       put_tile(lds.U, n, p);
       uh[n] = p.hi;
       ul[n] = p.lo;
     }
-    load_t(left - kC);
     lds_barrier();   // U is in LDS
     // S' = gam_C S0 + K^T (e^{G_C - G} U)
 #pragma unroll
     for (int f = 0; f < FT; ++f)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) S[f][n] *= gc;
+      for (int n = 0; n < NT; ++n) S[f][n] *= now.gc;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -224,23 +202,12 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
 #pragma unroll
         for (int f = 0; f < FT; ++f)
           if (wave * FT + f < 2 * KS) {
-            S[f][n] = mfma(ktf[f][t], hi, S[f][n]);
-            S[f][n] = mfma(ktf[f][t], lo, S[f][n]);
+            S[f][n] = mfma(now.kt[f][t], hi, S[f][n]);
+            S[f][n] = mfma(now.kt[f][t], lo, S[f][n]);
           }
       }
-    load_kt(left - kC);
-    if constexpr (SAVE) {
-      const Rsrc hr = buffer_at(up), lr = buffer_at(up + plane);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t at = (urow + 2 * i * (uint32_t)(a.Hv * a.Dv)) | dead | miss_from(16 * wave + 4 * q + i, left);
-        store_row<NT>(hr, at, uh, i);
-        store_row<NT>(lr, at, ul, i);
-      }
-      up += (int64_t)kC * a.Hv * a.Dv;
-      save_state();   // S0, whose parts the last put_state left
-    }
     if (left > kC) put_state();
+    if constexpr (SAVE) save_u(left);
   }
   if (a.hT && col < a.Dv) {
 #pragma unroll
@@ -255,29 +222,59 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
   }
 }
 
+// The tokens' waves: R = b (V - gam K S0) and O = s gam Q S0 + P U.
 template <int KS, int NT>
-__device__ __forceinline__ void scan_outputs(const Args& a, const Scan& s, const Lane& l, ScanLds<KS, NT>& lds) {
+__device__ __forceinline__ void scan_tokens(const Args& a, const Scan& s, const Lane& l, ScanLds<KS, NT>& lds) {
   const int wave = l.wave, q = l.q;
+  const uint32_t put_tok = (wave >> 1) * NT * 1024 + (wave & 1) * 512 + (l.r + 16 * (q >> 1)) * 16 + (q & 1) * 8;
   const auto get = [&](const uint8_t* buf, int f) {
     return *reinterpret_cast<const bf16x8*>(buf + f * 1024 + l.lane * 16);
   };
-  bf16x8 qf[KS], pf[2][2];
-  f32x4 gam;
-  const uint16_t* qp = a.q + s.b * a.q_sb + s.hk * a.q_sh + s.tok0 * a.q_st;
+  bf16x8 kf[KS], qf[KS], pf[2][2];
+  f32x4 gam, bt;
+  Cols<NT> vr[4];
+  // Operands of the next chunk: pointers that go along, per-lane offsets that
+  // stay, and the bit that masks rows past the sequence.  Each is loaded where
+  // its last value was used, in the order of use, which is the order in which
+  // loads are waited for.
+  // K and Q: rows of the caller's tensors, or their fragments (delta_prep.hip)
+  const bool copies = a.kf != nullptr;
+  const int64_t copy_at = ((int64_t)s.c0 * a.Hk + s.hk) * (4 * KS * 1024), copy_step = (int64_t)a.Hk * (4 * KS * 1024);
+  const uint8_t* kp = copies ? a.kf + copy_at
+                             : reinterpret_cast<const uint8_t*>(a.k + s.b * a.k_sb + s.hk * a.k_sh + s.tok0 * a.k_st);
+  const uint8_t* qp = copies ? a.qf + copy_at
+                             : reinterpret_cast<const uint8_t*>(a.q + s.b * a.q_sb + s.hk * a.q_sh + s.tok0 * a.q_st);
+  const int64_t k_step = copies ? copy_step : 2 * kC * a.k_st, q_step = copies ? copy_step : 2 * kC * a.q_st;
+  const uint32_t in_copy = wave * KS * 1024 + l.lane * 16, along = copies ? 1024 : 64;
+  const uint32_t krow = copies ? in_copy : 2 * ((16 * wave + l.r) * (uint32_t)a.k_st + 8 * q);
+  const uint32_t qrow = copies ? in_copy : 2 * ((16 * wave + l.r) * (uint32_t)a.q_st + 8 * q);
+  const uint16_t* vp = a.v + s.b * a.v_sb + s.hv * a.v_sh + s.tok0 * a.v_st;
   const uint8_t* trip = a.tri + ((size_t)s.c0 * a.Hv + s.hv) * kTriBytes;
   const float* scp = a.scal + ((size_t)s.c0 * a.Hv + s.hv) * kScal;
   uint16_t* op = a.o + (((int64_t)s.b * a.T + s.tok0) * a.Hv + s.hv) * a.Dv;
-  const uint32_t qrow = 2 * ((16 * wave + l.r) * (uint32_t)a.q_st + 8 * q);
+  const uint32_t vrow = 2 * ((16 * wave + 4 * q) * (uint32_t)a.v_st + l.col);
   const uint32_t orow = 2 * ((16 * wave + 4 * q) * (uint32_t)(a.Hv * a.Dv) + l.col);
-  const auto load_rows = [&](int left) {
-    const uint32_t miss = miss_from(16 * wave + l.r, left);
-    const Rsrc qr = buffer_at(qp), sr = buffer_at(scp);
+  const auto half_miss = [&](int ks) { return ks == KS - 1 ? l.last_half : ks == KS - 2 ? l.before_half : 0; };
+  const auto load_k = [&](int left) {
+    const uint32_t miss = miss_from(16 * wave + l.r, left), at = 4 * (16 * wave + 4 * q) | miss_from(0, left);
+    const Rsrc kr = buffer_at(kp), vr_ = buffer_at(vp), sr = buffer_at(scp);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-      qf[ks] = load_frag(qr, (qrow + 64 * ks) | miss | (ks == KS - 1 ? l.last_half : ks == KS - 2 ? l.before_half : 0));
-    gam = load_f4(sr, 4 * (16 * wave + 4 * q) | miss_from(0, left));
-    qp += kC * a.q_st;
+    for (int ks = 0; ks < KS; ++ks) kf[ks] = load_frag(kr, krow | miss | half_miss(ks), along * ks);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      vr[i].load(vr_, (vrow + 2 * i * (uint32_t)a.v_st) | l.dead | miss_from(16 * wave + 4 * q + i, left));
+    gam = load_f4(sr, at);
+    bt = load_f4(sr, at, 8 * kC);
+    kp += k_step;
+    vp += kC * a.v_st;
     scp += a.Hv * kScal;
+  };
+  const auto load_q = [&](int left) {
+    const uint32_t miss = miss_from(16 * wave + l.r, left);
+    const Rsrc qr = buffer_at(qp);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = load_frag(qr, qrow | miss | half_miss(ks), along * ks);
+    qp += q_step;
   };
   const auto load_p = [&](int left) {
     const Rsrc tr = buffer_at(trip);
@@ -291,12 +288,36 @@ __device__ __forceinline__ void scan_outputs(const Args& a, const Scan& s, const
     trip += (size_t)a.Hv * kTriBytes;
   };
   if (s.len > 0) {
-    load_rows(s.len);
+    load_k(s.len);
+    load_q(s.len);
     load_p(s.len);
     settle();
   }
   for (int left = s.len; left > 0; left -= kC) {
     lds_barrier();   // S0 is in LDS
+    {
+      f32x4 X[NT] = {}, X2[NT] = {};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          X[n] = mfma(kf[ks], get(lds.S[0], ks * NT + n), X[n]);
+          X2[n] = mfma(kf[ks], get(lds.S[1], ks * NT + n), X2[n]);
+        }
+      // rows behind the sequence's end have b = 0 and V = 0
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        f32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = vr[i].get(n);
+        const Parts p = parts_of(bt * (v - gam * (X[n] + X2[n])));
+        *reinterpret_cast<u32x2*>(lds.R[0] + put_tok + n * 1024) = p.hi;
+        *reinterpret_cast<u32x2*>(lds.R[1] + put_tok + n * 1024) = p.lo;
+      }
+    }
+    const f32x4 sgam = gam * a.scale;
+    lds_barrier();   // R is in LDS
+    load_k(left - kC);
     f32x4 O[NT] = {}, O2[NT] = {};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
@@ -307,12 +328,10 @@ __device__ __forceinline__ void scan_outputs(const Args& a, const Scan& s, const
       }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      O[n] = (O[n] + O2[n]) * (gam * a.scale);
+      O[n] = (O[n] + O2[n]) * sgam;
       O2[n] = f32x4{};
     }
-    load_rows(left - kC);
-    lds_barrier();   // R is in LDS
-    lds_barrier();   // U is in LDS
+    lds_barrier();   // U is in LDS, and nobody reads S0 any more
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
       if (ks <= wave >> 1)
@@ -323,6 +342,7 @@ __device__ __forceinline__ void scan_outputs(const Args& a, const Scan& s, const
           O2[n] = mfma(pf[ks][1], hi, O2[n]);
           O2[n] = mfma(pf[ks][0], lo, O2[n]);
         }
+    load_q(left - kC);
     load_p(left - kC);
     const Rsrc orsrc = buffer_at(op);
     u32x2 ow[NT];
@@ -345,7 +365,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Args a) {
   const Lane l{wave & 3, lane, r, q, col, miss_from(col, a.Dv), miss_from(32 * (KS - 1) + 8 * q, a.Dk),
                miss_from(32 * (KS - 2) + 8 * q, a.Dk)};
   if (wave < 4) scan_state<KS, NT, SAVE>(a, s, l, lds);
-  else scan_outputs<KS, NT>(a, s, l, lds);
+  else scan_tokens<KS, NT>(a, s, l, lds);
 }
 
 template <int KS, int NT>

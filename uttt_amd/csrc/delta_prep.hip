@@ -138,6 +138,15 @@ __device__ __forceinline__ void write_transposed(const uint16_t* lds, uint8_t* o
   }
 }
 
+// The same of staged rows as they are: 16 tokens by 32 features each.
+template <int KS, int LD>
+__device__ __forceinline__ void write_rows(const uint16_t* lds, uint8_t* out, int first, int step) {
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  for (int f = first; f < 4 * KS; f += step)
+    *reinterpret_cast<uint4*>(out + (size_t)f * 1024 + lane * 16) =
+        *reinterpret_cast<const uint4*>(lds + (16 * (f / KS) + r) * LD + 32 * (f % KS) + 8 * q);
+}
+
 constexpr int kLT = kC + 4;   // fp32 row stride of the 64 x 64 matrices
 
 // hi and lo fragments first, first + step, .. of a triangular matrix (or its
@@ -230,6 +239,8 @@ __global__ __launch_bounds__(256, KS <= 4 ? 4 : 2) void delta_prep_kernel(Args a
     const size_t frag = ((size_t)c * a.Hk + hk) * (4 * KS) * 1024;
     write_transposed<KS, LD>(Kl, a.kt + frag, wave - 1, 3);
     if constexpr (BWD) write_transposed<KS, LD>(Ql, a.qt + frag, wave - 1, 3);
+    if (a.kf) write_rows<KS, LD>(Kl, a.kf + frag, wave - 1, 3);
+    if (a.qf) write_rows<KS, LD>(Ql, a.qf + frag, wave - 1, 3);
   }
   __syncthreads();
   float* Am = reinterpret_cast<float*>(buf);
