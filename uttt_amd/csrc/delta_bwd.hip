@@ -26,8 +26,7 @@ struct ScanBwdLds {
   uint8_t U[2][2 * NT * 1024];    // dU
   uint8_t H[2][2 * NT * 1024];    // s gam dO
   uint8_t E[2][2 * NT * 1024];    // -b gam dR
-  f32x4 Z[4][NT][64];             // P^T dO and dR in fp32, as their waves' lanes hold them
-  f32x4 R[4][NT][64];
+  f32x4 R[4][NT][64];             // dR in fp32, as its waves' lanes hold it
 };
 
 template <int NT>
@@ -35,7 +34,8 @@ __device__ __forceinline__ uint32_t put_at(int wave, int r, int q) {
   return (wave >> 1) * NT * 1024 + (wave & 1) * 512 + (r + 16 * (q >> 1)) * 16 + (q & 1) * 8;
 }
 
-// The state's waves: 16 tokens of dU and dR and a quarter of dS's features each.
+// The state's waves: dR = T^T dU, 16 tokens each, and a quarter of dS's features
+// each.  While the others work on dU they store dS' and add Q^T (s gam dO).
 template <int KS, int NT>
 __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int wave, int lane,
                                                ScanBwdLds<KS, NT>& lds) {
@@ -43,10 +43,6 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
   const int r = lane & 15, q = lane >> 4, col = s.col0 + NT * r;
   const uint32_t dead = miss_from(col, a.Dv), put_tok = put_at<NT>(wave, r, q);
   const uint32_t put = (r + 16 * (q >> 1)) * 16 + (q & 1) * 8;
-  const auto put_tile = [&](uint8_t (*buf)[2 * NT * 1024], int n, const Parts& p) {
-    *reinterpret_cast<u32x2*>(buf[0] + put_tok + n * 1024) = p.hi;
-    *reinterpret_cast<u32x2*>(buf[1] + put_tok + n * 1024) = p.lo;
-  };
   const auto get = [&](const uint8_t* buf, int f) {
     return *reinterpret_cast<const bf16x8*>(buf + f * 1024 + lane * 16);
   };
@@ -63,34 +59,17 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
                          ? a.dhT[((int64_t)s.head * a.Dk + feat) * a.Dv + col + n] : 0.0f;
     }
 
-  bf16x8 kf[KS], tf[2][2], ktf[FT][2], qtf[FT][2];
-  f32x4 ge, bg;
+  bf16x8 qtf[FT][2], tf[2][2], ktf[FT][2];
+  f32x4 bg;
   float gc;
-  // Operands of the chunk before: pointers that go along, at first those of the last chunk.
+  // Operands of the chunk before: pointers that go along, at first those of the
+  // last chunk.  `left`: tokens from the chunk on to the sequence's end; 0
+  // before its first chunk.
   const int lastc = s.nc - 1;
-  const bool copies = a.kf != nullptr;   // K's fragments in place of its rows
-  const int64_t copy_step = (int64_t)a.Hk * (4 * KS * 1024);
-  const uint8_t* kp = copies ? a.kf + (s.c0 + lastc) * copy_step + s.hk * (4 * KS * 1024)
-                             : reinterpret_cast<const uint8_t*>(a.k + s.b * a.k_sb + s.hk * a.k_sh +
-                                                                (s.tok0 + (int64_t)lastc * kC) * a.k_st);
-  const int64_t k_step = copies ? copy_step : 2 * kC * a.k_st;
   const uint8_t* trip = a.tri + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kTriBytes;
   const int64_t trans_at = ((int64_t)(s.c0 + lastc) * a.Hk + s.hk) * (4 * KS * 1024);
   const uint8_t *ktp = a.kt + trans_at, *qtp = a.qt + trans_at;
   const float* scp = a.scal + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kScal;
-  const uint32_t krow = copies ? wave * KS * 1024 + lane * 16 : 2 * ((16 * wave + r) * (uint32_t)a.k_st + 8 * q);
-  const uint32_t along = copies ? 1024 : 64;
-  const uint32_t last_half = miss_from(32 * (KS - 1) + 8 * q, a.Dk), before_half = miss_from(32 * (KS - 2) + 8 * q, a.Dk);
-  // `left`: tokens from the chunk on to the sequence's end; 0 before its first chunk
-  const auto load_k = [&](int left) {
-    const uint32_t miss = miss_from(16 * wave + r, left);
-    const Rsrc kr = buffer_at(kp);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-      kf[ks] = load_frag(kr, krow | miss | (ks == KS - 1 ? last_half : ks == KS - 2 ? before_half : 0), along * ks);
-    ge = load_f4(buffer_at(scp), 4 * (16 * wave + 4 * q) | miss_from(0, left), 4 * kC);
-    kp -= k_step;
-  };
   const auto load_t = [&](int left) {
     const Rsrc tr = buffer_at(trip), sr = buffer_at(scp);
     const uint32_t at = lane * 16 | miss_from(0, left), s_at = 4 * (16 * wave + 4 * q) | miss_from(0, left);
@@ -102,7 +81,6 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
       tf[ks][1] = load_frag(tr, at, (kTFrags + f) * 1024);
     }
     bg = load_f4(sr, s_at) * load_f4(sr, s_at, 8 * kC);
-    gc = load_f1(sr, 4 * (kC - 1) | miss_from(0, left));
     scp -= a.Hv * kScal;
     trip -= (int64_t)a.Hv * kTriBytes;
   };
@@ -116,39 +94,53 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
         if (wave * FT + f < 2 * KS) x[f][t] = load_frag(tr, at, (2 * (wave * FT + f) + t) * 1024);
     p -= (int64_t)a.Hk * (4 * KS * 1024);
   };
-  // dS' to LDS and memory
+  const auto load_qt = [&](int left) {
+    gc = load_f1(buffer_at(scp), 4 * (kC - 1) | miss_from(0, left));
+    load_trans(left, qtp, qtf);
+  };
+  // dS' to LDS, and from its parts to memory
   uint16_t* dsp = a.ds + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * 2 * a.Dk * a.Dv;
+  Parts sw[FT][NT];
   const auto put_state = [&]() {
-    const Rsrc sr = buffer_at(dsp);
 #pragma unroll
     for (int f = 0; f < FT; ++f) {
       const int tile = wave * FT + f;
-      if (tile < 2 * KS) {
+      if (tile < 2 * KS)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          sw[f][n] = parts_of(S[f][n]);
+          const uint32_t at = ((tile >> 1) * NT + n) * 1024 + (tile & 1) * 512 + put;
+          *reinterpret_cast<u32x2*>(lds.S[0] + at) = sw[f][n].hi;
+          *reinterpret_cast<u32x2*>(lds.S[1] + at) = sw[f][n].lo;
+        }
+    }
+  };
+  const auto save_state = [&]() {
+    const Rsrc sr = buffer_at(dsp);
+#pragma unroll
+    for (int f = 0; f < FT; ++f)
+      if (wave * FT + f < 2 * KS) {
         u32x2 hi[NT], lo[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const Parts p = parts_of(S[f][n]);
-          const uint32_t at = ((tile >> 1) * NT + n) * 1024 + (tile & 1) * 512 + put;
-          *reinterpret_cast<u32x2*>(lds.S[0] + at) = hi[n] = p.hi;
-          *reinterpret_cast<u32x2*>(lds.S[1] + at) = lo[n] = p.lo;
+          hi[n] = sw[f][n].hi;
+          lo[n] = sw[f][n].lo;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int feat = 16 * tile + 4 * q + i;
+          const int feat = 16 * (wave * FT + f) + 4 * q + i;
           const uint32_t at = 2 * (feat * a.Dv + col) | dead | miss_from(feat, a.Dk);
           store_row<NT>(sr, at, hi, i);
           store_row<NT>(sr, at, lo, i, 2 * (uint32_t)(a.Dk * a.Dv));
         }
       }
-    }
     dsp -= (int64_t)a.Hv * 2 * a.Dk * a.Dv;
   };
 
   const int first_left = s.len - lastc * kC;
   if (lastc >= 0) {
-    load_k(first_left);
+    load_qt(first_left);
     load_t(first_left);
-    load_trans(first_left, qtp, qtf);
     load_trans(first_left, ktp, ktf);
     put_state();
     settle();
@@ -156,21 +148,26 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
   }
   for (int c = lastc; c >= 0; --c) {
     const int next = c > 0 ? kC : 0;
-    lds_barrier();   // dS', P^T dO and s gam dO are in LDS
-    // dU = e^{G_C - G} K dS' + P^T dO
-    {
-      f32x4 X[NT] = {}, X2[NT] = {};
+    lds_barrier();   // dS' and s gam dO are in LDS
+    save_state();
+    // dS0 = gam_C dS' + Q^T (s gam dO) - K^T (b gam dR): the first product here
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+    for (int f = 0; f < FT; ++f)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          X[n] = mfma(kf[ks], get(lds.S[0], ks * NT + n), X[n]);
-          X2[n] = mfma(kf[ks], get(lds.S[1], ks * NT + n), X2[n]);
-        }
+      for (int n = 0; n < NT; ++n) S[f][n] *= gc;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) put_tile(lds.U, n, parts_of(ge * (X[n] + X2[n]) + lds.Z[wave][n][lane]));
-    }
-    load_k(next);
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const bf16x8 hi = get(lds.H[0], t * NT + n), lo = get(lds.H[1], t * NT + n);
+#pragma unroll
+        for (int f = 0; f < FT; ++f)
+          if (wave * FT + f < 2 * KS) {
+            S[f][n] = mfma(qtf[f][t], hi, S[f][n]);
+            S[f][n] = mfma(qtf[f][t], lo, S[f][n]);
+          }
+      }
+    load_qt(next);
     lds_barrier();   // dU is in LDS
     f32x4 R[NT] = {};   // dR = T^T dU
     {
@@ -190,28 +187,12 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      put_tile(lds.E, n, parts_of(-bg * R[n]));
+      const Parts p = parts_of(-bg * R[n]);
+      *reinterpret_cast<u32x2*>(lds.E[0] + put_tok + n * 1024) = p.hi;
+      *reinterpret_cast<u32x2*>(lds.E[1] + put_tok + n * 1024) = p.lo;
       lds.R[wave][n][lane] = R[n];
     }
-    // dS0 = gam_C dS' + Q^T (s gam dO) - K^T (b gam dR): the first product here
-#pragma unroll
-    for (int f = 0; f < FT; ++f)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) S[f][n] *= gc;
     load_t(next);
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const bf16x8 hi = get(lds.H[0], t * NT + n), lo = get(lds.H[1], t * NT + n);
-#pragma unroll
-        for (int f = 0; f < FT; ++f)
-          if (wave * FT + f < 2 * KS) {
-            S[f][n] = mfma(qtf[f][t], hi, S[f][n]);
-            S[f][n] = mfma(qtf[f][t], lo, S[f][n]);
-          }
-      }
-    load_trans(next, qtp, qtf);
     lds_barrier();   // b gam dR is in LDS
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -225,8 +206,8 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
             S[f][n] = mfma(ktf[f][t], lo, S[f][n]);
           }
       }
-    load_trans(next, ktp, ktf);
     if (c > 0) put_state();
+    load_trans(next, ktp, ktf);
   }
   if (a.dh0 && col < a.Dv) {
 #pragma unroll
@@ -241,25 +222,46 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
   }
 }
 
-// The other waves: 16 tokens each of P^T dO and s gam dO, a chunk before the
-// state's waves need them, and of dR and dV on their way to memory.
+// The tokens' waves, 16 tokens each: dU = e^{G_C - G} K dS' + P^T dO, its second
+// term and s gam dO a chunk before they are needed, and dR and dV on their way
+// to memory.
 template <int KS, int NT>
 __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, int wave, int lane,
                                                 ScanBwdLds<KS, NT>& lds) {
   const int r = lane & 15, q = lane >> 4, col = s.col0 + NT * r;
   const uint32_t dead = miss_from(col, a.Dv), put_tok = put_at<NT>(wave, r, q);
-  bf16x8 pf[2][2];
-  f32x4 gam, bt;
+  bf16x8 kf[KS], pf[2][2];
+  f32x4 ge, gam, bt;
   Cols<NT> gr[4];
   const int lastc = s.nc - 1;
+  // K: rows of the caller's tensor, or their fragments
+  const bool copies = a.kf != nullptr;
+  const int64_t copy_step = (int64_t)a.Hk * (4 * KS * 1024);
+  const uint8_t* kp = copies ? a.kf + (s.c0 + lastc) * copy_step + s.hk * (4 * KS * 1024)
+                             : reinterpret_cast<const uint8_t*>(a.k + s.b * a.k_sb + s.hk * a.k_sh +
+                                                                (s.tok0 + (int64_t)lastc * kC) * a.k_st);
+  const int64_t k_step = copies ? copy_step : 2 * kC * a.k_st;
+  const uint32_t krow = copies ? wave * KS * 1024 + lane * 16 : 2 * ((16 * wave + r) * (uint32_t)a.k_st + 8 * q);
+  const uint32_t along = copies ? 1024 : 64;
+  const uint32_t last_half = miss_from(32 * (KS - 1) + 8 * q, a.Dk), before_half = miss_from(32 * (KS - 2) + 8 * q, a.Dk);
   const uint16_t* gp = a.dout + s.b * a.do_sb + s.hv * a.do_sh + (s.tok0 + (int64_t)lastc * kC) * a.do_st;
   const uint8_t* trip = a.tri + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kTriBytes;
   const float* gamp = a.scal + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kScal;   // goes with dO
-  const float* betap = gamp;                                                      // with dR
+  const float *betap = gamp, *gep = gamp;                                         // with dR, with K
   const uint32_t grow = 2 * ((16 * wave + 4 * q) * (uint32_t)a.do_st + col);
   const uint32_t orow = 2 * ((16 * wave + 4 * q) * (uint32_t)(a.Hv * a.Dv) + col);
   int64_t out_at = (((int64_t)s.b * a.T + s.tok0 + (int64_t)lastc * kC) * a.Hv + s.hv) * a.Dv;
   const int64_t plane = (int64_t)a.B * a.T * a.Hv * a.Dv;
+  const auto load_k = [&](int left) {
+    const uint32_t miss = miss_from(16 * wave + r, left);
+    const Rsrc kr = buffer_at(kp);
+    ge = load_f4(buffer_at(gep), 4 * (16 * wave + 4 * q) | miss_from(0, left), 4 * kC);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      kf[ks] = load_frag(kr, krow | miss | (ks == KS - 1 ? last_half : ks == KS - 2 ? before_half : 0), along * ks);
+    gep -= a.Hv * kScal;
+    kp -= k_step;
+  };
   const auto load_do = [&](int left) {
     const Rsrc gr_ = buffer_at(gp);
 #pragma unroll
@@ -284,6 +286,9 @@ __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, in
     bt = load_f4(buffer_at(betap), 4 * (16 * wave + 4 * q) | miss_from(0, left), 8 * kC);
     betap -= a.Hv * kScal;
   };
+  const auto get = [&](const uint8_t* buf, int f) {
+    return *reinterpret_cast<const bf16x8*>(buf + f * 1024 + lane * 16);
+  };
   const auto put_do = [&]() {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -291,8 +296,11 @@ __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, in
       *reinterpret_cast<u32x2*>(lds.G + put_tok + n * 1024) = g;
     }
   };
-  const auto put_z = [&]() {
-    f32x4 Z[NT] = {}, Z2[NT] = {};
+  f32x4 Z[NT];   // P^T dO
+  const auto make_z = [&]() {
+    f32x4 Z2[NT] = {};
+#pragma unroll
+    for (int n = 0; n < NT; ++n) Z[n] = f32x4{};
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
       if (ks >= wave >> 1)
@@ -303,7 +311,7 @@ __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, in
           Z2[n] = mfma(pf[ks][1], g, Z2[n]);
         }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) lds.Z[wave][n][lane] = Z[n] + Z2[n];
+    for (int n = 0; n < NT; ++n) Z[n] += Z2[n];
   };
   const auto put_h = [&]() {
 #pragma unroll
@@ -317,16 +325,17 @@ __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, in
     }
   };
 
-  // beta is a chunk behind dO and P: it is of the chunk whose dR comes out
+  // dO and P are a chunk ahead of K and beta
   const int first_left = s.len - lastc * kC;
   if (lastc >= 0) {
     load_do(first_left);
     load_p(first_left);
+    load_k(first_left);
     load_beta(first_left);
     settle();
     put_do();
     lds_barrier();   // dO is in LDS
-    put_z();
+    make_z();
     put_h();
     const int next = lastc > 0 ? kC : 0;
     load_do(next);
@@ -334,15 +343,32 @@ __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, in
     settle();
   }
   for (int c = lastc; c >= 0; --c) {
-    const int left = s.len - c * kC, later = c > 1 ? kC : 0;
-    lds_barrier();   // dS', P^T dO and s gam dO are in LDS
-    put_do();        // of the chunk before, as all that follows
-    lds_barrier();   // dU is in LDS, P^T dO read
-    put_z();
-    load_p(later);
-    lds_barrier();   // b gam dR is in LDS, s gam dO read
+    const int left = s.len - c * kC, next = c > 0 ? kC : 0, later = c > 1 ? kC : 0;
+    lds_barrier();   // dS' and s gam dO are in LDS
+    {
+      f32x4 X[NT] = {}, X2[NT] = {};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          X[n] = mfma(kf[ks], get(lds.S[0], ks * NT + n), X[n]);
+          X2[n] = mfma(kf[ks], get(lds.S[1], ks * NT + n), X2[n]);
+        }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const Parts p = parts_of(ge * (X[n] + X2[n]) + Z[n]);
+        *reinterpret_cast<u32x2*>(lds.U[0] + put_tok + n * 1024) = p.hi;
+        *reinterpret_cast<u32x2*>(lds.U[1] + put_tok + n * 1024) = p.lo;
+      }
+    }
+    put_do();        // of the chunk before
+    lds_barrier();   // dU and dO are in LDS, s gam dO read
+    load_k(next);
+    make_z();
     put_h();
+    load_p(later);
     load_do(later);
+    lds_barrier();   // dR is in LDS
     {
       const Rsrc vr = buffer_at(a.dv + out_at), hr = buffer_at(a.dr + out_at), lr = buffer_at(a.dr + plane + out_at);
       u32x2 v[NT], hi[NT], lo[NT];
@@ -354,6 +380,7 @@ __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, in
         lo[n] = p.lo;
         v[n] = round_of(bt * R);
       }
+      load_beta(next);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t at = (orow + 2 * i * (uint32_t)(a.Hv * a.Dv)) | dead | miss_from(16 * wave + 4 * q + i, left);
@@ -363,7 +390,6 @@ __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, in
       }
       out_at -= (int64_t)kC * a.Hv * a.Dv;
     }
-    load_beta(c > 0 ? kC : 0);
   }
 }
 
