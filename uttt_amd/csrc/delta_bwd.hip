@@ -98,9 +98,8 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
     gc = load_f1(buffer_at(scp), 4 * (kC - 1) | miss_from(0, left));
     load_trans(left, qtp, qtf);
   };
-  // dS' to LDS, and from its parts to memory
+  // dS' to LDS, and its lane's part from there to memory
   uint16_t* dsp = a.ds + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * 2 * a.Dk * a.Dv;
-  Parts sw[FT][NT];
   const auto put_state = [&]() {
 #pragma unroll
     for (int f = 0; f < FT; ++f) {
@@ -108,32 +107,35 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
       if (tile < 2 * KS)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          sw[f][n] = parts_of(S[f][n]);
+          const Parts p = parts_of(S[f][n]);
           const uint32_t at = ((tile >> 1) * NT + n) * 1024 + (tile & 1) * 512 + put;
-          *reinterpret_cast<u32x2*>(lds.S[0] + at) = sw[f][n].hi;
-          *reinterpret_cast<u32x2*>(lds.S[1] + at) = sw[f][n].lo;
+          *reinterpret_cast<u32x2*>(lds.S[0] + at) = p.hi;
+          *reinterpret_cast<u32x2*>(lds.S[1] + at) = p.lo;
         }
     }
   };
   const auto save_state = [&]() {
     const Rsrc sr = buffer_at(dsp);
 #pragma unroll
-    for (int f = 0; f < FT; ++f)
-      if (wave * FT + f < 2 * KS) {
+    for (int f = 0; f < FT; ++f) {
+      const int tile = wave * FT + f;
+      if (tile < 2 * KS) {
         u32x2 hi[NT], lo[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          hi[n] = sw[f][n].hi;
-          lo[n] = sw[f][n].lo;
+          const uint32_t at = ((tile >> 1) * NT + n) * 1024 + (tile & 1) * 512 + put;
+          hi[n] = *reinterpret_cast<const u32x2*>(lds.S[0] + at);
+          lo[n] = *reinterpret_cast<const u32x2*>(lds.S[1] + at);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int feat = 16 * (wave * FT + f) + 4 * q + i;
+          const int feat = 16 * tile + 4 * q + i;
           const uint32_t at = 2 * (feat * a.Dv + col) | dead | miss_from(feat, a.Dk);
           store_row<NT>(sr, at, hi, i);
           store_row<NT>(sr, at, lo, i, 2 * (uint32_t)(a.Dk * a.Dv));
         }
       }
+    }
     dsp -= (int64_t)a.Hv * 2 * a.Dk * a.Dv;
   };
 

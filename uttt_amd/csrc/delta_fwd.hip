@@ -70,7 +70,10 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
                          ? a.h0[((int64_t)s.head * a.Dk + feat) * a.Dv + col + n] : 0.0f;
     }
 
-  // Operands of this chunk, and of the next on their way.
+  // Operands of this chunk, and of the next on their way.  With 64 accumulators
+  // a lane there are no registers for K^T twice: it is then loaded for this
+  // chunk while R is made.
+  constexpr bool kAhead = FT * NT < 16;
   struct Ops {
     bf16x8 t[2][2], kt[FT][2];
     f32x4 ge;
@@ -82,7 +85,7 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
   const float* scp = a.scal + ((size_t)s.c0 * a.Hv + s.hv) * kScal;
   const auto load = [&](int left, Ops& o) {
     const uint32_t none = miss_from(0, left), at = l.lane * 16 | none;
-    const Rsrc tr = buffer_at(trip), kr = buffer_at(ktp), sr = buffer_at(scp);
+    const Rsrc tr = buffer_at(trip), sr = buffer_at(scp);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       // step 1 of the upper tiles is zero and not stored: step 0 again, unused
@@ -92,16 +95,19 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
     }
     o.ge = load_f4(sr, 4 * (16 * wave + 4 * q) | none, 4 * kC);
     o.gc = load_f1(sr, 4 * (kC - 1) | none);
+    trip += (size_t)a.Hv * kTriBytes;
+    scp += a.Hv * kScal;
+  };
+  const auto load_kt = [&](int left, Ops& o) {
+    const uint32_t at = l.lane * 16 | miss_from(0, left);
+    const Rsrc kr = buffer_at(ktp);
 #pragma unroll
     for (int f = 0; f < FT; ++f)
 #pragma unroll
       for (int t = 0; t < 2; ++t)
         if (wave * FT + f < 2 * KS) o.kt[f][t] = load_frag(kr, at, (2 * (wave * FT + f) + t) * 1024);
-    trip += (size_t)a.Hv * kTriBytes;
     ktp += (size_t)a.Hk * (4 * KS * 1024);
-    scp += a.Hv * kScal;
   };
-  Parts sw[FT][NT];   // the state's parts
   const auto put_state = [&]() {
 #pragma unroll
     for (int f = 0; f < FT; ++f) {
@@ -109,10 +115,10 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
       if (tile < 2 * KS)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          sw[f][n] = parts_of(S[f][n]);
+          const Parts p = parts_of(S[f][n]);
           const uint32_t at = ((tile >> 1) * NT + n) * 1024 + (tile & 1) * 512 + put;
-          *reinterpret_cast<u32x2*>(lds.S[0] + at) = sw[f][n].hi;
-          *reinterpret_cast<u32x2*>(lds.S[1] + at) = sw[f][n].lo;
+          *reinterpret_cast<u32x2*>(lds.S[0] + at) = p.hi;
+          *reinterpret_cast<u32x2*>(lds.S[1] + at) = p.lo;
         }
     }
   };
@@ -120,22 +126,25 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
   const auto save_state = [&]() {
     const Rsrc sr = buffer_at(s0p);
 #pragma unroll
-    for (int f = 0; f < FT; ++f)
-      if (wave * FT + f < 2 * KS) {
+    for (int f = 0; f < FT; ++f) {
+      const int tile = wave * FT + f;
+      if (tile < 2 * KS) {
         u32x2 hi[NT], lo[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          hi[n] = sw[f][n].hi;
-          lo[n] = sw[f][n].lo;
+          const uint32_t at = ((tile >> 1) * NT + n) * 1024 + (tile & 1) * 512 + put;
+          hi[n] = *reinterpret_cast<const u32x2*>(lds.S[0] + at);
+          lo[n] = *reinterpret_cast<const u32x2*>(lds.S[1] + at);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int feat = 16 * (wave * FT + f) + 4 * q + i;
+          const int feat = 16 * tile + 4 * q + i;
           const uint32_t at = 2 * (feat * a.Dv + col) | dead | miss_from(feat, a.Dk);
           store_row<NT>(sr, at, hi, i);
           store_row<NT>(sr, at, lo, i, 2 * (uint32_t)(a.Dk * a.Dv));
         }
       }
+    }
     s0p += (int64_t)a.Hv * 2 * a.Dk * a.Dv;
   };
   uint16_t* up = SAVE ? a.u + (((int64_t)s.b * a.T + s.tok0) * a.Hv + s.hv) * a.Dv : nullptr;
@@ -155,13 +164,16 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
 
   if (s.len > 0) {
     load(s.len, coming);
+    if constexpr (kAhead) load_kt(s.len, coming);
     put_state();
     settle();
   }
   for (int left = s.len; left > 0; left -= kC) {
     lds_barrier();   // S0 is in LDS
     now = coming;
+    if constexpr (!kAhead) load_kt(left, now);
     load(left - kC, coming);
+    if constexpr (kAhead) load_kt(left - kC, coming);
     if constexpr (SAVE) save_state();
     lds_barrier();   // R is in LDS
     f32x4 U[NT] = {};
