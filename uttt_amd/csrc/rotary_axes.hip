@@ -6,7 +6,11 @@
 //
 // Bound by memory: one read and one write of x.  A token's R cosines and sines
 // are computed once, in LDS, for all its heads; the angle in turns is reduced
-// in 64 bits, so that positions of any size keep fp32's precision.
+// in 64 bits, so that positions of any size keep fp32's precision.  A thread's
+// first piece of x is on its way while the angles are computed, and each next
+// one while the last is turned: 3 x 8191 tokens of 12 heads of 128 bf16
+// features 36 us, 4.2 TB/s (without this, and with 8-byte pieces where pairs
+// are side by side, 48).
 #include "common.h"
 
 namespace uttt {
@@ -15,6 +19,7 @@ namespace {
 constexpr int kRotThreads = 256;
 constexpr int kMaxAxes = 8;
 constexpr int kRotPairs = 2048;   // cosines and sines of a workgroup's tokens, 16 KiB
+constexpr int kRotTokens = 256;   // tokens of a workgroup at most
 
 struct RotArgs {
   const void* x;
@@ -51,14 +56,44 @@ template <class TT, int V, bool INTER>
 __global__ __launch_bounds__(kRotThreads) void rotary_axes_kernel(RotArgs a) {
   using S = typename TT::S;
   __shared__ float cs[kRotPairs], sn[kRotPairs];
+  __shared__ int64_t xat[kRotTokens], pat[kRotTokens];   // tokens' places in x and in the positions
   const int64_t first = (int64_t)blockIdx.x * a.tokens, all = (int64_t)a.B * a.L;
   const int nt = (int)min((int64_t)a.tokens, all - first);
+  for (int t = threadIdx.x; t < nt; t += kRotThreads) {
+    const uint32_t b = (uint32_t)(first + t) / (uint32_t)a.L, l = (uint32_t)(first + t) - b * (uint32_t)a.L;
+    xat[t] = b * a.x_sb + l * a.x_sl;
+    pat[t] = b * a.p_sb + l * a.p_sl;
+  }
+  __syncthreads();
+  // A piece is 2V features of a token's head: V pairs, or after the pairs
+  // features that pass through (turned by 0).  The next of a thread is
+  // kRotThreads further on, by sums and carries, and is loaded a piece ahead.
+  const int rp = a.R / V, per = (a.D + 2 * V - 1) / (2 * V);
+  const int dth = kRotThreads / per, de = kRotThreads - dth * per, dt = dth / a.H, dh = dth - dt * a.H;
+  struct Piece {
+    int t, h, e;
+    float u[V], w[V];
+  };
+  // first features of a piece's two halves, and whether it has the second
+  const auto at_u = [&](int e) { return INTER ? 2 * V * e : e < rp ? V * e : 2 * V * e; };
+  const auto at_w = [&](int e) { return INTER ? 2 * V * e + V : e < rp ? a.R + V * e : 2 * V * e + V; };
+  const auto load = [&](Piece& p) {
+    if (p.t >= nt) return;
+    const S* x = static_cast<const S*>(a.x) + xat[p.t] + p.h * a.x_sh;
+    Vec<TT, V>::load(x + at_u(p.e), p.u);
+    if (at_w(p.e) < a.D) Vec<TT, V>::load(x + at_w(p.e), p.w);
+  };
+  Piece next;
+  const int th = threadIdx.x / per;
+  next.e = threadIdx.x - th * per;
+  next.t = th / a.H;
+  next.h = th - next.t * a.H;
+  load(next);
   for (int i = threadIdx.x; i < nt * a.R; i += kRotThreads) {
     const int t = i / a.R, j = i - t * a.R;
     int axis = 0;
     while (j >= a.ends[axis]) ++axis;
-    const int64_t b = (first + t) / a.L, l = (first + t) - b * a.L;
-    const int64_t at = b * a.p_sb + l * a.p_sl + axis * a.p_sa;
+    const int64_t at = pat[t] + axis * a.p_sa;
     const double p = a.pos64 ? (double)static_cast<const int64_t*>(a.pos)[at]
                              : (double)static_cast<const int32_t*>(a.pos)[at];
     double half = p * (double)a.freq[j] * 0.31830988618379067154;   // angle / pi
@@ -69,49 +104,34 @@ __global__ __launch_bounds__(kRotThreads) void rotary_axes_kernel(RotArgs a) {
     sn[i] = a.sign * s;
   }
   __syncthreads();
-  // rotated pieces, V pairs each, then the features that pass through
-  const int rp = a.R / V, rest = (a.D - 2 * a.R) / V, per = rp + rest;
-  const int n = nt * a.H * per;
-  for (int i = threadIdx.x; i < n; i += kRotThreads) {
-    const int th = i / per, e = i - th * per, t = th / a.H, h = th - t * a.H;
-    const int64_t b = (first + t) / a.L, l = (first + t) - b * a.L;
-    const S* x = static_cast<const S*>(a.x) + b * a.x_sb + l * a.x_sl + h * a.x_sh;
-    S* y = static_cast<S*>(a.y) + ((first + t) * a.H + h) * a.D;
-    float u[V], w[V], c[V], s[V];
-    if (e >= rp) {
-      const int f = 2 * a.R + (e - rp) * V;
-      Vec<TT, V>::load(x + f, u);
-      Vec<TT, V>::store(y + f, u);
-      continue;
-    }
-    const int j = e * V;
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      c[k] = cs[t * a.R + j + k];
-      s[k] = sn[t * a.R + j + k];
-    }
-    if constexpr (INTER) {
-      float p[2 * V];
-      Vec<TT, 2 * V>::load(x + 2 * j, p);
+  while (next.t < nt) {
+    Piece p = next;
+    next.e += de;
+    next.h += dh;
+    next.t += dt;
+    if (next.e >= per) next.e -= per, ++next.h;
+    if (next.h >= a.H) next.h -= a.H, ++next.t;
+    load(next);
+    if (p.e < rp) {
+      const float *c = cs + p.t * a.R + V * p.e, *s = sn + p.t * a.R + V * p.e;
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const float m = p[2 * k], o = p[2 * k + 1];
-        p[2 * k] = m * c[k] - o * s[k];
-        p[2 * k + 1] = m * s[k] + o * c[k];
+        if constexpr (INTER) {   // pairs 0 .. V/2-1 of the piece in u, the others in w
+          float& m = 2 * k < V ? p.u[2 * k] : p.w[2 * k - V];
+          float& o = 2 * k + 1 < V ? p.u[2 * k + 1] : p.w[2 * k + 1 - V];
+          const float x = m, y = o;
+          m = x * c[k] - y * s[k];
+          o = x * s[k] + y * c[k];
+        } else {
+          const float x = p.u[k], y = p.w[k];
+          p.u[k] = x * c[k] - y * s[k];
+          p.w[k] = x * s[k] + y * c[k];
+        }
       }
-      Vec<TT, 2 * V>::store(y + 2 * j, p);
-    } else {
-      Vec<TT, V>::load(x + j, u);
-      Vec<TT, V>::load(x + a.R + j, w);
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float m = u[k], o = w[k];
-        u[k] = m * c[k] - o * s[k];
-        w[k] = m * s[k] + o * c[k];
-      }
-      Vec<TT, V>::store(y + j, u);
-      Vec<TT, V>::store(y + a.R + j, w);
     }
+    S* y = static_cast<S*>(a.y) + ((first + p.t) * a.H + p.h) * a.D;
+    Vec<TT, V>::store(y + at_u(p.e), p.u);
+    if (at_w(p.e) < a.D) Vec<TT, V>::store(y + at_w(p.e), p.w);
   }
 }
 
@@ -125,30 +145,26 @@ void launch_rotary_as(const RotArgs& a, bool inter, hipStream_t st) {
 template <class TT>
 int launch_rotary(RotArgs a, bool inter, hipStream_t st) {
   constexpr int V = 16 / sizeof(typename TT::S);
-  const int size = sizeof(typename TT::S);
-  const auto fits = [&](int v) {   // v pairs at a time, whole aligned pieces throughout
-    const int bytes = v * size > 16 ? 16 : v * size;
-    return a.R % v == 0 && a.D % v == 0 && (a.D * size) % bytes == 0 && (a.x_sb * size) % bytes == 0 &&
+  // v pairs at a time: whole pieces, aligned throughout.  2 x 8191 tokens, 12
+  // heads, read from memory: 16-byte pieces 2.9 TB/s, 8-byte ones (120 features,
+  // 60 pairs) 2.5, single features (100 and 41) 1.7.
+  const auto fits = [&](int v) {
+    const int size = sizeof(typename TT::S), bytes = size * v;
+    return a.R % v == 0 && (a.D * size) % bytes == 0 && (a.x_sb * size) % bytes == 0 &&
            (a.x_sl * size) % bytes == 0 && (a.x_sh * size) % bytes == 0 &&
            (reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y)) % bytes == 0;
   };
   // about four pieces a thread, and cosines that fit
   const int64_t pieces = (int64_t)a.H * a.D / (2 * V);
-  int64_t tokens = pieces ? (4 * kRotThreads) / pieces : 1;
-  tokens = tokens < 1 ? 1 : tokens;
+  int64_t tokens = pieces ? (4 * kRotThreads) / pieces : kRotTokens;
+  tokens = tokens < 1 ? 1 : tokens > kRotTokens ? kRotTokens : tokens;
   if (tokens > kRotPairs / a.R) tokens = kRotPairs / a.R;
   const int64_t all = (int64_t)a.B * a.L;
   if (all / tokens < 1024) tokens = (all + 1023) / 1024 < tokens ? (all + 1023) / 1024 : tokens;
   a.tokens = (int)tokens;
-  if (inter ? a.R % (V / 2) == 0 && fits(V / 2) && a.D % (V / 2) == 0 && a.D * size % 16 == 0 &&
-                  a.x_sb * size % 16 == 0 && a.x_sl * size % 16 == 0 && a.x_sh * size % 16 == 0 &&
-                  (reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y)) % 16 == 0
-            : fits(V)) {
-    if (inter) launch_rotary_as<TT, V / 2>(a, true, st);
-    else launch_rotary_as<TT, V>(a, false, st);
-  } else {
-    launch_rotary_as<TT, 1>(a, inter, st);
-  }
+  if (fits(V)) launch_rotary_as<TT, V>(a, inter, st);
+  else if (fits(V / 2)) launch_rotary_as<TT, V / 2>(a, inter, st);
+  else launch_rotary_as<TT, 1>(a, inter, st);
   return check_launch("rotary_axes");
 }
 
