@@ -97,6 +97,14 @@ def test_many_heads_take_wide_columns(Dk):
     check(*inputs(64, 70, 64, 4, 4, Dk, 40, seed=1), what=Dk)
 
 
+@pytest.mark.parametrize("Dk", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("B,Dv", [(32, 64), (65, 64), (64, 136)])
+def test_column_widths(Dk, B, Dv):
+    """Enough heads for 32 and for 64 columns a workgroup, a last block of which
+    has few; two value heads to a key head."""
+    check(*inputs(B, 70, B, 2, 4, Dk, Dv, seed=Dk + B), what=(Dk, B, Dv))
+
+
 @pytest.mark.parametrize("cu", [[0, 200], [0, 1, 1, 65, 130, 200], [0, 0, 0, 200], [0, 64, 128, 192, 200],
                                 [0, 200, 200], [7, 70, 135], [0, 63], [100, 100], [0, 3, 5, 190]])
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
@@ -490,3 +498,74 @@ def test_backward_in_a_graph():
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b), i
+
+
+def test_packed_without_tokens():
+    """The states pass through, forwards and backwards."""
+    x, do, dht = inputs(1, 0, 3, 1, 2, 64, 64)
+    got = check(x, do, dht, cu=[0, 0, 0, 0])
+    assert torch.equal(got["state"].detach().cpu(), x["h0"]) and torch.equal(got["dh0"].cpu(), dht)
+
+
+def test_step_without_rows_or_tokens():
+    from uttt_amd.delta import gated_delta_step
+    for B, T in ((0, 1), (2, 0)):
+        state = torch.randn(3, 2, 16, 16, device="cuda")
+        before = state.clone()
+        r = lambda *s: torch.randn(*s, device="cuda", dtype=BF16)  # noqa: E731
+        o = gated_delta_step(r(B, T, 1, 16), r(B, T, 1, 16), r(B, T, 2, 16), r(B, T, 2), r(B, T, 2), state)
+        assert o.shape == (B, T, 2, 16) and torch.equal(state, before)
+
+
+def test_tokens_far_apart():
+    """Rows 2^23 elements apart and more: past a chunk's 31-bit offsets."""
+    def far(name, t):
+        if name not in ("q", "k", "v"):
+            return t.cuda()
+        room = torch.zeros(t.shape[1], 2 ** 23 + 8, dtype=t.dtype, device="cuda")
+        view = room[:, :t[0, 0].numel()].view(1, t.shape[1], *t.shape[2:])
+        view.copy_(t)
+        return view.detach()
+
+    check(*inputs(1, 66, 1, 1, 2, 64, 64, seed=3), move=far)
+
+
+def test_offsets_past_32_bits():
+    """q, k, v, outputs and gradients of more than 2^31 elements: the tokens at
+    the end, and at the start, give the bits of calls that have only them."""
+    from uttt_amd.delta import gated_delta_rule
+    T, Hh, D = 2 ** 21 + 192, 16, 64
+    cut = T - 384
+
+    def make(*s):
+        gen = torch.Generator(device="cuda").manual_seed(len(s))
+        return torch.randn(1, T, Hh, *s, device="cuda", dtype=BF16, generator=gen)
+
+    q, k, v, do = make(D), make(D).mul_(0.1), make(D), make(D)
+    g, beta = -make().abs().float().mul_(0.1), torch.sigmoid(make().float())
+    leaf = [t.requires_grad_() for t in (q, k, v, g, beta)]
+    o, S = gated_delta_rule(*leaf, output_final_state=True)
+    grads = torch.autograd.grad(o, leaf, do)
+    with torch.no_grad():
+        start, S1 = gated_delta_rule(*(t[:, :cut] for t in leaf), output_final_state=True)
+        assert torch.equal(start[:, :256], o[:, :256])
+        del start
+    few = [t[:, cut:].detach().clone().requires_grad_() for t in leaf]
+    o2, S2 = gated_delta_rule(*few, initial_state=S1, output_final_state=True)
+    assert torch.equal(o[:, cut:], o2) and torch.equal(S, S2)
+    for n, a, b in zip(("q", "k", "v", "g", "beta"), grads, torch.autograd.grad(o2, few, do[:, cut:])):
+        assert torch.equal(a[:, cut:], b), n
+
+
+def test_step_in_a_slot_past_32_bits():
+    from uttt_amd.delta import gated_delta_step
+    slots = 2 ** 31 // (16 * 128 * 128) + 2
+    state = torch.zeros(slots, 16, 128, 128, device="cuda")
+    r = lambda *s: torch.randn(*s, device="cuda", dtype=BF16)  # noqa: E731
+    x = r(2, 1, 8, 128), r(2, 1, 8, 128).mul_(0.1), r(2, 1, 16, 128), -r(2, 1, 16).abs(), r(2, 1, 16).abs()
+    own = torch.randn(2, 16, 128, 128, device="cuda")
+    state[slots - 1], state[0] = own[0], own[1]
+    o = gated_delta_step(*x, state, state_indices=torch.tensor([slots - 1, 0], device="cuda"))
+    assert torch.equal(o, gated_delta_step(*x, own))
+    assert torch.equal(state[slots - 1], own[0]) and torch.equal(state[0], own[1])
+    assert not state[1:-1].any()

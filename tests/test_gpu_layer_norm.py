@@ -216,3 +216,20 @@ def test_twice_the_same_bits_and_in_a_graph():
         torch.cuda.synchronize()
         for s, t in zip(got, want):
             assert torch.equal(s, t)
+
+
+@pytest.mark.parametrize("N", [1024, 1025])
+def test_offsets_past_32_bits(N):
+    """The last rows of more than 2^31 elements give the bits of a call that has
+    only them."""
+    from uttt_amd.norm import layer_norm
+    rows, few = 2 ** 31 // 1024 + 5, 7
+    x = torch.randn(few, N, device="cuda", dtype=BF16).repeat(rows // few + 1, 1)[:rows].requires_grad_()
+    w = torch.randn(N, device="cuda")
+    y = layer_norm(x, w)
+    dy = torch.randn(few, N, device="cuda", dtype=BF16).repeat(rows // few + 1, 1)[:rows]
+    dx, = torch.autograd.grad(y, x, dy)
+    end = x[-few:].detach().clone().requires_grad_()
+    y2 = layer_norm(end, w)
+    assert torch.equal(y[-few:], y2)
+    assert torch.equal(dx[-few:], torch.autograd.grad(y2, end, dy[-few:])[0])

@@ -149,3 +149,23 @@ def test_empty_and_in_a_graph():
         want = run()
         torch.cuda.synchronize()
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("sections,D", [([20, 20, 20], 120), ([14, 13, 14], 100), ([2, 2], 12), ([5], 11)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_piece_widths(sections, D, interleaved):
+    """Pairs and features that divide into 8-byte pieces, into single ones, and
+    a last piece of half the features."""
+    for dtype in (BF16, F32):
+        check(*make(2, 37, 5, D, sections, dtype), sections, interleaved)
+
+
+def test_offsets_past_32_bits():
+    from uttt_amd.positions import axis_frequencies, rotary_axes
+    L, H, D = 2 ** 21 + 3, 16, 64
+    x = torch.randn(1, L, H, D, device="cuda", dtype=BF16)
+    pos = torch.arange(L, device="cuda")[:, None]
+    freq = axis_frequencies([32], device="cuda")
+    y = rotary_axes(x, pos, freq, [32])
+    assert torch.equal(y[:, -100:], rotary_axes(x[:, -100:], pos[-100:], freq, [32]))
+    assert torch.equal(y[:, :100], rotary_axes(x[:, :100], pos[:100], freq, [32]))

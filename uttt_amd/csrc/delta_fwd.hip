@@ -411,7 +411,7 @@ int check_args(const Args& a, int B, bool packed, const char* what) {
   UTTT_REQUIRE(packed ? B == 1 : a.nseq == B, "%s: %d sequences in a batch of %d", what, a.nseq, B);
   const int64_t slots = chunk_slots(B, a.T, a.nseq, packed);
   UTTT_REQUIRE(slots >= 0 && slots * a.Hv < (1LL << 31) &&
-                   ((int64_t)a.nseq * a.Hv + 8) * ((a.Dv + 63) / 64) < (1LL << 31),
+                   ((int64_t)a.nseq * a.Hv + 8) * ((a.Dv + 15) / 16) < (1LL << 31),
                "%s: too many chunks and heads for one launch", what);
   UTTT_REQUIRE(a.T == 0 || (a.q && a.k && a.v && a.g && a.beta), "%s: null pointer", what);
   UTTT_REQUIRE(aligned16(a.q) && aligned16(a.k) && aligned16(a.v), "%s: q, k and v must be 16-byte aligned",
@@ -473,7 +473,7 @@ extern "C" int uttt_gated_delta_fwd(const void* q, const int64_t* q_strides, con
   UTTT_REQUIRE(out || T == 0, "%s: null output", what);
   UTTT_REQUIRE(aligned16(out) && aligned16(u_saved) && aligned16(s_saved) && aligned16(workspace),
                "%s: tensors must be 16-byte aligned", what);
-  UTTT_REQUIRE((u_saved == nullptr) == (s_saved == nullptr), "%s: save both U and S or neither", what);
+  UTTT_REQUIRE(T == 0 || (u_saved == nullptr) == (s_saved == nullptr), "%s: save both U and S or neither", what);
   const Workspace w = workspace_of(B, T, nseq, Hk, Hv, Dk, Dv, packed, false);
   UTTT_REQUIRE(w.total == 0 || (workspace && workspace_bytes >= w.total),
                "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, w.total);

@@ -44,9 +44,10 @@ def _strides(t: Tensor):
 
 
 def _rows16(t: Tensor) -> Tensor:
-    """t itself where its rows can be read 16 bytes at a time, else a copy."""
+    """t itself where its rows can be read 16 bytes at a time and a chunk's by
+    31-bit offsets, else a copy."""
     sb, st, sh, sd = t.stride()
-    return t if sd == 1 and not (sb | st | sh) % 8 and not t.data_ptr() % 16 else t.contiguous()
+    return t if sd == 1 and not (sb | st | sh) % 8 and st < 1 << 23 and not t.data_ptr() % 16 else t.contiguous()
 
 
 _GATE_TYPES = (torch.float32, torch.bfloat16, torch.float16)
