@@ -279,15 +279,20 @@ struct Scan {
 inline unsigned scan_blocks(const Args& a, int width) {
   return (unsigned)(((int64_t)a.nseq * a.Hv + 7) / 8 * 8 * ((a.Dv + width - 1) / width));
 }
-// 16-column tiles of a scan's workgroup.  One workgroup runs on a CU at a
-// time, and its chunk takes about 2.0, 2.3 and 3.0 us for 1, 2 and 4 tiles
-// (128 features): wide ones do more a CU, narrow ones end a long sequence
-// sooner.  What is estimated: rounds of workgroups over the 256 CUs, and of
-// packed sequences, whose lengths the host does not know, the work over the
-// CUs and a longest sequence of three times the mean.  Measured (us for 1, 2,
-// 4): 12 prompts of 1 to 5000 tokens, 16 heads 269, 180, 230; 16 x 2048 tokens,
-// 12 heads, with what a backward reads 631, 420, 353; one of 4096 tokens, 4
-// heads of 192 141, 158, 264.
+// 16-column tiles of a scan's workgroup.  Wide ones do more work a CU, narrow
+// ones end a long sequence sooner.  What is estimated: rounds of workgroups
+// over the 256 CUs, a chunk of them as 2.0, 2.3 and 3.0 us for 1, 2 and 4 tiles
+// (what a busy card takes at 128 features), and of packed sequences, whose
+// lengths the host does not know, the work over the CUs and a longest sequence
+// of three times the mean.  Measured, forward scans, us for 1, 2, 4 tiles:
+//   4096 tokens, 4 heads of 192                         85, 135, 301
+//   8192 tokens, 16 heads of 128                       159, 210, 312
+//   4 x 4096 tokens, 16 heads of 128                   229, 164, 189
+//   12 prompts of 1 to 5000 tokens, 16 heads of 128    230, 169, 212
+// and with what a backward reads
+//   8 x 1024 tokens, 4 heads of 192                     81,  61,  97
+//   16 x 2048 tokens, 12 heads of 128                  577, 418, 344
+//   16 x 2048 tokens, 4 heads of 256                   528, 406, 297
 inline int scan_tiles(int64_t T, int nseq, int Hv, int Dv, bool packed) {
   const int tiles[3] = {1, 2, 4}, tenths[3] = {20, 23, 30};
   const int64_t total = T / kC + nseq, mean = (total + nseq - 1) / nseq, cps = (T + kC - 1) / kC;

@@ -13,6 +13,10 @@
 //        + sum_{j < t} (e^{G_C - G} k.(dS' U))_j + gam_C <S0, dS'>
 // a sum without cancelling terms, where differences of running sums of o.do
 // and v.dv would lose a strong decay's small gradient.
+//
+// Measured, 16 x 2048 tokens, 12 heads of 128 by 128: scan 330 us (0.7 GB
+// stored, 0.55 GB loaded: 3.8 TB/s), gradients 562 us (1.8 GB from and to
+// memory, 0.6 GB once more from cache).
 #include "delta.h"
 
 namespace uttt {

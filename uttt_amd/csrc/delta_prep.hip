@@ -2,6 +2,12 @@
 // the chunk table of packed sequences, and per chunk and head the decays, T =
 // (I + A)^-1, P and the transposed keys, laid out as the matrix instruction's
 // operand fragments for the scans that follow.
+//
+// Bound by memory: K and Q read once, 24 KiB of T and P and 256 bytes a feature
+// of K^T (and Q^T, K, Q where asked for) written per chunk and head.  16 x 2048
+// tokens, 12 heads of 128: 119 us forward, 137 backward, 3.9 and 4.1 TB/s.  The
+// backward makes its operands again: kept from the forward they would hold 350
+// MB of that layer to save a tenth of its step.
 #include "delta.h"
 
 namespace uttt {

@@ -4,7 +4,9 @@
 // Both products of a token come from one pass over the state, so it is read
 // once and written once per call whatever the tokens: 8 bytes per element,
 // which is what bounds it.  A workgroup holds a block of one head's columns in
-// registers, a lane four of them (16 bytes) of every (256 / LC)-th row.
+// registers, a lane four of them (16 bytes) of every (256 / LC)-th row.  250
+// rows of 16 heads of 128 x 128: 91 us, 5.7 TB/s; one row of 4 heads of 192 x
+// 192: 5.6 us.
 //
 // Rows whose slot is that of an earlier row are taken up by that row's
 // workgroup, after it and in order, so that a slot named twice is two calls in
@@ -186,8 +188,11 @@ void launch_step_as(const StepArgs& a, hipStream_t st) {
 
 template <class TT>
 int launch_step(const StepArgs& a, hipStream_t st) {
-  // 16 columns a workgroup where 64 leave CUs without one
-  const bool narrow = (int64_t)a.B * a.Hv * ((a.Dv + 63) / 64) < 512;
+  // 16 columns a workgroup, whose rows are only 64 bytes, where 64 columns make
+  // less than 64 workgroups: 32 (16 heads of 128 x 128) 4.4 us against 4.8, 16
+  // (4 of 256 x 256) 4.8 against 6.0; with 64 of them 5.0 against 4.9 and 6.3
+  // against 6.5, with 256 10.0 against 5.9 and 15.0 against 8.8
+  const bool narrow = (int64_t)a.B * a.Hv * ((a.Dv + 63) / 64) < 64;
   if (narrow) {
     if (a.Dk <= 64) launch_step_as<TT, 4, 1>(a, st);
     else if (a.Dk <= 128) launch_step_as<TT, 4, 2>(a, st);

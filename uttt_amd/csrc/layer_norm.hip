@@ -13,6 +13,8 @@
 // be added in a fixed order by a second launch.  Rows too long for registers
 // (over 2048 pieces of 16 bytes, or 8192 elements where no such piece divides
 // them) are read again from cache for each pass, their sums in 64 bits.
+// 65536 rows of 768 bf16: forward 46 us (4.4 TB/s), backward 65 (4.6) and the
+// sum over the workgroups 5.
 #include "common.h"
 
 namespace uttt {
