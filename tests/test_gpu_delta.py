@@ -375,6 +375,12 @@ def test_step(dtype, B, T, Hk, Hv, Dk, Dv):
             assert (o[b] == 0).all()
 
 
+@pytest.mark.parametrize("Dk,Dv", [(40, 64), (100, 132), (128, 128), (256, 68)])
+def test_step_of_many_rows(Dk, Dv):
+    """Enough workgroups for 64 columns each, a last block of which has few."""
+    test_step(BF16, 33, 2, 1, 2, Dk, Dv)
+
+
 @pytest.mark.parametrize("width", [(64, 64), (128, 128)])
 def test_step_rows_of_one_slot_follow_one_another(width):
     from uttt_amd.delta import gated_delta_step
