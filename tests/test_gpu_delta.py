@@ -155,6 +155,17 @@ def test_many_sequences_fill_several_rounds_of_the_table():
     check(x, do, dht, cu, what="many")
 
 
+@pytest.mark.parametrize("n", [255, 256, 257])
+def test_sequences_ranked_by_length(n):
+    """Up to 256 sequences are taken up longest first, each with its own states."""
+    gen = torch.Generator().manual_seed(n)
+    lens = torch.randint(0, 4, (n,), generator=gen)
+    lens[n // 2], lens[n - 1] = 200, 131
+    cu = [0] + lens.cumsum(0).tolist()
+    x, do, dht = inputs(1, cu[-1], n, 1, 2, 16, 24)
+    check(x, do, dht, cu, what=n)
+
+
 def test_decays():
     """No decay, a strong one everywhere, single tokens that forget everything
     (-inf, also twice in a row and first in a chunk), none at all between."""

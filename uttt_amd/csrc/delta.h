@@ -50,7 +50,7 @@ struct Args {
   int cps;                       // chunks per sequence where there is no table
   float scale;
   const int4* table;             // [nchunks] sequence, first token, tokens; packed sequences only
-  const int4* seqs;              // [nseq] first chunk, chunks
+  const int4* seqs;              // [nseq] first chunk, sequence, first token, tokens
   uint8_t* tri;                  // [nchunks, Hv] kTriBytes
   float* scal;                   // [nchunks, Hv, kScal]
   uint8_t* kt;                   // [nchunks, Hk, 4 KS] KiB: K^T fragments
@@ -260,19 +260,21 @@ struct Scan {
   __device__ __forceinline__ bool init(const Args& a, int width) {
     const int ncb = (a.Dv + width - 1) / width;
     const int grp = blockIdx.x / (8 * ncb), in = blockIdx.x % (8 * ncb);
-    head = grp * 8 + (in & 7);
-    if (head >= a.nseq * a.Hv) return false;
+    const int at = grp * 8 + (in & 7);
+    if (at >= a.nseq * a.Hv) return false;
     col0 = (in >> 3) * width;
-    seq = head / a.Hv;
-    hv = head % a.Hv;
+    seq = at / a.Hv;
+    hv = at % a.Hv;
     hk = hv / (a.Hv / a.Hk);
     b = a.table ? 0 : seq;
     if (a.table) {
       const int4 s = a.seqs[seq];
-      c0 = s.x; nc = s.y; tok0 = s.z; len = s.w;
+      c0 = s.x; seq = s.y; tok0 = s.z; len = s.w;
+      nc = (len + kC - 1) / kC;
     } else {
       c0 = seq * a.cps; nc = a.cps; tok0 = 0; len = a.T;
     }
+    head = seq * a.Hv + hv;
     return true;
   }
 };
