@@ -698,7 +698,10 @@ __global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads
       }
     }
     lds_barrier();
-    load_rows(0, 3, 8);
+    load_rows(0, 3, 8);   // for the second pass, as the states
+    bf16x8 dh, dl;
+    load_state(sp, 0, sh, sl);
+    load_state(dp, 0, dh, dl);
     // dQ += D K, dK += D^T Q + (M + M^T) K
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
@@ -716,9 +719,6 @@ __global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads
     // the second pass: U dS'^T and <S0, dS'>
     f32x4 EU[4] = {}, dot = {};
     {
-      bf16x8 dh, dl;
-      load_state(sp, 0, sh, sl);
-      load_state(dp, 0, dh, dl);
       int half = 0;
       for (int e0 = 0; e0 < a.Dv; e0 += 32, half ^= 1) {
         uint8_t* stage = buf + half * 8 * 1024;

@@ -27,7 +27,7 @@ import torch
 from torch import Tensor
 
 from . import _lib as L
-from ._ops import run_function, traced_op
+from ._ops import new_like, run_function, traced_op
 
 MAX_KEY_DIM = 256
 
@@ -98,7 +98,7 @@ def _state_like(v, q, cu_seqlens, wanted):
 
 
 def _infer_fake(q, k, v, g, beta, initial_state, cu_seqlens, scale, want_state):
-    return (torch.empty(v.shape, dtype=v.dtype, device=v.device),
+    return (new_like(v),
             _state_like(v, q, cu_seqlens, want_state))
 
 
@@ -136,8 +136,7 @@ def _bwd_fake(q, k, v, g, beta, cu_seqlens, scale, u, s0, do, dstate, want_dh0):
     B, T, Hk, Dk = q.shape
     Hv, Dv = v.shape[2:]
     dh0 = v.new_empty((_seqs(q, cu_seqlens), Hv, Dk, Dv) if want_dh0 else (0,), dtype=torch.float32)
-    return [q.new_empty(q.shape), q.new_empty(q.shape), v.new_empty(v.shape), g.new_empty(g.shape),
-            beta.new_empty(beta.shape), dh0]
+    return [new_like(q), new_like(q), new_like(v), new_like(g), new_like(beta), dh0]
 
 
 @traced_op("gated_delta_bwd", _bwd_fake)
@@ -238,7 +237,7 @@ def gated_delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, *
 
 
 def _step_fake(q, k, v, g, beta, state, scale, state_indices):
-    return torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    return new_like(v)
 
 
 @traced_op("gated_delta_step", _step_fake, mutates_args=("state",))

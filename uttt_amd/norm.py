@@ -9,7 +9,7 @@ import torch
 from torch import Tensor
 
 from . import _lib as L
-from ._ops import none_if_empty, run_function, traced_op
+from ._ops import new_like, none_if_empty, run_function, traced_op
 
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -25,7 +25,7 @@ def _launch_fwd(x, weight, bias, eps, y, stats):
 
 
 def _infer_fake(x, weight, bias, eps):
-    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    return new_like(x)
 
 
 @traced_op("layer_norm_infer", _infer_fake)
@@ -50,8 +50,8 @@ def _fwd(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor],
 
 
 def _bwd_fake(x, dy, weight, bias, stats, want_dw, want_db):
-    return [x.new_empty(x.shape), weight.new_empty(weight.shape) if want_dw else x.new_empty((0,)),
-            bias.new_empty(bias.shape) if want_db else x.new_empty((0,))]
+    return [new_like(x), new_like(weight) if want_dw else x.new_empty((0,)),
+            new_like(bias) if want_db else x.new_empty((0,))]
 
 
 @traced_op("layer_norm_bwd", _bwd_fake)

@@ -11,7 +11,7 @@ import torch
 from torch import Tensor
 
 from . import _lib as L
-from ._ops import run_function, traced_op
+from ._ops import new_like, run_function, traced_op
 
 MAX_AXES = 8
 
@@ -33,7 +33,7 @@ def _host(ctype, *values):
 
 
 def _turn_fake(x, positions, inv_freq, sections, interleaved, inverse):
-    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    return new_like(x)
 
 
 @traced_op("rotary_axes", _turn_fake)
