@@ -287,7 +287,7 @@ inline unsigned scan_blocks(const Args& a, int width) {
 // (what a busy card takes at 128 features), and of packed sequences, whose
 // lengths the host does not know, the work over the CUs and a longest sequence
 // of three times the mean.  Measured, forward scans, us for 1, 2, 4 tiles:
-//   4096 tokens, 4 heads of 192                         85, 135, 301
+//   4096 tokens, 4 heads of 192                         79, 135, 301
 //   8192 tokens, 16 heads of 128                       159, 210, 312
 //   4 x 4096 tokens, 16 heads of 128                   229, 164, 189
 //   12 prompts of 1 to 5000 tokens, 16 heads of 128    230, 169, 212

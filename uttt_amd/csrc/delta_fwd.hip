@@ -13,7 +13,7 @@
 // read by one wave, straight into its registers and a chunk ahead; S, R and U
 // pass through LDS, from the wave that made them to all: three barriers a chunk.
 //
-// Measured: one sequence of 4096 tokens, 4 heads of 192 by 192, 85 us (1.3 us a
+// Measured: one sequence of 4096 tokens, 4 heads of 192 by 192, 79 us (1.2 us a
 // chunk; with X in the state's waves and K read by rows 140); 16 x 2048 tokens,
 // 12 heads of 128 by 128, with U and S0 stored for a backward, 338 us: 0.7 GB of
 // stores and 0.55 GB of loads at 3.7 TB/s (a copy reaches 5.1).
@@ -237,6 +237,11 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
 // The tokens' waves: R = b (V - gam K S0) and O = s gam Q S0 + P U.
 template <int KS, int NT>
 __device__ __forceinline__ void scan_tokens(const Args& a, const Scan& s, const Lane& l, ScanLds<KS, NT>& lds) {
+  // With one tile there are registers to read S0 from LDS once for both products
+  // (4096 tokens, 4 heads of 192: 85 -> 79 us; four chains of products instead of
+  // two, or K and V two chunks ahead, gave nothing).
+  constexpr bool kHold = NT == 1;
+  constexpr int kHeld = kHold ? KS : 1;
   const int wave = l.wave, q = l.q;
   const uint32_t put_tok = (wave >> 1) * NT * 1024 + (wave & 1) * 512 + (l.r + 16 * (q >> 1)) * 16 + (q & 1) * 8;
   const auto get = [&](const uint8_t* buf, int f) {
@@ -307,14 +312,23 @@ __device__ __forceinline__ void scan_tokens(const Args& a, const Scan& s, const 
   }
   for (int left = s.len; left > 0; left -= kC) {
     lds_barrier();   // S0 is in LDS
+    bf16x8 held[kHeld][2];
+    const auto state = [&](int part, int f) { return kHold ? held[f < kHeld ? f : 0][part] : get(lds.S[part], f); };
+    if constexpr (kHold) {
+#pragma unroll
+      for (int f = 0; f < kHeld; ++f) {
+        held[f][0] = get(lds.S[0], f);
+        held[f][1] = get(lds.S[1], f);
+      }
+    }
     {
       f32x4 X[NT] = {}, X2[NT] = {};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          X[n] = mfma(kf[ks], get(lds.S[0], ks * NT + n), X[n]);
-          X2[n] = mfma(kf[ks], get(lds.S[1], ks * NT + n), X2[n]);
+          X[n] = mfma(kf[ks], state(0, ks * NT + n), X[n]);
+          X2[n] = mfma(kf[ks], state(1, ks * NT + n), X2[n]);
         }
       // rows behind the sequence's end have b = 0 and V = 0
 #pragma unroll
@@ -335,8 +349,8 @@ __device__ __forceinline__ void scan_tokens(const Args& a, const Scan& s, const 
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        O[n] = mfma(qf[ks], get(lds.S[0], ks * NT + n), O[n]);
-        O2[n] = mfma(qf[ks], get(lds.S[1], ks * NT + n), O2[n]);
+        O[n] = mfma(qf[ks], state(0, ks * NT + n), O[n]);
+        O2[n] = mfma(qf[ks], state(1, ks * NT + n), O2[n]);
       }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
