@@ -586,3 +586,24 @@ def test_step_in_a_slot_past_32_bits():
     assert torch.equal(o, gated_delta_step(*x, own))
     assert torch.equal(state[slots - 1], own[0]) and torch.equal(state[0], own[1])
     assert not state[1:-1].any()
+
+
+def test_addresses_between_pieces_and_strides_of_one():
+    """Contiguous tensors that start 2 bytes behind a multiple of 16, and axes of
+    one with strides of no use."""
+    def behind(name, t):
+        if name not in ("q", "k", "v"):
+            return t.cuda()
+        room = torch.zeros(t.numel() + 1, dtype=t.dtype, device="cuda")
+        room[1:] = t.flatten().cuda()
+        return room[1:].view(t.shape).detach()
+
+    def odd(name, t):
+        if name not in ("q", "k", "v"):
+            return t.cuda()
+        room = torch.zeros(t.numel() + 16, dtype=t.dtype, device="cuda")
+        room[:t.numel()] = t.flatten().cuda()
+        return room.as_strided(t.shape, (13, 7, *t.stride()[2:])).detach()
+
+    check(*inputs(1, 70, 1, 1, 2, 64, 64, seed=4), move=behind)
+    check(*inputs(1, 1, 1, 2, 2, 64, 64, seed=5), move=odd)

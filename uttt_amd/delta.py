@@ -38,16 +38,25 @@ def _int64s(*values):
     return (ctypes.c_int64 * len(values))(*values)
 
 
+def _steps(t: Tensor):
+    """Element strides of [B, T, H, D]'s first three axes, 0 along an axis of one,
+    whose stride says nothing."""
+    (B, T, H, _), (sb, st, sh, _) = t.shape, t.stride()
+    return sb if B > 1 else 0, st if T > 1 else 0, sh if H > 1 else 0
+
+
 def _strides(t: Tensor):
-    """Element strides of [B, T, H, D] with D contiguous."""
-    return _int64s(*t.stride()[:3])
+    return _int64s(*_steps(t))
 
 
 def _rows16(t: Tensor) -> Tensor:
     """t itself where its rows can be read 16 bytes at a time and a chunk's by
-    31-bit offsets, else a copy."""
-    sb, st, sh, sd = t.stride()
-    return t if sd == 1 and not (sb | st | sh) % 8 and st < 1 << 23 and not t.data_ptr() % 16 else t.contiguous()
+    31-bit offsets, else a copy (contiguous() gives back a t that is contiguous
+    and starts at another address)."""
+    sb, st, sh = _steps(t)
+    if t.stride(3) == 1 and not (sb | st | sh) % 8 and st < 1 << 23 and not t.data_ptr() % 16:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 _GATE_TYPES = (torch.float32, torch.bfloat16, torch.float16)
