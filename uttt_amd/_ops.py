@@ -69,6 +69,29 @@ def run_function(fn, *args, graph=True):
     return fn.forward(_NoGraph(), *unwrap_dead_wrappers(args))
 
 
+class _FirstOrder(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, what, n, *tensors):
+        ctx.what = what
+        return tensors[:n]
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.what}: gradients of its gradients are not built")
+
+
+def first_order_only(what, grads, *inputs):
+    """A backward's `grads`, through which no gradient passes: under
+    create_graph=True they hang on `inputs` (what they are computed from, the
+    given gradients included) by a node that raises, so that a loss made of them
+    raises too and loses no term in silence.  (torch's once_differentiable lets
+    gradients through without a graph where the given ones require none, as
+    those of any loss linear in the outputs.)"""
+    if not torch.is_grad_enabled():
+        return grads
+    return _FirstOrder.apply(what, len(grads), *grads, *(t for t in inputs if t is not None))
+
+
 def none_if_empty(t):
     """Optional outputs travel through the ops as 0-element tensors."""
     return None if t is None or t.numel() == 0 else t

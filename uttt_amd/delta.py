@@ -14,7 +14,8 @@ this layer beside uTTT (uttt_llm/flame/custom_models/gated_deltanet_swa/,
 uttt_nvs/models/gated_deltanet_block.py) and takes its kernels from a package
 that is not part of it.
 
-`gated_delta_rule` is differentiable in q, k, v, g, beta and initial_state.
+`gated_delta_rule` is differentiable once in q, k, v, g, beta and initial_state
+(gradients of its gradients are refused).
 There is no CPU path.
 """
 from __future__ import annotations
@@ -27,7 +28,7 @@ import torch
 from torch import Tensor
 
 from . import _lib as L
-from ._ops import new_like, run_function, traced_op
+from ._ops import first_order_only, new_like, run_function, traced_op
 
 MAX_KEY_DIM = 256
 
@@ -180,7 +181,8 @@ class _GatedDeltaRule(torch.autograd.Function):
         o, state, u, s0 = _fwd(*args)
         ctx.save_for_backward(q, k, v, g, beta, cu_seqlens, u, s0)
         ctx.scale = scale
-        ctx.want_dh0 = initial_state is not None and initial_state.requires_grad
+        # its values are not needed again (no saved tensor, which must not change)
+        ctx.h0 = initial_state if initial_state is not None and initial_state.requires_grad else None
         ctx.set_materialize_grads(False)
         return o, state
 
@@ -191,9 +193,11 @@ class _GatedDeltaRule(torch.autograd.Function):
             do = torch.zeros_like(v)
         if dstate is not None:
             dstate = dstate.contiguous()
-        dq, dk, dv, dg, dbeta, dh0 = _bwd(q, k, v, g, beta, cu, ctx.scale, u, s0, do, dstate,
-                                          ctx.want_dh0)
-        return (dq, dk, dv, dg, dbeta, dh0 if ctx.want_dh0 else None, None, None, None, None)
+        want_dh0 = ctx.h0 is not None
+        grads = _bwd(q, k, v, g, beta, cu, ctx.scale, u, s0, do, dstate, want_dh0)
+        dq, dk, dv, dg, dbeta, dh0 = first_order_only("gated_delta_rule", grads, q, k, v, g, beta,
+                                                      ctx.h0, do, dstate)
+        return (dq, dk, dv, dg, dbeta, dh0 if want_dh0 else None, None, None, None, None)
 
 
 def gated_delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, *,
