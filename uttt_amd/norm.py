@@ -9,7 +9,7 @@ import torch
 from torch import Tensor
 
 from . import _lib as L
-from ._ops import new_like, none_if_empty, run_function, traced_op
+from ._ops import first_order_only, new_like, none_if_empty, run_function, traced_op
 
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -82,7 +82,8 @@ class _LayerNorm(torch.autograd.Function):
         x, weight, bias, stats = ctx.saved_tensors
         _, want_dw, want_db = ctx.needs_input_grad[:3]
         dy = dy if dy.stride(-1) == 1 or dy.shape[-1] == 1 else dy.contiguous()
-        dx, dw, db = _bwd(x, dy, weight, bias, stats, want_dw, want_db)
+        grads = _bwd(x, dy, weight, bias, stats, want_dw, want_db)
+        dx, dw, db = first_order_only("layer_norm", grads, x, weight, bias, dy)
         return dx, none_if_empty(dw), none_if_empty(db), None, None
 
 
@@ -95,7 +96,8 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
     of the three (fp32 weights with bf16 activations included).  Gradients have
     their inputs' dtypes; those of weight and bias are summed over the rows in
     fp32, in an order that the shape alone decides.  x may be a view whose rows
-    are evenly spaced (a slice of the last axis); other views are copied."""
+    are evenly spaced (a slice of the last axis); other views are copied.
+    Gradients of its gradients are refused."""
     L.require_device(x, weight, bias)
     assert x.dim() >= 1 and x.shape[-1] >= 1, "layer_norm: x must be [..., N] with N of 1 or more"
     assert x.dtype in _TYPES, f"layer_norm: dtype {x.dtype}"
