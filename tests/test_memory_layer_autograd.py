@@ -3,7 +3,7 @@ pass, without a GPU: the kernels' fake implementations carry the shapes."""
 import pytest
 import torch
 
-from uttt_amd import delta, norm
+from uttt_amd import delta, norm, positions
 
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -58,3 +58,41 @@ def test_second_order_of_layer_norm_is_refused(monkeypatch, linear, one):
         for t in wanted:
             with pytest.raises(RuntimeError, match="gradients of its gradients"):
                 torch.autograd.grad(loss + g.float().square().sum(), t, retain_graph=True)
+
+
+def turn_in_torch(x, positions, inv_freq, sections, interleaved, inverse):
+    """The rotary kernel's product, for tensors on the CPU."""
+    R = sum(sections)
+    axis = torch.repeat_interleave(torch.arange(len(sections)), torch.tensor(sections))
+    angle = (positions[..., axis] * inv_freq)[:, :, None] * (-1 if inverse else 1)
+    a, b = (x[..., 0:2 * R:2], x[..., 1:2 * R:2]) if interleaved else (x[..., :R], x[..., R:2 * R])
+    u, w = a * angle.cos() - b * angle.sin(), a * angle.sin() + b * angle.cos()
+    return torch.cat([torch.stack([u, w], -1).flatten(-2) if interleaved else torch.cat([u, w], -1),
+                      x[..., 2 * R:]], -1).detach()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_is_differentiable_any_number_of_times(monkeypatch, interleaved):
+    """Linear in x: its gradient's gradient is the turn itself, here with the
+    kernel's product in torch.  Up to third order, against differences."""
+    monkeypatch.setattr(positions, "_turn", turn_in_torch)
+    monkeypatch.setattr(positions.L, "require_device", lambda *t: None)
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn(2, 3, 2, 10, generator=gen, dtype=F32).requires_grad_()
+    pos = torch.randint(-9, 9, (2, 3, 2), generator=gen)
+    f = lambda t: positions.rotary_axes(t, pos, torch.tensor([1.0, 0.3, 0.1]), [1, 2], interleaved=interleaved)  # noqa: E731
+    w = torch.randn(x.shape, generator=gen)
+    # y.y is |x|^2, so that its gradient is 2 x and that of |gradient|^2 8 x
+    (g,) = torch.autograd.grad(f(x).square().sum(), x, create_graph=True)
+    assert torch.allclose(g, 2 * x, atol=1e-5)
+    (gg,) = torch.autograd.grad(g.square().sum(), x, create_graph=True)
+    assert torch.allclose(gg, 8 * x, atol=1e-4)
+    (ggg,) = torch.autograd.grad(gg.square().sum(), x)
+    assert torch.allclose(ggg, 128 * x, atol=1e-3)
+    # a loss linear in y: the gradient does not depend on x, but on what it is given
+    v = w.clone().requires_grad_()
+    (g,) = torch.autograd.grad(f(x), x, v, create_graph=True)
+    (gv,) = torch.autograd.grad(g, v, w)
+    assert torch.allclose(gv, f(w), atol=1e-5)
+    (g,) = torch.autograd.grad((f(x) * w).sum(), x, create_graph=True)
+    assert torch.allclose(f(g.detach()), w, atol=1e-5)

@@ -53,16 +53,18 @@ def _turn(x: Tensor, positions: Tensor, inv_freq: Tensor, sections: List[int], i
 
 class _RotaryAxes(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, positions, inv_freq, sections, interleaved):
+    def forward(ctx, x, positions, inv_freq, sections, interleaved, inverse):
         ctx.save_for_backward(positions, inv_freq)
-        ctx.args = (sections, interleaved)
-        return _turn(x, positions, inv_freq, sections, interleaved, False)
+        ctx.args = (sections, interleaved, inverse)
+        return _turn(x, positions, inv_freq, sections, interleaved, inverse)
 
     @staticmethod
     def backward(ctx, dy):
+        """The turn back, itself differentiable in dy."""
         positions, inv_freq = ctx.saved_tensors
-        sections, interleaved = ctx.args
-        return _turn(dy, positions, inv_freq, sections, interleaved, True), None, None, None, None
+        sections, interleaved, inverse = ctx.args
+        turn = _RotaryAxes.apply if torch.is_grad_enabled() else _turn
+        return turn(dy, positions, inv_freq, sections, interleaved, not inverse), None, None, None, None, None
 
 
 def rotary_axes(x: Tensor, positions: Tensor, inv_freq: Tensor, sections: Sequence[int], *,
@@ -77,8 +79,8 @@ def rotary_axes(x: Tensor, positions: Tensor, inv_freq: Tensor, sections: Sequen
     inv_freq    [R] fp32: pair j turns by position * inv_freq[j] (axis_frequencies).
     interleaved pairs are features (2j, 2j + 1) instead of (j, j + R).
 
-    Features from 2R on pass through.  Differentiable in x.  x may be a view with
-    contiguous features (one of a fused projection's parts)."""
+    Features from 2R on pass through.  Differentiable in x, any number of times.
+    x may be a view with contiguous features (one of a fused projection's parts)."""
     what = "rotary_axes"
     L.require_device(x, positions, inv_freq)
     assert x.dim() == 4, f"{what}: x must be [B, L, H, D]"
@@ -97,4 +99,4 @@ def rotary_axes(x: Tensor, positions: Tensor, inv_freq: Tensor, sections: Sequen
     if positions.dim() == 2:
         positions = positions.expand(B, Lx, A)
     return run_function(_RotaryAxes, x, positions, inv_freq.contiguous(), sections, bool(interleaved),
-                        graph=x.requires_grad)
+                        False, graph=x.requires_grad)
