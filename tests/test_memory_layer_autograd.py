@@ -96,3 +96,20 @@ def test_rotary_is_differentiable_any_number_of_times(monkeypatch, interleaved):
     assert torch.allclose(gv, f(w), atol=1e-5)
     (g,) = torch.autograd.grad((f(x) * w).sum(), x, create_graph=True)
     assert torch.allclose(f(g.detach()), w, atol=1e-5)
+
+
+def test_rotary_refuses_frequencies_that_require_gradients():
+    """None would reach them."""
+    x, pos = leaf(1, 3, 2, 8), torch.empty(1, 3, 1, dtype=torch.int32, device="meta")
+    freq = leaf(4, dtype=F32)
+    with pytest.raises(AssertionError, match="inv_freq"):
+        positions.rotary_axes(x, pos, freq, [4])
+    with pytest.raises(AssertionError, match="inv_freq"):
+        positions.rotary_axes(x.detach(), pos, freq, [4])
+
+
+def test_rotary_takes_such_frequencies_where_gradients_are_off(monkeypatch):
+    monkeypatch.setattr(positions, "_turn", positions._turn_fake)
+    x, pos = leaf(1, 3, 2, 8), torch.empty(1, 3, 1, dtype=torch.int32, device="meta")
+    with torch.no_grad():
+        assert positions.rotary_axes(x, pos, leaf(4, dtype=F32), [4]).shape == x.shape

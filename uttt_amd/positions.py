@@ -76,7 +76,8 @@ def rotary_axes(x: Tensor, positions: Tensor, inv_freq: Tensor, sections: Sequen
                 values, negative and far ones included (angles are reduced in 64 bits).
     sections    the pairs of each of the A axes (up to 8), R = sum(sections) in all, 2R <= D:
                 the first sections[0] pairs turn by the first axis' position, and so on.
-    inv_freq    [R] fp32: pair j turns by position * inv_freq[j] (axis_frequencies).
+    inv_freq    [R] fp32: pair j turns by position * inv_freq[j] (axis_frequencies); no gradient
+                flows to it.
     interleaved pairs are features (2j, 2j + 1) instead of (j, j + R).
 
     Features from 2R on pass through.  Differentiable in x, any number of times.
@@ -95,6 +96,8 @@ def rotary_axes(x: Tensor, positions: Tensor, inv_freq: Tensor, sections: Sequen
         f"{what}: positions must be [{B}, {Lx}, {A}] or [{Lx}, {A}], got {tuple(positions.shape)}")
     assert inv_freq.shape == (R,) and inv_freq.dtype == torch.float32, (
         f"{what}: inv_freq must be [{R}] fp32")
+    assert not (inv_freq.requires_grad and torch.is_grad_enabled()), (
+        f"{what}: no gradient flows to inv_freq; detach it")
     assert positions.get_device() == inv_freq.get_device() == x.get_device(), f"{what}: tensors on several devices"
     if positions.dim() == 2:
         positions = positions.expand(B, Lx, A)
