@@ -113,3 +113,48 @@ def test_rotary_takes_such_frequencies_where_gradients_are_off(monkeypatch):
     x, pos = leaf(1, 3, 2, 8), torch.empty(1, 3, 1, dtype=torch.int32, device="meta")
     with torch.no_grad():
         assert positions.rotary_axes(x, pos, leaf(4, dtype=F32), [4]).shape == x.shape
+
+
+def step_inputs(slots=3, device="meta"):
+    e = lambda *s, dtype=BF16: torch.empty(*s, dtype=dtype, device=device)  # noqa: E731
+    return [e(2, 1, 1, 64), e(2, 1, 1, 64), e(2, 1, 2, 32), e(2, 1, 2, dtype=F32), e(2, 1, 2, dtype=F32)], e(
+        slots, 2, 64, 32, dtype=F32)
+
+
+@pytest.fixture
+def launched(monkeypatch):
+    """The step up to its launch, on meta tensors."""
+    calls = []
+    monkeypatch.setattr(delta.L, "call_on", lambda t, name, *args: calls.append((name, args)))
+    monkeypatch.setattr(delta.L, "stream_of", lambda t: 0)
+    return calls
+
+
+def test_the_step_says_that_it_changes_the_state(launched):
+    """A state that another op has saved for its backward raises there, as after
+    any torch operation in place; through a view of a pool too."""
+    x, state = step_inputs()
+    state.requires_grad_()
+    loss = state.square().sum()
+    with torch.no_grad():
+        delta.gated_delta_step(*x, state)
+    assert len(launched) == 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    pool = torch.empty(3, 4, 2, 64, 32, device="meta")
+    before = pool._version
+    delta.gated_delta_step(*x, pool[:, 1])
+    assert pool._version == before + 1
+    before = [t._version for t in x]
+    delta.gated_delta_step(*x, pool[:, 1])
+    assert [t._version for t in x] == before
+
+
+def test_the_step_takes_states_of_inference_mode(launched):
+    x, state = step_inputs()
+    with torch.inference_mode():
+        own = torch.empty_like(state)
+        delta.gated_delta_step(*x, own)
+        delta.gated_delta_step(*x, state)
+    delta.gated_delta_step(*x, own)   # which nothing can save for a backward
+    assert len(launched) == 3

@@ -5,11 +5,14 @@ instead of breaking the graph at every kernel call.
 
 `traced_op(name, fake)` registers a function as torch.ops.uttt_hip.<name>
 and returns a wrapper that calls the registered op while torch.compile
-traces, and the function itself otherwise (eager calls skip the dispatcher).
+traces, and the function itself otherwise (eager calls skip the dispatcher,
+and count a change of the arguments that they write to themselves, so that
+autograd refuses a backward that saved one of them before).
 """
 from __future__ import annotations
 
 import functools
+import inspect
 
 import torch
 from torch._C._functorch import is_dead_tensor_wrapper
@@ -21,12 +24,19 @@ def traced_op(name, fake, mutates_args=()):
     def deco(fn):
         op = torch.library.custom_op(f"uttt_hip::{name}", fn, mutates_args=mutates_args)
         op.register_fake(fake)
+        names = list(inspect.signature(fn).parameters)
+        written = [names.index(n) for n in mutates_args]
 
         @functools.wraps(fn)
         def call(*args, **kwargs):
             if torch.compiler.is_compiling():
                 return op(*args, **kwargs)
-            return fn(*args, **kwargs)
+            out = fn(*args, **kwargs)
+            for i in written:
+                t = args[i] if i < len(args) else kwargs[names[i]]
+                if not t.is_inference():   # those have no count, and nothing saves them
+                    torch.autograd.graph.increment_version(t)
+            return out
 
         call.op = op
         return call
