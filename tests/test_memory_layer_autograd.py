@@ -2,6 +2,7 @@
 pass, without a GPU: the kernels' fake implementations carry the shapes."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from uttt_amd import delta, norm, positions
 
@@ -158,3 +159,31 @@ def test_the_step_takes_states_of_inference_mode(launched):
         delta.gated_delta_step(*x, state)
     delta.gated_delta_step(*x, own)   # which nothing can save for a backward
     assert len(launched) == 3
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_the_step_refuses_forward_gradients(launched, which):
+    """Their tangents would be lost in silence."""
+    x, state = step_inputs()
+    args = x + [state]
+    with forward_ad.dual_level():
+        delta.gated_delta_step(*args)   # none of them has one
+        args[which] = forward_ad.make_dual(args[which], torch.empty_like(args[which]))
+        with pytest.raises(AssertionError, match="no gradient"):
+            delta.gated_delta_step(*args)
+    assert len(launched) == 1
+
+
+def test_the_others_refuse_forward_gradients(monkeypatch):
+    monkeypatch.setattr(delta, "_infer", delta._infer_fake)
+    monkeypatch.setattr(norm, "_infer", norm._infer_fake)
+    monkeypatch.setattr(positions, "_turn", positions._turn_fake)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t.detach(), torch.empty_like(t))  # noqa: E731
+        q, k, v, g, beta = rule_leaves()
+        for call in (lambda: delta.gated_delta_rule(dual(q), k.detach(), v.detach(), g.detach(), beta.detach()),
+                     lambda: norm.layer_norm(dual(leaf(4, 16))),
+                     lambda: positions.rotary_axes(dual(leaf(1, 2, 1, 8)), torch.empty(2, 1, dtype=torch.int32, device="meta"),
+                                                   torch.empty(4, device="meta"), [4])):
+            with pytest.raises(NotImplementedError):
+                call()

@@ -26,6 +26,7 @@ from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from ._ops import first_order_only, new_like, run_function, traced_op
@@ -285,7 +286,7 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
                    index is no slot (-1: padding) leaves every state alone and gets zeros.  Rows
                    that name one slot follow one another in row order.
 
-    No gradient flows through it."""
+    No gradient flows through it, backward or forward: tensors that have one are refused."""
     what = "gated_delta_step"
     B, T, Hk, Hv, Dk, Dv = _check(q, k, v, g, beta, what)
     assert q.dtype in (torch.float32, torch.bfloat16, torch.float16), f"{what}: dtype {q.dtype}"
@@ -305,6 +306,8 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
         state_indices = state_indices.contiguous()
     else:
         assert B <= state.shape[0], f"{what}: {B} rows, {state.shape[0]} states"
-    assert not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state))), (
+    tensors = (q, k, v, g, beta, state)
+    assert not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) and not (
+        forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)), (
         f"{what}: no gradient flows through a state that is updated in place")
     return _step(q, k, v, g, beta, state, Dk ** -0.5 if scale is None else float(scale), state_indices)
