@@ -262,11 +262,12 @@ def _step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, state: Tenso
     q, k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k, v))
     g, beta = g.contiguous(), beta.contiguous()
     o = _step_fake(q, k, v, g, beta, state, scale, state_indices)
+    slots = state.shape[0]
+    apart = state.stride(0) if slots > 1 else Hv * Dk * Dv   # of one slot it says nothing
     L.call_on(q, "uttt_gated_delta_step", L.ptr(q), _strides(q), L.ptr(k), _strides(k), L.ptr(v),
               _strides(v), L.dtype_code(q.dtype), L.ptr(g), L.dtype_code(g.dtype), L.ptr(beta),
-              L.dtype_code(beta.dtype), B, T, Hk, Hv, Dk, Dv, scale, L.ptr(state),
-              max(state.stride(0), Hv * Dk * Dv),
-              state.shape[0], L.ptr(state_indices),
+              L.dtype_code(beta.dtype), B, T, Hk, Hv, Dk, Dv, scale, L.ptr(state), apart,
+              slots, L.ptr(state_indices),
               int(state_indices is not None and state_indices.dtype == torch.int64), L.ptr(o),
               L.stream_of(q))
     return o
