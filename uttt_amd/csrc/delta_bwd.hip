@@ -442,6 +442,7 @@ __global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads
   __shared__ __attribute__((aligned(16))) uint8_t buf[kBuf > kOut ? kBuf : kOut];
   __shared__ __attribute__((aligned(16))) float Sc[kScal];
   __shared__ float bsum[PW][16], zsum[PW][kC], rvs[kC], dots[NW];
+  __shared__ int bad;   // the first column of X that is not finite
   float* Xl = reinterpret_cast<float*>(buf);
   __bf16* Dl = reinterpret_cast<__bf16*>(buf);
   __bf16* DTl = Dl + kC * LM;
@@ -477,6 +478,7 @@ __global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads
     int r = r0, q = q0;
     asm volatile("" : "+v"(r), "+v"(q));
     const int feat = 16 * wave + r;
+    if (tid == 0) bad = kC;
     for (int i = tid; i < kScal; i += kThreads) Sc[i] = a.scal[((size_t)c * a.Hv + hv) * kScal + i];
     const int64_t oat = tok * orow + (int64_t)hv * a.Dv;
     const uint16_t* gp = a.dout + ch.b * a.do_sb + ch.t0 * a.do_st + hv * a.do_sh;
@@ -602,6 +604,7 @@ __global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads
         if (r >> 2 == q) rvs[16 * rw + r] = d;
       }
       f32x4 bs = {};
+      float zero = 0.0f;   // NaN where some X is not finite
 #pragma unroll
       for (int x = 0; x < CT; ++x) {
         const int j = 16 * (cw + x) + r;
@@ -610,15 +613,30 @@ __global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads
           const int row = 16 * rw + 4 * q + i;
           const float E = row >= j ? __expf((Sc[3 * kC + row] - Sc[3 * kC + j]) +
                                             (Sc[4 * kC + row] - Sc[4 * kC + j])) : 0.0f;
-          const float D = a.scale * E * dP[x][i];
+          const float D = row >= j ? a.scale * E * dP[x][i] : 0.0f;
           const float m = row > j ? -E * dA[x][i] : 0.0f;
           const float M = Sc[2 * kC + row] * m;
           bs[i] = __builtin_fmaf(m, kk[x][i], bs[i]);
-          Xl[row * LX + j] = D * qk[x][i] + M * kk[x][i];
+          const float xv = D * qk[x][i] + M * kk[x][i];
+          Xl[row * LX + j] = xv;
+          zero = __builtin_fmaf(xv, 0.0f, zero);
           dP[x][i] = D;
           dA[x][i] = M;
         }
       }
+      // An X that is not finite comes from a U of token j that is not.  It is left
+      // out of the sums over j < t, whose product multiplies zeros with it, and dg
+      // is NaN behind j.
+      if (__builtin_expect(zero != 0.0f, 0))
+        for (int x = 0; x < CT; ++x)
+          for (int i = 0; i < 4; ++i) {
+            const int j = 16 * (cw + x) + r;
+            float* xp = Xl + (16 * rw + 4 * q + i) * LX + j;
+            if (*xp * 0.0f != 0.0f) {
+              *xp = 0.0f;
+              atomicMin(&bad, j);
+            }
+          }
 #pragma unroll
       for (int i = 0; i < 4; ++i) bs[i] = sum16(bs[i]);
       if (r == 0)
@@ -780,7 +798,7 @@ __global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads
       for (int w = 0; w < PW / 4; ++w) b += bsum[(lane >> 4) + 4 * w][lane & 15];
       if (lane < ch.n) {
         const int64_t at = (tok + lane) * a.Hv + hv;
-        store_any(a.dg, a.g_dtype, at, z + suf + pre + Sc[kC - 1] * all);
+        store_any(a.dg, a.g_dtype, at, lane > bad ? __builtin_nanf("") : z + suf + pre + Sc[kC - 1] * all);
         store_any(a.dbeta, a.beta_dtype, at, rvs[lane] - gam * s[1] + b);
       }
     }

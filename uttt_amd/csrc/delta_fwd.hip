@@ -13,6 +13,14 @@
 // read by one wave, straight into its registers and a chunk ahead; S, R and U
 // pass through LDS, from the wave that made them to all: three barriers a chunk.
 //
+// Values that are not finite.  U = T R and P U multiply the zeros above the
+// diagonal with later tokens' R and U, and a zero by an infinity is NaN.  So an R
+// that is not finite goes in as zero, and what becomes of it is put in behind the
+// products: NaN in its column from its token on, in the outputs, in U as saved
+// and in what goes to the state.  With ordinary values that is one test of R and
+// two of a flag a chunk (one sequence of 8192 tokens, 16 heads of 64 by 64, whose
+// chunks are the shortest: scan 105 -> 113 us; other scans 0 to 1 %).
+//
 // Measured: one sequence of 4096 tokens, 4 heads of 192 by 192, 79 us (1.2 us a
 // chunk; with X in the state's waves and K read by rows 140); 16 x 2048 tokens,
 // 12 heads of 128 by 128, with U and S0 stored for a backward, 338 us: 0.7 GB of
@@ -31,7 +39,16 @@ struct ScanLds {
   uint8_t R[2][2 * NT * 1024];
   uint8_t U[2][2 * NT * 1024];
   uint8_t E[2][2 * NT * 1024];   // e^{G_C - G} U
+  int first[NT][16];             // a column's first token in the chunk whose R is not finite
+  int bad;                       // whether there is one
 };
+
+// NaN in rows from `first` on.
+__device__ __forceinline__ void spoil(f32x4& x, int row, int first) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (row + i >= first) x[i] = __builtin_nanf("");
+}
 
 // What both kinds of waves know of their place.
 struct Lane {
@@ -176,6 +193,7 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
     if constexpr (kAhead) load_kt(left - kC, coming);
     if constexpr (SAVE) save_state();
     lds_barrier();   // R is in LDS
+    int bad = lds.bad;
     f32x4 U[NT] = {};
     {
       f32x4 U2[NT] = {};
@@ -189,17 +207,26 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
             U2[n] = mfma(now.t[ks][1], hi, U2[n]);
             U2[n] = mfma(now.t[ks][0], lo, U2[n]);
           }
+      asm volatile("" : "+v"(bad));   // read with R, not when U is made
 #pragma unroll
       for (int n = 0; n < NT; ++n) U[n] += U2[n];
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      put_tile(lds.E, n, parts_of(now.ge * U[n]));
       const Parts p = parts_of(U[n]);
       put_tile(lds.U, n, p);
       uh[n] = p.hi;
       ul[n] = p.lo;
     }
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(bad), 0)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        spoil(U[n], 16 * wave + 4 * q, lds.first[n][r]);
+        uh[n] = parts_of(U[n]).hi;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) put_tile(lds.E, n, parts_of(now.ge * U[n]));
     lds_barrier();   // U is in LDS
     // S' = gam_C S0 + K^T (e^{G_C - G} U)
 #pragma unroll
@@ -331,19 +358,36 @@ __device__ __forceinline__ void scan_tokens(const Args& a, const Scan& s, const 
           X2[n] = mfma(kf[ks], state(1, ks * NT + n), X2[n]);
         }
       // rows behind the sequence's end have b = 0 and V = 0
+      f32x4 zero = {};   // NaN where some value is not finite
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         f32x4 v;
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = vr[i].get(n);
-        const Parts p = parts_of(bt * (v - gam * (X[n] + X2[n])));
+        X[n] = bt * (v - gam * (X[n] + X2[n]));
+        const Parts p = parts_of(X[n]);
         *reinterpret_cast<u32x2*>(lds.R[0] + put_tok + n * 1024) = p.hi;
         *reinterpret_cast<u32x2*>(lds.R[1] + put_tok + n * 1024) = p.lo;
+        zero += X[n] * 0.0f;
+      }
+      if (__builtin_expect(__any((zero[0] + zero[1]) + (zero[2] + zero[3]) != 0.0f), 0)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (X[n][i] * 0.0f != 0.0f) {
+              *reinterpret_cast<uint16_t*>(lds.R[0] + put_tok + n * 1024 + 2 * i) = 0;
+              *reinterpret_cast<uint16_t*>(lds.R[1] + put_tok + n * 1024 + 2 * i) = 0;
+              atomicMin(&lds.first[n][l.r], 16 * wave + 4 * q + i);
+            }
+        lds.bad = 1;
       }
     }
     const f32x4 sgam = gam * a.scale;
     lds_barrier();   // R is in LDS
-    load_k(left - kC);
+    int next = left - kC;
+    asm volatile("" : "+s"(next));   // offsets of the next loads: here, not in front of the barrier
+    load_k(next);
     f32x4 O[NT] = {}, O2[NT] = {};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
@@ -368,8 +412,11 @@ __device__ __forceinline__ void scan_tokens(const Args& a, const Scan& s, const 
           O2[n] = mfma(pf[ks][1], hi, O2[n]);
           O2[n] = mfma(pf[ks][0], lo, O2[n]);
         }
-    load_q(left - kC);
-    load_p(left - kC);
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(lds.bad), 0))
+#pragma unroll
+      for (int n = 0; n < NT; ++n) spoil(O[n], 16 * wave + 4 * q, lds.first[n][l.r]);
+    load_q(next);
+    load_p(next);
     const Rsrc orsrc = buffer_at(op);
     u32x2 ow[NT];
 #pragma unroll
@@ -381,13 +428,20 @@ __device__ __forceinline__ void scan_tokens(const Args& a, const Scan& s, const 
   }
 }
 
+// The smallest variants keep to the 128 registers with which two workgroups
+// share a CU.
 template <int KS, int NT, bool SAVE>
-__global__ __launch_bounds__(512) void delta_scan_kernel(Args a) {
+__global__ __launch_bounds__(512, KS * NT <= 4 ? 4 : 2) void delta_scan_kernel(Args a) {
   __shared__ __attribute__((aligned(16))) ScanLds<KS, NT> lds;
   Scan s;
   if (!s.init(a, 16 * NT)) return;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, q = lane >> 4, col = s.col0 + NT * r;
+  if (wave == 4 && q == 0) {   // one of the waves that write it
+#pragma unroll
+    for (int n = 0; n < NT; ++n) lds.first[n][r] = kC;
+    lds.bad = 0;
+  }
   const Lane l{wave & 3, lane, r, q, col, miss_from(col, a.Dv), miss_from(32 * (KS - 1) + 8 * q, a.Dk),
                miss_from(32 * (KS - 2) + 8 * q, a.Dk)};
   if (wave < 4) scan_state<KS, NT, SAVE>(a, s, l, lds);

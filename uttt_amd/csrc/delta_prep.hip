@@ -203,6 +203,7 @@ __global__ __launch_bounds__(256, KS <= 4 ? 4 : 2) void delta_prep_kernel(Args a
   __shared__ __attribute__((aligned(16))) uint8_t buf[kRows > kMats ? kRows : kMats];
   __shared__ double Gd[kC];
   __shared__ float bet[kC];
+  __shared__ int bad;   // the first row of A that is not finite
   const int c = blockIdx.x / a.Hk, hk = blockIdx.x % a.Hk;
   const Chunk ch = chunk_of(a, c);
   if (ch.seq < 0) {
@@ -234,6 +235,7 @@ __global__ __launch_bounds__(256, KS <= 4 ? 4 : 2) void delta_prep_kernel(Args a
     sc[3 * kC + lane] = (float)G;
     sc[4 * kC + lane] = (float)(G - (double)(float)G);
   };
+  if (tid == 0) bad = kC;
   if (wave == 0) load_gates(hk * group);
   uint16_t* Kl = reinterpret_cast<uint16_t*>(buf);
   uint16_t* Ql = Kl + kC * LD;
@@ -267,6 +269,7 @@ __global__ __launch_bounds__(256, KS <= 4 ? 4 : 2) void delta_prep_kernel(Args a
   float* Pm = Am + kC * kLT;
   float* Tm = Pm;   // T takes P's place once P's fragments are written
   for (int hv = hk * group; hv < (hk + 1) * group; ++hv) {
+    float zero = 0.0f;   // NaN where some value is not finite
 #pragma unroll
     for (int ct = 0; ct < 4; ++ct) {
       const int j = 16 * ct + r;
@@ -275,11 +278,30 @@ __global__ __launch_bounds__(256, KS <= 4 ? 4 : 2) void delta_prep_kernel(Args a
       for (int i = 0; i < 4; ++i) {
         const int row = 16 * wave + 4 * q + i;
         const float e = row >= j ? exp_diff(Gd[row] - Gj) : 0.0f;
-        Am[row * kLT + j] = row > j ? bet[row] * e * kk[ct][i] : 0.0f;
+        const float x = row > j ? bet[row] * e * kk[ct][i] : 0.0f;
+        Am[row * kLT + j] = x;
+        zero = __builtin_fmaf(x, 0.0f, zero);
         Pm[row * kLT + j] = row >= j ? a.scale * e * qk[ct][i] : 0.0f;
       }
     }
+    if (__builtin_expect(zero != 0.0f, 0))
+      for (int i = 0; i < 4; ++i)
+        for (int ct = 0; ct < 4; ++ct) {
+          const int row = 16 * wave + 4 * q + i;
+          if (Am[row * kLT + 16 * ct + r] * 0.0f != 0.0f) atomicMin(&bad, row);
+        }
     __syncthreads();
+    // T's blocks are joined by products whose zeros would make NaN of earlier
+    // tokens' rows: from the first row on that is not finite A is left out, and a
+    // beta of NaN gives that token's R and so all that comes after it.
+    const int first_bad = __builtin_amdgcn_readfirstlane(bad);
+    if (__builtin_expect(first_bad < kC, 0)) {
+      for (int i = first_bad * kLT + tid; i < kC * kLT; i += 256) Am[i] = 0.0f;
+      if (wave == 0 && lane >= first_bad)
+        a.scal[((size_t)c * a.Hv + hv) * kScal + 2 * kC + lane] = __builtin_nanf("");
+      __syncthreads();
+      if (tid == 0) bad = kC;   // for the next head
+    }
     uint8_t* tri = a.tri + ((size_t)c * a.Hv + hv) * kTriBytes;
     // wave 0: column r of diagonal block q, top to bottom; the others: P's fragments
     float t[16];

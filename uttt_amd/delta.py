@@ -220,6 +220,11 @@ def gated_delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, *
                    allowed.  Offsets must ascend; tokens of no sequence get zeros as outputs
                    and gradients.
 
+    A value that is not finite reaches the results of its token and later ones of its sequence
+    (of q: of its token alone; of v: in its column alone), as in the recurrence, and no others:
+    what lies behind a padded sequence's tokens does not matter to their outputs.  Of v this
+    holds for the gradients too, where those given for the later outputs are zeros.
+
     q, k and v may be views with any strides of their first three axes that are multiples of
     8 elements; others are copied.  Everything but q, k, v, the outputs and the gradients of
     q, k and v is kept to fp32's order.  The backward keeps U and the state at every 64th
