@@ -6,11 +6,11 @@
 //
 // Bound by memory: one read and one write of x.  A token's R cosines and sines
 // are computed once, in LDS, for all its heads; the angle in turns is reduced
-// in 64 bits, so that positions of any size keep fp32's precision.  A thread's
-// first piece of x is on its way while the angles are computed, and each next
-// one while the last is turned: 3 x 8191 tokens of 12 heads of 128 bf16
-// features 36 us, 4.2 TB/s (without this, and with 8-byte pieces where pairs
-// are side by side, 48).
+// with products in two doubles, so that any 64-bit position keeps fp32's
+// precision.  A thread's first piece of x is on its way while the angles are
+// computed, and each next one while the last is turned: 3 x 8191 tokens of 12
+// heads of 128 bf16 features 36 us, 4.2 TB/s (without this, and with 8-byte
+// pieces where pairs are side by side, 48).
 #include "common.h"
 
 namespace uttt {
@@ -51,6 +51,16 @@ struct Vec {
     __builtin_memcpy(__builtin_assume_aligned(p, V * sizeof(S) > 16 ? 16 : V * sizeof(S)), w, sizeof w);
   }
 };
+
+// p f / pi without whole turns, in [-1, 1], to 2^-106 of |p f|: f / pi and its
+// product with p in two doubles each.
+__device__ __forceinline__ double half_turns(double p, double f) {
+  constexpr double kInvPi = 0x1.45f306dc9c883p-2, kInvPiLow = -0x1.6b01ec5417056p-56;
+  const double fh = f * kInvPi, fl = __builtin_fma(f, kInvPiLow, __builtin_fma(f, kInvPi, -fh));
+  const double h = p * fh, l = __builtin_fma(p, fl, __builtin_fma(p, fh, -h));
+  const double x = (h - 2.0 * rint(0.5 * h)) + l;
+  return x - 2.0 * rint(0.5 * x);
+}
 
 template <class TT, int V, bool INTER>
 __global__ __launch_bounds__(kRotThreads) void rotary_axes_kernel(RotArgs a) {
@@ -94,10 +104,15 @@ __global__ __launch_bounds__(kRotThreads) void rotary_axes_kernel(RotArgs a) {
     int axis = 0;
     while (j >= a.ends[axis]) ++axis;
     const int64_t at = pat[t] + axis * a.p_sa;
-    const double p = a.pos64 ? (double)static_cast<const int64_t*>(a.pos)[at]
-                             : (double)static_cast<const int32_t*>(a.pos)[at];
-    double half = p * (double)a.freq[j] * 0.31830988618379067154;   // angle / pi
-    half -= 2.0 * rint(0.5 * half);
+    const double f = (double)a.freq[j];
+    double half;
+    if (a.pos64) {
+      const int64_t p = static_cast<const int64_t*>(a.pos)[at];
+      half = half_turns((double)(p >> 32) * 4294967296.0, f) + half_turns((double)(uint32_t)p, f);
+      half -= 2.0 * rint(0.5 * half);
+    } else {
+      half = half_turns((double)static_cast<const int32_t*>(a.pos)[at], f);
+    }
     float s, c;
     sincospif((float)half, &s, &c);
     cs[i] = c;

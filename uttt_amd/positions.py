@@ -73,7 +73,7 @@ def rotary_axes(x: Tensor, positions: Tensor, inv_freq: Tensor, sections: Sequen
     bf16 or fp16; rotated in fp32 and rounded once).
 
     positions   [B, L, A] or, the same for every batch row, [L, A] int32 or int64; any
-                values, negative and far ones included (angles are reduced in 64 bits).
+                values, negative and far ones included (to the end of int64 angles keep fp32's precision).
     sections    the pairs of each of the A axes (up to 8), R = sum(sections) in all, 2R <= D:
                 the first sections[0] pairs turn by the first axis' position, and so on.
     inv_freq    [R] fp32: pair j turns by position * inv_freq[j] (axis_frequencies); no gradient
