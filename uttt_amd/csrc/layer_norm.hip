@@ -311,33 +311,37 @@ __global__ __launch_bounds__(kLnThreads) void ln_cols_kernel(LnArgs a, int64_t r
 }
 
 // The workgroups' totals added: 16 columns by 64 slices of the workgroups, in
-// a fixed order.
-constexpr int kSumSlices = 64;
+// a fixed order.  Past kSumBlocks * 16 columns (of dw and db together) a
+// workgroup has several such runs: a launch has fewer than 2^32 threads.
+constexpr int kSumSlices = 64, kSumBlocks = 1 << 20;
 __global__ __launch_bounds__(16 * kSumSlices) void ln_sum_kernel(const float* __restrict__ part, int n, int N,
                                                                  void* dw, int w_dtype, void* db, int b_dtype) {
   __shared__ float red[kSumSlices][17];
   const int c = threadIdx.x & 15, s = threadIdx.x >> 4;
-  const int64_t e = (int64_t)blockIdx.x * 16 + c;   // over dw then db
-  float sum = 0.0f;
-  if (e < 2 * (int64_t)N)
+  for (int64_t base = (int64_t)blockIdx.x * 16; base < 2 * (int64_t)N; base += (int64_t)kSumBlocks * 16) {
+    const int64_t e = base + c;   // over dw then db
+    float sum = 0.0f;
+    if (e < 2 * (int64_t)N)
 #pragma unroll 8
-    for (int i = s; i < n; i += kSumSlices) sum += part[(int64_t)i * 2 * N + e];
-  red[s][c] = sum;
-  __syncthreads();
-#pragma unroll
-  for (int d = kSumSlices / 2; d > 0; d >>= 1) {
-    if (s < d) red[s][c] += red[s + d][c];
+      for (int i = s; i < n; i += kSumSlices) sum += part[(int64_t)i * 2 * N + e];
+    __syncthreads();   // the run before is read
+    red[s][c] = sum;
     __syncthreads();
+#pragma unroll
+    for (int d = kSumSlices / 2; d > 0; d >>= 1) {
+      if (s < d) red[s][c] += red[s + d][c];
+      __syncthreads();
+    }
+    if (s != 0 || e >= 2 * (int64_t)N) continue;
+    sum = red[0][c];
+    const bool second = e >= N;
+    void* out = second ? db : dw;
+    const int dt = second ? b_dtype : w_dtype;
+    const int64_t at = second ? e - N : e;
+    if (!out) continue;
+    if (dt == UTTT_F32) static_cast<float*>(out)[at] = sum;
+    else static_cast<uint16_t*>(out)[at] = dt == UTTT_BF16 ? f32_to_bf16(sum) : f32_to_f16(sum);
   }
-  if (s != 0 || e >= 2 * (int64_t)N) return;
-  sum = red[0][c];
-  const bool second = e >= N;
-  void* out = second ? db : dw;
-  const int dt = second ? b_dtype : w_dtype;
-  const int64_t at = second ? e - N : e;
-  if (!out) return;
-  if (dt == UTTT_F32) static_cast<float*>(out)[at] = sum;
-  else static_cast<uint16_t*>(out)[at] = dt == UTTT_BF16 ? f32_to_bf16(sum) : f32_to_f16(sum);
 }
 
 constexpr int kLnPieces = 2048, kLnOddMost = 8192;   // longest rows held in registers
@@ -465,7 +469,8 @@ extern "C" int uttt_layer_norm_bwd(const void* x, int dtype, int64_t x_stride, c
     default: rc = ln_rows<F16T>(a, true, st); break;
   }
   if (rc || !sums) return rc;
-  hipLaunchKernelGGL(ln_sum_kernel, dim3((unsigned)((2 * (int64_t)N + 15) / 16)), dim3(16 * kSumSlices), 0,
-                     st, a.part, (int)bwd_blocks(rows, N), N, dweight, weight_dtype, dbias, bias_dtype);
+  const int64_t runs = (2 * (int64_t)N + 15) / 16;
+  hipLaunchKernelGGL(ln_sum_kernel, dim3((unsigned)(runs < kSumBlocks ? runs : kSumBlocks)), dim3(16 * kSumSlices), 0, st,
+                     a.part, (int)bwd_blocks(rows, N), N, dweight, weight_dtype, dbias, bias_dtype);
   return check_launch("layer_norm_sum");
 }

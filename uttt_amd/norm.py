@@ -89,8 +89,8 @@ class _LayerNorm(torch.autograd.Function):
 
 def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None,
                eps: float = 1e-5) -> Tensor:
-    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis, of any
-    length; mean, variance and the products in fp32, rounded once to x's dtype.
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis, of up to
+    2^27 elements; mean, variance and the products in fp32, rounded once to x's dtype.
 
     x [..., N] in fp32, bf16 or fp16; weight and bias [N], each None or in any
     of the three (fp32 weights with bf16 activations included).  Gradients have
