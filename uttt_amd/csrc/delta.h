@@ -278,8 +278,8 @@ struct Scan {
     return true;
   }
 };
-inline unsigned scan_blocks(const Args& a, int width) {
-  return (unsigned)(((int64_t)a.nseq * a.Hv + 7) / 8 * 8 * ((a.Dv + width - 1) / width));
+inline int64_t scan_blocks(const Args& a, int width) {
+  return ((int64_t)a.nseq * a.Hv + 7) / 8 * 8 * ((a.Dv + width - 1) / width);
 }
 // 16-column tiles of a scan's workgroup.  Wide ones do more work a CU, narrow
 // ones end a long sequence sooner.  What is estimated: rounds of workgroups
@@ -397,7 +397,7 @@ inline void bind_workspace(Args& a, const Workspace& w, uint8_t* ws, bool packed
 }
 
 // delta_fwd.hip: the argument checks of both directions.
-int check_args(const Args& a, int B, bool packed, const char* what);
+int check_args(const Args& a, int B, bool packed, bool backward, const char* what);
 
 }  // namespace delta
 }  // namespace uttt

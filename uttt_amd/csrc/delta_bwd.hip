@@ -830,13 +830,13 @@ template <int KS>
 int launch_bwd(const Args& a, hipStream_t st) {
   switch (scan_tiles(a)) {
     case 1:
-      hipLaunchKernelGGL((delta_scan_bwd_kernel<KS, 1>), dim3(scan_blocks(a, 16)), dim3(512), 0, st, a);
+      hipLaunchKernelGGL((delta_scan_bwd_kernel<KS, 1>), dim3((unsigned)scan_blocks(a, 16)), dim3(512), 0, st, a);
       break;
     case 2:
-      hipLaunchKernelGGL((delta_scan_bwd_kernel<KS, 2>), dim3(scan_blocks(a, 32)), dim3(512), 0, st, a);
+      hipLaunchKernelGGL((delta_scan_bwd_kernel<KS, 2>), dim3((unsigned)scan_blocks(a, 32)), dim3(512), 0, st, a);
       break;
     default:
-      hipLaunchKernelGGL((delta_scan_bwd_kernel<KS, 4>), dim3(scan_blocks(a, 64)), dim3(512), 0, st, a);
+      hipLaunchKernelGGL((delta_scan_bwd_kernel<KS, 4>), dim3((unsigned)scan_blocks(a, 64)), dim3(512), 0, st, a);
   }
   if (const int rc = check_launch("delta_scan_bwd")) return rc;
   if (a.nchunks == 0) return UTTT_OK;
@@ -878,7 +878,7 @@ extern "C" int uttt_gated_delta_bwd(const void* q, const int64_t* q_strides, con
   a.B = B; a.T = T; a.Hk = Hk; a.Hv = Hv; a.Dk = Dk; a.Dv = Dv; a.nseq = nseq;
   a.cps = (T + kC - 1) / kC;
   a.scale = scale;
-  if (const int rc = check_args(a, B, packed, what)) return rc;
+  if (const int rc = check_args(a, B, packed, true, what)) return rc;
   a.nchunks = chunk_slots(B, T, nseq, packed);
   UTTT_REQUIRE(T == 0 || (u_saved && s_saved && dout && dq && dk && dv && dg && dbeta), "%s: null pointer", what);
   for (const void* p : {u_saved, s_saved, dout, (const void*)dq, (const void*)dk, (const void*)dv,

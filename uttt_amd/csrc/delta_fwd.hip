@@ -450,7 +450,7 @@ __global__ __launch_bounds__(512, KS * NT <= 4 ? 4 : 2) void delta_scan_kernel(A
 
 template <int KS, int NT>
 void launch_scan_as(const Args& a, hipStream_t st) {
-  const dim3 grid(scan_blocks(a, 16 * NT));
+  const dim3 grid((unsigned)scan_blocks(a, 16 * NT));
   if (a.s0) hipLaunchKernelGGL((delta_scan_kernel<KS, NT, true>), grid, dim3(512), 0, st, a);
   else hipLaunchKernelGGL((delta_scan_kernel<KS, NT, false>), grid, dim3(512), 0, st, a);
 }
@@ -468,7 +468,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 }  // namespace
 
-int check_args(const Args& a, int B, bool packed, const char* what) {
+int check_args(const Args& a, int B, bool packed, bool backward, const char* what) {
   UTTT_REQUIRE(B >= 1 && a.T >= 0 && a.nseq >= 1 && a.Hk >= 1 && a.Hv >= 1,
                "%s: bad sizes B=%d T=%d sequences=%d Hk=%d Hv=%d", what, B, a.T, a.nseq, a.Hk, a.Hv);
   UTTT_REQUIRE(a.Hv % a.Hk == 0, "%s: Hv=%d must be a multiple of Hk=%d", what, a.Hv, a.Hk);
@@ -478,8 +478,12 @@ int check_args(const Args& a, int B, bool packed, const char* what) {
                "%s: Dv=%d must be a multiple of 8 up to 65536", what, a.Dv);
   UTTT_REQUIRE(packed ? B == 1 : a.nseq == B, "%s: %d sequences in a batch of %d", what, a.nseq, B);
   const int64_t slots = chunk_slots(B, a.T, a.nseq, packed);
-  UTTT_REQUIRE(slots >= 0 && slots * a.Hv < (1LL << 31) &&
-                   ((int64_t)a.nseq * a.Hv + 8) * ((a.Dv + 15) / 16) < (1LL << 31),
+  // a launch has fewer than 2^32 threads: of a chunk and key head (operands,
+  // gradients), of a workgroup of the scans
+  const int64_t chunk = backward && steps_of(a.Dk) > 2 ? 128 * steps_of(a.Dk) : 256;
+  const int64_t scans = scan_blocks(a, 16 * scan_tiles(a.T, a.nseq, a.Hv, a.Dv, packed));
+  UTTT_REQUIRE(slots >= 0 && slots * a.Hv < (1LL << 31) && slots * a.Hk * chunk < (1LL << 32) &&
+                   scans * 512 < (1LL << 32),
                "%s: too many chunks and heads for one launch", what);
   UTTT_REQUIRE(a.T == 0 || (a.q && a.k && a.v && a.g && a.beta), "%s: null pointer", what);
   UTTT_REQUIRE(aligned16(a.q) && aligned16(a.k) && aligned16(a.v), "%s: q, k and v must be 16-byte aligned",
@@ -536,7 +540,7 @@ extern "C" int uttt_gated_delta_fwd(const void* q, const int64_t* q_strides, con
   a.B = B; a.T = T; a.Hk = Hk; a.Hv = Hv; a.Dk = Dk; a.Dv = Dv; a.nseq = nseq;
   a.cps = (T + kC - 1) / kC;
   a.scale = scale;
-  if (const int rc = check_args(a, B, packed, what)) return rc;
+  if (const int rc = check_args(a, B, packed, false, what)) return rc;
   a.nchunks = chunk_slots(B, T, nseq, packed);
   UTTT_REQUIRE(out || T == 0, "%s: null output", what);
   UTTT_REQUIRE(aligned16(out) && aligned16(u_saved) && aligned16(s_saved) && aligned16(workspace),

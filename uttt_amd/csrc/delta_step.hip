@@ -179,9 +179,11 @@ __global__ __launch_bounds__(kStepThreads) void delta_step_kernel(StepArgs a) {
   }
 }
 
+int64_t step_blocks(const StepArgs& a, int LC) { return (int64_t)a.B * a.Hv * ((a.Dv + 4 * LC - 1) / (4 * LC)); }
+
 template <class TT, int LC, int RPT>
 void launch_step_as(const StepArgs& a, hipStream_t st) {
-  const int64_t blocks = (int64_t)a.B * a.Hv * ((a.Dv + 4 * LC - 1) / (4 * LC));
+  const int64_t blocks = step_blocks(a, LC);
   hipLaunchKernelGGL((delta_step_kernel<TT, LC, RPT>), dim3((unsigned)blocks), dim3(kStepThreads), 0,
                      st, a);
 }
@@ -192,7 +194,7 @@ int launch_step(const StepArgs& a, hipStream_t st) {
   // less than 64 workgroups: 32 (16 heads of 128 x 128) 4.4 us against 4.8, 16
   // (4 of 256 x 256) 4.8 against 6.0; with 64 of them 5.0 against 4.9 and 6.3
   // against 6.5, with 256 10.0 against 5.9 and 15.0 against 8.8
-  const bool narrow = (int64_t)a.B * a.Hv * ((a.Dv + 63) / 64) < 64;
+  const bool narrow = step_blocks(a, 16) < 64;
   if (narrow) {
     if (a.Dk <= 64) launch_step_as<TT, 4, 1>(a, st);
     else if (a.Dk <= 128) launch_step_as<TT, 4, 2>(a, st);
@@ -228,7 +230,8 @@ extern "C" int uttt_gated_delta_step(const void* q, const int64_t* q_strides, co
   UTTT_REQUIRE(dtype_bytes(dtype) && dtype_bytes(g_dtype) && dtype_bytes(beta_dtype),
                "%s: dtype codes %d, %d, %d", what, dtype, g_dtype, beta_dtype);
   UTTT_REQUIRE(indices || B <= slots, "%s: %d rows without indices, %d slots", what, B, slots);
-  UTTT_REQUIRE((int64_t)B * Hv * ((Dv + 15) / 16) < (1LL << 31), "%s: too many rows and heads", what);
+  // of 256 threads, and a launch has fewer than 2^32
+  UTTT_REQUIRE((int64_t)B * Hv * ((Dv + 63) / 64) < (1LL << 24), "%s: too many rows and heads", what);
   if (B == 0 || T == 0) return UTTT_OK;
   UTTT_REQUIRE(q && k && v && g && beta && state && out && q_strides && k_strides && v_strides,
                "%s: null pointer", what);

@@ -177,6 +177,8 @@ int launch_rotary(RotArgs a, bool inter, hipStream_t st) {
   const int64_t all = (int64_t)a.B * a.L;
   if (all / tokens < 1024) tokens = (all + 1023) / 1024 < tokens ? (all + 1023) / 1024 : tokens;
   a.tokens = (int)tokens;
+  UTTT_REQUIRE((all + tokens - 1) / tokens * kRotThreads < (1LL << 32),
+               "rotary_axes: too many tokens of %d features for one launch", a.H * a.D);
   if (fits(V)) launch_rotary_as<TT, V>(a, inter, st);
   else if (fits(V / 2)) launch_rotary_as<TT, V / 2>(a, inter, st);
   else launch_rotary_as<TT, 1>(a, inter, st);
