@@ -17,8 +17,9 @@ Q = 8 * H * H
 BF16, F32 = torch.bfloat16, torch.float32
 
 # lens: one number of tokens and rows B, or packed sequences of a token axis that
-# starts with `front` and ends with `back` tokens of none; tiles: the 16-column
-# tiles a scan's workgroup takes, which a change of that choice has to keep here
+# starts with `front` and ends with `behind` tokens of none; tiles: the 16-column
+# tiles a scan's workgroup takes (back: in the backward, where it takes others),
+# which a change of that choice has to keep here
 CASES = [
     dict(B=2, lens=[330], Hk=1, Hv=2, Dk=64, Dv=64, tiles=1),
     dict(B=1, lens=[200], Hk=2, Hv=2, Dk=192, Dv=72, tiles=1),
@@ -29,13 +30,13 @@ CASES = [
     dict(B=24, lens=[330], Hk=4, Hv=8, Dk=64, Dv=40, tiles=4),
     dict(B=32, lens=[200], Hk=2, Hv=4, Dk=96, Dv=72, tiles=4, gates=BF16),
     dict(B=32, lens=[200], Hk=4, Hv=4, Dk=128, Dv=72, tiles=4),
-    dict(B=16, lens=[200], Hk=2, Hv=4, Dk=192, Dv=136, tiles=4),
-    dict(B=8, lens=[270], Hk=4, Hv=8, Dk=256, Dv=136, tiles=4),
-    dict(B=0, lens=[300, 1, 0, 129, 250], front=7, back=13, Hk=8, Hv=16, Dk=64, Dv=64, tiles=1),
-    dict(B=0, lens=[64, 200, 0, 65, 40], front=20, back=11, Hk=32, Hv=96, Dk=40, Dv=40, tiles=2),
-    dict(B=0, lens=[271, 1, 128], front=0, back=0, Hk=48, Hv=48, Dk=64, Dv=136, tiles=2),
-    dict(B=0, lens=[330, 3, 0, 64, 65, 100, 10, 100], front=28, back=0, Hk=32, Hv=64, Dk=96, Dv=72, tiles=4),
-    dict(B=0, lens=[200, 0, 0, 17, 63, 80, 1, 20], front=0, back=19, Hk=16, Hv=32, Dk=128, Dv=136, tiles=4),
+    dict(B=16, lens=[200], Hk=2, Hv=4, Dk=192, Dv=136, tiles=4, back=2),
+    dict(B=8, lens=[270], Hk=4, Hv=8, Dk=256, Dv=136, tiles=2),
+    dict(B=0, lens=[300, 1, 0, 129, 250], front=7, behind=13, Hk=8, Hv=16, Dk=64, Dv=64, tiles=1),
+    dict(B=0, lens=[64, 200, 0, 65, 40], front=20, behind=11, Hk=32, Hv=96, Dk=40, Dv=40, tiles=2),
+    dict(B=0, lens=[271, 1, 128], front=0, behind=0, Hk=48, Hv=48, Dk=64, Dv=136, tiles=2),
+    dict(B=0, lens=[330, 3, 0, 64, 65, 100, 10, 100], front=28, behind=0, Hk=32, Hv=64, Dk=96, Dv=72, tiles=4),
+    dict(B=0, lens=[200, 0, 0, 17, 63, 80, 1, 20], front=0, behind=19, Hk=16, Hv=32, Dk=128, Dv=136, tiles=4),
 ]
 
 
@@ -44,12 +45,14 @@ def name_of(c):
     return f"{rows}-{c['Hk']}-{c['Hv']}-{c['Dk']}x{c['Dv']}-{c['tiles']}"
 
 
-def scan_tiles(T, nseq, Hv, Dv, packed):
+def scan_tiles(T, nseq, Hv, Dk, Dv, packed, backward=False):
     """The choice of csrc/delta.h."""
     total, cps = T // 64 + nseq, (T + 63) // 64
     mean = -(-total // nseq)
     cost = {}
     for tiles, tenths in ((1, 20), (2, 23), (4, 30)):
+        if tiles == 4 and Dk > (128 if backward else 192):
+            continue
         blocks = -(-Dv // (16 * tiles))
         if packed:
             cost[tiles] = max(min(3 * mean, total), total * Hv * blocks // 256) * tenths
@@ -62,7 +65,7 @@ def shape(c):
     """tokens, sequences, packed"""
     if c["B"]:
         return c["lens"][0], c["B"], False
-    return c["front"] + sum(c["lens"]) + c["back"], len(c["lens"]), True
+    return c["front"] + sum(c["lens"]) + c["behind"], len(c["lens"]), True
 
 
 def make(c, seed=0):

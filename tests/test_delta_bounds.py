@@ -26,10 +26,11 @@ def test_gradients_of_the_oracle():
 @pytest.mark.parametrize("c", CASES, ids=name_of)
 def test_cases_take_their_column_widths(c):
     T, n, packed = shape(c)
-    assert scan_tiles(T, n, c["Hv"], c["Dv"], packed) == c["tiles"]
+    assert scan_tiles(T, n, c["Hv"], c["Dk"], c["Dv"], packed) == c["tiles"]
+    assert scan_tiles(T, n, c["Hv"], c["Dk"], c["Dv"], packed, True) == c.get("back", c["tiles"])
     assert max(c["lens"]) > 2 * C   # three chunks or more
     if packed:
-        assert offsets(c)[-1] + c["back"] == T and len(by_sequence(c, torch.zeros(1, T))) == n
+        assert offsets(c)[-1] + c["behind"] == T and len(by_sequence(c, torch.zeros(1, T))) == n
 
 
 def terms(c, a, got):

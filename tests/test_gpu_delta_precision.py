@@ -1,0 +1,38 @@
+"""The fp32 results of the gated delta rule are exact to fp32's order: against the
+64-bit recurrence, per case in the 2-norm, within N = 16 * 2^-24.
+
+A chunk's part of the state passes through at most Dk / 32 + 1 accumulations of
+K S0, R, 12 of U = T R, 6 of K^T U and the decay, some 30 roundings of at most
+2^-24 that add up as their square root, 5.5; T and its norm (up to 2 for these
+keys) carry U's to at most 11 of them, decays and earlier chunks come in as they
+are.  16 are allowed.  A product with an operand cut to two bf16 values, 2^-16 of
+it left out, is off by 20 N."""
+import pytest
+import torch
+
+from delta_cases import CASES, F32, groups_of_heads, make, name_of, offsets, reference
+
+pytestmark = pytest.mark.gpu
+N = 16 * 2.0 ** -24
+EXACT = [dict(c, gates=F32) for c in CASES]
+
+
+@pytest.mark.parametrize("c", EXACT, ids=name_of)
+def test_states_and_their_gradients(c):
+    """The gradient's chain has Q^T dO, P^T dO and K dS' beside T^T dU and K^T dR: as
+    many roundings again."""
+    from uttt_amd.delta import gated_delta_rule
+    x, do, dht = make(c)
+    y = {n: t.cuda() for n, t in x.items()}
+    cu = None if c["B"] else torch.tensor(offsets(c), dtype=torch.int32, device="cuda")
+    args = [y[n] for n in ("q", "k", "v", "g", "beta")]
+    S = gated_delta_rule(*args, initial_state=y["h0"], output_final_state=True, cu_seqlens=cu)[1]
+    y["h0"].requires_grad_()   # with what a backward reads
+    o, S2 = gated_delta_rule(*args, initial_state=y["h0"], output_final_state=True, cu_seqlens=cu)
+    assert torch.equal(S2, S)
+    (dh0,) = torch.autograd.grad([o, S2], y["h0"], [do.cuda(), dht.cuda()])
+    for heads in groups_of_heads(c):
+        ref = reference(c, x, do, dht, heads, "cuda")[1]
+        for name, got, want in (("state", S, ref["S"][:, -1]), ("dh0", dh0, ref["dh0"])):
+            off, norm = (got[:, heads].double() - want).norm().item(), want.norm().item()
+            assert off <= N * norm, (name, heads.tolist(), off / norm)

@@ -16,11 +16,12 @@
 //   dS0 = gam_C dS' + (s gam Q)^T dO - (b gam K)^T dR
 //
 // Precision.  The state and its gradient are fp32 and stay exact to fp32's
-// order: a product with one of them, with U, T, P, R or their gradients takes
-// that fp32 operand as the sum of two bf16 values (hi = bf16(x), lo = bf16(x -
-// hi); at most 2^-16 of x is left out) and adds both products in fp32; q, k, v
-// and do are bf16 as given.  What a backward keeps or exchanges (U, S0, dR,
-// dS') is stored as the two parts too, planes hi and lo.
+// order: a product with one of them, with U, T, R, P, e^{G_C - G} U or their
+// gradients takes that fp32 operand as the sum of three bf16 values (x1 = bf16(x),
+// x2 = bf16(x - x1), x3 = bf16(x - x1 - x2), all of its 24 bits) and adds the
+// products that are not below 2^-24 in fp32; q, k, v and do are bf16 as given.
+// Where only bf16 results come of it, the first two parts go in (at most 2^-16
+// left out): S0, U and P for the outputs.
 //
 // Fragments.  v_mfma_f32_16x16x32_bf16 takes from lane (r = lane % 16, q =
 // lane / 16) eight consecutive values 8q..8q+7 of the contracted axis for row
@@ -38,7 +39,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kC = 64;           // tokens of a chunk
 constexpr int kTFrags = 6;       // nonzero 16 x 32 fragments of a triangular 64 x 64 operand
-constexpr int kTriBytes = 4 * kTFrags * 1024;   // T hi, T lo, P hi, P lo
+constexpr int kPFrag = 3 * kTFrags;                  // P's first fragment, behind T's three parts
+constexpr int kTriBytes = (kPFrag + 2 * kTFrags) * 1024;      // P in two parts
+constexpr int kTriBwdBytes = (kPFrag + 3 * kTFrags) * 1024;   // P^T in three
 constexpr int kScal = 5 * kC;    // gam, e^{G_C - G}, beta and G in two parts, per token
 
 struct Args {
@@ -51,7 +54,7 @@ struct Args {
   float scale;
   const int4* table;             // [nchunks] sequence, first token, tokens; packed sequences only
   const int4* seqs;              // [nseq] first chunk, sequence, first token, tokens
-  uint8_t* tri;                  // [nchunks, Hv] kTriBytes
+  uint8_t* tri;                  // [nchunks, Hv] kTriBytes, in the backward kTriBwdBytes
   float* scal;                   // [nchunks, Hv, kScal]
   uint8_t* kt;                   // [nchunks, Hk, 4 KS] KiB: K^T fragments
   uint8_t* qt;                   // the same of Q (backward)
@@ -117,6 +120,20 @@ __device__ __forceinline__ void split8(f32x4 a, f32x4 b, bf16x8& hi, bf16x8& lo)
     lo[i] = (__bf16)(a[i] - (float)hi[i]);
     lo[4 + i] = (__bf16)(b[i] - (float)hi[4 + i]);
   }
+}
+
+// The first PARTS bf16 parts of a, b.
+template <int PARTS>
+__device__ __forceinline__ void split8(f32x4 a, f32x4 b, bf16x8 (&out)[PARTS]) {
+#pragma unroll
+  for (int k = 0; k < PARTS; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      out[k][i] = (__bf16)a[i];
+      out[k][4 + i] = (__bf16)b[i];
+      a[i] -= (float)out[k][i];
+      b[i] -= (float)out[k][4 + i];
+    }
 }
 
 // Raw buffers: a lane whose offset has bit 31 (past any record count) reads
@@ -188,6 +205,24 @@ __device__ __forceinline__ Parts parts_of(f32x4 x) {
     p.lo[i] = pack_bf16x2(x[2 * i] - __uint_as_float(h << 16), x[2 * i + 1] - __uint_as_float(h & 0xffff0000u));
   }
   return p;
+}
+// The same as three parts.
+struct Parts3 {
+  u32x2 p[3];
+};
+__device__ __forceinline__ Parts3 parts3_of(f32x4 x) {
+  Parts3 r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      r.p[k][i] = pack_bf16x2(a, b);
+      a -= __uint_as_float(r.p[k][i] << 16);
+      b -= __uint_as_float(r.p[k][i] & 0xffff0000u);
+    }
+  }
+  return r;
 }
 __device__ __forceinline__ u32x2 round_of(f32x4 x) {
   u32x2 p;
@@ -295,12 +330,16 @@ inline int64_t scan_blocks(const Args& a, int width) {
 //   8 x 1024 tokens, 4 heads of 192                     81,  61,  97
 //   16 x 2048 tokens, 12 heads of 128                  577, 418, 344
 //   16 x 2048 tokens, 4 heads of 256                   528, 406, 297
-inline int scan_tiles(int64_t T, int nseq, int Hv, int Dv, bool packed) {
+// The three parts of 64 columns fit in LDS up to 192 features, the backward's up
+// to 128.
+constexpr int scan_widest(int KS, bool backward) { return KS <= (backward ? 4 : 6) ? 4 : 2; }
+inline int scan_tiles(int64_t T, int nseq, int Hv, int Dk, int Dv, bool packed, bool backward) {
   const int tiles[3] = {1, 2, 4}, tenths[3] = {20, 23, 30};
+  const int widths = scan_widest((Dk + 31) / 32, backward) == 4 ? 3 : 2;
   const int64_t total = T / kC + nseq, mean = (total + nseq - 1) / nseq, cps = (T + kC - 1) / kC;
   int best = 1;
   int64_t least = INT64_MAX;
-  for (int i = 0; i < 3; ++i) {
+  for (int i = 0; i < widths; ++i) {
     const int64_t blocks = (Dv + 16 * tiles[i] - 1) / (16 * tiles[i]);
     int64_t cost;
     if (packed) {
@@ -316,7 +355,9 @@ inline int scan_tiles(int64_t T, int nseq, int Hv, int Dv, bool packed) {
   }
   return best;
 }
-inline int scan_tiles(const Args& a) { return scan_tiles(a.T, a.nseq, a.Hv, a.Dv, a.table != nullptr); }
+inline int scan_tiles(const Args& a, bool backward) {
+  return scan_tiles(a.T, a.nseq, a.Hv, a.Dk, a.Dv, a.table != nullptr, backward);
+}
 
 // Features up to which a kernel instance goes, in steps of 32: the next of 2,
 // 3, 4, 6, 8 (K, Q past Dk are zeros in LDS).
@@ -364,12 +405,12 @@ inline Workspace workspace_of(int64_t B, int64_t T, int nseq, int Hk, int Hv, in
   w.seqs = take(packed ? (size_t)nseq * 16 : 0);
   w.scal = take(n * Hv * kScal * 4);
   w.kt = take(frags);
-  w.tri = take(n * Hv * kTriBytes);
+  w.tri = take(n * Hv * (backward ? kTriBwdBytes : kTriBytes));
   // Where 16 columns a workgroup are taken, each of them loads all of K and Q:
   // then from a copy in fragment order, 1 KiB a load, and not 64 bytes of each
   // of 16 rows (a chunk of 192 features 2.1 -> 1.5 us; with more columns a
   // workgroup the copy costs more than it saves).
-  const bool copies = scan_tiles(T, nseq, Hv, Dv, packed) == 1;
+  const bool copies = scan_tiles(T, nseq, Hv, Dk, Dv, packed, backward) == 1;
   w.kf = take(copies ? frags : 0);
   w.qf = take(copies && !backward ? frags : 0);
   if (!copies) w.kf = w.qf = SIZE_MAX;

@@ -25,11 +25,11 @@ namespace {
 
 template <int KS, int NT>
 struct ScanBwdLds {
-  uint8_t S[2][KS * NT * 1024];   // dS'
+  uint8_t S[3][KS * NT * 1024];   // dS', in three parts as the others
   uint8_t G[2 * NT * 1024];       // dO
-  uint8_t U[2][2 * NT * 1024];    // dU
-  uint8_t H[2][2 * NT * 1024];    // s gam dO
-  uint8_t E[2][2 * NT * 1024];    // -b gam dR
+  uint8_t U[3][2 * NT * 1024];    // dU
+  uint8_t H[3][2 * NT * 1024];    // s gam dO
+  uint8_t E[3][2 * NT * 1024];    // -b gam dR
   f32x4 R[4][NT][64];             // dR in fp32, as its waves' lanes hold it
 };
 
@@ -63,14 +63,14 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
                          ? a.dhT[((int64_t)s.head * a.Dk + feat) * a.Dv + col + n] : 0.0f;
     }
 
-  bf16x8 qtf[FT][2], tf[2][2], ktf[FT][2];
+  bf16x8 qtf[FT][2], tf[2][3], ktf[FT][2];
   f32x4 bg;
   float gc;
   // Operands of the chunk before: pointers that go along, at first those of the
   // last chunk.  `left`: tokens from the chunk on to the sequence's end; 0
   // before its first chunk.
   const int lastc = s.nc - 1;
-  const uint8_t* trip = a.tri + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kTriBytes;
+  const uint8_t* trip = a.tri + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kTriBwdBytes;
   const int64_t trans_at = ((int64_t)(s.c0 + lastc) * a.Hk + s.hk) * (4 * KS * 1024);
   const uint8_t *ktp = a.kt + trans_at, *qtp = a.qt + trans_at;
   const float* scp = a.scal + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kScal;
@@ -81,12 +81,12 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
     for (int ks = 0; ks < 2; ++ks) {
       // step 0 of the lower tiles is zero and not stored: step 1 again, unused
       const int f = upper_frag(wave, wave < 2 ? ks : 1);
-      tf[ks][0] = load_frag(tr, at, f * 1024);
-      tf[ks][1] = load_frag(tr, at, (kTFrags + f) * 1024);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) tf[ks][k] = load_frag(tr, at, (k * kTFrags + f) * 1024);
     }
     bg = load_f4(sr, s_at) * load_f4(sr, s_at, 8 * kC);
     scp -= a.Hv * kScal;
-    trip -= (int64_t)a.Hv * kTriBytes;
+    trip -= (int64_t)a.Hv * kTriBwdBytes;
   };
   const auto load_trans = [&](int left, const uint8_t*& p, bf16x8 (&x)[FT][2]) {
     const Rsrc tr = buffer_at(p);
@@ -111,10 +111,10 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
       if (tile < 2 * KS)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const Parts p = parts_of(S[f][n]);
+          const Parts3 p = parts3_of(S[f][n]);
           const uint32_t at = ((tile >> 1) * NT + n) * 1024 + (tile & 1) * 512 + put;
-          *reinterpret_cast<u32x2*>(lds.S[0] + at) = p.hi;
-          *reinterpret_cast<u32x2*>(lds.S[1] + at) = p.lo;
+#pragma unroll
+          for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x2*>(lds.S[k] + at) = p.p[k];
         }
     }
   };
@@ -165,37 +165,40 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const bf16x8 hi = get(lds.H[0], t * NT + n), lo = get(lds.H[1], t * NT + n);
 #pragma unroll
-        for (int f = 0; f < FT; ++f)
-          if (wave * FT + f < 2 * KS) {
-            S[f][n] = mfma(qtf[f][t], hi, S[f][n]);
-            S[f][n] = mfma(qtf[f][t], lo, S[f][n]);
-          }
+        for (int k = 0; k < 3; ++k) {
+          const bf16x8 h = get(lds.H[k], t * NT + n);
+#pragma unroll
+          for (int f = 0; f < FT; ++f)
+            if (wave * FT + f < 2 * KS) S[f][n] = mfma(qtf[f][t], h, S[f][n]);
+        }
       }
     load_qt(next);
     lds_barrier();   // dU is in LDS
     f32x4 R[NT] = {};   // dR = T^T dU
     {
-      f32x4 R2[NT] = {};
+      f32x4 R2[NT] = {}, R3[NT] = {};   // the products below 2^-7, below 2^-15 of the first
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
         if (ks >= wave >> 1)
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const bf16x8 hi = get(lds.U[0], ks * NT + n), lo = get(lds.U[1], ks * NT + n);
-            R[n] = mfma(tf[ks][0], hi, R[n]);
-            R2[n] = mfma(tf[ks][1], hi, R2[n]);
-            R2[n] = mfma(tf[ks][0], lo, R2[n]);
+            const bf16x8 u1 = get(lds.U[0], ks * NT + n), u2 = get(lds.U[1], ks * NT + n), u3 = get(lds.U[2], ks * NT + n);
+            R[n] = mfma(tf[ks][0], u1, R[n]);
+            R2[n] = mfma(tf[ks][1], u1, R2[n]);
+            R3[n] = mfma(tf[ks][2], u1, R3[n]);
+            R2[n] = mfma(tf[ks][0], u2, R2[n]);
+            R3[n] = mfma(tf[ks][1], u2, R3[n]);
+            R3[n] = mfma(tf[ks][0], u3, R3[n]);
           }
 #pragma unroll
-      for (int n = 0; n < NT; ++n) R[n] += R2[n];
+      for (int n = 0; n < NT; ++n) R[n] += R2[n] + R3[n];
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const Parts p = parts_of(-bg * R[n]);
-      *reinterpret_cast<u32x2*>(lds.E[0] + put_tok + n * 1024) = p.hi;
-      *reinterpret_cast<u32x2*>(lds.E[1] + put_tok + n * 1024) = p.lo;
+      const Parts3 p = parts3_of(-bg * R[n]);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x2*>(lds.E[k] + put_tok + n * 1024) = p.p[k];
       lds.R[wave][n][lane] = R[n];
     }
     load_t(next);
@@ -204,13 +207,13 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const bf16x8 hi = get(lds.E[0], t * NT + n), lo = get(lds.E[1], t * NT + n);
 #pragma unroll
-        for (int f = 0; f < FT; ++f)
-          if (wave * FT + f < 2 * KS) {
-            S[f][n] = mfma(ktf[f][t], hi, S[f][n]);
-            S[f][n] = mfma(ktf[f][t], lo, S[f][n]);
-          }
+        for (int k = 0; k < 3; ++k) {
+          const bf16x8 e = get(lds.E[k], t * NT + n);
+#pragma unroll
+          for (int f = 0; f < FT; ++f)
+            if (wave * FT + f < 2 * KS) S[f][n] = mfma(ktf[f][t], e, S[f][n]);
+        }
       }
     if (c > 0) put_state();
     load_trans(next, ktp, ktf);
@@ -236,7 +239,7 @@ __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, in
                                                 ScanBwdLds<KS, NT>& lds) {
   const int r = lane & 15, q = lane >> 4, col = s.col0 + NT * r;
   const uint32_t dead = miss_from(col, a.Dv), put_tok = put_at<NT>(wave, r, q);
-  bf16x8 kf[KS], pf[2][2];
+  bf16x8 kf[KS], pf[2][3];
   f32x4 ge, gam, bt;
   Cols<NT> gr[4];
   const int lastc = s.nc - 1;
@@ -251,7 +254,7 @@ __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, in
   const uint32_t along = copies ? 1024 : 64;
   const uint32_t last_half = miss_from(32 * (KS - 1) + 8 * q, a.Dk), before_half = miss_from(32 * (KS - 2) + 8 * q, a.Dk);
   const uint16_t* gp = a.dout + s.b * a.do_sb + s.hv * a.do_sh + (s.tok0 + (int64_t)lastc * kC) * a.do_st;
-  const uint8_t* trip = a.tri + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kTriBytes;
+  const uint8_t* trip = a.tri + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kTriBwdBytes;
   const float* gamp = a.scal + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kScal;   // goes with dO
   const float *betap = gamp, *gep = gamp;                                         // with dR, with K
   const uint32_t grow = 2 * ((16 * wave + 4 * q) * (uint32_t)a.do_st + col);
@@ -282,11 +285,11 @@ __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, in
     const uint32_t at = lane * 16 | miss_from(0, left);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      const int f = 2 * kTFrags + upper_frag(wave, wave < 2 ? ks : 1);
-      pf[ks][0] = load_frag(tr, at, f * 1024);
-      pf[ks][1] = load_frag(tr, at, (kTFrags + f) * 1024);
+      const int f = kPFrag + upper_frag(wave, wave < 2 ? ks : 1);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) pf[ks][k] = load_frag(tr, at, (k * kTFrags + f) * 1024);
     }
-    trip -= (int64_t)a.Hv * kTriBytes;
+    trip -= (int64_t)a.Hv * kTriBwdBytes;
   };
   const auto load_beta = [&](int left) {
     bt = load_f4(buffer_at(betap), 4 * (16 * wave + 4 * q) | miss_from(0, left), 8 * kC);
@@ -304,7 +307,7 @@ __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, in
   };
   f32x4 Z[NT];   // P^T dO
   const auto make_z = [&]() {
-    f32x4 Z2[NT] = {};
+    f32x4 Z2[NT] = {}, Z3[NT] = {};
 #pragma unroll
     for (int n = 0; n < NT; ++n) Z[n] = f32x4{};
 #pragma unroll
@@ -315,9 +318,10 @@ __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, in
           const bf16x8 g = *reinterpret_cast<const bf16x8*>(lds.G + (ks * NT + n) * 1024 + lane * 16);
           Z[n] = mfma(pf[ks][0], g, Z[n]);
           Z2[n] = mfma(pf[ks][1], g, Z2[n]);
+          Z3[n] = mfma(pf[ks][2], g, Z3[n]);
         }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) Z[n] += Z2[n];
+    for (int n = 0; n < NT; ++n) Z[n] += Z2[n] + Z3[n];
   };
   const auto put_h = [&]() {
 #pragma unroll
@@ -325,9 +329,9 @@ __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, in
       f32x4 g;
 #pragma unroll
       for (int i = 0; i < 4; ++i) g[i] = gr[i].get(n);
-      const Parts p = parts_of(g * (gam * a.scale));
-      *reinterpret_cast<u32x2*>(lds.H[0] + put_tok + n * 1024) = p.hi;
-      *reinterpret_cast<u32x2*>(lds.H[1] + put_tok + n * 1024) = p.lo;
+      const Parts3 p = parts3_of(g * (gam * a.scale));
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x2*>(lds.H[k] + put_tok + n * 1024) = p.p[k];
     }
   };
 
@@ -352,19 +356,20 @@ __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, in
     const int left = s.len - c * kC, next = c > 0 ? kC : 0, later = c > 1 ? kC : 0;
     lds_barrier();   // dS' and s gam dO are in LDS
     {
-      f32x4 X[NT] = {}, X2[NT] = {};
+      f32x4 X[NT] = {}, X2[NT] = {}, X3[NT] = {};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           X[n] = mfma(kf[ks], get(lds.S[0], ks * NT + n), X[n]);
           X2[n] = mfma(kf[ks], get(lds.S[1], ks * NT + n), X2[n]);
+          X3[n] = mfma(kf[ks], get(lds.S[2], ks * NT + n), X3[n]);
         }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const Parts p = parts_of(ge * (X[n] + X2[n]) + Z[n]);
-        *reinterpret_cast<u32x2*>(lds.U[0] + put_tok + n * 1024) = p.hi;
-        *reinterpret_cast<u32x2*>(lds.U[1] + put_tok + n * 1024) = p.lo;
+        const Parts3 p = parts3_of(ge * (X[n] + (X2[n] + X3[n])) + Z[n]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x2*>(lds.U[k] + put_tok + n * 1024) = p.p[k];
       }
     }
     put_do();        // of the chunk before
@@ -828,7 +833,7 @@ __global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads
 
 template <int KS>
 int launch_bwd(const Args& a, hipStream_t st) {
-  switch (scan_tiles(a)) {
+  switch (scan_tiles(a, true)) {
     case 1:
       hipLaunchKernelGGL((delta_scan_bwd_kernel<KS, 1>), dim3((unsigned)scan_blocks(a, 16)), dim3(512), 0, st, a);
       break;
@@ -836,7 +841,8 @@ int launch_bwd(const Args& a, hipStream_t st) {
       hipLaunchKernelGGL((delta_scan_bwd_kernel<KS, 2>), dim3((unsigned)scan_blocks(a, 32)), dim3(512), 0, st, a);
       break;
     default:
-      hipLaunchKernelGGL((delta_scan_bwd_kernel<KS, 4>), dim3((unsigned)scan_blocks(a, 64)), dim3(512), 0, st, a);
+      if constexpr (scan_widest(KS, true) == 4)
+        hipLaunchKernelGGL((delta_scan_bwd_kernel<KS, 4>), dim3((unsigned)scan_blocks(a, 64)), dim3(512), 0, st, a);
   }
   if (const int rc = check_launch("delta_scan_bwd")) return rc;
   if (a.nchunks == 0) return UTTT_OK;

@@ -32,13 +32,13 @@ namespace delta {
 namespace {
 
 // LDS of a scan's workgroup: operand fragments (32 contracted rows x 16
-// columns, 1 KiB), in two bf16 parts.
+// columns, 1 KiB) of each bf16 part.
 template <int KS, int NT>
 struct ScanLds {
-  uint8_t S[2][KS * NT * 1024];
-  uint8_t R[2][2 * NT * 1024];
+  uint8_t S[3][KS * NT * 1024];
+  uint8_t R[3][2 * NT * 1024];
   uint8_t U[2][2 * NT * 1024];
-  uint8_t E[2][2 * NT * 1024];   // e^{G_C - G} U
+  uint8_t E[3][2 * NT * 1024];   // e^{G_C - G} U
   int first[NT][16];             // a column's first token in the chunk whose R is not finite
   int bad;                       // whether there is one
 };
@@ -67,10 +67,6 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
   const uint32_t dead = l.dead;
   const uint32_t put = (r + 16 * (q >> 1)) * 16 + (q & 1) * 8;   // 4 rows of a tile in a fragment
   const uint32_t put_tok = (wave >> 1) * NT * 1024 + (wave & 1) * 512 + put;
-  const auto put_tile = [&](uint8_t (*buf)[2 * NT * 1024], int n, const Parts& p) {
-    *reinterpret_cast<u32x2*>(buf[0] + put_tok + n * 1024) = p.hi;
-    *reinterpret_cast<u32x2*>(buf[1] + put_tok + n * 1024) = p.lo;
-  };
   const auto get = [&](const uint8_t* buf, int f) {
     return *reinterpret_cast<const bf16x8*>(buf + f * 1024 + l.lane * 16);
   };
@@ -92,7 +88,7 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
   // chunk while R is made.
   constexpr bool kAhead = FT * NT < 16;
   struct Ops {
-    bf16x8 t[2][2], kt[FT][2];
+    bf16x8 t[2][3], kt[FT][2];
     f32x4 ge;
     float gc;
   };
@@ -107,8 +103,8 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
     for (int ks = 0; ks < 2; ++ks) {
       // step 1 of the upper tiles is zero and not stored: step 0 again, unused
       const int f = lower_frag(wave, wave < 2 ? 0 : ks);
-      o.t[ks][0] = load_frag(tr, at, f * 1024);
-      o.t[ks][1] = load_frag(tr, at, (kTFrags + f) * 1024);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) o.t[ks][k] = load_frag(tr, at, (k * kTFrags + f) * 1024);
     }
     o.ge = load_f4(sr, 4 * (16 * wave + 4 * q) | none, 4 * kC);
     o.gc = load_f1(sr, 4 * (kC - 1) | none);
@@ -132,10 +128,10 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
       if (tile < 2 * KS)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const Parts p = parts_of(S[f][n]);
+          const Parts3 p = parts3_of(S[f][n]);
           const uint32_t at = ((tile >> 1) * NT + n) * 1024 + (tile & 1) * 512 + put;
-          *reinterpret_cast<u32x2*>(lds.S[0] + at) = p.hi;
-          *reinterpret_cast<u32x2*>(lds.S[1] + at) = p.lo;
+#pragma unroll
+          for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x2*>(lds.S[k] + at) = p.p[k];
         }
     }
   };
@@ -196,25 +192,29 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
     int bad = lds.bad;
     f32x4 U[NT] = {};
     {
-      f32x4 U2[NT] = {};
+      f32x4 U2[NT] = {}, U3[NT] = {};   // the products below 2^-7, below 2^-15 of the first
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
         if (ks <= wave >> 1)
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const bf16x8 hi = get(lds.R[0], ks * NT + n), lo = get(lds.R[1], ks * NT + n);
-            U[n] = mfma(now.t[ks][0], hi, U[n]);
-            U2[n] = mfma(now.t[ks][1], hi, U2[n]);
-            U2[n] = mfma(now.t[ks][0], lo, U2[n]);
+            const bf16x8 r1 = get(lds.R[0], ks * NT + n), r2 = get(lds.R[1], ks * NT + n), r3 = get(lds.R[2], ks * NT + n);
+            U[n] = mfma(now.t[ks][0], r1, U[n]);
+            U2[n] = mfma(now.t[ks][1], r1, U2[n]);
+            U3[n] = mfma(now.t[ks][2], r1, U3[n]);
+            U2[n] = mfma(now.t[ks][0], r2, U2[n]);
+            U3[n] = mfma(now.t[ks][1], r2, U3[n]);
+            U3[n] = mfma(now.t[ks][0], r3, U3[n]);
           }
       asm volatile("" : "+v"(bad));   // read with R, not when U is made
 #pragma unroll
-      for (int n = 0; n < NT; ++n) U[n] += U2[n];
+      for (int n = 0; n < NT; ++n) U[n] += U2[n] + U3[n];
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const Parts p = parts_of(U[n]);
-      put_tile(lds.U, n, p);
+      *reinterpret_cast<u32x2*>(lds.U[0] + put_tok + n * 1024) = p.hi;
+      *reinterpret_cast<u32x2*>(lds.U[1] + put_tok + n * 1024) = p.lo;
       uh[n] = p.hi;
       ul[n] = p.lo;
     }
@@ -226,7 +226,11 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
       }
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) put_tile(lds.E, n, parts_of(now.ge * U[n]));
+    for (int n = 0; n < NT; ++n) {
+      const Parts3 p = parts3_of(now.ge * U[n]);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x2*>(lds.E[k] + put_tok + n * 1024) = p.p[k];
+    }
     lds_barrier();   // U is in LDS
     // S' = gam_C S0 + K^T (e^{G_C - G} U)
 #pragma unroll
@@ -237,13 +241,13 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const bf16x8 hi = get(lds.E[0], t * NT + n), lo = get(lds.E[1], t * NT + n);
 #pragma unroll
-        for (int f = 0; f < FT; ++f)
-          if (wave * FT + f < 2 * KS) {
-            S[f][n] = mfma(now.kt[f][t], hi, S[f][n]);
-            S[f][n] = mfma(now.kt[f][t], lo, S[f][n]);
-          }
+        for (int k = 0; k < 3; ++k) {
+          const bf16x8 e = get(lds.E[k], t * NT + n);
+#pragma unroll
+          for (int f = 0; f < FT; ++f)
+            if (wave * FT + f < 2 * KS) S[f][n] = mfma(now.kt[f][t], e, S[f][n]);
+        }
       }
     if (left > kC) put_state();
     if constexpr (SAVE) save_u(left);
@@ -325,7 +329,7 @@ __device__ __forceinline__ void scan_tokens(const Args& a, const Scan& s, const 
     const uint32_t at = l.lane * 16 | miss_from(0, left);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      const int f = 2 * kTFrags + lower_frag(wave, wave < 2 ? 0 : ks);
+      const int f = kPFrag + lower_frag(wave, wave < 2 ? 0 : ks);
       pf[ks][0] = load_frag(tr, at, f * 1024);
       pf[ks][1] = load_frag(tr, at, (kTFrags + f) * 1024);
     }
@@ -349,13 +353,14 @@ __device__ __forceinline__ void scan_tokens(const Args& a, const Scan& s, const 
       }
     }
     {
-      f32x4 X[NT] = {}, X2[NT] = {};
+      f32x4 X[NT] = {}, X2[NT] = {}, X3[NT] = {};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           X[n] = mfma(kf[ks], state(0, ks * NT + n), X[n]);
           X2[n] = mfma(kf[ks], state(1, ks * NT + n), X2[n]);
+          X3[n] = mfma(kf[ks], get(lds.S[2], ks * NT + n), X3[n]);
         }
       // rows behind the sequence's end have b = 0 and V = 0
       f32x4 zero = {};   // NaN where some value is not finite
@@ -364,10 +369,10 @@ __device__ __forceinline__ void scan_tokens(const Args& a, const Scan& s, const 
         f32x4 v;
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = vr[i].get(n);
-        X[n] = bt * (v - gam * (X[n] + X2[n]));
-        const Parts p = parts_of(X[n]);
-        *reinterpret_cast<u32x2*>(lds.R[0] + put_tok + n * 1024) = p.hi;
-        *reinterpret_cast<u32x2*>(lds.R[1] + put_tok + n * 1024) = p.lo;
+        X[n] = bt * (v - gam * (X[n] + (X2[n] + X3[n])));
+        const Parts3 p = parts3_of(X[n]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x2*>(lds.R[k] + put_tok + n * 1024) = p.p[k];
         zero += X[n] * 0.0f;
       }
       if (__builtin_expect(__any((zero[0] + zero[1]) + (zero[2] + zero[3]) != 0.0f), 0)) {
@@ -376,8 +381,8 @@ __device__ __forceinline__ void scan_tokens(const Args& a, const Scan& s, const 
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (X[n][i] * 0.0f != 0.0f) {
-              *reinterpret_cast<uint16_t*>(lds.R[0] + put_tok + n * 1024 + 2 * i) = 0;
-              *reinterpret_cast<uint16_t*>(lds.R[1] + put_tok + n * 1024 + 2 * i) = 0;
+#pragma unroll
+              for (int k = 0; k < 3; ++k) *reinterpret_cast<uint16_t*>(lds.R[k] + put_tok + n * 1024 + 2 * i) = 0;
               atomicMin(&lds.first[n][l.r], 16 * wave + 4 * q + i);
             }
         lds.bad = 1;
@@ -431,7 +436,7 @@ __device__ __forceinline__ void scan_tokens(const Args& a, const Scan& s, const 
 // The smallest variants keep to the 128 registers with which two workgroups
 // share a CU.
 template <int KS, int NT, bool SAVE>
-__global__ __launch_bounds__(512, KS * NT <= 4 ? 4 : 2) void delta_scan_kernel(Args a) {
+__global__ __launch_bounds__(512, KS * NT <= 2 ? 4 : 2) void delta_scan_kernel(Args a) {
   __shared__ __attribute__((aligned(16))) ScanLds<KS, NT> lds;
   Scan s;
   if (!s.init(a, 16 * NT)) return;
@@ -456,10 +461,10 @@ void launch_scan_as(const Args& a, hipStream_t st) {
 }
 
 int launch_scan(const Args& a, hipStream_t st) {
-  UTTT_DELTA_STEPS(steps_of(a.Dk), KS, switch (scan_tiles(a)) {
+  UTTT_DELTA_STEPS(steps_of(a.Dk), KS, switch (scan_tiles(a, false)) {
     case 1: launch_scan_as<KS, 1>(a, st); break;
     case 2: launch_scan_as<KS, 2>(a, st); break;
-    default: launch_scan_as<KS, 4>(a, st); break;
+    default: if constexpr (scan_widest(KS, false) == 4) launch_scan_as<KS, 4>(a, st);
   });
   return check_launch("delta_scan");
 }
@@ -481,7 +486,7 @@ int check_args(const Args& a, int B, bool packed, bool backward, const char* wha
   // a launch has fewer than 2^32 threads: of a chunk and key head (operands,
   // gradients), of a workgroup of the scans
   const int64_t chunk = backward && steps_of(a.Dk) > 2 ? 128 * steps_of(a.Dk) : 256;
-  const int64_t scans = scan_blocks(a, 16 * scan_tiles(a.T, a.nseq, a.Hv, a.Dv, packed));
+  const int64_t scans = scan_blocks(a, 16 * scan_tiles(a.T, a.nseq, a.Hv, a.Dk, a.Dv, packed, backward));
   UTTT_REQUIRE(slots >= 0 && slots * a.Hv < (1LL << 31) && slots * a.Hk * chunk < (1LL << 32) &&
                    scans * 512 < (1LL << 32),
                "%s: too many chunks and heads for one launch", what);

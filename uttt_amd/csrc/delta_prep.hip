@@ -169,9 +169,9 @@ __device__ __forceinline__ void write_rows(const uint16_t* lds, uint8_t* out, in
 
 constexpr int kLT = kC + 4;   // fp32 row stride of the 64 x 64 matrices
 
-// hi and lo fragments first, first + step, .. of a triangular matrix (or its
-// transpose) in LDS.
-template <bool TRANS>
+// Fragments first, first + step, .. of a triangular matrix (or its transpose) in
+// LDS, each part's behind the part before it.
+template <bool TRANS, int PARTS>
 __device__ __forceinline__ void write_tri(const float* m, uint8_t* out, int first, int step) {
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   for (int f = first; f < kTFrags; f += step) {
@@ -184,10 +184,11 @@ __device__ __forceinline__ void write_tri(const float* m, uint8_t* out, int firs
       x[i] = TRANS ? m[(c0 + i) * kLT + row] : m[row * kLT + c0 + i];
       y[i] = TRANS ? m[(c0 + 4 + i) * kLT + row] : m[row * kLT + c0 + 4 + i];
     }
-    bf16x8 hi, lo;
-    split8(x, y, hi, lo);
-    *reinterpret_cast<bf16x8*>(out + f * 1024 + lane * 16) = hi;
-    *reinterpret_cast<bf16x8*>(out + (kTFrags + f) * 1024 + lane * 16) = lo;
+    bf16x8 part[PARTS];
+    split8(x, y, part);
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k)
+      *reinterpret_cast<bf16x8*>(out + (k * kTFrags + f) * 1024 + lane * 16) = part[k];
   }
 }
 
@@ -302,7 +303,7 @@ __global__ __launch_bounds__(256, KS <= 4 ? 4 : 2) void delta_prep_kernel(Args a
       __syncthreads();
       if (tid == 0) bad = kC;   // for the next head
     }
-    uint8_t* tri = a.tri + ((size_t)c * a.Hv + hv) * kTriBytes;
+    uint8_t* tri = a.tri + ((size_t)c * a.Hv + hv) * (BWD ? kTriBwdBytes : kTriBytes);
     // wave 0: column r of diagonal block q, top to bottom; the others: P's fragments
     float t[16];
     if (wave == 0) {
@@ -315,7 +316,7 @@ __global__ __launch_bounds__(256, KS <= 4 ? 4 : 2) void delta_prep_kernel(Args a
         t[i] = x;
       }
     } else {
-      write_tri<BWD>(Pm, tri + 2 * kTFrags * 1024, wave - 1, 3);
+      write_tri<BWD, BWD ? 3 : 2>(Pm, tri + kPFrag * 1024, wave - 1, 3);
     }
     __syncthreads();
     if (wave == 0) {
@@ -366,7 +367,7 @@ __global__ __launch_bounds__(256, KS <= 4 ? 4 : 2) void delta_prep_kernel(Args a
       load_gates(hv + 1);
       put_decays(hv + 1);
     }
-    write_tri<BWD>(Tm, tri, more ? (wave == 0 ? kTFrags : wave - 1) : wave, more ? 3 : 4);
+    write_tri<BWD, 3>(Tm, tri, more ? (wave == 0 ? kTFrags : wave - 1) : wave, more ? 3 : 4);
     __syncthreads();
   }
 }
