@@ -696,9 +696,9 @@ int uttt_dense_scatter_heads(const void* y, int b, int l, int H, int d, void* ou
  * zeros.  States are [nseq, Hv, Dk, Dv] fp32 contiguous.
  *
  * fwd: out [B, T, Hv, Dv] bf16; initial_state NULL: zeros; final_state NULL:
- * not wanted.  u_saved [2, B, T, Hv, Dv] and s_saved [chunks, Hv, 2, Dk, Dv]
- * bf16 (uttt_gated_delta_chunks slots; fp32 values as two parts each) are what
- * the backward reads; both NULL without one.  bwd: dout [B, T, Hv, Dv] bf16 with strides, dfinal_state NULL:
+ * not wanted.  u_saved [B, T, Hv, Dv] and s_saved [chunks, Hv, Dk, Dv] fp32
+ * (uttt_gated_delta_chunks slots) are what the backward reads; both NULL
+ * without one.  bwd: dout [B, T, Hv, Dv] bf16 with strides, dfinal_state NULL:
  * zeros, dinitial_state NULL: not wanted; dq, dk, dv bf16 contiguous, dg and
  * dbeta in g's and beta's dtypes.  The reference's gated delta layers
  * (gated_deltanet_swa/, uttt_nvs/models/gated_deltanet_block.py) call an

@@ -1,5 +1,6 @@
-"""The fp32 results of the gated delta rule are exact to fp32's order: against the
-64-bit recurrence, per case in the 2-norm, within N = 16 * 2^-24.
+"""The fp32 results of the gated delta rule are exact to fp32's order: states and
+their gradients against the 64-bit recurrence, per case in the 2-norm, within N =
+16 * 2^-24.
 
 A chunk's part of the state passes through at most Dk / 32 + 1 accumulations of
 K S0, R, 12 of U = T R, 6 of K^T U and the decay, some 30 roundings of at most
@@ -10,7 +11,7 @@ it left out, is off by 20 N."""
 import pytest
 import torch
 
-from delta_cases import CASES, F32, groups_of_heads, make, name_of, offsets, reference
+from delta_cases import BF16, CASES, F32, by_sequence, groups_of_heads, make, name_of, offsets, reference
 
 pytestmark = pytest.mark.gpu
 N = 16 * 2.0 ** -24
@@ -36,3 +37,28 @@ def test_states_and_their_gradients(c):
         for name, got, want in (("state", S, ref["S"][:, -1]), ("dh0", dh0, ref["dh0"])):
             off, norm = (got[:, heads].double() - want).norm().item(), want.norm().item()
             assert off <= N * norm, (name, heads.tolist(), off / norm)
+
+
+@pytest.mark.parametrize("types", [(F32, F32), (F32, BF16), (BF16, F32)])
+@pytest.mark.parametrize("c", EXACT, ids=name_of)
+def test_gradients_of_fp32_gates(c, types):
+    """dg and dbeta of a head: N of the norms of the products that they are sums of
+    (tests/delta_cases.py), as their factors are off by N, and 2^-24 of themselves
+    for every one of the 64 + 16 additions in a row at most, 9 as their square root.
+    Where one of the two gates is fp32, its gradient is; the other's is rounded."""
+    from uttt_amd.delta import gated_delta_rule
+    x, do, dht = make(c)
+    x["g"], x["beta"] = x["g"].to(types[0]), x["beta"].to(types[1])
+    leaf = {n: t.cuda().requires_grad_(n in ("g", "beta")) for n, t in x.items()}
+    cu = None if c["B"] else torch.tensor(offsets(c), dtype=torch.int32, device="cuda")
+    out = gated_delta_rule(*(leaf[n] for n in ("q", "k", "v", "g", "beta")), initial_state=leaf["h0"],
+                           output_final_state=True, cu_seqlens=cu)
+    grads = torch.autograd.grad(out, [leaf["g"], leaf["beta"]], [do.cuda(), dht.cuda()])
+    for heads in groups_of_heads(c):
+        ref = reference(c, x, do, dht, heads, "cuda")[1]
+        for name, got, dtype in zip(("g", "beta"), grads, types):
+            mine = torch.nn.utils.rnn.pad_sequence(by_sequence(c, got[:, :, heads]), batch_first=True).double()
+            off, norm = (mine - ref["d" + name]).norm(dim=1), ref["d" + name].norm(dim=1)
+            n = c["Dk"] * c["Dv"] if name == "g" else c["Dv"]
+            bound = (torch.finfo(dtype).eps / 2 + 9 * 2.0 ** -24 + N) * norm + 4 * N * ref["size_" + name].norm(dim=1) / n ** 0.5
+            assert got.dtype == dtype and (off <= bound).all(), (name, (off / bound).max().item())

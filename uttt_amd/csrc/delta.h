@@ -62,15 +62,15 @@ struct Args {
   const float* h0;               // [nseq, Hv, Dk, Dv] or null
   uint16_t* o;                   // [B, T, Hv, Dv]
   float* hT;                     // final states or null
-  uint16_t* u;                   // [2, B, T, Hv, Dv] parts of U, or null
-  uint16_t* s0;                  // [nchunks, Hv, 2, Dk, Dv] parts of S0, or null
+  float* u;                      // [B, T, Hv, Dv], or null
+  float* s0;                     // [nchunks, Hv, Dk, Dv], or null
   // backward
   const uint16_t* dout;          // [B, T, Hv, Dv]
   int64_t do_sb, do_st, do_sh;
   const float* dhT;              // or null
   float* dh0;                    // or null
-  uint16_t* ds;                  // [nchunks, Hv, 2, Dk, Dv] parts of dS'
-  uint16_t* dr;                  // [2, B, T, Hv, Dv] parts of dR
+  float* ds;                     // [nchunks, Hv, Dk, Dv] dS'
+  float* dr;                     // [B, T, Hv, Dv]
   uint16_t *dq, *dk;             // [B, T, Hk, Dk]
   uint16_t* dv;                  // [B, T, Hv, Dv]
   void *dg, *dbeta;              // [B, T, Hv] in their inputs' types
@@ -109,17 +109,6 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
 }
 __device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
-}
-
-// x[0..3] = a, x[4..7] = b as bf16 parts hi + lo.
-__device__ __forceinline__ void split8(f32x4 a, f32x4 b, bf16x8& hi, bf16x8& lo) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    hi[i] = (__bf16)a[i];
-    hi[4 + i] = (__bf16)b[i];
-    lo[i] = (__bf16)(a[i] - (float)hi[i]);
-    lo[4 + i] = (__bf16)(b[i] - (float)hi[4 + i]);
-  }
 }
 
 // The first PARTS bf16 parts of a, b.
@@ -232,19 +221,30 @@ __device__ __forceinline__ u32x2 round_of(f32x4 x) {
 }
 // Row i of NT columns' words to memory as adjacent bf16.
 template <int NT>
-__device__ __forceinline__ void store_row(Rsrc r, uint32_t off, const u32x2 (&x)[NT], int i, uint32_t uniform = 0) {
+__device__ __forceinline__ void store_row(Rsrc r, uint32_t off, const u32x2 (&x)[NT], int i) {
   const auto pair = [&](int n) -> uint32_t {
     const uint32_t a = x[n][i >> 1], b = x[n + 1][i >> 1];
     return i & 1 ? (a >> 16) | (b & 0xffff0000u) : (a & 0xffffu) | (b << 16);
   };
   if constexpr (NT == 1)
-    __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(i & 1 ? x[0][i >> 1] >> 16 : x[0][i >> 1]), r, off, uniform, 0);
+    __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(i & 1 ? x[0][i >> 1] >> 16 : x[0][i >> 1]), r, off, 0, 0);
   else if constexpr (NT == 2)
-    __builtin_amdgcn_raw_buffer_store_b32(pair(0), r, off, uniform, 0);
+    __builtin_amdgcn_raw_buffer_store_b32(pair(0), r, off, 0, 0);
   else {
     const u32x2 w = {pair(0), pair(2)};
-    __builtin_amdgcn_raw_buffer_store_b64(w, r, off, uniform, 0);
+    __builtin_amdgcn_raw_buffer_store_b64(w, r, off, 0, 0);
   }
+}
+// Row i of NT columns to memory as adjacent fp32.
+template <int NT>
+__device__ __forceinline__ void store_row(Rsrc r, uint32_t off, const f32x4 (&x)[NT], int i) {
+  if constexpr (NT == 1)
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[0][i]), r, off, 0, 0);
+  else if constexpr (NT == 2)
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(x[0][i]), __float_as_uint(x[1][i])}, r, off, 0, 0);
+  else
+    __builtin_amdgcn_raw_buffer_store_b128(u32x4{__float_as_uint(x[0][i]), __float_as_uint(x[1][i]),
+                                                 __float_as_uint(x[2][i]), __float_as_uint(x[3][i])}, r, off, 0, 0);
 }
 
 // Sum over the 16 lanes of equal lane / 16, in all of them: four additions
@@ -432,8 +432,8 @@ inline void bind_workspace(Args& a, const Workspace& w, uint8_t* ws, bool packed
   a.qf = w.qf == SIZE_MAX ? nullptr : ws + w.qf;
   if (backward) {
     a.qt = ws + w.qt;
-    a.ds = reinterpret_cast<uint16_t*>(ws + w.ds);
-    a.dr = reinterpret_cast<uint16_t*>(ws + w.dr);
+    a.ds = reinterpret_cast<float*>(ws + w.ds);
+    a.dr = reinterpret_cast<float*>(ws + w.dr);
   }
 }
 

@@ -102,8 +102,7 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
     gc = load_f1(buffer_at(scp), 4 * (kC - 1) | miss_from(0, left));
     load_trans(left, qtp, qtf);
   };
-  // dS' to LDS, and its lane's part from there to memory
-  uint16_t* dsp = a.ds + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * 2 * a.Dk * a.Dv;
+  float* dsp = a.ds + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * a.Dk * a.Dv;
   const auto put_state = [&]() {
 #pragma unroll
     for (int f = 0; f < FT; ++f) {
@@ -121,26 +120,14 @@ __device__ __forceinline__ void scan_bwd_state(const Args& a, const Scan& s, int
   const auto save_state = [&]() {
     const Rsrc sr = buffer_at(dsp);
 #pragma unroll
-    for (int f = 0; f < FT; ++f) {
-      const int tile = wave * FT + f;
-      if (tile < 2 * KS) {
-        u32x2 hi[NT], lo[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const uint32_t at = ((tile >> 1) * NT + n) * 1024 + (tile & 1) * 512 + put;
-          hi[n] = *reinterpret_cast<const u32x2*>(lds.S[0] + at);
-          lo[n] = *reinterpret_cast<const u32x2*>(lds.S[1] + at);
-        }
+    for (int f = 0; f < FT; ++f)
+      if (wave * FT + f < 2 * KS)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int feat = 16 * tile + 4 * q + i;
-          const uint32_t at = 2 * (feat * a.Dv + col) | dead | miss_from(feat, a.Dk);
-          store_row<NT>(sr, at, hi, i);
-          store_row<NT>(sr, at, lo, i, 2 * (uint32_t)(a.Dk * a.Dv));
+          const int feat = 16 * (wave * FT + f) + 4 * q + i;
+          store_row<NT>(sr, 4 * (feat * a.Dv + col) | dead | miss_from(feat, a.Dk), S[f], i);
         }
-      }
-    }
-    dsp -= (int64_t)a.Hv * 2 * a.Dk * a.Dv;
+    dsp -= (int64_t)a.Hv * a.Dk * a.Dv;
   };
 
   const int first_left = s.len - lastc * kC;
@@ -258,9 +245,7 @@ __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, in
   const float* gamp = a.scal + ((int64_t)(s.c0 + lastc) * a.Hv + s.hv) * kScal;   // goes with dO
   const float *betap = gamp, *gep = gamp;                                         // with dR, with K
   const uint32_t grow = 2 * ((16 * wave + 4 * q) * (uint32_t)a.do_st + col);
-  const uint32_t orow = 2 * ((16 * wave + 4 * q) * (uint32_t)(a.Hv * a.Dv) + col);
-  int64_t out_at = (((int64_t)s.b * a.T + s.tok0 + (int64_t)lastc * kC) * a.Hv + s.hv) * a.Dv;
-  const int64_t plane = (int64_t)a.B * a.T * a.Hv * a.Dv;
+  int64_t out_at = (((int64_t)s.b * a.T + s.tok0 + (int64_t)lastc * kC + 16 * wave) * a.Hv + s.hv) * a.Dv;
   const auto load_k = [&](int left) {
     const uint32_t miss = miss_from(16 * wave + r, left);
     const Rsrc kr = buffer_at(kp);
@@ -381,23 +366,21 @@ __device__ __forceinline__ void scan_bwd_tokens(const Args& a, const Scan& s, in
     load_do(later);
     lds_barrier();   // dR is in LDS
     {
-      const Rsrc vr = buffer_at(a.dv + out_at), hr = buffer_at(a.dr + out_at), lr = buffer_at(a.dr + plane + out_at);
-      u32x2 v[NT], hi[NT], lo[NT];
+      const Rsrc vr = buffer_at(a.dv + out_at), rr = buffer_at(a.dr + out_at);
+      f32x4 R[NT];
+      u32x2 v[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const f32x4 R = lds.R[wave][n][lane];
-        const Parts p = parts_of(R);
-        hi[n] = p.hi;
-        lo[n] = p.lo;
-        v[n] = round_of(bt * R);
+        R[n] = lds.R[wave][n][lane];
+        v[n] = round_of(bt * R[n]);
       }
       load_beta(next);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t at = (orow + 2 * i * (uint32_t)(a.Hv * a.Dv)) | dead | miss_from(16 * wave + 4 * q + i, left);
-        store_row<NT>(vr, at, v, i);
-        store_row<NT>(hr, at, hi, i);
-        store_row<NT>(lr, at, lo, i);
+        const uint32_t at = (4 * q + i) * (uint32_t)(a.Hv * a.Dv) + col;
+        const uint32_t none = dead | miss_from(16 * wave + 4 * q + i, left);
+        store_row<NT>(vr, 2 * at | none, v, i);
+        store_row<NT>(rr, 4 * at | none, R, i);
       }
       out_at -= (int64_t)kC * a.Hv * a.Dv;
     }
@@ -429,19 +412,20 @@ __global__ __launch_bounds__(512) void delta_scan_bwd_kernel(Args a) {
 // done, which reads U and S0 (for <S0, dS'>) once more from cache.  With all
 // of them in one pass and one workgroup a CU 6144 chunks of 128 x 128 took 745
 // us, with two workgroups and the registers spilled 1129.
-constexpr int grads_waves(int KS, bool shared) {   // per SIMD, at least
-  return KS == 8 ? 4 : KS == 6 ? 3 : shared ? 2 : 4;
+constexpr int grads_waves(int KS, bool shared, int parts) {   // per SIMD, at least
+  return KS == 8 ? 4 : KS == 6 ? 3 : shared || (parts == 3 && KS < 4) ? 2 : 4;
 }
 
-template <int KS, bool SHARED>
-__global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads_kernel(Args a) {
+template <int KS, bool SHARED, int PARTS>
+__global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED, PARTS)) void delta_grads_kernel(Args a) {
   constexpr int NW = 2 * KS, PW = NW >= 16 ? 16 : NW >= 8 ? 8 : 4, CT = 16 / PW;
   constexpr int LX = kC + 4, LM = kC + 8, LO = 32 * KS + 8;
-  constexpr int kThreads = 64 * NW, kStage = 5 * 4 * 1024;   // dO, dR hi, lo, U hi, lo: 4 fragments each
+  constexpr int kThreads = 64 * NW, kStage = (1 + 2 * PARTS) * 4 * 1024;   // dO, dR's parts, U's: 4 fragments each
+  constexpr int kHalves = PARTS == 2 ? 2 : 1;                 // the stage twice, where two workgroups share a CU
   constexpr int kMats = 3 * kC * LM * 2;                      // D, D^T, M + M^T; before them X
   constexpr int kRows = 3 * NW * kC * 4, kOut = kC * LO * 2;
   constexpr int kPair = 8 * KS * 1024;                         // K and Q fragments
-  constexpr int kBig = 2 * kStage > kMats + kRows ? 2 * kStage : kMats + kRows;
+  constexpr int kBig = kHalves * kStage > kMats + kRows ? kHalves * kStage : kMats + kRows;
   constexpr int kBuf = kBig > kPair ? kBig : kPair;
   __shared__ __attribute__((aligned(16))) uint8_t trans[NW][4 * 1024];   // a wave's K^T and Q^T fragments
   __shared__ __attribute__((aligned(16))) uint8_t buf[kBuf > kOut ? kBuf : kOut];
@@ -474,7 +458,6 @@ __global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads
   }
   f32x4 dQ[4] = {}, dK[4] = {};
   const int64_t orow = (int64_t)a.Hv * a.Dv, tok = (int64_t)ch.b * a.T + ch.t0;
-  const int64_t plane = (int64_t)a.B * a.T * orow;
   const int hv_end = SHARED ? (hk + 1) * group : hk + 1;
   for (int hv = SHARED ? hk * group : hk; hv < hv_end; ++hv) {
     // Behind this the compiler takes r and q for new values in every turn: the
@@ -488,37 +471,51 @@ __global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads
     const int64_t oat = tok * orow + (int64_t)hv * a.Dv;
     const uint16_t* gp = a.dout + ch.b * a.do_sb + ch.t0 * a.do_st + hv * a.do_sh;
     const Rsrc vp = buffer_at(a.v + ch.b * a.v_sb + ch.t0 * a.v_st + hv * a.v_sh);
-    const int64_t sat = ((int64_t)c * a.Hv + hv) * 2 * a.Dk * a.Dv;
+    const int64_t sat = ((int64_t)c * a.Hv + hv) * a.Dk * a.Dv;
     const Rsrc sp = buffer_at(a.s0 + sat), dp = buffer_at(a.ds + sat);
-    const uint32_t lo_at = 2 * (uint32_t)(a.Dk * a.Dv);
-    const uint32_t srow = 2 * (feat * a.Dv + 8 * q) | miss_from(feat, a.Dk);
-    bf16x8 st[(20 + NW - 1) / NW], sh, sl;
-    // Rows of 16 tokens by 32 columns to LDS: wave w has fragments w, w + NW, ..
-    // of `count`, four of each tensor, the first of them tensor `from` of dO, dR
-    // hi, lo, U hi, lo.
+    const uint32_t srow = 4 * (feat * a.Dv + 8 * q) | miss_from(feat, a.Dk);
+    // Rows of 16 tokens by 32 columns to LDS, 16 bytes a lane at a time: four
+    // fragments of dO, then eight half ones each of dR and U in fp32.  Wave w has
+    // pieces w, w + NW, .. of `count` from `from` on.
+    u32x4 st[(20 + NW - 1) / NW];
     const auto load_rows = [&](int e0, int from, int count) {
-      const uint32_t miss = miss_from(e0 + 8 * q, a.Dv);
 #pragma unroll
       for (int i = 0; i < (20 + NW - 1) / NW; ++i) {
-        const int f = i * NW + wave;
+        const int f = i * NW + wave, g = from + f;
         if (f < count) {
-          const int t = 16 * (f & 3) + r, which = from + (f >> 2);
-          const uint32_t ld = which == 0 ? (uint32_t)a.do_st : (uint32_t)orow;
-          const uint16_t* p = which == 0 ? gp : (which < 3 ? a.dr : a.u) + oat + (which & 1 ? 0 : plane);
-          st[i] = load_frag(buffer_at(p), 2 * (t * ld + e0 + 8 * q) | miss_from(t, ch.n) | miss);
+          const int tile = g < 4 ? g : (g >> 1) & 3, half = g < 4 ? 0 : 4 * (g & 1);
+          const uint32_t miss = miss_from(16 * tile + r, ch.n) | miss_from(e0 + 8 * q, a.Dv);
+          const uint32_t col = e0 + 8 * q + half;
+          const Rsrc p = g < 4 ? buffer_at(gp + 16 * tile * a.do_st)
+                               : buffer_at((g < 12 ? a.dr : a.u) + oat + 16 * tile * orow);
+          const uint32_t at = g < 4 ? 2 * (r * (uint32_t)a.do_st + col) : 4 * (r * (uint32_t)orow + col);
+          st[i] = __builtin_amdgcn_raw_buffer_load_b128(p, at | miss, 0, 0);
         }
       }
     };
-    const auto put_rows = [&](uint8_t* stage, int count) {
+    const auto put_rows = [&](uint8_t* stage, int from, int count) {
 #pragma unroll
-      for (int i = 0; i < (20 + NW - 1) / NW; ++i)
-        if (i * NW + wave < count)
-          *reinterpret_cast<bf16x8*>(stage + (i * NW + wave) * 1024 + lane * 16) = st[i];
+      for (int i = 0; i < (20 + NW - 1) / NW; ++i) {
+        const int f = i * NW + wave, g = from + f;
+        if (f < count) {
+          if (g < 4) {
+            *reinterpret_cast<u32x4*>(stage + g * 1024 + lane * 16) = st[i];
+          } else {   // part k of dR or U behind the parts before it; of U alone from the start
+            const int base = from ? 0 : g < 12 ? 4 : 4 + 4 * PARTS;
+            const Parts3 x = parts3_of(__builtin_bit_cast(f32x4, st[i]));
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k)
+              *reinterpret_cast<u32x2*>(stage + (base + 4 * k + ((g >> 1) & 3)) * 1024 + lane * 16 + 8 * (g & 1)) = x.p[k];
+          }
+        }
+      }
     };
-    const auto load_state = [&](Rsrc p, int e0, bf16x8& hi, bf16x8& lo) {
-      const uint32_t at = (srow + 2 * e0) | miss_from(e0 + 8 * q, a.Dv);
-      hi = load_frag(p, at);
-      lo = load_frag(p, at, lo_at);
+    struct Eight {
+      f32x4 a, b;
+    };
+    const auto load_state = [&](Rsrc p, int e0) {
+      const uint32_t at = (srow + 4 * e0) | miss_from(e0 + 8 * q, a.Dv);
+      return Eight{load_f4(p, at), load_f4(p, at, 16)};
     };
     // a wave's own 16 x 16 products, of which the diagonal is wanted
     const auto diagonal = [&](f32x4 x) {
@@ -535,43 +532,52 @@ __global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads
         vf = load_frag(vp, 2 * (t * (uint32_t)a.v_st + e0 + 8 * q) | miss_from(t, ch.n) | miss_from(e0 + 8 * q, a.Dv));
       };
       load_rows(0, 0, 20);
-      load_state(sp, 0, sh, sl);
+      Eight s8 = load_state(sp, 0);
       if (wave < 4) load_v(0);
       int half = 0;
-      for (int e0 = 0; e0 < a.Dv; e0 += 32, half ^= 1) {
+      for (int e0 = 0; e0 < a.Dv; e0 += 32, half ^= kHalves - 1) {
         uint8_t* stage = buf + half * kStage;
-        put_rows(stage, 20);
+        if (kHalves == 1 && e0 > 0) lds_barrier();   // the step before is read
+        put_rows(stage, 0, 20);
         load_rows(e0 + 32, 0, 20);   // past Dv: nothing is read
         lds_barrier();               // the step's rows are in LDS; the other half is free after the next one
-        const auto row = [&](int which, int rt) {
+        const auto row = [&](int which, int rt) {   // 0: dO, then the parts of dR, of U
           return *reinterpret_cast<const bf16x8*>(stage + (4 * which + rt) * 1024 + lane * 16);
         };
+        bf16x8 sf[PARTS];
+        split8(s8.a, s8.b, sf);
+        s8 = load_state(sp, e0 + 32);
 #pragma unroll
         for (int rt = 0; rt < 4; ++rt) {
-          const bf16x8 g = row(0, rt), rh = row(1, rt), rl = row(2, rt);
-          EQ[rt] = mfma(g, sh, EQ[rt]);
-          ER[rt] = mfma(rh, sh, ER[rt]);
-          EQ[rt] = mfma(g, sl, EQ[rt]);
-          ER[rt] = mfma(rh, sl, ER[rt]);
-          ER[rt] = mfma(rl, sh, ER[rt]);
+          const bf16x8 g = row(0, rt);
+#pragma unroll
+          for (int k = 0; k < PARTS; ++k) EQ[rt] = mfma(g, sf[k], EQ[rt]);
+#pragma unroll
+          for (int j = 0; j < PARTS; ++j) {
+            const bf16x8 x = row(1 + j, rt);
+#pragma unroll
+            for (int k = 0; j + k < PARTS; ++k) ER[rt] = mfma(x, sf[k], ER[rt]);
+          }
         }
-        load_state(sp, e0 + 32, sh, sl);
         if (wave < PW) {
-          const bf16x8 gw = row(0, rw), rh = row(1, rw), rl = row(2, rw);
+          const bf16x8 gw = row(0, rw);
+          bf16x8 x[PARTS];
+#pragma unroll
+          for (int j = 0; j < PARTS; ++j) x[j] = row(1 + j, rw);
           if (wave < 4) {   // dR.v
-            rv = mfma(rh, vf, rv);
-            rv = mfma(rl, vf, rv);
+#pragma unroll
+            for (int j = 0; j < PARTS; ++j) rv = mfma(x[j], vf, rv);
             load_v(e0 + 32);
           }
 #pragma unroll
-          for (int x = 0; x < CT; ++x) {
-            const bf16x8 uh = row(3, cw + x), ul = row(4, cw + x);
-            dP[x] = mfma(gw, uh, dP[x]);
-            dA[x] = mfma(rh, uh, dA[x]);
-            dP[x] = mfma(gw, ul, dP[x]);
-            dA[x] = mfma(rh, ul, dA[x]);
-            dA[x] = mfma(rl, uh, dA[x]);
-          }
+          for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k) {
+              const bf16x8 u = row(1 + PARTS + k, cw + c);
+              dP[c] = mfma(gw, u, dP[c]);
+#pragma unroll
+              for (int j = 0; j + k < PARTS; ++j) dA[c] = mfma(x[j], u, dA[c]);
+            }
         }
       }
     }
@@ -671,14 +677,14 @@ __global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads
     }
     lds_barrier();
     asm volatile("" : "+v"(r), "+v"(q));
-    // sum_{j < t} X_ij as a product with the strictly upper ones, X in two bf16 parts
+    // sum_{j < t} X_ij as a product with the strictly upper ones
     if (wave < PW) {
       f32x4 Z[CT] = {};
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
         const float* xp = Xl + (16 * rw + r) * LX + 32 * ks + 8 * q;
-        bf16x8 hi, lo;
-        split8(*reinterpret_cast<const f32x4*>(xp), *reinterpret_cast<const f32x4*>(xp + 4), hi, lo);
+        bf16x8 xf[PARTS];
+        split8(*reinterpret_cast<const f32x4*>(xp), *reinterpret_cast<const f32x4*>(xp + 4), xf);
 #pragma unroll
         for (int x = 0; x < CT; ++x) {
           const int below = 16 * (cw + x) + r - (32 * ks + 8 * q);   // ones in places under it
@@ -686,8 +692,8 @@ __global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             ones[i] = 2 * i + 1 < below ? 0x3f803f80u : 2 * i < below ? 0x3f80u : 0u;
-          Z[x] = mfma(hi, __builtin_bit_cast(bf16x8, ones), Z[x]);
-          Z[x] = mfma(lo, __builtin_bit_cast(bf16x8, ones), Z[x]);
+#pragma unroll
+          for (int k = 0; k < PARTS; ++k) Z[x] = mfma(xf[k], __builtin_bit_cast(bf16x8, ones), Z[x]);
         }
       }
 #pragma unroll
@@ -721,10 +727,8 @@ __global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads
       }
     }
     lds_barrier();
-    load_rows(0, 3, 8);   // for the second pass, as the states
-    bf16x8 dh, dl;
-    load_state(sp, 0, sh, sl);
-    load_state(dp, 0, dh, dl);
+    load_rows(0, 12, 8);   // for the second pass, as the states
+    Eight s8 = load_state(sp, 0), d8 = load_state(dp, 0);
     // dQ += D K, dK += D^T Q + (M + M^T) K
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
@@ -744,23 +748,27 @@ __global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED)) void delta_grads
     {
       int half = 0;
       for (int e0 = 0; e0 < a.Dv; e0 += 32, half ^= 1) {
-        uint8_t* stage = buf + half * 8 * 1024;
-        put_rows(stage, 8);
-        load_rows(e0 + 32, 3, 8);
+        uint8_t* stage = buf + half * 4 * PARTS * 1024;
+        put_rows(stage, 12, 8);
+        load_rows(e0 + 32, 12, 8);
         lds_barrier();
+        bf16x8 sf[PARTS], df[PARTS];
+        split8(d8.a, d8.b, df);
+        d8 = load_state(dp, e0 + 32);
 #pragma unroll
-        for (int rt = 0; rt < 4; ++rt) {
-          const bf16x8 uh = *reinterpret_cast<const bf16x8*>(stage + rt * 1024 + lane * 16);
-          const bf16x8 ul = *reinterpret_cast<const bf16x8*>(stage + (4 + rt) * 1024 + lane * 16);
-          EU[rt] = mfma(uh, dh, EU[rt]);
-          EU[rt] = mfma(uh, dl, EU[rt]);
-          EU[rt] = mfma(ul, dh, EU[rt]);
-        }
-        dot = mfma(sh, dh, dot);
-        dot = mfma(sh, dl, dot);
-        dot = mfma(sl, dh, dot);
-        load_state(sp, e0 + 32, sh, sl);
-        load_state(dp, e0 + 32, dh, dl);
+        for (int rt = 0; rt < 4; ++rt)
+#pragma unroll
+          for (int j = 0; j < PARTS; ++j) {
+            const bf16x8 u = *reinterpret_cast<const bf16x8*>(stage + (4 * j + rt) * 1024 + lane * 16);
+#pragma unroll
+            for (int k = 0; j + k < PARTS; ++k) EU[rt] = mfma(u, df[k], EU[rt]);
+          }
+        split8(s8.a, s8.b, sf);
+        s8 = load_state(sp, e0 + 32);
+#pragma unroll
+        for (int j = 0; j < PARTS; ++j)
+#pragma unroll
+          for (int k = 0; j + k < PARTS; ++k) dot = mfma(sf[j], df[k], dot);
       }
     }
 #pragma unroll
@@ -847,8 +855,10 @@ int launch_bwd(const Args& a, hipStream_t st) {
   if (const int rc = check_launch("delta_scan_bwd")) return rc;
   if (a.nchunks == 0) return UTTT_OK;
   const dim3 grid((unsigned)((int64_t)a.nchunks * a.Hk));
-  if (a.Hv > a.Hk) hipLaunchKernelGGL((delta_grads_kernel<KS, true>), grid, dim3(128 * KS), 0, st, a);
-  else hipLaunchKernelGGL((delta_grads_kernel<KS, false>), grid, dim3(128 * KS), 0, st, a);
+  const bool shared = a.Hv > a.Hk, exact = a.g_dtype == UTTT_F32 || a.beta_dtype == UTTT_F32;
+  const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(128 * KS), 0, st, a); };
+  if (shared) exact ? launch(delta_grads_kernel<KS, true, 3>) : launch(delta_grads_kernel<KS, true, 2>);
+  else exact ? launch(delta_grads_kernel<KS, false, 3>) : launch(delta_grads_kernel<KS, false, 2>);
   return check_launch("delta_grads");
 }
 
@@ -897,8 +907,8 @@ extern "C" int uttt_gated_delta_bwd(const void* q, const int64_t* q_strides, con
   UTTT_REQUIRE(w.total == 0 || (workspace && workspace_bytes >= w.total),
                "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, w.total);
   bind_workspace(a, w, static_cast<uint8_t*>(workspace), packed, true);
-  a.u = static_cast<uint16_t*>(const_cast<void*>(u_saved));
-  a.s0 = static_cast<uint16_t*>(const_cast<void*>(s_saved));
+  a.u = static_cast<float*>(const_cast<void*>(u_saved));
+  a.s0 = static_cast<float*>(const_cast<void*>(s_saved));
   a.dout = static_cast<const uint16_t*>(dout);
   a.dhT = dfinal_state;
   a.dh0 = dinitial_state;

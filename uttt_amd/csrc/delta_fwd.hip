@@ -135,44 +135,27 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
         }
     }
   };
-  uint16_t* s0p = SAVE ? a.s0 + ((int64_t)s.c0 * a.Hv + s.hv) * 2 * a.Dk * a.Dv : nullptr;
+  float* s0p = SAVE ? a.s0 + ((int64_t)s.c0 * a.Hv + s.hv) * a.Dk * a.Dv : nullptr;
   const auto save_state = [&]() {
     const Rsrc sr = buffer_at(s0p);
 #pragma unroll
-    for (int f = 0; f < FT; ++f) {
-      const int tile = wave * FT + f;
-      if (tile < 2 * KS) {
-        u32x2 hi[NT], lo[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const uint32_t at = ((tile >> 1) * NT + n) * 1024 + (tile & 1) * 512 + put;
-          hi[n] = *reinterpret_cast<const u32x2*>(lds.S[0] + at);
-          lo[n] = *reinterpret_cast<const u32x2*>(lds.S[1] + at);
-        }
+    for (int f = 0; f < FT; ++f)
+      if (wave * FT + f < 2 * KS)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int feat = 16 * tile + 4 * q + i;
-          const uint32_t at = 2 * (feat * a.Dv + col) | dead | miss_from(feat, a.Dk);
-          store_row<NT>(sr, at, hi, i);
-          store_row<NT>(sr, at, lo, i, 2 * (uint32_t)(a.Dk * a.Dv));
+          const int feat = 16 * (wave * FT + f) + 4 * q + i;
+          store_row<NT>(sr, 4 * (feat * a.Dv + col) | dead | miss_from(feat, a.Dk), S[f], i);
         }
-      }
-    }
-    s0p += (int64_t)a.Hv * 2 * a.Dk * a.Dv;
+    s0p += (int64_t)a.Hv * a.Dk * a.Dv;
   };
-  uint16_t* up = SAVE ? a.u + (((int64_t)s.b * a.T + s.tok0) * a.Hv + s.hv) * a.Dv : nullptr;
-  const int64_t plane = (int64_t)a.B * a.T * a.Hv * a.Dv;
-  const uint32_t urow = 2 * ((16 * wave + 4 * q) * (uint32_t)(a.Hv * a.Dv) + col);
-  u32x2 uh[NT], ul[NT];
-  const auto save_u = [&](int left) {
-    const Rsrc hr = buffer_at(up), lr = buffer_at(up + plane);
+  const int64_t token = (int64_t)a.Hv * a.Dv;
+  float* up = SAVE ? a.u + ((int64_t)s.b * a.T + s.tok0 + 16 * wave) * token + s.hv * a.Dv : nullptr;
+  const auto save_u = [&](const f32x4 (&U)[NT], int left) {
+    const Rsrc ur = buffer_at(up);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t at = (urow + 2 * i * (uint32_t)(a.Hv * a.Dv)) | dead | miss_from(16 * wave + 4 * q + i, left);
-      store_row<NT>(hr, at, uh, i);
-      store_row<NT>(lr, at, ul, i);
-    }
-    up += (int64_t)kC * a.Hv * a.Dv;
+    for (int i = 0; i < 4; ++i)
+      store_row<NT>(ur, 4 * ((4 * q + i) * (uint32_t)token + col) | dead | miss_from(16 * wave + 4 * q + i, left), U, i);
+    up += kC * token;
   };
 
   if (s.len > 0) {
@@ -215,16 +198,10 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
       const Parts p = parts_of(U[n]);
       *reinterpret_cast<u32x2*>(lds.U[0] + put_tok + n * 1024) = p.hi;
       *reinterpret_cast<u32x2*>(lds.U[1] + put_tok + n * 1024) = p.lo;
-      uh[n] = p.hi;
-      ul[n] = p.lo;
     }
-    if (__builtin_expect(__builtin_amdgcn_readfirstlane(bad), 0)) {
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(bad), 0))
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        spoil(U[n], 16 * wave + 4 * q, lds.first[n][r]);
-        uh[n] = parts_of(U[n]).hi;
-      }
-    }
+      for (int n = 0; n < NT; ++n) spoil(U[n], 16 * wave + 4 * q, lds.first[n][r]);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const Parts3 p = parts3_of(now.ge * U[n]);
@@ -250,7 +227,7 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
         }
       }
     if (left > kC) put_state();
-    if constexpr (SAVE) save_u(left);
+    if constexpr (SAVE) save_u(U, left);
   }
   if (a.hT && col < a.Dv) {
 #pragma unroll
@@ -558,8 +535,8 @@ extern "C" int uttt_gated_delta_fwd(const void* q, const int64_t* q_strides, con
   a.h0 = initial_state;
   a.hT = final_state;
   a.o = static_cast<uint16_t*>(out);
-  a.u = static_cast<uint16_t*>(u_saved);
-  a.s0 = static_cast<uint16_t*>(s_saved);
+  a.u = static_cast<float*>(u_saved);
+  a.s0 = static_cast<float*>(s_saved);
   const hipStream_t st = as_stream(stream);
   if (packed)
     if (const int rc = launch_table(cu_seqlens, cu_is_int64, nseq, T, a.nchunks,

@@ -128,7 +128,8 @@ def _fwd_fake(q, k, v, g, beta, initial_state, cu_seqlens, scale, want_state):
     Hv, Dv = v.shape[2:]
     slots = T // 64 + _seqs(q, cu_seqlens) + 2 if cu_seqlens is not None else B * ((T + 63) // 64)
     return (*_infer_fake(q, k, v, g, beta, initial_state, cu_seqlens, scale, want_state),
-            v.new_empty((2, B, T, Hv, Dv)), v.new_empty((slots, Hv, 2, Dk, Dv)))
+            v.new_empty((B, T, Hv, Dv), dtype=torch.float32),
+            v.new_empty((slots, Hv, Dk, Dv), dtype=torch.float32))
 
 
 @traced_op("gated_delta_fwd", _fwd_fake)
@@ -136,7 +137,7 @@ def _fwd(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, initial_state
          cu_seqlens: Optional[Tensor], scale: float,
          want_state: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
     """_infer, and what the backward reads: U and the states at the chunks'
-    starts, as bf16 parts hi and lo."""
+    starts."""
     o, state, u, s0 = _fwd_fake(q, k, v, g, beta, initial_state, cu_seqlens, scale, want_state)
     _launch_fwd(q, k, v, g, beta, initial_state, cu_seqlens, scale, o, state if want_state else None,
                 u, s0)
