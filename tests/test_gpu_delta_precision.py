@@ -62,3 +62,32 @@ def test_gradients_of_fp32_gates(c, types):
             n = c["Dk"] * c["Dv"] if name == "g" else c["Dv"]
             bound = (torch.finfo(dtype).eps / 2 + 9 * 2.0 ** -24 + N) * norm + 4 * N * ref["size_" + name].norm(dim=1) / n ** 0.5
             assert got.dtype == dtype and (off <= bound).all(), (name, (off / bound).max().item())
+
+
+@pytest.mark.parametrize("c", CASES, ids=name_of)
+def test_bf16_results_are_rounded_once(c):
+    """o, dq, dk and dv are the 64-bit results rounded to bf16 but where those lie
+    next to a border: values off by Q = 8 H^2 of their size end up on its other side
+    in 2 Q / H = 16 H of the cases, as a step is H or 2 H of the value.  An operand
+    rounded to bf16 on the way moves a third of the values."""
+    from uttt_amd.delta import gated_delta_rule
+    names = ("q", "k", "v", "g", "beta", "h0")
+    x, do, dht = make(c)
+    leaf = {n: t.cuda().requires_grad_() for n, t in x.items()}
+    cu = None if c["B"] else torch.tensor(offsets(c), dtype=torch.int32, device="cuda")
+    o, S = gated_delta_rule(*(leaf[n] for n in names[:5]), initial_state=leaf["h0"], output_final_state=True, cu_seqlens=cu)
+    ours = dict(zip(("dq", "dk", "dv"), torch.autograd.grad([o, S], [leaf[n] for n in names[:3]], [do.cuda(), dht.cuda()])),
+                o=o.detach())
+    pad = lambda t: torch.nn.utils.rnn.pad_sequence(by_sequence(c, t), batch_first=True)  # noqa: E731
+    per = c["Hv"] // c["Hk"]
+    moved = dict.fromkeys(ours, 0)
+    for heads in groups_of_heads(c):
+        a, ref = reference(c, x, do, dht, heads, "cuda")
+        real = ref["size_g"] > 0
+        want = {n: ref[n].unflatten(2, (-1, per)).sum(3) for n in ("dq", "dk")}
+        want.update(dv=ref["dv"], o=(a["q"][..., None] * ref["S"][:, 1:]).sum(-2) * c["Dk"] ** -0.5 * real[..., None])
+        for n, w in want.items():
+            mine = pad(ours[n][:, :, heads[::per] // per if n in ("dq", "dk") else heads])
+            moved[n] += (mine != w.to(BF16)).sum().item()
+    for n, m in moved.items():
+        assert m <= 16 * 2.0 ** -8 * ours[n].numel(), (n, m / ours[n].numel())

@@ -708,41 +708,52 @@ __global__ __launch_bounds__(128 * KS, grads_waves(KS, SHARED, PARTS)) void delt
       }
     }
     lds_barrier();   // X is read: D, D^T and M + M^T take its place
-    if (wave < PW) {
+    // dQ += D K, dK += D^T Q + (M + M^T) K, the matrices in two bf16 parts, one
+    // after the other through LDS
+    Eight s8, d8;
 #pragma unroll
-      for (int x = 0; x < CT; ++x) {
-        const int j = 16 * (cw + x) + r, row0 = 16 * rw + 4 * q;
-        const u32x2 d = round_of(dP[x]), m = round_of(dA[x]);
-        *reinterpret_cast<u32x2*>(DTl + j * LM + row0) = d;
+    for (int part = 0; part < 2; ++part) {
+      if (wave < PW) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = row0 + i;
-          const uint16_t mw = (uint16_t)(i & 1 ? m[i >> 1] >> 16 : m[i >> 1]);
-          reinterpret_cast<uint16_t*>(Dl)[row * LM + j] = (uint16_t)(i & 1 ? d[i >> 1] >> 16 : d[i >> 1]);
-          if (row >= j) {   // M is zero on the diagonal
-            reinterpret_cast<uint16_t*>(Nl)[row * LM + j] = mw;
-            reinterpret_cast<uint16_t*>(Nl)[j * LM + row] = mw;
+        for (int x = 0; x < CT; ++x) {
+          const int j = 16 * (cw + x) + r, row0 = 16 * rw + 4 * q;
+          const u32x2 d = round_of(dP[x]), m = round_of(dA[x]);
+          *reinterpret_cast<u32x2*>(DTl + j * LM + row0) = d;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = row0 + i;
+            const uint32_t dw = i & 1 ? d[i >> 1] & 0xffff0000u : d[i >> 1] << 16;
+            const uint32_t mw = i & 1 ? m[i >> 1] & 0xffff0000u : m[i >> 1] << 16;
+            reinterpret_cast<uint16_t*>(Dl)[row * LM + j] = (uint16_t)(dw >> 16);
+            if (row >= j) {   // M is zero on the diagonal
+              reinterpret_cast<uint16_t*>(Nl)[row * LM + j] = (uint16_t)(mw >> 16);
+              reinterpret_cast<uint16_t*>(Nl)[j * LM + row] = (uint16_t)(mw >> 16);
+            }
+            dP[x][i] -= __uint_as_float(dw);
+            dA[x][i] -= __uint_as_float(mw);
           }
         }
       }
-    }
-    lds_barrier();
-    load_rows(0, 12, 8);   // for the second pass, as the states
-    Eight s8 = load_state(sp, 0), d8 = load_state(dp, 0);
-    // dQ += D K, dK += D^T Q + (M + M^T) K
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const bf16x8 kb = *reinterpret_cast<const bf16x8*>(trans[wave] + ks * 1024 + lane * 16);
-      const bf16x8 qb = *reinterpret_cast<const bf16x8*>(trans[wave] + (2 + ks) * 1024 + lane * 16);
-#pragma unroll
-      for (int rt = 0; rt < 4; ++rt) {
-        const int o = (16 * rt + r) * LM + 32 * ks + 8 * q;
-        if (ks == 0 || rt >= 2) dQ[rt] = mfma(*reinterpret_cast<const bf16x8*>(Dl + o), kb, dQ[rt]);
-        if (ks == 1 || rt < 2) dK[rt] = mfma(*reinterpret_cast<const bf16x8*>(DTl + o), qb, dK[rt]);
-        dK[rt] = mfma(*reinterpret_cast<const bf16x8*>(Nl + o), kb, dK[rt]);
+      lds_barrier();
+      if (part == 1) {   // for the second pass
+        load_rows(0, 12, 8);
+        s8 = load_state(sp, 0);
+        d8 = load_state(dp, 0);
       }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const bf16x8 kb = *reinterpret_cast<const bf16x8*>(trans[wave] + ks * 1024 + lane * 16);
+        const bf16x8 qb = *reinterpret_cast<const bf16x8*>(trans[wave] + (2 + ks) * 1024 + lane * 16);
+#pragma unroll
+        for (int rt = 0; rt < 4; ++rt) {
+          const int o = (16 * rt + r) * LM + 32 * ks + 8 * q;
+          if (ks == 0 || rt >= 2) dQ[rt] = mfma(*reinterpret_cast<const bf16x8*>(Dl + o), kb, dQ[rt]);
+          if (ks == 1 || rt < 2) dK[rt] = mfma(*reinterpret_cast<const bf16x8*>(DTl + o), qb, dK[rt]);
+          dK[rt] = mfma(*reinterpret_cast<const bf16x8*>(Nl + o), kb, dK[rt]);
+        }
+      }
+      lds_barrier();   // every wave is done with the 64 x 64 matrices
     }
-    lds_barrier();   // every wave is done with the 64 x 64 matrices
     // the second pass: U dS'^T and <S0, dS'>
     f32x4 EU[4] = {}, dot = {};
     {
