@@ -33,10 +33,10 @@ CASES = [
     dict(B=16, lens=[200], Hk=2, Hv=4, Dk=192, Dv=136, tiles=4, back=2),
     dict(B=8, lens=[270], Hk=4, Hv=8, Dk=256, Dv=136, tiles=2),
     dict(B=0, lens=[300, 1, 0, 129, 250], front=7, behind=13, Hk=8, Hv=16, Dk=64, Dv=64, tiles=1),
-    dict(B=0, lens=[64, 200, 0, 65, 40], front=20, behind=11, Hk=32, Hv=96, Dk=40, Dv=40, tiles=2),
+    dict(B=0, lens=[64, 200, 0, 65, 40], front=20, behind=11, Hk=32, Hv=128, Dk=40, Dv=40, tiles=2),
     dict(B=0, lens=[271, 1, 128], front=0, behind=0, Hk=48, Hv=48, Dk=64, Dv=136, tiles=2),
-    dict(B=0, lens=[330, 3, 0, 64, 65, 100, 10, 100], front=28, behind=0, Hk=32, Hv=64, Dk=96, Dv=72, tiles=4),
-    dict(B=0, lens=[200, 0, 0, 17, 63, 80, 1, 20], front=0, behind=19, Hk=16, Hv=32, Dk=128, Dv=136, tiles=4),
+    dict(B=0, lens=[330, 3, 0, 64, 65, 100, 10, 100], front=28, behind=0, Hk=32, Hv=96, Dk=96, Dv=72, tiles=4),
+    dict(B=0, lens=[200, 0, 0, 17, 63, 80, 1, 20], front=0, behind=19, Hk=24, Hv=48, Dk=128, Dv=136, tiles=4),
 ]
 
 
@@ -45,12 +45,12 @@ def name_of(c):
     return f"{rows}-{c['Hk']}-{c['Hv']}-{c['Dk']}x{c['Dv']}-{c['tiles']}"
 
 
-def scan_tiles(T, nseq, Hv, Dk, Dv, packed, backward=False):
+def scan_tiles(T, nseq, Hv, Dk, Dv, packed, backward=False, stored=True):
     """The choice of csrc/delta.h."""
     total, cps = T // 64 + nseq, (T + 63) // 64
     mean = -(-total // nseq)
     cost = {}
-    for tiles, tenths in ((1, 20), (2, 23), (4, 30)):
+    for tiles, tenths in ((1, 20), (2, 28), (4, 40 if stored else 43)):
         if tiles == 4 and Dk > (128 if backward else 192):
             continue
         blocks = -(-Dv // (16 * tiles))

@@ -318,23 +318,32 @@ inline int64_t scan_blocks(const Args& a, int width) {
 }
 // 16-column tiles of a scan's workgroup.  Wide ones do more work a CU, narrow
 // ones end a long sequence sooner.  What is estimated: rounds of workgroups
-// over the 256 CUs, a chunk of them as 2.0, 2.3 and 3.0 us for 1, 2 and 4 tiles
-// (what a busy card takes at 128 features), and of packed sequences, whose
+// over the 256 CUs, a chunk of them as 2.0, 2.8 and 4.3 us for 1, 2 and 4 tiles
+// (what a busy card takes at 128 features; 4.0 for 4 tiles in the backward and
+// where what it reads is stored, which is most of the time then), and of packed
+// sequences, whose
 // lengths the host does not know, the work over the CUs and a longest sequence
 // of three times the mean.  Measured, forward scans, us for 1, 2, 4 tiles:
-//   4096 tokens, 4 heads of 192                         79, 135, 301
-//   8192 tokens, 16 heads of 128                       159, 210, 312
-//   4 x 4096 tokens, 16 heads of 128                   229, 164, 189
-//   12 prompts of 1 to 5000 tokens, 16 heads of 128    230, 169, 212
-// and with what a backward reads
-//   8 x 1024 tokens, 4 heads of 192                     81,  61,  97
-//   16 x 2048 tokens, 12 heads of 128                  577, 418, 344
-//   16 x 2048 tokens, 4 heads of 256                   528, 406, 297
+//   4096 tokens, 4 heads of 192                         96, 163, 358
+//   8192 tokens, 16 heads of 128                       177, 249, 532
+//   4 x 4096 tokens, 16 heads of 128                   258, 178, 297
+//   16 x 2048 tokens, 12 heads of 128                  387, 284, 333
+//   16 x 4096 tokens, 16 heads of 64 x 128             711, 589, 530
+//   12 prompts of 1 to 5000 tokens, 16 heads of 128    256, 195, 346
+//   8 packed sequences of 1024, 4 heads of 192          60,  52, 102
+// and with what a backward reads, then the backward's
+//   8 x 1024 tokens, 4 heads of 192                     78,  61, 106    95,  70
+//   16 x 2048 tokens, 12 heads of 128                  569, 398, 380   556, 385, 392
+//   16 x 2048 tokens, 16 heads of 64                   280, 194, 154   291, 204, 182
+//   32 x 2048 tokens, 4 heads of 96                    280, 223, 171   297, 289, 221
+//   16 x 2048 tokens, 4 heads of 256                   527, 412        534, 397
+// The packed rows are one where the guess of the longest sequence is near and one
+// where it is three times too long and takes the narrower scan.
 // The three parts of 64 columns fit in LDS up to 192 features, the backward's up
 // to 128.
 constexpr int scan_widest(int KS, bool backward) { return KS <= (backward ? 4 : 6) ? 4 : 2; }
-inline int scan_tiles(int64_t T, int nseq, int Hv, int Dk, int Dv, bool packed, bool backward) {
-  const int tiles[3] = {1, 2, 4}, tenths[3] = {20, 23, 30};
+inline int scan_tiles(int64_t T, int nseq, int Hv, int Dk, int Dv, bool packed, bool backward, bool stored) {
+  const int tiles[3] = {1, 2, 4}, tenths[3] = {20, 28, stored ? 40 : 43};
   const int widths = scan_widest((Dk + 31) / 32, backward) == 4 ? 3 : 2;
   const int64_t total = T / kC + nseq, mean = (total + nseq - 1) / nseq, cps = (T + kC - 1) / kC;
   int best = 1;
@@ -356,7 +365,7 @@ inline int scan_tiles(int64_t T, int nseq, int Hv, int Dk, int Dv, bool packed, 
   return best;
 }
 inline int scan_tiles(const Args& a, bool backward) {
-  return scan_tiles(a.T, a.nseq, a.Hv, a.Dk, a.Dv, a.table != nullptr, backward);
+  return scan_tiles(a.T, a.nseq, a.Hv, a.Dk, a.Dv, a.table != nullptr, backward, a.s0 != nullptr);
 }
 
 // Features up to which a kernel instance goes, in steps of 32: the next of 2,
@@ -410,7 +419,7 @@ inline Workspace workspace_of(int64_t B, int64_t T, int nseq, int Hk, int Hv, in
   // then from a copy in fragment order, 1 KiB a load, and not 64 bytes of each
   // of 16 rows (a chunk of 192 features 2.1 -> 1.5 us; with more columns a
   // workgroup the copy costs more than it saves).
-  const bool copies = scan_tiles(T, nseq, Hv, Dk, Dv, packed, backward) == 1;
+  const bool copies = scan_tiles(T, nseq, Hv, Dk, Dv, packed, backward, backward) == 1;
   w.kf = take(copies ? frags : 0);
   w.qf = take(copies && !backward ? frags : 0);
   if (!copies) w.kf = w.qf = SIZE_MAX;

@@ -463,7 +463,7 @@ int check_args(const Args& a, int B, bool packed, bool backward, const char* wha
   // a launch has fewer than 2^32 threads: of a chunk and key head (operands,
   // gradients), of a workgroup of the scans
   const int64_t chunk = backward && steps_of(a.Dk) > 2 ? 128 * steps_of(a.Dk) : 256;
-  const int64_t scans = scan_blocks(a, 16 * scan_tiles(a.T, a.nseq, a.Hv, a.Dk, a.Dv, packed, backward));
+  const int64_t scans = scan_blocks(a, 16 * scan_tiles(a.T, a.nseq, a.Hv, a.Dk, a.Dv, packed, backward, backward));
   UTTT_REQUIRE(slots >= 0 && slots * a.Hv < (1LL << 31) && slots * a.Hk * chunk < (1LL << 32) &&
                    scans * 512 < (1LL << 32),
                "%s: too many chunks and heads for one launch", what);
