@@ -20,8 +20,14 @@
 // gradients takes that fp32 operand as the sum of three bf16 values (x1 = bf16(x),
 // x2 = bf16(x - x1), x3 = bf16(x - x1 - x2), all of its 24 bits) and adds the
 // products that are not below 2^-24 in fp32; q, k, v and do are bf16 as given.
-// Where only bf16 results come of it, the first two parts go in (at most 2^-16
-// left out): S0, U and P for the outputs.
+// Where only 16-bit results come of it the first two parts go in, at most 2^-16
+// left out where the result's rounding is 2^-8 or 2^-11: S0, U and P for the
+// outputs; D, M and X of the gradients, and there U, S0, dR and dS' where g and
+// beta are both 16-bit types.  What a backward keeps or exchanges (U, S0, dR, dS')
+// is stored in fp32.  With two parts throughout states came out 4e-6 off the
+// 64-bit recurrence and dg and dbeta 5e-6, with three 1.3e-7 and 3e-7, as the same
+// sums in plain fp32.  Decays are e^x by the hardware's 2^x, off by |x| 2^-24 and
+// an ulp or two, of differences of sums held in 64 bits.
 //
 // Fragments.  v_mfma_f32_16x16x32_bf16 takes from lane (r = lane % 16, q =
 // lane / 16) eight consecutive values 8q..8q+7 of the contracted axis for row

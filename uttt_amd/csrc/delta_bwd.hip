@@ -14,9 +14,9 @@
 // a sum without cancelling terms, where differences of running sums of o.do
 // and v.dv would lose a strong decay's small gradient.
 //
-// Measured, 16 x 2048 tokens, 12 heads of 128 by 128: scan 330 us (0.7 GB
-// stored, 0.55 GB loaded: 3.8 TB/s), gradients 562 us (1.8 GB from and to
-// memory, 0.6 GB once more from cache).
+// Measured, 16 x 2048 tokens, 12 heads of 128 by 128, 16-bit gates: scan 395 us
+// (0.7 GB stored, 0.63 loaded: 3.4 TB/s), gradients 565 us (2 GB from and to
+// memory, 0.6 once more from cache).
 #include "delta.h"
 
 namespace uttt {
@@ -411,7 +411,10 @@ __global__ __launch_bounds__(512) void delta_scan_bwd_kernel(Args a) {
 // with dS' come in a second pass, when those with S0 and the [64, 64] ones are
 // done, which reads U and S0 (for <S0, dS'>) once more from cache.  With all
 // of them in one pass and one workgroup a CU 6144 chunks of 128 x 128 took 745
-// us, with two workgroups and the registers spilled 1129.
+// us, with two workgroups and the registers spilled 1129, as it is now 565.
+// D, M and M^T go through LDS a part at a time; the second is 34 us of that.  PARTS: bf16 parts
+// of U, S0, dR, dS' and X, 3 where g or beta is fp32 and its gradient shows what a
+// third holds, 2 where both are 16-bit.
 constexpr int grads_waves(int KS, bool shared, int parts) {   // per SIMD, at least
   return KS == 8 ? 4 : KS == 6 ? 3 : shared || (parts == 3 && KS < 4) ? 2 : 4;
 }

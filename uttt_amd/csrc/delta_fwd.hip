@@ -19,12 +19,15 @@
 // products: NaN in its column from its token on, in the outputs, in U as saved
 // and in what goes to the state.  With ordinary values that is one test of R and
 // two of a flag a chunk (one sequence of 8192 tokens, 16 heads of 64 by 64, whose
-// chunks are the shortest: scan 105 -> 113 us; other scans 0 to 1 %).
+// chunks are the shortest: scan 105 -> 113 us with operands in two parts; other
+// scans 0 to 1 %).
 //
-// Measured: one sequence of 4096 tokens, 4 heads of 192 by 192, 79 us (1.2 us a
-// chunk; with X in the state's waves and K read by rows 140); 16 x 2048 tokens,
-// 12 heads of 128 by 128, with U and S0 stored for a backward, 338 us: 0.7 GB of
-// stores and 0.55 GB of loads at 3.7 TB/s (a copy reaches 5.1).
+// Measured: one sequence of 4096 tokens, 4 heads of 192 by 192, 97 us (1.5 us a
+// chunk); 16 x 2048 tokens, 12 heads of 128 by 128, with U and S0 stored for a
+// backward, 383 us: 0.7 GB of stores and 0.6 GB of loads at 3.4 TB/s (a copy
+// reaches 5.1).  The third part of the operands is 15 to 20 % of a scan that a
+// chunk's chain bounds: with two 80 us and 348.  With T and K^T loaded where their
+// last value was used, not a whole chunk ahead, the first takes 15 us more.
 #include "delta.h"
 
 namespace uttt {
@@ -245,9 +248,8 @@ __device__ __forceinline__ void scan_state(const Args& a, const Scan& s, const L
 // The tokens' waves: R = b (V - gam K S0) and O = s gam Q S0 + P U.
 template <int KS, int NT>
 __device__ __forceinline__ void scan_tokens(const Args& a, const Scan& s, const Lane& l, ScanLds<KS, NT>& lds) {
-  // With one tile there are registers to read S0 from LDS once for both products
-  // (4096 tokens, 4 heads of 192: 85 -> 79 us; four chains of products instead of
-  // two, or K and V two chunks ahead, gave nothing).
+  // With one tile there are registers to read S0's first two parts from LDS once
+  // for both products (4096 tokens, 4 heads of 192, with two parts: 85 -> 79 us).
   constexpr bool kHold = NT == 1;
   constexpr int kHeld = kHold ? KS : 1;
   const int wave = l.wave, q = l.q;

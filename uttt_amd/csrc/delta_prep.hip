@@ -3,11 +3,12 @@
 // (I + A)^-1, P and the transposed keys, laid out as the matrix instruction's
 // operand fragments for the scans that follow.
 //
-// Bound by memory: K and Q read once, 24 KiB of T and P and 256 bytes a feature
-// of K^T (and Q^T, K, Q where asked for) written per chunk and head.  16 x 2048
-// tokens, 12 heads of 128: 119 us forward, 137 backward, 3.9 and 4.1 TB/s.  The
-// backward makes its operands again: kept from the forward they would hold 350
-// MB of that layer to save a tenth of its step.
+// Bound by memory: K and Q read once; T and P written, 30 KiB a chunk and value
+// head (36 in the backward), and K^T (Q^T, K, Q where asked for), 128 bytes a
+// feature of a chunk and key head each.  16 x 2048 tokens, 12 heads of 128: 129 us
+// forward, 150 backward, 3.9 and 4.2 TB/s.  The backward makes its operands again:
+// kept from the forward, transposed, they would hold 430 MB of that layer to save
+// a tenth of its step.
 #include "delta.h"
 
 namespace uttt {

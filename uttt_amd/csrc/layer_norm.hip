@@ -356,7 +356,8 @@ bool whole_pieces(const LnArgs& a, int size) {
 // Workgroups of the backward: each writes 8 bytes per column, so that it has
 // 4 rows or more to walk over (4099 rows of 1537 fp32: 256 workgroups 55 us,
 // 1024 23 us).  A function of the sizes alone, so that its sums come out the
-// same on every run.
+// same on every run (the rows of a workgroup are added in an order that also goes
+// by whether 16-byte pieces fit).
 int64_t bwd_blocks(int64_t rows, int N) {
   const int64_t per = N <= 64 ? 16 : 4;
   const int64_t n = (rows + per - 1) / per;

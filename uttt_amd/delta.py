@@ -227,9 +227,9 @@ def gated_delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, *
     holds for the gradients too, where those given for the later outputs are zeros.
 
     q, k and v may be views with any strides of their first three axes that are multiples of
-    8 elements; others are copied.  Everything but q, k, v, the outputs and the gradients of
-    q, k and v is kept to fp32's order.  The backward keeps U and the state at every 64th
-    token, 4 bytes an element."""
+    8 elements; others are copied.  States, their gradients and those of fp32 g and beta are
+    exact to fp32's order, outputs and the other gradients are rounded to their types once.
+    The backward keeps U and the state at every 64th token, 4 bytes an element."""
     what = "gated_delta_rule"
     B, T, Hk, Hv, Dk, Dv = _check(q, k, v, g, beta, what)
     assert q.dtype == torch.bfloat16, f"{what}: q, k and v must be bf16, got {q.dtype}"

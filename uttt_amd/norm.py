@@ -95,9 +95,9 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
     x [..., N] in fp32, bf16 or fp16; weight and bias [N], each None or in any
     of the three (fp32 weights with bf16 activations included).  Gradients have
     their inputs' dtypes; those of weight and bias are summed over the rows in
-    fp32, in an order that the shape alone decides.  x may be a view whose rows
-    are evenly spaced (a slice of the last axis); other views are copied.
-    Gradients of its gradients are refused."""
+    fp32, in an order that the shape and the 16-byte alignment of tensors and
+    rows decide.  x may be a view whose rows are evenly spaced (a slice of the
+    last axis); other views are copied.  Gradients of its gradients are refused."""
     L.require_device(x, weight, bias)
     assert x.dim() >= 1 and x.shape[-1] >= 1, "layer_norm: x must be [..., N] with N of 1 or more"
     assert x.dtype in _TYPES, f"layer_norm: dtype {x.dtype}"
