@@ -765,6 +765,124 @@ int uttt_rotary_axes(const void* x, int dtype, const int64_t* x_strides, int B, 
                      const float* inv_freq, const int* sections, int axes, int interleaved,
                      int inverse, void* out, void* stream);
 
+/* ---- The state space layer: short causal convolution and selective scan ----
+ * Sequences as the gated delta rule's: cu_seqlens NULL: B sequences of T
+ * tokens, nseq = B; else B = 1 and sequence n is tokens cu_seqlens[n] ..
+ * cu_seqlens[n + 1] (nseq + 1 ascending offsets on the device, clamped to
+ * [0, T]); outputs and gradients of tokens of no sequence are zeros.  x and
+ * what has its shape: element strides {batch, token}, channels contiguous;
+ * B and C: {batch, token, group}, states contiguous.  Outputs and gradients
+ * are contiguous.  workspaces lie on 16 bytes.
+ *
+ * Convolution: y_t = act(b + sum_k w[k] x_{t-W+1+k}) per channel, W 2 to 8,
+ * act the identity or silu; weight [D, W], bias [D] or NULL, each in its own
+ * dtype code.  initial_state [nseq, W - 1, D] (x's dtype, the oldest input
+ * first; NULL: zeros) are the inputs before a sequence's first, final_state
+ * the last W - 1 of them all (NULL: not wanted).  bwd: dfinal_state NULL:
+ * zeros; dweight, dbias, dinitial_state NULL where not wanted. */
+int uttt_causal_conv_fwd(const void* x, const int64_t* x_strides, int dtype, const void* weight,
+                         int weight_dtype, const void* bias, int bias_dtype, int silu,
+                         const void* initial_state, const void* cu_seqlens, int cu_is_int64, int B,
+                         int T, int nseq, int D, int W, void* out, void* final_state,
+                         void* stream);
+size_t uttt_causal_conv_bwd_workspace_bytes(int B, int T, int nseq, int packed, int D, int W);
+int uttt_causal_conv_bwd(const void* x, const int64_t* x_strides, int dtype, const void* weight,
+                         int weight_dtype, const void* bias, int bias_dtype, int silu,
+                         const void* initial_state, const void* cu_seqlens, int cu_is_int64, int B,
+                         int T, int nseq, int D, int W, const void* dout,
+                         const int64_t* dout_strides, const void* dfinal_state, void* dx,
+                         void* dweight, void* dbias, void* dinitial_state, void* workspace,
+                         size_t workspace_bytes, void* stream);
+/* T tokens per row against state [slots, W - 1, D] in place, slots
+ * state_stride elements apart; indices as uttt_gated_delta_step's. */
+int uttt_causal_conv_step(const void* x, const int64_t* x_strides, int dtype, const void* weight,
+                          int weight_dtype, const void* bias, int bias_dtype, int silu, int B,
+                          int T, int D, int W, void* state, int64_t state_stride, int slots,
+                          const void* indices, int indices_int64, void* out, void* stream);
+
+/* Scan, per channel d of group g = d / (D / G) with a state h [N], N up to 64:
+ *   dt = softplus(dt_t + dt_bias) or dt_t + dt_bias
+ *   h_t[n] = e^{dt A[n]} h_{t-1}[n] + dt x_t B_t[g, n]
+ *   y_t = sum_n C_t[g, n] h_t[n] + skip x_t,  out_t = y_t silu(gate_t)
+ * x, gate, out [B, T, D] and B, C [B, T, G, N] of one dtype code, dt [B, T, D]
+ * in its own; A [D, N], skip, dt_bias [D] fp32 (skip, gate, dt_bias NULL: left
+ * out); states [nseq, D, N] fp32, A and states on 16 bytes.  tile_states
+ * [uttt_selective_scan_tiles, D, N] fp32 are the states at every 16th token
+ * for the backward, NULL without one.  bwd: dskip, dgate and ddt_bias belong
+ * to skip, gate and dt_bias; dinitial_state NULL where not wanted. */
+int uttt_selective_scan_tiles(int B, int T, int nseq, int packed);
+size_t uttt_selective_scan_fwd_workspace_bytes(int B, int T, int nseq, int packed, int D, int N,
+                                               int G);
+int uttt_selective_scan_fwd(const void* x, const int64_t* x_strides, int dtype, const void* dt,
+                            const int64_t* dt_strides, int dt_dtype, const float* A, const void* Bm,
+                            const int64_t* B_strides, const void* Cm, const int64_t* C_strides,
+                            const float* skip, const void* gate, const int64_t* gate_strides,
+                            const float* dt_bias, int dt_softplus, const float* initial_state,
+                            const void* cu_seqlens, int cu_is_int64, int B, int T, int nseq, int D,
+                            int N, int G, void* out, float* final_state, float* tile_states,
+                            void* workspace, size_t workspace_bytes, void* stream);
+size_t uttt_selective_scan_bwd_workspace_bytes(int B, int T, int nseq, int packed, int D, int N,
+                                               int G);
+int uttt_selective_scan_bwd(const void* x, const int64_t* x_strides, int dtype, const void* dt,
+                            const int64_t* dt_strides, int dt_dtype, const float* A, const void* Bm,
+                            const int64_t* B_strides, const void* Cm, const int64_t* C_strides,
+                            const float* skip, const void* gate, const int64_t* gate_strides,
+                            const float* dt_bias, int dt_softplus, const void* cu_seqlens,
+                            int cu_is_int64, int B, int T, int nseq, int D, int N, int G,
+                            const float* tile_states, const void* dout, const int64_t* dout_strides,
+                            const float* dfinal_state, void* dx, void* ddt, float* dA, void* dB,
+                            void* dC, float* dskip, void* dgate, float* ddt_bias,
+                            float* dinitial_state, void* workspace, size_t workspace_bytes,
+                            void* stream);
+/* T tokens per row against state [slots, D, N] fp32 in place, slots
+ * state_stride elements apart (where N is a multiple of 4 on 16 bytes);
+ * indices as uttt_gated_delta_step's. */
+int uttt_selective_scan_step(const void* x, const int64_t* x_strides, int dtype, const void* dt,
+                             const int64_t* dt_strides, int dt_dtype, const float* A,
+                             const void* Bm, const int64_t* B_strides, const void* Cm,
+                             const int64_t* C_strides, const float* skip, const void* gate,
+                             const int64_t* gate_strides, const float* dt_bias, int dt_softplus,
+                             int B, int T, int D, int N, int G, float* state, int64_t state_stride,
+                             int slots, const void* indices, int indices_int64, void* out,
+                             void* stream);
+
+/* ---- The norms around a block ----------------------------------------------
+ * Over rows of N up to 8192 elements, rms(v) = sqrt(sum(v^2) / N + eps):
+ *   after:  y = residual + s (x / rms(x)) weight silu(gate)
+ *   before: sum = residual + s x,  y = sum / rms(sum) weight
+ * with s = alpha scale.  Rows are in groups of `heads`: row i at i / heads *
+ * strides[0] + i % heads * strides[1].  gate has x's dtype; weight and scale
+ * [N], NULL: ones, each in its own dtype code.  after: residual and gate NULL:
+ * left out; y in out_dtype, which is the residual's.  before: y in x's dtype,
+ * sum in the residual's.  Outputs contiguous; rstd [rows] fp32, NULL where no
+ * backward follows.  bwd: dout (before: and dsum) with strides, NULL (before):
+ * zeros; dweight, dscale in weight's and scale's dtype, NULL where not wanted,
+ * else the workspace; the residual's gradient of `after` is dout itself. */
+int uttt_norm_after_fwd(const void* x, const int64_t* x_strides, int dtype, const void* weight,
+                        int weight_dtype, const void* gate, const int64_t* gate_strides,
+                        const void* residual, const int64_t* residual_strides, int out_dtype,
+                        const void* scale, int scale_dtype, float alpha, int64_t rows, int heads,
+                        int N, float eps, void* out, float* rstd, void* stream);
+int uttt_norm_before_fwd(const void* x, const int64_t* x_strides, int dtype, const void* residual,
+                         const int64_t* residual_strides, int residual_dtype, const void* weight,
+                         int weight_dtype, const void* scale, int scale_dtype, float alpha,
+                         int64_t rows, int heads, int N, float eps, void* out, void* sum,
+                         float* rstd, void* stream);
+size_t uttt_norm_bwd_workspace_bytes(int64_t rows, int N);
+int uttt_norm_after_bwd(const void* x, const int64_t* x_strides, int dtype, const void* weight,
+                        int weight_dtype, const void* gate, const int64_t* gate_strides,
+                        const void* scale, int scale_dtype, float alpha, int64_t rows, int heads,
+                        int N, const float* rstd, const void* dout, const int64_t* dout_strides,
+                        int dout_dtype, void* dx, void* dgate, void* dweight, void* dscale,
+                        void* workspace, size_t workspace_bytes, void* stream);
+int uttt_norm_before_bwd(const void* x, const int64_t* x_strides, int dtype, const void* residual,
+                         const int64_t* residual_strides, int residual_dtype, const void* weight,
+                         int weight_dtype, const void* scale, int scale_dtype, float alpha,
+                         int64_t rows, int heads, int N, const float* rstd, const void* dout,
+                         const int64_t* dout_strides, const void* dsum, const int64_t* dsum_strides,
+                         void* dx, void* dresidual, void* dweight, void* dscale, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,6 +18,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libuttt_hip.so")
 
 c_int, c_i64, c_sz, c_p = ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_void_p
+c_float = ctypes.c_float
 
 # dtype codes of the C ABI
 F32, BF16, F16 = 0, 1, 2
@@ -229,6 +230,79 @@ SIGNATURES = {
         c_int,
         [c_p, c_int, c_p, c_int, c_int, c_int, c_int, c_p, c_int, c_p, c_p, c_p, c_int, c_int,
          c_int, c_p, c_p],
+    ),
+    "uttt_causal_conv_fwd": (
+        c_int,
+        [c_p, c_p, c_int, c_p, c_int, c_p, c_int, c_int, c_p, c_p, c_int, c_int, c_int,
+         c_int, c_int, c_int, c_p, c_p, c_p],
+    ),
+    "uttt_causal_conv_bwd_workspace_bytes": (
+        c_sz,
+        [c_int, c_int, c_int, c_int, c_int, c_int],
+    ),
+    "uttt_causal_conv_bwd": (
+        c_int,
+        [c_p, c_p, c_int, c_p, c_int, c_p, c_int, c_int, c_p, c_p, c_int, c_int, c_int,
+         c_int, c_int, c_int, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_sz, c_p],
+    ),
+    "uttt_causal_conv_step": (
+        c_int,
+        [c_p, c_p, c_int, c_p, c_int, c_p, c_int, c_int, c_int, c_int, c_int, c_int,
+         c_p, c_i64, c_int, c_p, c_int, c_p, c_p],
+    ),
+    "uttt_selective_scan_tiles": (
+        c_int,
+        [c_int, c_int, c_int, c_int],
+    ),
+    "uttt_selective_scan_fwd_workspace_bytes": (
+        c_sz,
+        [c_int, c_int, c_int, c_int, c_int, c_int, c_int],
+    ),
+    "uttt_selective_scan_fwd": (
+        c_int,
+        [c_p, c_p, c_int, c_p, c_p, c_int, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p,
+         c_int, c_p, c_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_p, c_p,
+         c_p, c_p, c_sz, c_p],
+    ),
+    "uttt_selective_scan_bwd_workspace_bytes": (
+        c_sz,
+        [c_int, c_int, c_int, c_int, c_int, c_int, c_int],
+    ),
+    "uttt_selective_scan_bwd": (
+        c_int,
+        [c_p, c_p, c_int, c_p, c_p, c_int, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p,
+         c_int, c_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_p, c_p, c_p,
+         c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_sz, c_p],
+    ),
+    "uttt_selective_scan_step": (
+        c_int,
+        [c_p, c_p, c_int, c_p, c_p, c_int, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p,
+         c_int, c_int, c_int, c_int, c_int, c_int, c_p, c_i64, c_int, c_p, c_int, c_p,
+         c_p],
+    ),
+    "uttt_norm_after_fwd": (
+        c_int,
+        [c_p, c_p, c_int, c_p, c_int, c_p, c_p, c_p, c_p, c_int, c_p, c_int, c_float,
+         c_i64, c_int, c_int, c_float, c_p, c_p, c_p],
+    ),
+    "uttt_norm_before_fwd": (
+        c_int,
+        [c_p, c_p, c_int, c_p, c_p, c_int, c_p, c_int, c_p, c_int, c_float, c_i64,
+         c_int, c_int, c_float, c_p, c_p, c_p, c_p],
+    ),
+    "uttt_norm_bwd_workspace_bytes": (
+        c_sz,
+        [c_i64, c_int],
+    ),
+    "uttt_norm_after_bwd": (
+        c_int,
+        [c_p, c_p, c_int, c_p, c_int, c_p, c_p, c_p, c_int, c_float, c_i64, c_int,
+         c_int, c_p, c_p, c_p, c_int, c_p, c_p, c_p, c_p, c_p, c_sz, c_p],
+    ),
+    "uttt_norm_before_bwd": (
+        c_int,
+        [c_p, c_p, c_int, c_p, c_p, c_int, c_p, c_int, c_p, c_int, c_float, c_i64,
+         c_int, c_int, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_sz, c_p],
     ),
 }
 

@@ -11,6 +11,7 @@ autograd refuses a backward that saved one of them before).
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 import inspect
 
@@ -100,6 +101,27 @@ def first_order_only(what, grads, *inputs):
     if not torch.is_grad_enabled():
         return grads
     return _FirstOrder.apply(what, len(grads), *grads, *(t for t in inputs if t is not None))
+
+
+def no_gradient(what, *tensors):
+    """Refuses tensors through which a gradient would have to flow, backward or
+    forward, in a call that changes its states in place."""
+    tensors = [t for t in tensors if t is not None]
+    assert not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) and not (
+        forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)), (
+        f"{what}: no gradient flows through a state that is updated in place")
+
+
+@functools.lru_cache(maxsize=256)
+def _int64s(*values):
+    """Host integers as the C ABI takes them (read during a call, never written)."""
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def strides_of(t, axes):
+    """Element strides of t's first `axes` axes as the C ABI takes them, 0 along an
+    axis of one, whose stride says nothing."""
+    return _int64s(*(s if n > 1 else 0 for s, n in zip(t.stride()[:axes], t.shape)))
 
 
 def none_if_empty(t):

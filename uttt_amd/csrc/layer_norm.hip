@@ -15,7 +15,7 @@
 // them) are read again from cache for each pass, their sums in 64 bits.
 // 65536 rows of 768 bf16: forward 46 us (4.4 TB/s), backward 65 (4.6) and the
 // sum over the workgroups 5.
-#include "common.h"
+#include "rows.h"
 
 namespace uttt {
 namespace {
@@ -37,34 +37,6 @@ struct LnArgs {
   float* part;           // [workgroups, 2, N]
 };
 
-template <class TT, int V>
-__device__ __forceinline__ void load_piece(const typename TT::S* p, float (&v)[V]) {
-  typename TT::S w[V];
-  __builtin_memcpy(w, __builtin_assume_aligned(p, sizeof w > 16 ? 16 : sizeof w), sizeof w);
-#pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = TT::load(w[i]);
-}
-template <class TT, int V>
-__device__ __forceinline__ void store_piece(typename TT::S* p, const float (&v)[V]) {
-  typename TT::S w[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) w[i] = TT::store(v[i]);
-  __builtin_memcpy(__builtin_assume_aligned(p, sizeof w), w, sizeof w);
-}
-// V weights from element e, `none` where there is no weight tensor.
-template <int V>
-__device__ __forceinline__ void load_weights(const void* p, int dtype, int e, float none, float (&v)[V]) {
-  if (p == nullptr) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = none;
-  } else if (dtype == UTTT_F32) {
-    load_piece<F32T, V>(static_cast<const float*>(p) + e, v);
-  } else if (dtype == UTTT_BF16) {
-    load_piece<BF16T, V>(static_cast<const uint16_t*>(p) + e, v);
-  } else {
-    load_piece<F16T, V>(static_cast<const uint16_t*>(p) + e, v);
-  }
-}
 __device__ __forceinline__ float load_w(const void* p, int dtype, int i) {
   if (dtype == UTTT_F32) return static_cast<const float*>(p)[i];
   const uint16_t h = static_cast<const uint16_t*>(p)[i];

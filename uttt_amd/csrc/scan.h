@@ -1,0 +1,149 @@
+// The selective state space scan's geometry (scan_fwd.hip, scan_bwd.hip).  Per
+// channel d of group g = d / (D / G), with a state h [N]:
+//   dt_t = softplus(raw_t + bias) or raw_t + bias
+//   h_t[n] = e^{dt_t A[n]} h_{t-1}[n] + dt_t x_t B_t[g, n]
+//   y_t = sum_n C_t[g, n] h_t[n] + Dskip x_t,  out_t = y_t silu(z_t) (y_t without a gate)
+// Everything between the loads and the stores is fp32; decays are 2^(dt A log2 e)
+// by the hardware's 2^x.
+//
+// A lane holds four states of CS channels, LN = ceil(N / 4) lanes (a power of
+// two) hold a channel, a workgroup of four waves CB channels of one group.  It
+// walks over a run of a sequence's tokens in tiles of 16: its threads load
+// x, dt (and z, the outputs' gradient), turn them into what the recurrence
+// takes and put that into LDS, where the lanes of a channel read it.
+#pragma once
+
+#include <float.h>
+
+#include "state_space.h"
+
+namespace uttt {
+namespace ssm {
+
+constexpr int kTile = 16;            // tokens of a tile; a backward's states are kept at their starts
+constexpr int kScanThreads = 256;
+constexpr int kMaxStates = 64;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+struct ScanArgs {
+  Seqs seqs;
+  int D, N, G, Dg;         // Dg = D / G channels share B and C
+  int R;                   // tokens of a run, a multiple of kTile
+  int nruns, ncb;          // runs; workgroups for a run and group
+  const void *x, *dt, *Bm, *Cm, *z;
+  int64_t x_sb, x_st, dt_sb, dt_st, z_sb, z_st, B_sb, B_st, B_sg, C_sb, C_st, C_sg;
+  int dt_dtype, soft;
+  const float *A, *Dskip, *bias, *h0;   // [D, N], [D] or null, [D] or null, [nseq, D, N] or null
+  void* out;               // [B, T, D]
+  float *hT, *hs;          // [nseq, D, N] or null; [tiles, D, N] or null
+  float *ends, *starts;    // [nruns, D, N]: of each run on its own; with what came before it
+  float* decay;            // [nruns, D] sums of dt over a run
+  // backward
+  const void* dout;        // [B, T, D]
+  int64_t do_sb, do_st;
+  const float* dhT;        // or null
+  void *dx, *ddt, *dz;     // [B, T, D] in x's, dt's and x's type
+  float* dh0;              // or null
+  float *part_A, *part_D, *part_bias;   // [nruns, D, N], [nruns, D], [nruns, D] or null
+  float* part_bc;          // [ncb, B, T, 2, G, N]
+};
+
+template <int LN>
+struct Geo {
+  static constexpr int NP = 4 * LN;               // states with those that only fill up
+  static constexpr int CS = LN >= 4 ? 2 : 1;      // channels of a lane
+  static constexpr int WC = CS * 64 / LN;         // of a wave
+  static constexpr int CB = 4 * WC;               // of a workgroup
+  static constexpr int TPP = kScanThreads / CB;   // tokens that the threads cover at a time
+  static constexpr int EPT = kTile / TPP;         // elements of a tile per thread
+  static constexpr int BPT = (kTile * NP + kScanThreads - 1) / kScanThreads;   // of B or C
+};
+
+inline int scan_lanes(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
+inline int scan_width(int N) {   // Geo<scan_lanes(N)>::CB
+  const int ln = scan_lanes(N);
+  return (ln >= 4 ? 512 : 256) / ln;
+}
+
+// Sum over the LN lanes of a channel, in all of them.
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float x) {
+  return x + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+template <int LN>
+__device__ __forceinline__ float sum_lanes(float x) {
+  if constexpr (LN > 1) x = dpp_add<0xb1>(x);    // lane ^ 1
+  if constexpr (LN > 2) x = dpp_add<0x4e>(x);    // lane ^ 2
+  if constexpr (LN > 4) x = dpp_add<0x141>(x);   // 7 - lane % 8
+  if constexpr (LN > 8) x = dpp_add<0x140>(x);   // 15 - lane % 16
+  return x;
+}
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A log2 e within fp32's finite range: a step of zero then decays nothing for
+// an A of -inf too (which a tile's empty tokens rely on).
+__device__ __forceinline__ float log2_rate(float A) {
+  const float v = A * kLog2e;
+  return v < -FLT_MAX ? -FLT_MAX : v > FLT_MAX ? FLT_MAX : v;
+}
+
+// Four states from index n of a row of N.
+__device__ __forceinline__ float4 load_states(const float* p, int n, int N) {
+  if ((N & 3) == 0) return n < N ? *reinterpret_cast<const float4*>(p + n) : make_float4(0, 0, 0, 0);
+  return make_float4(n < N ? p[n] : 0.0f, n + 1 < N ? p[n + 1] : 0.0f, n + 2 < N ? p[n + 2] : 0.0f,
+                     n + 3 < N ? p[n + 3] : 0.0f);
+}
+__device__ __forceinline__ void store_states(float* p, int n, int N, float4 v) {
+  if ((N & 3) == 0) {
+    if (n < N) *reinterpret_cast<float4*>(p + n) = v;
+    return;
+  }
+  if (n < N) p[n] = v.x;
+  if (n + 1 < N) p[n + 1] = v.y;
+  if (n + 2 < N) p[n + 2] = v.z;
+  if (n + 3 < N) p[n + 3] = v.w;
+}
+__device__ __forceinline__ void unpack(float4 v, float (&x)[4]) {
+  x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+}
+
+// An element as its bits, to be widened where it is used and not where it is loaded.
+__device__ __forceinline__ uint32_t load_bits(const void* p, int dtype, int64_t i) {
+  return dtype == UTTT_F32 ? static_cast<const uint32_t*>(p)[i] : static_cast<const uint16_t*>(p)[i];
+}
+__device__ __forceinline__ float widen(uint32_t bits, int dtype) {
+  return dtype == UTTT_F32 ? __uint_as_float(bits)
+         : dtype == UTTT_BF16 ? __uint_as_float(bits << 16) : f16_to_f32((uint16_t)bits);
+}
+
+// What a workgroup works on.
+struct Place {
+  Run run;
+  int t0, n;     // its tokens within the sequence
+  int g, d0, nc; // group, first channel, channels
+  __device__ __forceinline__ bool init(const ScanArgs& a, int CB) {
+    const int per = a.G * a.ncb;
+    const int at = blockIdx.x / per, blk = blockIdx.x % per;
+    g = blk / a.ncb;
+    const int c0 = (blk % a.ncb) * CB;
+    d0 = g * a.Dg + c0;
+    nc = min(CB, a.Dg - c0);
+    if (at >= a.nruns) {
+      run.seq = -1;
+      return false;
+    }
+    run = run_of(a.seqs, at, a.R);
+    t0 = run.c * a.R;
+    n = min(a.R, run.len - t0);
+    return run.seq >= 0;
+  }
+};
+
+int scan_check(const ScanArgs& a, int dtype, const char* what);
+// Runs of the tokens: enough that `want` workgroups have work.
+void scan_runs(ScanArgs& a, int want);
+bool scan_fits(const ScanArgs& a);
+
+}  // namespace ssm
+}  // namespace uttt
