@@ -805,10 +805,11 @@ int uttt_causal_conv_step(const void* x, const int64_t* x_strides, int dtype, co
  *   h_t[n] = e^{dt A[n]} h_{t-1}[n] + dt x_t B_t[g, n]
  *   y_t = sum_n C_t[g, n] h_t[n] + skip x_t,  out_t = y_t silu(gate_t)
  * x, gate, out [B, T, D] and B, C [B, T, G, N] of one dtype code, dt [B, T, D]
- * in its own; A [D, N], skip, dt_bias [D] fp32 (skip, gate, dt_bias NULL: left
- * out); states [nseq, D, N] fp32, A and states on 16 bytes.  tile_states
- * [uttt_selective_scan_tiles, D, N] fp32 are the states at every 16th token
- * for the backward, NULL without one.  bwd: dskip, dgate and ddt_bias belong
+ * of fp32 or theirs; A [D, N], skip, dt_bias [D] fp32 (skip, gate, dt_bias NULL: left
+ * out); states [nseq, D, N] fp32, A and states on 16 bytes; fewer than 2^24
+ * elements between tokens.  tile_states [uttt_selective_scan_tiles, K, D] fp32
+ * are the states at every 16th token for the backward, NULL without one, K
+ * being N up to the next power of two of 4 or more.  bwd: dskip, dgate and ddt_bias belong
  * to skip, gate and dt_bias; dinitial_state NULL where not wanted. */
 int uttt_selective_scan_tiles(int B, int T, int nseq, int packed);
 size_t uttt_selective_scan_fwd_workspace_bytes(int B, int T, int nseq, int packed, int D, int N,

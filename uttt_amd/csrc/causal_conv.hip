@@ -20,7 +20,7 @@ namespace {
 
 constexpr int kConvThreads = 256;
 constexpr int kMinWidth = 2, kMaxWidth = 8;
-constexpr int kLooseRuns = 8;   // runs' places behind the last run for the tokens of no sequence
+
 
 struct ConvArgs {
   Seqs seqs;

@@ -35,8 +35,8 @@ struct ScanArgs {
   int dt_dtype, soft;
   const float *A, *Dskip, *bias, *h0;   // [D, N], [D] or null, [D] or null, [nseq, D, N] or null
   void* out;               // [B, T, D]
-  float *hT, *hs;          // [nseq, D, N] or null; [tiles, D, N] or null
-  float *ends, *starts;    // [nruns, D, N]: of each run on its own; with what came before it
+  float *hT, *hs;          // [nseq, D, N] or null; [tiles, NP, D] or null
+  float *ends, *starts;    // [nruns, NP, D]: of each run on its own; with what came before it
   float* decay;            // [nruns, D] sums of dt over a run
   // backward
   const void* dout;        // [B, T, D]
@@ -117,6 +117,60 @@ __device__ __forceinline__ float widen(uint32_t bits, int dtype) {
          : dtype == UTTT_BF16 ? __uint_as_float(bits << 16) : f16_to_f32((uint16_t)bits);
 }
 
+// All the states of a channel, zeros behind the last, as the caller's tensors
+// hold them (side by side) and as the kernels keep them: NP states of all
+// channels, a state of a wave's channels side by side.
+template <int NP>
+__device__ __forceinline__ void load_row(const float* p, int N, float (&v)[NP]) {
+#pragma unroll
+  for (int j = 0; j < NP; ++j) v[j] = p[min(j, N - 1)];
+#pragma unroll
+  for (int j = 0; j < NP; ++j) v[j] = j < N ? v[j] : 0.0f;
+}
+template <int NP>
+__device__ __forceinline__ void store_row(float* p, int N, const float (&v)[NP]) {
+#pragma unroll
+  for (int j = 0; j < NP; ++j)
+    if (j < N) p[j] = v[j];
+}
+template <int NP>
+__device__ __forceinline__ void load_kept(const float* p, int D, uint32_t d, float (&v)[NP]) {
+#pragma unroll
+  for (int j = 0; j < NP; ++j) v[j] = (p + (int64_t)j * D)[d];
+}
+template <int NP>
+__device__ __forceinline__ void store_kept(float* p, int D, uint32_t d, const float (&v)[NP]) {
+#pragma unroll
+  for (int j = 0; j < NP; ++j) (p + (int64_t)j * D)[d] = v[j];
+}
+inline int kept_states(int N) { return 4 * scan_lanes(N); }
+
+// Waves of a SIMD in the kernels with a lane per channel: the loads of tokens
+// ahead and other tokens' decays take the registers that are left.
+constexpr int fwd_waves(int NP) { return NP <= 16 ? 4 : NP <= 32 ? 3 : 2; }
+
+// B or C of a tile on the way from memory to LDS.
+template <class TT, int NP>
+struct Rows16 {
+  static constexpr int kEach = (kTile * NP + kScanThreads - 1) / kScanThreads;
+  typename TT::S v[kEach];
+  // the tile's first token, tokens, states; row stride (a tile's offsets fit 32 bits)
+  __device__ __forceinline__ void load(const typename TT::S* p, uint32_t step, int n, int N) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const uint32_t e = threadIdx.x + i * kScanThreads;
+      v[i] = p[(uint32_t)min((int)(e / NP), n - 1) * step + (uint32_t)min((int)(e % NP), N - 1)];
+    }
+  }
+  __device__ __forceinline__ void write(float4* to, int n, int N) const {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int e = threadIdx.x + i * kScanThreads;
+      if (e < kTile * NP) reinterpret_cast<float*>(to)[e] = e / NP < n && e % NP < N ? TT::load(v[i]) : 0.0f;
+    }
+  }
+};
+
 // What a workgroup works on.
 struct Place {
   Run run;
@@ -141,8 +195,8 @@ struct Place {
 };
 
 int scan_check(const ScanArgs& a, int dtype, const char* what);
-// Runs of the tokens: enough that `want` workgroups have work.
-void scan_runs(ScanArgs& a, int want);
+// Runs of the tokens: enough that `want` workgroups of `width` channels have work.
+void scan_runs(ScanArgs& a, int width, int want);
 bool scan_fits(const ScanArgs& a);
 
 }  // namespace ssm

@@ -20,147 +20,173 @@ namespace uttt {
 namespace ssm {
 namespace {
 
-// What a run adds to the adjoint at its start, and the sum of its steps.
-template <class TT, int LN>
-__global__ __launch_bounds__(kScanThreads) void scan_adjoint_kernel(ScanArgs a) {
+// What a run adds to the adjoint at its start, and the sum of its steps: a lane
+// per channel, as in the forward.
+template <class TT, class DT, int NP, bool GATE>
+__global__ __launch_bounds__(kScanThreads, fwd_waves(NP)) void scan_adjoint_kernel(ScanArgs a) {
   using S = typename TT::S;
-  using M = Geo<LN>;
-  constexpr int CS = M::CS, CB = M::CB, NP = M::NP, EPT = M::EPT, BPT = M::BPT;
-  __shared__ float sDy[kTile][CB], sDt[kTile][CB];
-  __shared__ float4 sC[kTile][LN];
-  const int tid = threadIdx.x, c = tid % CB, tq = tid / CB;
+  using SD = typename DT::S;
+  __shared__ float4 sC[2][kTile][NP / 4];
+  const int tid = threadIdx.x;
   Place p;
-  if (!p.init(a, CB) || p.run.c == 0) return;   // nothing comes before the first one
+  if (!p.init(a, kScanThreads) || p.run.c == 0) return;   // nothing comes before the first one
   const int at = p.run.base + p.run.c;
-  const int64_t tok = p.run.tok0 + p.t0;
-  const bool live = c < p.nc;
-  const int64_t dt_at = p.run.b * a.dt_sb + tok * a.dt_st + p.d0 + c;
-  const S* gp = static_cast<const S*>(a.dout) + p.run.b * a.do_sb + tok * a.do_st + p.d0 + c;
-  const S* zp = static_cast<const S*>(a.z) + p.run.b * a.z_sb + tok * a.z_st + p.d0 + c;
-  const S* Cp = static_cast<const S*>(a.Cm) + p.run.b * a.C_sb + tok * a.C_st + p.g * a.C_sg;
-  const float bias = live && a.bias ? a.bias[p.d0 + c] : 0.0f;
-  const int wave = tid >> 6, lane = tid & 63, ln = lane % LN;
-  const int ch = wave * M::WC + lane / LN * CS;
-  float q[CS][4], A2[CS][4];
+  const int last = (p.n - 1) / kTile * kTile;             // it has tokens
+  const int64_t tok = p.run.tok0 + p.t0, end = tok + p.n - 1;
+  const bool busy = (tid & ~(kWave - 1)) < p.nc;
+  const uint32_t c = min(tid, p.nc - 1), d = p.d0 + c;
+  const SD* tp = static_cast<const SD*>(a.dt) + p.run.b * a.dt_sb + end * a.dt_st + p.d0;
+  const S* gp = static_cast<const S*>(a.dout) + p.run.b * a.do_sb + end * a.do_st + p.d0;
+  const S* zp = static_cast<const S*>(a.z) + p.run.b * a.z_sb + end * a.z_st + p.d0;
+  const S* Cp = static_cast<const S*>(a.Cm) + p.run.b * a.C_sb + (tok + last) * a.C_st + p.g * a.C_sg;
+  const float bias = a.bias ? a.bias[d] : 0.0f;
+  const bool soft = a.soft;
+  float q[NP], A2[NP];
+  load_row<NP>(a.A + (int64_t)d * a.N, a.N, A2);
 #pragma unroll
-  for (int s = 0; s < CS; ++s) {
-    unpack(ch + s < p.nc ? load_states(a.A + (int64_t)(p.d0 + ch + s) * a.N, 4 * ln, a.N) : make_float4(0, 0, 0, 0),
-           A2[s]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      A2[s][j] = log2_rate(A2[s][j]);
-      q[s][j] = 0.0f;
-    }
+  for (int j = 0; j < NP; ++j) {
+    A2[j] = log2_rate(A2[j]);
+    q[j] = 0.0f;
   }
-  S rg[EPT], rz[EPT], rC[BPT];
-  uint32_t rdt[EPT];
-  auto load_tile = [&](int tt) {
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      const int t = tt + tq + i * M::TPP;
-      rg[i] = rz[i] = S(0);
-      rdt[i] = 0;
-      if (live && t < p.n) {
-        rg[i] = gp[(int64_t)t * a.do_st];
-        rdt[i] = load_bits(a.dt, a.dt_dtype, dt_at + (int64_t)t * a.dt_st);
-        if (a.z) rz[i] = zp[(int64_t)t * a.z_st];
-      }
+  float sum_dt = 0.0f;
+  auto token = [&](const float4* qC, S gbits, SD dtbits, S zbits) {
+    const float raw = DT::load(dtbits) + bias, grown = softplus(raw), dt = soft ? grown : raw;
+    float dy = TT::load(gbits);
+    if (GATE) {
+      const float z = TT::load(zbits);
+      dy *= z * sigmoid(z);
     }
+    sum_dt += dt;
 #pragma unroll
-    for (int i = 0; i < BPT; ++i) {
-      const int e = tid + i * kScanThreads, t = tt + e / NP, n = e % NP;
-      rC[i] = e < kTile * NP && t < p.n && n < a.N ? Cp[(int64_t)t * a.C_st + n] : S(0);
+    for (int k = 0; k < NP / 4; ++k) {
+      float cc[4];
+      unpack(qC[k], cc);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        q[4 * k + j] = exp2_hw(dt * A2[4 * k + j]) * __builtin_fmaf(cc[j], dy, q[4 * k + j]);
     }
   };
-  float sum_dt = 0.0f;
-  const int last = (p.n - 1) / kTile * kTile;   // a run has tokens, or it is the first
-  load_tile(last);
-  for (int tt = last; tt >= 0; tt -= kTile) {
+  auto back = [&]() {
+    tp -= a.dt_st;
+    gp -= a.do_st;
+    if (GATE) zp -= a.z_st;
+  };
+  constexpr int U = 4;   // tokens that are loaded ahead
+  S rg[U], rz[U];
+  SD rdt[U];
+  auto load = [&]() {
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      const int tl = tq + i * M::TPP;
-      float dt = 0.0f, dy = TT::load(rg[i]);
-      if (a.z) {
-        const float z = TT::load(rz[i]);
-        dy *= z * sigmoid(z);
-      }
-      if (tt + tl < p.n) {
-        dt = widen(rdt[i], a.dt_dtype) + bias;
-        if (a.soft) dt = softplus(dt);
-      }
-      sum_dt += dt;
-      sDt[tl][c] = dt;
-      sDy[tl][c] = dy;
+    for (int i = 0; i < U; ++i) {
+      rg[i] = gp[c];
+      rdt[i] = tp[c];
+      if (GATE) rz[i] = zp[c];
+      back();
     }
-#pragma unroll
-    for (int i = 0; i < BPT; ++i) {
-      const int e = tid + i * kScanThreads;
-      if (e < kTile * NP) reinterpret_cast<float*>(sC)[e] = TT::load(rC[i]);
-    }
-    __syncthreads();
-    if (tt > 0) load_tile(tt - kTile);
-#pragma unroll
-    for (int t = kTile - 1; t >= 0; --t) {
-      float cc[4];
-      unpack(sC[t][ln], cc);
-#pragma unroll
-      for (int s = 0; s < CS; ++s) {
-        const float dt = sDt[t][ch + s], dy = sDy[t][ch + s];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) q[s][j] = exp2_hw(dt * A2[s][j]) * __builtin_fmaf(cc[j], dy, q[s][j]);
-      }
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int s = 0; s < CS; ++s)
-    if (ch + s < p.nc)
-      store_states(a.ends + ((int64_t)at * a.D + p.d0 + ch + s) * a.N, 4 * ln, a.N,
-                   make_float4(q[s][0], q[s][1], q[s][2], q[s][3]));
-  float* red = &sDt[0][0];
-  red[tid] = sum_dt;
+  };
+  Rows16<TT, NP> rC;
+  rC.load(Cp, (uint32_t)a.C_st, p.n - last, a.N);
+  rC.write(sC[0][0], p.n - last, a.N);
   __syncthreads();
-  if (tq == 0 && live) {
+  int t = p.n, buf = 0;
+  for (int tt = last; tt >= 0; tt -= kTile, buf ^= 1) {
+    if (tt > 0) {
+      Cp -= kTile * a.C_st;
+      rC.load(Cp, (uint32_t)a.C_st, kTile, a.N);
+    }
+    if (busy) {
+      const float4* qC = sC[buf][0] + (t - tt) * (NP / 4);
+      if (tt == last) {   // the last few, and the first loads
+#pragma unroll 1
+        for (; t % U; --t) {
+          qC -= NP / 4;
+          token(qC, gp[c], tp[c], GATE ? zp[c] : S(0));
+          back();
+        }
+        if (t > 0) load();
+      }
+#pragma unroll 1
+      for (; t > tt; t -= U) {
+        S g[U], z[U];
+        SD dt[U];
 #pragma unroll
-    for (int i = 1; i < M::TPP; ++i) sum_dt += red[c + i * CB];
-    a.decay[(int64_t)at * a.D + p.d0 + c] = sum_dt;
+        for (int i = 0; i < U; ++i) {
+          g[i] = rg[i];
+          dt[i] = rdt[i];
+          z[i] = rz[i];
+        }
+        if (t > U) load();
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          qC -= NP / 4;
+          token(qC, g[i], dt[i], z[i]);
+          __builtin_amdgcn_sched_barrier(0);   // as in the forward
+        }
+      }
+    }
+    if (tt > 0) rC.write(sC[buf ^ 1][0], kTile, a.N);
+    __syncthreads();
   }
+  if (!busy) return;
+  store_kept<NP>(a.ends + (int64_t)at * NP * a.D, a.D, d, q);
+  a.decay[(int64_t)at * a.D + d] = sum_dt;
 }
 
 // The adjoint behind each run of a sequence but the last.
-__global__ __launch_bounds__(kScanThreads) void scan_join_back_kernel(ScanArgs a, const float* __restrict__ ends,
+__global__ __launch_bounds__(kScanThreads) void scan_join_back_kernel(ScanArgs a, int keep, const float* __restrict__ ends,
                                                                       const float* __restrict__ decay,
                                                                       float* __restrict__ starts) {
-  const int64_t e = (int64_t)blockIdx.x * kScanThreads + threadIdx.x, M = (int64_t)a.D * a.N;
-  if (e >= M * a.seqs.nseq) return;
-  const int seq = (int)(e / M);
-  const int64_t at = e % M, d = at / a.N;
+  const int64_t e = (int64_t)blockIdx.x * kScanThreads + threadIdx.x, K = (int64_t)a.D * keep;   // K: states kept of a run
+  if (e >= K * a.seqs.nseq) return;
+  const int seq = (int)(e / K);
+  const int64_t in = e % K, d = in % a.D, n = in / a.D;
+  const bool real = n < a.N;   // the others stay zero
+  const int64_t own = d * a.N + n, M = (int64_t)a.D * a.N;   // as the caller holds it
   const Run r = span_of(a.seqs, seq, a.R);
   const int runs = (int)(((int64_t)r.len + a.R - 1) / a.R);
-  const float A2 = log2_rate(a.A[at]);
-  float q = a.dhT ? a.dhT[e] : 0.0f;
+  const float A2 = real ? log2_rate(a.A[own]) : 0.0f;
+  float q = a.dhT && real ? a.dhT[seq * M + own] : 0.0f;
 #pragma unroll 8
   for (int c = runs - 1; c > 0; --c) {
     const int64_t i = r.base + c;
-    q = __builtin_fmaf(exp2_hw(decay[i * a.D + d] * A2), q, ends[i * M + at]);
-    starts[(i - 1) * M + at] = q;
+    q = __builtin_fmaf(exp2_hw(decay[i * a.D + d] * A2), q, ends[i * K + in]);
+    starts[(i - 1) * K + in] = q;
   }
 }
 
 template <int LN>
 struct BwdLds {
   using M = Geo<LN>;
-  static constexpr int kGroup = 4;        // tokens whose sums over lanes are taken together
-  static constexpr int kRow = 64 + 4;     // float4 of one token's dB or dC, four to leave the banks
-  float u[kTile][M::CB], dt[kTile][M::CB], dy[kTile][M::CB];   // then du, sum A w, y
+  float u[kTile][M::CB], dt[kTile][M::CB], dy[kTile][M::CB];   // u: then du
+  float aw[kTile][M::CB], y[kTile][M::CB];                     // sums over the states
+  float slope[kTile][M::CB], dgate[kTile][M::CB];              // of the step by its input; dout silu'(z)
   float4 B[kTile][LN], C[kTile][LN];
-  float4 red[4][kGroup * 2][kRow];        // by wave
-  float4 sum[4][kTile][2][LN];
+  float sum[4][kTile][2][M::NP];   // dB and dC, by wave
 };
 
-template <class TT, int LN>
+// a + (lane ^ 32's) in the lower 32 lanes, b's in the upper ones.
+__device__ __forceinline__ float halves_add(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// a + (lane ^ 16's) in lanes 0..15 and 32..47, b's in the others.
+__device__ __forceinline__ float rows_add(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// Sum over the lanes of a row of 16 that are LN apart, in all of them.
+template <int LN>
+__device__ __forceinline__ float sum_apart(float x) {
+  if constexpr (LN < 16) x = dpp_add<0x128>(x);   // rotations by 8, 4, 2, 1
+  if constexpr (LN < 8) x = dpp_add<0x124>(x);
+  if constexpr (LN < 4) x = dpp_add<0x122>(x);
+  if constexpr (LN < 2) x = dpp_add<0x121>(x);
+  return x;
+}
+
+template <class TT, class DT, int LN, bool GATE>
 __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanArgs a) {
   using S = typename TT::S;
+  using SD = typename DT::S;
   using M = Geo<LN>;
   using L = BwdLds<LN>;
   constexpr int CS = M::CS, CB = M::CB, NP = M::NP, EPT = M::EPT, BPT = M::BPT;
@@ -183,32 +209,34 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanArgs a) {
         if (a.part_bias) a.part_bias[(int64_t)num * a.D + p.d0 + c] = 0.0f;
       }
     } else {   // the tokens of no sequence
-      for (int i = tq;; i += M::TPP) {
+      for (int i = num - a.nruns;; i += kLooseRuns) {
         const int t = loose_token(a.seqs, i);
         if (t < 0) break;
-        if (live) {
+        if (live && tq == 0) {
           const int64_t e = (int64_t)t * a.D + p.d0 + c;
           static_cast<S*>(a.dx)[e] = TT::store(0.0f);
-          store_any(a.ddt, a.dt_dtype, e, 0.0f);
-          if (a.z) static_cast<S*>(a.dz)[e] = TT::store(0.0f);
+          static_cast<SD*>(a.ddt)[e] = DT::store(0.0f);
+          if (GATE) static_cast<S*>(a.dz)[e] = TT::store(0.0f);
         }
         const int64_t row = ((int64_t)(p.d0 - p.g * a.Dg) / CB * a.seqs.T + t) * 2;
-        for (int n = c; n < 2 * a.N; n += CB)
+        for (int n = tid; n < 2 * a.N; n += kScanThreads)
           a.part_bc[((row + n / a.N) * a.G + p.g) * a.N + n % a.N] = 0.0f;
       }
     }
     return;
   }
   const int64_t tok = p.run.tok0 + p.t0;
-  const S* xp = static_cast<const S*>(a.x) + p.run.b * a.x_sb + tok * a.x_st + p.d0 + c;
-  const S* zp = static_cast<const S*>(a.z) + p.run.b * a.z_sb + tok * a.z_st + p.d0 + c;
-  const S* gp = static_cast<const S*>(a.dout) + p.run.b * a.do_sb + tok * a.do_st + p.d0 + c;
-  const int64_t dt_at = p.run.b * a.dt_sb + tok * a.dt_st + p.d0 + c;
+  const int cl = live ? c : p.nc - 1;   // loads of a thread without a channel are the last one's
+  const S* xp = static_cast<const S*>(a.x) + p.run.b * a.x_sb + tok * a.x_st + p.d0;
+  const S* zp = static_cast<const S*>(a.z) + p.run.b * a.z_sb + tok * a.z_st + p.d0;
+  const S* gp = static_cast<const S*>(a.dout) + p.run.b * a.do_sb + tok * a.do_st + p.d0;
+  const SD* tp = static_cast<const SD*>(a.dt) + p.run.b * a.dt_sb + tok * a.dt_st + p.d0;
   const S* Bp = static_cast<const S*>(a.Bm) + p.run.b * a.B_sb + tok * a.B_st + p.g * a.B_sg;
   const S* Cp = static_cast<const S*>(a.Cm) + p.run.b * a.C_sb + tok * a.C_st + p.g * a.C_sg;
-  const int64_t out0 = ((int64_t)p.run.b * a.seqs.T + tok) * a.D + p.d0 + c;
-  const float bias = live && a.bias ? a.bias[p.d0 + c] : 0.0f;
-  const float skip = live && a.Dskip ? a.Dskip[p.d0 + c] : 0.0f;
+  const int64_t out0 = ((int64_t)p.run.b * a.seqs.T + tok) * a.D + p.d0;
+  const float bias = a.bias ? a.bias[p.d0 + cl] : 0.0f;
+  const float skip = a.Dskip ? a.Dskip[p.d0 + cl] : 0.0f;
+  const bool soft = a.soft;
 
   float A2[CS][4], q[CS][4], dA[CS][4];
 #pragma unroll
@@ -218,8 +246,10 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanArgs a) {
     unpack(on ? load_states(a.A + row * a.N, 4 * ln, a.N) : make_float4(0, 0, 0, 0), A2[s]);
     float4 v = make_float4(0, 0, 0, 0);
     if (on) {
-      if (p.t0 + p.n < p.run.len) v = load_states(a.starts + ((int64_t)num * a.D + row) * a.N, 4 * ln, a.N);
-      else if (a.dhT) v = load_states(a.dhT + ((int64_t)p.run.seq * a.D + row) * a.N, 4 * ln, a.N);
+      if (p.t0 + p.n < p.run.len) {
+        const float* from = a.starts + ((int64_t)num * NP + 4 * ln) * a.D + row;
+        v = make_float4(from[0], from[a.D], from[2 * (int64_t)a.D], from[3 * (int64_t)a.D]);
+      } else if (a.dhT) v = load_states(a.dhT + ((int64_t)p.run.seq * a.D + row) * a.N, 4 * ln, a.N);
     }
     unpack(v, q[s]);
 #pragma unroll
@@ -230,161 +260,190 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanArgs a) {
   }
   const int64_t tile0 = first_run(a.seqs, p.run.seq, kTile) + p.t0 / kTile;
   float sum_D = 0.0f, sum_bias = 0.0f;
+  const bool busy = wave * M::WC < p.nc;   // a wave without channels adds nothing
+  if (!busy)
+    for (int e = lane; e < kTile * 2 * NP; e += kWave) (&lds.sum[wave][0][0][0])[e] = 0.0f;
 
-  for (int tt = p.n > 0 ? (p.n - 1) / kTile * kTile : -1; tt >= 0; tt -= kTile) {
-    const int nt = min(kTile, p.n - tt);
-    float x[EPT], dt[EPT], dy[EPT], slope[EPT], dgate[EPT];   // slope: of the step by its input
-    {
-      S rx[EPT], rg[EPT], rz[EPT], rB[BPT], rC[BPT];
-      uint32_t rdt[EPT];
+  // What a tile reads, a tile ahead.  Tokens behind the run's last are loaded as
+  // the last and count for nothing.
+  S rx[EPT], rg[EPT], rz[EPT], rB[BPT], rC[BPT];
+  SD rdt[EPT];
+  float rh[CS][4];
+  auto load_tile = [&](int tt) {
+    const int most = min(p.n - 1 - tt, kTile - 1);
+    const S *x0 = xp + tt * a.x_st, *g0 = gp + tt * a.do_st, *z0 = zp + tt * a.z_st;
+    const SD* t0 = tp + tt * a.dt_st;
+    const S *B0 = Bp + tt * a.B_st, *C0 = Cp + tt * a.C_st;
+    // within a tile 32 bits hold any offset
+    const uint32_t xs = (uint32_t)a.x_st, gs = (uint32_t)a.do_st, zs = (uint32_t)a.z_st, ts = (uint32_t)a.dt_st;
 #pragma unroll
-      for (int i = 0; i < EPT; ++i) {
-        const int tl = tq + i * M::TPP;
-        rx[i] = rg[i] = rz[i] = S(0);
-        rdt[i] = 0;
-        if (live && tl < nt) {
-          rx[i] = xp[(int64_t)(tt + tl) * a.x_st];
-          rg[i] = gp[(int64_t)(tt + tl) * a.do_st];
-          rdt[i] = load_bits(a.dt, a.dt_dtype, dt_at + (int64_t)(tt + tl) * a.dt_st);
-          if (a.z) rz[i] = zp[(int64_t)(tt + tl) * a.z_st];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < BPT; ++i) {
-        const int e = tid + i * kScanThreads, tl = e / NP, n = e % NP;
-        rB[i] = rC[i] = S(0);
-        if (e < kTile * NP && tl < nt && n < a.N) {
-          rB[i] = Bp[(int64_t)(tt + tl) * a.B_st + n];
-          rC[i] = Cp[(int64_t)(tt + tl) * a.C_st + n];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < EPT; ++i) {
-        const int tl = tq + i * M::TPP;
-        x[i] = TT::load(rx[i]);
-        const float raw = widen(rdt[i], a.dt_dtype) + bias, g = TT::load(rg[i]);
-        dt[i] = tl < nt ? a.soft ? softplus(raw) : raw : 0.0f;
-        slope[i] = a.soft ? sigmoid(raw) : 1.0f;
-        dy[i] = g;
-        dgate[i] = 0.0f;
-        if (a.z) {
-          const float z = TT::load(rz[i]), s = sigmoid(z);
-          dy[i] = g * (z * s);
-          dgate[i] = g * s * __builtin_fmaf(z, 1.0f - s, 1.0f);
-        }
-        lds.dt[tl][c] = dt[i];
-        lds.u[tl][c] = dt[i] * x[i];
-        lds.dy[tl][c] = dy[i];
-      }
-#pragma unroll
-      for (int i = 0; i < BPT; ++i) {
-        const int e = tid + i * kScanThreads;
-        if (e < kTile * NP) {
-          reinterpret_cast<float*>(lds.B)[e] = TT::load(rB[i]);
-          reinterpret_cast<float*>(lds.C)[e] = TT::load(rC[i]);
-        }
-      }
+    for (int i = 0; i < EPT; ++i) {
+      const uint32_t t = (uint32_t)min(tq + i * M::TPP, most);
+      rx[i] = x0[t * xs + cl];
+      rg[i] = g0[t * gs + cl];
+      rdt[i] = t0[t * ts + cl];
+      if (GATE) rz[i] = z0[t * zs + cl];
     }
-    __syncthreads();
-    float h0[CS][4], h[kTile][CS][4];
+#pragma unroll
+    for (int i = 0; i < BPT; ++i) {
+      const int e = tid + i * kScanThreads;
+      const uint32_t t = (uint32_t)min(e / NP, most), n = (uint32_t)min(e % NP, a.N - 1);
+      rB[i] = B0[t * (uint32_t)a.B_st + n];
+      rC[i] = C0[t * (uint32_t)a.C_st + n];
+    }
 #pragma unroll
     for (int s = 0; s < CS; ++s)
-      unpack(ch + s < p.nc ? load_states(a.hs + ((tile0 + tt / kTile) * a.D + p.d0 + ch + s) * a.N, 4 * ln, a.N)
-                           : make_float4(0, 0, 0, 0),
-             h0[s]);
 #pragma unroll
-    for (int t = 0; t < kTile; ++t) {
-      float b[4];
-      unpack(lds.B[t][ln], b);
+      for (int j = 0; j < 4; ++j)
+        rh[s][j] = (a.hs + (tile0 + tt / kTile) * NP * a.D + p.d0)[(uint32_t)((4 * ln + j) * a.D + min(ch + s, p.nc - 1))];
+  };
+
+  // One token forward.
+  auto forward = [&](int t, const float (&from)[CS][4], float (&to)[CS][4]) {
+    float b[4];
+    unpack(lds.B[t][ln], b);
+#pragma unroll
+    for (int s = 0; s < CS; ++s) {
+      const float dts = lds.dt[t][ch + s], u = lds.u[t][ch + s];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) to[s][j] = __builtin_fmaf(exp2_hw(dts * A2[s][j]), from[s][j], u * b[j]);
+    }
+  };
+  // What a token's backward step reads, a token ahead.
+  struct Token {
+    float b[4], c[4], dt[CS], u[CS], dy[CS];
+  };
+  auto read = [&](int t, Token& k) {
+    unpack(lds.B[t][ln], k.b);
+    unpack(lds.C[t][ln], k.c);
+#pragma unroll
+    for (int s = 0; s < CS; ++s) {
+      k.dt[s] = lds.dt[t][ch + s];
+      k.u[s] = lds.u[t][ch + s];
+      k.dy[s] = lds.dy[t][ch + s];
+    }
+  };
+  // One token backward, from the states before and behind it.
+  auto backward = [&](int t, const Token& k, const float (&before)[CS][4], const float (&h)[CS][4]) {
+    float db[4] = {}, dc[4] = {}, y[CS] = {}, du[CS] = {}, aw[CS] = {};
+#pragma unroll
+    for (int s = 0; s < CS; ++s) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float qj = __builtin_fmaf(k.c[j], k.dy[s], q[s][j]);
+        if (GATE) y[s] = __builtin_fmaf(k.c[j], h[s][j], y[s]);
+        dc[j] = __builtin_fmaf(k.dy[s], h[s][j], dc[j]);
+        db[j] = __builtin_fmaf(qj, k.u[s], db[j]);
+        du[s] = __builtin_fmaf(qj, k.b[j], du[s]);
+        q[s][j] = exp2_hw(k.dt[s] * A2[s][j]) * qj;
+        const float w = q[s][j] * before[s][j];
+        aw[s] = __builtin_fmaf(A2[s][j], w, aw[s]);
+        dA[s][j] = __builtin_fmaf(k.dt[s], w, dA[s][j]);
+      }
+      if (GATE) y[s] = sum_lanes<LN>(y[s]);
+      du[s] = sum_lanes<LN>(du[s]);
+      aw[s] = sum_lanes<LN>(aw[s]) * kLn2;
+    }
+    // over the wave's channels: rows of 16 lanes end with dB 0 1, dB 2 3, dC 0 1, dC 2 3
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = halves_add(db[j], dc[j]);
+    const float v0 = sum_apart<LN>(rows_add(v[0], v[2])), v1 = sum_apart<LN>(rows_add(v[1], v[3]));
+    if (ln == 0)
 #pragma unroll
       for (int s = 0; s < CS; ++s) {
-        const float dts = lds.dt[t][ch + s], u = lds.u[t][ch + s];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          h[t][s][j] = __builtin_fmaf(exp2_hw(dts * A2[s][j]), t ? h[t - 1][s][j] : h0[s][j], u * b[j]);
+        lds.u[t][ch + s] = du[s];
+        lds.aw[t][ch + s] = aw[s];
+        if (GATE) lds.y[t][ch + s] = y[s];
       }
+    if ((lane & 15) < LN)
+      *reinterpret_cast<float2*>(&lds.sum[wave][t][lane >> 5][4 * ln + (lane >> 3 & 2)]) = make_float2(v0, v1);
+  };
+
+  if (p.n > 0) load_tile((p.n - 1) / kTile * kTile);
+  for (int tt = p.n > 0 ? (p.n - 1) / kTile * kTile : -1; tt >= 0; tt -= kTile) {
+    const int nt = min(kTile, p.n - tt);
+    S x[EPT];
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      const int tl = tq + i * M::TPP;
+      const bool in = tl < nt && live;
+      x[i] = rx[i];
+      const float raw = DT::load(rdt[i]) + bias, g = TT::load(rg[i]);
+      float slope, dy = g;
+      const float grown = softplus(raw, slope), dt = soft ? grown : raw;
+      if (GATE) {
+        const float z = TT::load(rz[i]), s = sigmoid(z);
+        dy = g * (z * s);
+        lds.dgate[tl][c] = g * s * __builtin_fmaf(z, 1.0f - s, 1.0f);
+      }
+      lds.slope[tl][c] = soft ? slope : 1.0f;
+      lds.dt[tl][c] = in ? dt : 0.0f;
+      lds.u[tl][c] = in ? dt * TT::load(x[i]) : 0.0f;
+      lds.dy[tl][c] = in ? dy : 0.0f;
     }
 #pragma unroll
-    for (int t = kTile - 1; t >= 0; --t) {
-      float b[4], cc[4], db[4] = {}, dc[4] = {};
-      if (t < nt) {   // behind the run's end there is nothing
-        unpack(lds.B[t][ln], b);
-        unpack(lds.C[t][ln], cc);
-#pragma unroll
-        for (int s = 0; s < CS; ++s) {
-          const float dts = lds.dt[t][ch + s], u = lds.u[t][ch + s], g = lds.dy[t][ch + s];
-          float y = 0.0f, du = 0.0f, aw = 0.0f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float qj = __builtin_fmaf(cc[j], g, q[s][j]);
-            y = __builtin_fmaf(cc[j], h[t][s][j], y);
-            dc[j] = __builtin_fmaf(g, h[t][s][j], dc[j]);
-            db[j] = __builtin_fmaf(qj, u, db[j]);
-            du = __builtin_fmaf(qj, b[j], du);
-            q[s][j] = exp2_hw(dts * A2[s][j]) * qj;
-            const float w = q[s][j] * (t ? h[t - 1][s][j] : h0[s][j]);
-            aw = __builtin_fmaf(A2[s][j], w, aw);
-            dA[s][j] = __builtin_fmaf(dts, w, dA[s][j]);
-          }
-          y = sum_lanes<LN>(y);
-          du = sum_lanes<LN>(du);
-          aw = sum_lanes<LN>(aw);
-          if (ln == 0) {
-            lds.u[t][ch + s] = du;
-            lds.dt[t][ch + s] = aw * kLn2;
-            lds.dy[t][ch + s] = y;
-          }
-        }
+    for (int i = 0; i < BPT; ++i) {
+      const int e = tid + i * kScanThreads;
+      if (e < kTile * NP) {
+        const bool in = e / NP < nt && e % NP < a.N;
+        reinterpret_cast<float*>(lds.B)[e] = in ? TT::load(rB[i]) : 0.0f;
+        reinterpret_cast<float*>(lds.C)[e] = in ? TT::load(rC[i]) : 0.0f;
       }
-      lds.red[wave][t % L::kGroup * 2][lane] = make_float4(db[0], db[1], db[2], db[3]);
-      lds.red[wave][t % L::kGroup * 2 + 1][lane] = make_float4(dc[0], dc[1], dc[2], dc[3]);
-      if (t % L::kGroup == 0) {   // the wave's lanes of equal states added, 8 values a lane
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        constexpr int OUT = 2 * L::kGroup * LN;            // float4 sums
-        constexpr int PER = OUT > 64 ? 1 : 64 / OUT;       // lanes that share one
-        constexpr int EACH = 64 / LN / PER;                // values that a lane adds
+    }
+    float h0[CS][4], h8[CS][4];
 #pragma unroll
-        for (int o0 = 0; o0 < OUT; o0 += 64) {
-          const int o = o0 + lane % (OUT < 64 ? OUT : 64), part = OUT < 64 ? lane / OUT : 0;
-          const int row = o / LN, l = o % LN;
-          float v[4] = {};
+    for (int s = 0; s < CS; ++s)
 #pragma unroll
-          for (int i = 0; i < EACH; ++i) {
-            const float4 r = lds.red[wave][row][(part * EACH + i) * LN + l];
-            v[0] += r.x; v[1] += r.y; v[2] += r.z; v[3] += r.w;
-          }
+      for (int j = 0; j < 4; ++j) h0[s][j] = ch + s < p.nc ? rh[s][j] : 0.0f;
+    __syncthreads();
+    if (tt > 0) load_tile(tt - kTile);
+    // the tile's second half from the state in its middle, then the first: the
+    // states of half a tile stay in registers
+    if (busy) {
 #pragma unroll
-          for (int d = OUT; d < 64; d <<= 1)
+    for (int s = 0; s < CS; ++s)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] += __shfl_xor(v[j], d);
-          if (part == 0) lds.sum[wave][t + row / 2][row % 2][l] = make_float4(v[0], v[1], v[2], v[3]);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      for (int j = 0; j < 4; ++j) h8[s][j] = h0[s][j];
+#pragma unroll
+    for (int t = 0; t < kTile / 2; ++t) forward(t, h8, h8);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int half = 1; half >= 0; --half) {
+      const int t0 = half * (kTile / 2);
+      float h[kTile / 2][CS][4];
+#pragma unroll
+      for (int t = 0; t < kTile / 2; ++t) forward(t0 + t, t ? h[t ? t - 1 : 0] : half ? h8 : h0, h[t]);
+      Token now, next;
+      read(t0 + kTile / 2 - 1, now);
+#pragma unroll
+      for (int t = kTile / 2 - 1; t >= 0; --t) {
+        if (t) read(t0 + t - 1, next);
+        if (t0 + t < nt) backward(t0 + t, now, t ? h[t ? t - 1 : 0] : half ? h8 : h0, h[t]);
+        now = next;
+        __builtin_amdgcn_sched_barrier(0);   // as in the forward
       }
+    }
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
       const int tl = tq + i * M::TPP;
       if (!live || tl >= nt) continue;
-      const int64_t e = out0 + (int64_t)(tt + tl) * a.D;
-      const float du = lds.u[tl][c];
-      const float ddt = __builtin_fmaf(du, x[i], lds.dt[tl][c]) * slope[i];
-      static_cast<S*>(a.dx)[e] = TT::store(__builtin_fmaf(du, dt[i], skip * dy[i]));
-      store_any(a.ddt, a.dt_dtype, e, ddt);
-      if (a.z) static_cast<S*>(a.dz)[e] = TT::store(dgate[i] * __builtin_fmaf(skip, x[i], lds.dy[tl][c]));
-      sum_D = __builtin_fmaf(dy[i], x[i], sum_D);
+      const int64_t e = out0 + (int64_t)(tt + tl) * a.D + c;
+      const float du = lds.u[tl][c], dy = lds.dy[tl][c], xf = TT::load(x[i]);
+      const float ddt = __builtin_fmaf(du, xf, lds.aw[tl][c]) * lds.slope[tl][c];
+      static_cast<S*>(a.dx)[e] = TT::store(__builtin_fmaf(du, lds.dt[tl][c], skip * dy));
+      static_cast<SD*>(a.ddt)[e] = DT::store(ddt);
+      if (GATE) static_cast<S*>(a.dz)[e] = TT::store(lds.dgate[tl][c] * __builtin_fmaf(skip, xf, lds.y[tl][c]));
+      sum_D = __builtin_fmaf(dy, xf, sum_D);
       sum_bias += ddt;
     }
     const int64_t row0 = ((int64_t)(p.d0 - p.g * a.Dg) / CB * a.seqs.B + p.run.b) * a.seqs.T + tok + tt;
     for (int e = tid; e < nt * 2 * NP; e += kScanThreads) {
       const int tl = e / (2 * NP), k = e / NP % 2, n = e % NP;
       if (n >= a.N) continue;
-      const float* s = reinterpret_cast<const float*>(lds.sum) + e;
+      const float* s = &lds.sum[0][0][0][0] + e;
       constexpr int W = kTile * 2 * NP;
       a.part_bc[(((row0 + tl) * 2 + k) * a.G + p.g) * a.N + n] = (s[0] + s[W]) + (s[2 * W] + s[3 * W]);
     }
@@ -452,31 +511,39 @@ __global__ __launch_bounds__(256) void sums_kernel(const float* __restrict__ par
   }
 }
 
-template <class TT, int LN>
-int launch_bwd_as(const ScanArgs& a, hipStream_t st) {
+template <class TT, class DT, int LN, bool GATE>
+int launch_bwd_gated(const ScanArgs& a, hipStream_t st) {
   const unsigned per = (unsigned)(a.G * a.ncb), blocks = (unsigned)a.nruns * per;
   if (a.ends) {
-    hipLaunchKernelGGL((scan_adjoint_kernel<TT, LN>), dim3(blocks), dim3(kScanThreads), 0, st, a);
-    const int64_t states = (int64_t)a.seqs.nseq * a.D * a.N;
+    ScanArgs b = a;
+    b.ncb = (a.Dg + kScanThreads - 1) / kScanThreads;
+    hipLaunchKernelGGL((scan_adjoint_kernel<TT, DT, 4 * LN, GATE>), dim3((unsigned)a.nruns * (unsigned)(a.G * b.ncb)),
+                       dim3(kScanThreads), 0, st, b);
+    const int64_t states = (int64_t)a.seqs.nseq * a.D * kept_states(a.N);
     hipLaunchKernelGGL(scan_join_back_kernel, dim3((unsigned)((states + kScanThreads - 1) / kScanThreads)),
-                       dim3(kScanThreads), 0, st, a, a.ends, a.decay, a.starts);
+                       dim3(kScanThreads), 0, st, a, 4 * LN, a.ends, a.decay, a.starts);
   }
-  hipLaunchKernelGGL((scan_bwd_kernel<TT, LN>), dim3(blocks + (a.seqs.cu ? per : 0)), dim3(kScanThreads), 0, st, a);
+  hipLaunchKernelGGL((scan_bwd_kernel<TT, DT, LN, GATE>), dim3(blocks + (a.seqs.cu ? kLooseRuns * per : 0)),
+                     dim3(kScanThreads), 0, st, a);
   return check_launch("selective_scan_bwd");
 }
+template <class TT, class DT, int LN>
+int launch_bwd_as(const ScanArgs& a, hipStream_t st) {
+  return a.z ? launch_bwd_gated<TT, DT, LN, true>(a, st) : launch_bwd_gated<TT, DT, LN, false>(a, st);
+}
 
-template <class TT>
+template <class TT, class DT>
 int launch_bwd(const ScanArgs& a, hipStream_t st) {
   switch (scan_lanes(a.N)) {
-    case 1: return launch_bwd_as<TT, 1>(a, st);
-    case 2: return launch_bwd_as<TT, 2>(a, st);
-    case 4: return launch_bwd_as<TT, 4>(a, st);
-    case 8: return launch_bwd_as<TT, 8>(a, st);
-    default: return launch_bwd_as<TT, 16>(a, st);
+    case 1: return launch_bwd_as<TT, DT, 1>(a, st);
+    case 2: return launch_bwd_as<TT, DT, 2>(a, st);
+    case 4: return launch_bwd_as<TT, DT, 4>(a, st);
+    case 8: return launch_bwd_as<TT, DT, 8>(a, st);
+    default: return launch_bwd_as<TT, DT, 16>(a, st);
   }
 }
 
-constexpr int kBwdBlocks = 512;   // workgroups that are wanted at once
+constexpr int kBwdBlocks = 3072;   // workgroups that are wanted at once
 
 // Floats of the workspace's parts.
 struct Parts {
@@ -486,7 +553,7 @@ struct Parts {
 Parts bwd_parts(const ScanArgs& a) {
   const size_t states = (size_t)a.nruns * a.D * a.N, chans = (size_t)a.nruns * a.D;
   Parts p{};
-  p.joins = a.R >= a.seqs.T ? 0 : 2 * states + chans;
+  p.joins = a.R >= a.seqs.T ? 0 : (2 * (size_t)kept_states(a.N) + 1) * chans;
   p.A = states;
   p.D = p.bias = chans;
   p.bc = (size_t)a.ncb * a.seqs.B * a.seqs.T * 2 * a.G * a.N;
@@ -515,7 +582,7 @@ extern "C" size_t uttt_selective_scan_bwd_workspace_bytes(int B, int T, int nseq
   a.seqs = Seqs{packed ? &a : nullptr, 0, B, T, nseq};
   a.D = D; a.N = N; a.G = G;
   if (!seqs_ok(a.seqs) || D < 1 || G < 1 || D % G || N < 1 || N > kMaxStates) return 0;
-  scan_runs(a, kBwdBlocks);
+  scan_runs(a, scan_width(N), kBwdBlocks);
   return bwd_parts(a).bytes();
 }
 
@@ -539,7 +606,6 @@ extern "C" int uttt_selective_scan_bwd(const void* x, const int64_t* x_strides, 
   a.hs = const_cast<float*>(tile_states);
   a.dout = dout; a.dhT = dfinal_state;
   a.dx = dx; a.ddt = ddt; a.dz = dgate; a.dh0 = dinitial_state;
-  if (const int rc = scan_check(a, dtype, what)) return rc;
   UTTT_REQUIRE(x_strides && dt_strides && B_strides && C_strides && dout_strides && (gate_strides || !gate),
                "%s: null strides", what);
   UTTT_REQUIRE(dA && (T == 0 || (tile_states && dout && dx && ddt && dB && dC && (dgate || !gate))),
@@ -550,7 +616,8 @@ extern "C" int uttt_selective_scan_bwd(const void* x, const int64_t* x_strides, 
   a.C_sb = C_strides[0]; a.C_st = C_strides[1]; a.C_sg = C_strides[2];
   a.do_sb = dout_strides[0]; a.do_st = dout_strides[1];
   if (gate) { a.z_sb = gate_strides[0]; a.z_st = gate_strides[1]; }
-  scan_runs(a, kBwdBlocks);
+  if (const int rc = scan_check(a, dtype, what)) return rc;
+  scan_runs(a, scan_width(N), kBwdBlocks);
   UTTT_REQUIRE(scan_fits(a), "%s: too many sequences, channels or states", what);
   const Parts parts = bwd_parts(a);
   UTTT_REQUIRE(workspace && workspace_bytes >= parts.bytes() && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0,
@@ -558,8 +625,8 @@ extern "C" int uttt_selective_scan_bwd(const void* x, const int64_t* x_strides, 
   float* w = static_cast<float*>(workspace);
   if (parts.joins) {
     a.ends = w;
-    a.starts = a.ends + (size_t)a.nruns * D * N;
-    a.decay = a.starts + (size_t)a.nruns * D * N;
+    a.starts = a.ends + (size_t)a.nruns * D * kept_states(N);
+    a.decay = a.starts + (size_t)a.nruns * D * kept_states(N);
   }
   a.part_A = w += parts.joins;
   w += parts.A;
@@ -570,9 +637,9 @@ extern "C" int uttt_selective_scan_bwd(const void* x, const int64_t* x_strides, 
   const hipStream_t st = as_stream(stream);
   int rc = UTTT_OK;
   switch (dtype) {
-    case UTTT_F32: rc = launch_bwd<F32T>(a, st); break;
-    case UTTT_BF16: rc = launch_bwd<BF16T>(a, st); break;
-    default: rc = launch_bwd<F16T>(a, st); break;
+    case UTTT_F32: rc = launch_bwd<F32T, F32T>(a, st); break;
+    case UTTT_BF16: rc = dt_dtype == UTTT_F32 ? launch_bwd<BF16T, F32T>(a, st) : launch_bwd<BF16T, BF16T>(a, st); break;
+    default: rc = dt_dtype == UTTT_F32 ? launch_bwd<F16T, F32T>(a, st) : launch_bwd<F16T, F16T>(a, st); break;
   }
   if (rc) return rc;
   const int64_t rows = (int64_t)B * T;

@@ -11,232 +11,237 @@ namespace uttt {
 namespace ssm {
 namespace {
 
-template <class TT, int LN, bool LOCAL>
-__global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanArgs a) {
+template <class TT, class DT, int NP, bool LOCAL, bool GATE>
+__global__ __launch_bounds__(kScanThreads, fwd_waves(NP)) void scan_fwd_kernel(ScanArgs a) {
   using S = typename TT::S;
-  using M = Geo<LN>;
-  constexpr int CS = M::CS, CB = M::CB, NP = M::NP, EPT = M::EPT, BPT = M::BPT;
-  __shared__ float sU[kTile][CB], sDt[kTile][CB], sY[LOCAL ? 1 : kTile][CB];
-  __shared__ float4 sB[kTile][LN], sC[LOCAL ? 1 : kTile][LN];
+  using SD = typename DT::S;
+  __shared__ float4 sB[2][kTile][NP / 4], sC[2][LOCAL ? 1 : kTile][NP / 4];
   const int tid = threadIdx.x;
-  const int c = tid % CB, tq = tid / CB;   // the element column that this thread loads and stores
   Place p;
-  if (!p.init(a, CB)) {
-    // the workgroups past the last run: zeros for the tokens of no sequence
-    if (!LOCAL && a.seqs.cu && (int)(blockIdx.x / (a.G * a.ncb)) >= a.nruns && c < p.nc)
-      for (int i = tq;; i += M::TPP) {
-        const int t = loose_token(a.seqs, i);
-        if (t < 0) break;
-        static_cast<S*>(a.out)[(int64_t)t * a.D + p.d0 + c] = TT::store(0.0f);
-      }
+  if (!p.init(a, kScanThreads)) {
+    if (!LOCAL && a.seqs.cu) {   // the workgroups past the last run: zeros for the tokens of no sequence
+      const int first = (int)(blockIdx.x / (a.G * a.ncb)) - a.nruns;
+      if (first >= 0 && tid < p.nc)
+        for (int i = first;; i += kLooseRuns) {
+          const int t = loose_token(a.seqs, i);
+          if (t < 0) break;
+          static_cast<S*>(a.out)[(int64_t)t * a.D + p.d0 + tid] = TT::store(0.0f);
+        }
+    }
     return;
   }
   if (LOCAL && p.t0 + p.n >= p.run.len) return;   // nothing follows it
   const int at = p.run.base + p.run.c;
   const int64_t tok = p.run.tok0 + p.t0;
-  const bool live = c < p.nc;
-  const S* xp = static_cast<const S*>(a.x) + p.run.b * a.x_sb + tok * a.x_st + p.d0 + c;
-  const S* zp = static_cast<const S*>(a.z) + p.run.b * a.z_sb + tok * a.z_st + p.d0 + c;
-  const int64_t dt_at = p.run.b * a.dt_sb + tok * a.dt_st + p.d0 + c;
+  // a lane without a channel does the last one's work again, a wave without any none
+  const bool busy = (tid & ~(kWave - 1)) < p.nc;
+  const uint32_t c = min(tid, p.nc - 1), d = p.d0 + c;
+  const S* xp = static_cast<const S*>(a.x) + p.run.b * a.x_sb + tok * a.x_st + p.d0;
+  const S* zp = static_cast<const S*>(a.z) + p.run.b * a.z_sb + tok * a.z_st + p.d0;
+  const SD* tp = static_cast<const SD*>(a.dt) + p.run.b * a.dt_sb + tok * a.dt_st + p.d0;
   const S* Bp = static_cast<const S*>(a.Bm) + p.run.b * a.B_sb + tok * a.B_st + p.g * a.B_sg;
   const S* Cp = static_cast<const S*>(a.Cm) + p.run.b * a.C_sb + tok * a.C_st + p.g * a.C_sg;
-  const float bias = live && a.bias ? a.bias[p.d0 + c] : 0.0f;
-  const float skip = !LOCAL && live && a.Dskip ? a.Dskip[p.d0 + c] : 0.0f;
-  const bool gate = !LOCAL && a.z != nullptr;
+  S* yp = static_cast<S*>(a.out) + ((int64_t)p.run.b * a.seqs.T + tok) * a.D + p.d0;
+  const float bias = a.bias ? a.bias[d] : 0.0f;
+  const float skip = !LOCAL && a.Dskip ? a.Dskip[d] : 0.0f;
+  const bool soft = a.soft;
 
-  const int wave = tid >> 6, lane = tid & 63, ln = lane % LN;
-  const int ch = wave * M::WC + lane / LN * CS;   // first channel of this lane
-  float h[CS][4], A2[CS][4];
+  float h[NP], A2[NP];
+  load_row<NP>(a.A + (int64_t)d * a.N, a.N, A2);
 #pragma unroll
-  for (int s = 0; s < CS; ++s) {
-    const bool on = ch + s < p.nc;
-    const int64_t row = p.d0 + ch + s;
-    unpack(on ? load_states(a.A + row * a.N, 4 * ln, a.N) : make_float4(0, 0, 0, 0), A2[s]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) A2[s][j] = log2_rate(A2[s][j]);
-    float4 v = make_float4(0, 0, 0, 0);
-    if (!LOCAL && on) {
-      if (p.run.c > 0) v = load_states(a.starts + ((int64_t)at * a.D + row) * a.N, 4 * ln, a.N);
-      else if (a.h0) v = load_states(a.h0 + ((int64_t)p.run.seq * a.D + row) * a.N, 4 * ln, a.N);
-    }
-    unpack(v, h[s]);
+  for (int j = 0; j < NP; ++j) {
+    A2[j] = log2_rate(A2[j]);
+    h[j] = 0.0f;
   }
-
-  S rx[EPT], rz[EPT], rB[BPT], rC[BPT];
-  uint32_t rdt[EPT];
-  auto load_tile = [&](int tt) {
+  if (!LOCAL) {
+    if (p.run.c > 0) load_kept<NP>(a.starts + (int64_t)at * NP * a.D, a.D, d, h);
+    else if (a.h0) load_row<NP>(a.h0 + ((int64_t)p.run.seq * a.D + d) * a.N, a.N, h);
+  }
+  float sum_dt = 0.0f;
+  // one token with B and C at q
+  auto token = [&](const float4* qB, const float4* qC, S* y0, S xbits, SD dtbits, S zbits) {
+    const float x = TT::load(xbits);
+    const float raw = DT::load(dtbits) + bias, grown = softplus(raw), dt = soft ? grown : raw;
+    const float u = dt * x;
+    if (LOCAL) sum_dt += dt;
+    float y[4] = {};
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      const int t = tt + tq + i * M::TPP;
-      rx[i] = rz[i] = S(0);
-      rdt[i] = 0;
-      if (live && t < p.n) {
-        rx[i] = xp[(int64_t)t * a.x_st];
-        rdt[i] = load_bits(a.dt, a.dt_dtype, dt_at + (int64_t)t * a.dt_st);
-        if (gate) rz[i] = zp[(int64_t)t * a.z_st];
+    for (int q = 0; q < NP / 4; ++q) {
+      float b[4], cc[4];
+      unpack(qB[q], b);
+      if (!LOCAL) unpack(qC[q], cc);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float& hj = h[4 * q + j];
+        hj = __builtin_fmaf(exp2_hw(dt * A2[4 * q + j]), hj, u * b[j]);
+        if (!LOCAL) y[j] = __builtin_fmaf(cc[j], hj, y[j]);
       }
     }
+    if (LOCAL) return;
+    float v = __builtin_fmaf(skip, x, (y[0] + y[1]) + (y[2] + y[3]));
+    if (GATE) {
+      const float z = TT::load(zbits);
+      v *= z * sigmoid(z);
+    }
+    y0[c] = TT::store(v);
+  };
+
+  constexpr int U = 4;   // tokens whose x, dt and z are loaded ahead
+  S rx[U], rz[U];
+  SD rdt[U];
+  auto load = [&]() {    // the next U tokens'
 #pragma unroll
-    for (int i = 0; i < BPT; ++i) {
-      const int e = tid + i * kScanThreads, t = tt + e / NP, n = e % NP;
-      rB[i] = rC[i] = S(0);
-      if (e < kTile * NP && t < p.n && n < a.N) {
-        rB[i] = Bp[(int64_t)t * a.B_st + n];
-        if (!LOCAL) rC[i] = Cp[(int64_t)t * a.C_st + n];
+    for (int i = 0; i < U; ++i) {
+      rx[i] = xp[c];
+      xp += a.x_st;
+      rdt[i] = tp[c];
+      tp += a.dt_st;
+      if (GATE) {
+        rz[i] = zp[c];
+        zp += a.z_st;
       }
     }
   };
-  float sum_dt = 0.0f;
-  load_tile(0);
-  const int64_t tile0 = a.hs ? first_run(a.seqs, p.run.seq, kTile) + p.t0 / kTile : 0;
-  for (int tt = 0; tt < p.n; tt += kTile) {
-    float x[EPT], z[EPT];
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      const int tl = tq + i * M::TPP;
-      float dt = 0.0f;
-      x[i] = TT::load(rx[i]);
-      z[i] = TT::load(rz[i]);
-      if (tt + tl < p.n) {
-        dt = widen(rdt[i], a.dt_dtype) + bias;
-        if (a.soft) dt = softplus(dt);
-      }
-      sum_dt += dt;
-      sDt[tl][c] = dt;
-      sU[tl][c] = dt * x[i];
-    }
-#pragma unroll
-    for (int i = 0; i < BPT; ++i) {
-      const int e = tid + i * kScanThreads;
-      if (e < kTile * NP) {
-        reinterpret_cast<float*>(sB)[e] = TT::load(rB[i]);
-        if (!LOCAL) reinterpret_cast<float*>(sC)[e] = TT::load(rC[i]);
-      }
-    }
-    __syncthreads();
-    if (tt + kTile < p.n) load_tile(tt + kTile);
-    if (!LOCAL && a.hs) {
-#pragma unroll
-      for (int s = 0; s < CS; ++s)
-        if (ch + s < p.nc)
-          store_states(a.hs + ((tile0 + tt / kTile) * a.D + p.d0 + ch + s) * a.N, 4 * ln, a.N,
-                       make_float4(h[s][0], h[s][1], h[s][2], h[s][3]));
-    }
-#pragma unroll
-    for (int t = 0; t < kTile; ++t) {
-      float b[4], cc[4];
-      unpack(sB[t][ln], b);
-      if (!LOCAL) unpack(sC[t][ln], cc);
-#pragma unroll
-      for (int s = 0; s < CS; ++s) {
-        const float dt = sDt[t][ch + s], u = sU[t][ch + s];
-        float y = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          h[s][j] = __builtin_fmaf(exp2_hw(dt * A2[s][j]), h[s][j], u * b[j]);
-          if (!LOCAL) y = __builtin_fmaf(cc[j], h[s][j], y);
-        }
-        if (!LOCAL) {
-          y = sum_lanes<LN>(y);
-          if (ln == 0) sY[t][ch + s] = y;
-        }
-      }
-    }
-    __syncthreads();
-    if (LOCAL) continue;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      const int tl = tq + i * M::TPP;
-      if (!live || tt + tl >= p.n) continue;
-      float y = __builtin_fmaf(skip, x[i], sY[tl][c]);
-      if (gate) y *= z[i] * sigmoid(z[i]);
-      static_cast<S*>(a.out)[((int64_t)p.run.b * a.seqs.T + tok + tt + tl) * a.D + p.d0 + c] = TT::store(y);
-    }
+  float* keep = a.hs ? a.hs + ((int64_t)first_run(a.seqs, p.run.seq, kTile) + p.t0 / kTile) * NP * a.D : nullptr;
+  const int whole = p.n / U * U;
+  Rows16<TT, NP> rB, rC;
+  if (p.n > 0) {
+    rB.load(Bp, (uint32_t)a.B_st, min(p.n, kTile), a.N);
+    if (!LOCAL) rC.load(Cp, (uint32_t)a.C_st, min(p.n, kTile), a.N);
+    if (busy && whole) load();
+    rB.write(sB[0][0], p.n, a.N);
+    if (!LOCAL) rC.write(sC[0][0], p.n, a.N);
   }
-  float* to = LOCAL ? a.ends + (int64_t)at * a.D * a.N
-              : a.hT && p.t0 + p.n >= p.run.len ? a.hT + (int64_t)p.run.seq * a.D * a.N : nullptr;
-  if (to)
-#pragma unroll
-    for (int s = 0; s < CS; ++s)
-      if (ch + s < p.nc)
-        store_states(to + (int64_t)(p.d0 + ch + s) * a.N, 4 * ln, a.N,
-                     make_float4(h[s][0], h[s][1], h[s][2], h[s][3]));
-  if (LOCAL) {
-    float* red = &sU[0][0];   // the last tile is read
-    red[tid] = sum_dt;
-    __syncthreads();
-    if (tq == 0 && live) {
-#pragma unroll
-      for (int i = 1; i < M::TPP; ++i) sum_dt += red[c + i * CB];
-      a.decay[(int64_t)at * a.D + p.d0 + c] = sum_dt;
+  __syncthreads();
+  for (int tt = 0; tt < p.n; tt += kTile) {
+    const int buf = tt / kTile & 1, left = p.n - tt - kTile;   // tokens behind the tile
+    if (left > 0) {
+      Bp += kTile * a.B_st;
+      Cp += kTile * a.C_st;
+      rB.load(Bp, (uint32_t)a.B_st, min(left, kTile), a.N);
+      if (!LOCAL) rC.load(Cp, (uint32_t)a.C_st, min(left, kTile), a.N);
     }
+    if (busy) {
+      if (!LOCAL && keep) {
+        store_kept<NP>(keep, a.D, d, h);
+        keep += (int64_t)NP * a.D;
+      }
+      const float4 *qB = sB[buf][0], *qC = sC[LOCAL ? 0 : buf][0];
+      int t = tt;
+#pragma unroll 1
+      for (; t < min(tt + kTile, whole); t += U) {
+        S x[U], z[U];
+        SD dt[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          x[i] = rx[i];
+          dt[i] = rdt[i];
+          z[i] = rz[i];
+        }
+        if (t + 2 * U <= p.n) load();
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          token(qB, qC, yp, x[i], dt[i], z[i]);
+          qB += NP / 4;
+          qC += NP / 4;
+          yp += a.D;
+          // without it decays of many tokens ahead are computed and spilled
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if (left <= 0)   // the last few
+#pragma unroll 1
+        for (; t < p.n; ++t) {
+          token(qB, qC, yp, xp[c], tp[c], GATE ? zp[c] : S(0));
+          xp += a.x_st;
+          tp += a.dt_st;
+          if (GATE) zp += a.z_st;
+          qB += NP / 4;
+          qC += NP / 4;
+          yp += a.D;
+        }
+    }
+    if (left > 0) {
+      rB.write(sB[buf ^ 1][0], left, a.N);
+      if (!LOCAL) rC.write(sC[LOCAL ? 0 : buf ^ 1][0], left, a.N);
+    }
+    __syncthreads();
+  }
+  if (!busy) return;
+  if (LOCAL) {
+    store_kept<NP>(a.ends + (int64_t)at * NP * a.D, a.D, d, h);
+    a.decay[(int64_t)at * a.D + d] = sum_dt;
+  } else if (a.hT && p.t0 + p.n >= p.run.len) {
+    store_row<NP>(a.hT + ((int64_t)p.run.seq * a.D + d) * a.N, a.N, h);
   }
 }
 
 // The states that a sequence's runs start with, from the second on.
-__global__ __launch_bounds__(kScanThreads) void scan_join_kernel(ScanArgs a, const float* __restrict__ ends,
+__global__ __launch_bounds__(kScanThreads) void scan_join_kernel(ScanArgs a, int keep, const float* __restrict__ ends,
                                                                  const float* __restrict__ decay,
                                                                  float* __restrict__ starts) {
-  const int64_t e = (int64_t)blockIdx.x * kScanThreads + threadIdx.x, M = (int64_t)a.D * a.N;
-  if (e >= M * a.seqs.nseq) return;
-  const int seq = (int)(e / M);
-  const int64_t at = e % M, d = at / a.N;
+  const int64_t e = (int64_t)blockIdx.x * kScanThreads + threadIdx.x, K = (int64_t)a.D * keep;   // K: states kept of a run
+  if (e >= K * a.seqs.nseq) return;
+  const int seq = (int)(e / K);
+  const int64_t in = e % K, d = in % a.D, n = in / a.D;
+  const bool real = n < a.N;   // the others stay zero
+  const int64_t own = d * a.N + n, M = (int64_t)a.D * a.N;   // as the caller holds it
   const Run r = span_of(a.seqs, seq, a.R);
   const int runs = (int)(((int64_t)r.len + a.R - 1) / a.R);
-  const float A2 = log2_rate(a.A[at]);
-  float h = a.h0 ? a.h0[e] : 0.0f;
+  const float A2 = real ? log2_rate(a.A[own]) : 0.0f;
+  float h = a.h0 && real ? a.h0[seq * M + own] : 0.0f;
 #pragma unroll 8
   for (int c = 1; c < runs; ++c) {
     const int64_t i = r.base + c - 1;
-    h = __builtin_fmaf(exp2_hw(decay[i * a.D + d] * A2), h, ends[i * M + at]);
-    starts[(i + 1) * M + at] = h;
+    h = __builtin_fmaf(exp2_hw(decay[i * a.D + d] * A2), h, ends[i * K + in]);
+    starts[(i + 1) * K + in] = h;
   }
 }
 
-template <class TT, int LN>
+template <class TT, class DT, int NP>
 int launch_fwd_as(const ScanArgs& a, hipStream_t st) {
   const unsigned per = (unsigned)(a.G * a.ncb), blocks = (unsigned)a.nruns * per;
+  const dim3 threads(kScanThreads), all(blocks + (a.seqs.cu ? kLooseRuns * per : 0));
   if (a.ends) {
-    hipLaunchKernelGGL((scan_fwd_kernel<TT, LN, true>), dim3(blocks), dim3(kScanThreads), 0, st, a);
-    const int64_t states = (int64_t)a.seqs.nseq * a.D * a.N;
+    hipLaunchKernelGGL((scan_fwd_kernel<TT, DT, NP, true, false>), dim3(blocks), threads, 0, st, a);
+    const int64_t states = (int64_t)a.seqs.nseq * a.D * kept_states(a.N);
     hipLaunchKernelGGL(scan_join_kernel, dim3((unsigned)((states + kScanThreads - 1) / kScanThreads)),
-                       dim3(kScanThreads), 0, st, a, a.ends, a.decay, a.starts);
+                       dim3(kScanThreads), 0, st, a, NP, a.ends, a.decay, a.starts);
   }
-  hipLaunchKernelGGL((scan_fwd_kernel<TT, LN, false>), dim3(blocks + (a.seqs.cu ? per : 0)), dim3(kScanThreads), 0,
-                     st, a);
+  if (a.z) hipLaunchKernelGGL((scan_fwd_kernel<TT, DT, NP, false, true>), all, threads, 0, st, a);
+  else hipLaunchKernelGGL((scan_fwd_kernel<TT, DT, NP, false, false>), all, threads, 0, st, a);
   return check_launch("selective_scan");
 }
 
-template <class TT>
+template <class TT, class DT>
 int launch_fwd(const ScanArgs& a, hipStream_t st) {
-  switch (scan_lanes(a.N)) {
-    case 1: return launch_fwd_as<TT, 1>(a, st);
-    case 2: return launch_fwd_as<TT, 2>(a, st);
-    case 4: return launch_fwd_as<TT, 4>(a, st);
-    case 8: return launch_fwd_as<TT, 8>(a, st);
-    default: return launch_fwd_as<TT, 16>(a, st);
-  }
+  if (a.N <= 4) return launch_fwd_as<TT, DT, 4>(a, st);
+  if (a.N <= 8) return launch_fwd_as<TT, DT, 8>(a, st);
+  if (a.N <= 16) return launch_fwd_as<TT, DT, 16>(a, st);
+  if (a.N <= 32) return launch_fwd_as<TT, DT, 32>(a, st);
+  return launch_fwd_as<TT, DT, 64>(a, st);
 }
 
-constexpr int kFwdBlocks = 1024;   // workgroups that are wanted at once
+constexpr int kFwdBlocks = 1536;   // workgroups that are wanted at once
+
+void fwd_runs(ScanArgs& a) { scan_runs(a, kScanThreads, kFwdBlocks); }
 
 }  // namespace
 
-// A sequence that no cut would help is one run.
-void scan_runs(ScanArgs& a, int want) {
+// Runs that a wave of workgroups holds at once: one workgroup more would take
+// as long again (16 x 2048 tokens of 1536 channels: 1056 workgroups where 1024
+// fit 447 us, 960 of them TODO).
+void scan_runs(ScanArgs& a, int width, int want) {
   a.Dg = a.D / a.G;
-  const int cb = scan_width(a.N);
-  a.ncb = (a.Dg + cb - 1) / cb;
-  const int64_t per = (int64_t)a.G * a.ncb, tokens = (int64_t)a.seqs.B * a.seqs.T;
-  const int64_t runs = (want + per - 1) / per;       // wanted over all tokens
-  int64_t R = (tokens + runs - 1) / runs;
-  if (R < 4 * kTile) R = 4 * kTile;
-  if (!a.seqs.cu) {                                  // equal runs
-    const int64_t k = R < a.seqs.T ? (a.seqs.T + R - 1) / R : 1;
-    R = (a.seqs.T + k - 1) / k;
-  }
-  if (R > a.seqs.T) R = a.seqs.T;
-  R = (R + kTile - 1) / kTile * kTile;
+  a.ncb = (a.Dg + width - 1) / width;
+  const int64_t per = (int64_t)a.G * a.ncb, T = a.seqs.T;
+  const int64_t seqs = a.seqs.cu ? 1 : a.seqs.nseq;     // that share the workgroups
+  int64_t runs = want / (per * seqs);                   // of a sequence, of all packed tokens
+  if (a.seqs.cu && runs > a.seqs.nseq + 1) runs -= a.seqs.nseq;   // a sequence has one run more than whole ones
+  const int64_t most = T / (4 * kTile);                 // shorter ones would be mostly beginnings
+  if (runs > most) runs = most;
+  if (runs < 1) runs = 1;
+  const int64_t R = ((T + runs - 1) / runs + kTile - 1) / kTile * kTile;
   a.R = (int)(R < kTile ? kTile : R);
   a.nruns = (int)run_count(a.seqs, a.R);
 }
@@ -246,7 +251,11 @@ int scan_check(const ScanArgs& a, int dtype, const char* what) {
                "%s: bad sizes B=%d T=%d nseq=%d", what, a.seqs.B, a.seqs.T, a.seqs.nseq);
   UTTT_REQUIRE(a.D >= 1 && a.G >= 1 && a.D % a.G == 0, "%s: D=%d must be a multiple of G=%d", what, a.D, a.G);
   UTTT_REQUIRE(a.N >= 1 && a.N <= kMaxStates, "%s: N=%d must be at most %d", what, a.N, kMaxStates);
-  UTTT_REQUIRE(dtype_bytes(dtype) && dtype_bytes(a.dt_dtype), "%s: dtype codes %d, %d", what, dtype, a.dt_dtype);
+  UTTT_REQUIRE(dtype_bytes(dtype) && (a.dt_dtype == UTTT_F32 || a.dt_dtype == dtype), "%s: dtype codes %d, %d", what,
+               dtype, a.dt_dtype);
+  // offsets within a tile are 32 bits
+  for (const int64_t st : {a.x_st, a.dt_st, a.z_st, a.B_st, a.C_st, a.do_st})
+    UTTT_REQUIRE(st >= 0 && st < (1 << 24), "%s: %lld elements between tokens", what, (long long)st);
   const bool empty = a.seqs.T == 0;
   UTTT_REQUIRE(a.A && (empty || (a.x && a.dt && a.Bm && a.Cm)), "%s: null pointer", what);
   const uintptr_t rows = reinterpret_cast<uintptr_t>(a.A) | reinterpret_cast<uintptr_t>(a.h0) |
@@ -257,14 +266,14 @@ int scan_check(const ScanArgs& a, int dtype, const char* what) {
 }
 
 bool scan_fits(const ScanArgs& a) {   // a launch has fewer than 2^32 threads
-  const int64_t runs = run_count(a.seqs, a.R), states = (int64_t)a.seqs.nseq * a.D * a.N;
-  return runs < (1 << 30) && (runs + 1) * a.G * a.ncb < (1LL << 24) && states < (1LL << 31);
+  const int64_t runs = run_count(a.seqs, a.R), states = (int64_t)a.seqs.nseq * a.D * kept_states(a.N);
+  return runs < (1 << 30) && (runs + kLooseRuns) * a.G * a.ncb < (1LL << 24) && states < (1LL << 31);
 }
 
 namespace {
 size_t fwd_bytes(const ScanArgs& a) {
   const bool whole = a.R >= a.seqs.T;
-  return whole ? 0 : (size_t)a.nruns * a.D * (2 * (size_t)a.N + 1) * 4;
+  return whole ? 0 : (size_t)a.nruns * a.D * (2 * (size_t)kept_states(a.N) + 1) * 4;
 }
 }  // namespace
 
@@ -284,7 +293,7 @@ extern "C" size_t uttt_selective_scan_fwd_workspace_bytes(int B, int T, int nseq
   a.seqs = Seqs{packed ? &a : nullptr, 0, B, T, nseq};
   a.D = D; a.N = N; a.G = G;
   if (!seqs_ok(a.seqs) || D < 1 || G < 1 || D % G || N < 1 || N > kMaxStates) return 0;
-  scan_runs(a, kFwdBlocks);
+  fwd_runs(a);
   return fwd_bytes(a);
 }
 
@@ -304,7 +313,6 @@ extern "C" int uttt_selective_scan_fwd(const void* x, const int64_t* x_strides, 
   a.dt_dtype = dt_dtype; a.soft = dt_softplus;
   a.A = A; a.Dskip = skip; a.bias = dt_bias; a.h0 = initial_state;
   a.out = out; a.hT = final_state; a.hs = tile_states;
-  if (const int rc = scan_check(a, dtype, what)) return rc;
   UTTT_REQUIRE(x_strides && dt_strides && B_strides && C_strides && (gate_strides || !gate) && (out || T == 0),
                "%s: null pointer", what);
   a.x_sb = x_strides[0]; a.x_st = x_strides[1];
@@ -312,7 +320,8 @@ extern "C" int uttt_selective_scan_fwd(const void* x, const int64_t* x_strides, 
   a.B_sb = B_strides[0]; a.B_st = B_strides[1]; a.B_sg = B_strides[2];
   a.C_sb = C_strides[0]; a.C_st = C_strides[1]; a.C_sg = C_strides[2];
   if (gate) { a.z_sb = gate_strides[0]; a.z_st = gate_strides[1]; }
-  scan_runs(a, kFwdBlocks);
+  if (const int rc = scan_check(a, dtype, what)) return rc;
+  fwd_runs(a);
   UTTT_REQUIRE(scan_fits(a), "%s: too many sequences, channels or states", what);
   const size_t need = fwd_bytes(a);
   UTTT_REQUIRE(!need || (workspace && workspace_bytes >= need), "%s: workspace of %zu bytes, %zu needed", what,
@@ -320,9 +329,11 @@ extern "C" int uttt_selective_scan_fwd(const void* x, const int64_t* x_strides, 
   if (need) {
     UTTT_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "%s: workspace must be 16-byte aligned", what);
     a.ends = static_cast<float*>(workspace);
-    a.starts = a.ends + (size_t)a.nruns * D * N;
-    a.decay = a.starts + (size_t)a.nruns * D * N;
+    a.starts = a.ends + (size_t)a.nruns * D * kept_states(N);
+    a.decay = a.starts + (size_t)a.nruns * D * kept_states(N);
   }
-  UTTT_DTYPE_SWITCH_LR(dtype, TT, return launch_fwd<TT>(a, as_stream(stream)));
+  const hipStream_t st = as_stream(stream);
+  UTTT_DTYPE_SWITCH_LR(dtype, TT,
+                       return dt_dtype == UTTT_F32 ? launch_fwd<TT, F32T>(a, st) : launch_fwd<TT, TT>(a, st));
   return UTTT_OK;
 }

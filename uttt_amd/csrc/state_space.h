@@ -62,6 +62,7 @@ __device__ __forceinline__ Run run_of(const Seqs& s, int at, int R) {
   return r;
 }
 
+constexpr int kLooseRuns = 8;   // places behind the last run for the tokens of no sequence
 // Token i of the tokens of no sequence of a packed call, -1 past the last one.
 __device__ __forceinline__ int loose_token(const Seqs& s, int i) {
   const int head = s.offset(0), tail = s.offset(s.nseq);
@@ -84,10 +85,32 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float x
   else static_cast<uint16_t*>(p)[i] = dtype == UTTT_BF16 ? f32_to_bf16(x) : f32_to_f16(x);
 }
 
-// 1 / (1 + e^-x), off by 2 ulp: e^x to an ulp and the hardware's reciprocal.
-__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + expf(-x)); }
-// ln(1 + e^x); above 20 they are the same to fp32's rounding.
-__device__ __forceinline__ float softplus(float x) { return x > 20.0f ? x : log1pf(expf(x)); }
+// e^-|x| (to e^-100, below which it is no normal fp32): the hardware's 2^x, an
+// ulp off, of x log2 e, whose rounding is made good to the first order.
+__device__ __forceinline__ float exp_neg_abs(float x) {
+  constexpr float c = 1.44269504088896340736f, c_low = 1.92596303e-8f, ln2 = 0.69314718055994530942f;
+  const float v = -fminf(fabsf(x), 100.0f), t = v * c;
+  const float low = __builtin_fmaf(v, c_low, __builtin_fmaf(v, c, -t));
+  const float e = __builtin_amdgcn_exp2f(t);
+  return __builtin_fmaf(e, low * ln2, e);
+}
+// 1 / (1 + e^-x), off by 2 ulp or so.
+__device__ __forceinline__ float sigmoid(float x) {
+  const float e = exp_neg_abs(x), r = __builtin_amdgcn_rcpf(1.0f + e);
+  return x < 0.0f ? e * r : r;
+}
+// ln(1 + e^x) and its slope 1 / (1 + e^-x), with s = 1 + e^-|x| and what its
+// rounding left out: ln(1 + e) = ln(s) + (e - (s - 1)) / s to the first order.
+__device__ __forceinline__ float softplus(float x, float& slope) {
+  const float e = exp_neg_abs(x), s = 1.0f + e, r = __builtin_amdgcn_rcpf(s);
+  slope = x < 0.0f ? e * r : r;
+  const float l = __builtin_fmaf(__builtin_amdgcn_logf(s), 0.69314718055994530942f, (e - (s - 1.0f)) * r);
+  return (x < 0.0f ? 0.0f : x) + l;
+}
+__device__ __forceinline__ float softplus(float x) {
+  float slope;
+  return softplus(x, slope);
+}
 
 // The rows of a step against a pool's slots.  Rows of one slot follow one
 // another in row order: the first one's workgroup takes them all up.

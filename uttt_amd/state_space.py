@@ -35,8 +35,11 @@ _ACTIVATIONS = {None: 0, "silu": 1}
 
 
 def _inner(t: Optional[Tensor]) -> Optional[Tensor]:
-    """t itself where its last axis is contiguous, else a copy."""
-    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """t itself where its last axis is contiguous and its tokens are not too far
+    apart (a tile's offsets are 32 bits), else a copy."""
+    if t is None or ((t.stride(-1) == 1 or t.shape[-1] == 1) and (t.stride(1) < 1 << 24 or t.shape[1] == 1)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _on16(t: Optional[Tensor]) -> Optional[Tensor]:
@@ -289,11 +292,16 @@ def _scan_infer(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optio
     return y, state
 
 
+def _kept_states(N):
+    """N up to the next power of two of 4 or more, as the kernels keep states."""
+    return max(4, 1 << (N - 1).bit_length())
+
+
 def _scan_fwd_fake(x, dt, A, B, C, D, gate, dt_bias, softplus, initial_state, cu_seqlens, want_state):
     n, T = x.shape[:2]
     tiles = T // TILE + _seqs(x, cu_seqlens) if cu_seqlens is not None else n * max(1, (T + TILE - 1) // TILE)
     return (*_scan_infer_fake(x, dt, A, B, C, D, gate, dt_bias, softplus, initial_state, cu_seqlens, want_state),
-            x.new_empty((tiles, *A.shape), dtype=torch.float32))
+            x.new_empty((tiles, _kept_states(A.shape[1]), A.shape[0]), dtype=torch.float32))
 
 
 @traced_op("selective_scan_fwd", _scan_fwd_fake)
@@ -371,7 +379,7 @@ def _check_scan(what, x, dt, A, B, C, D, gate, dt_bias):
     assert x.dtype in _TYPES, f"{what}: dtype {x.dtype}"
     n, T, Dm = x.shape
     assert dt.shape == x.shape, f"{what}: dt {tuple(dt.shape)} must have x's shape {tuple(x.shape)}"
-    assert dt.dtype in _TYPES, f"{what}: dt must be fp32, bf16 or fp16, got {dt.dtype}"
+    assert dt.dtype in (torch.float32, x.dtype), f"{what}: dt must be fp32 or of x's dtype {x.dtype}, got {dt.dtype}"
     assert A.dim() == 2 and A.shape[0] == Dm and 1 <= A.shape[1] <= MAX_STATES, (
         f"{what}: A must be [{Dm}, N] with N of 1 to {MAX_STATES}, got {tuple(A.shape)}")
     assert B.dim() == 4 and B.shape[:2] == (n, T) and B.shape[3] == A.shape[1], (
@@ -397,7 +405,7 @@ def selective_scan(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, *, D:
     final states [N_seqs, D, N] fp32 or None).
 
     x              [B, T, D] in fp32, bf16 or fp16.
-    dt             [B, T, D] steps in any of the three, to which dt_bias [D] is added and, with
+    dt             [B, T, D] steps in fp32 or x's dtype, to which dt_bias [D] is added and, with
                    dt_softplus, ln(1 + e^x) applied.
     A              [D, N] fp32, N up to 64: the states' rates, below zero where they decay.
     B, C           [B, T, G, N] in x's dtype; channels D / G * g onwards read group g.
