@@ -22,19 +22,20 @@ namespace uttt {
 namespace {
 
 using ssm::launch_sums;
-using ssm::sigmoid;
+using ssm::sigmoid_for;
 
 constexpr int kMaxRow = 8192;
 
 // Row i of a tensor of rows in groups of `heads`: at i / heads * outer + i % heads * inner.
+struct Row {
+  uint32_t group, head;
+  __device__ __forceinline__ Row(int64_t row, int heads)
+      : group((uint32_t)row / (uint32_t)heads), head((uint32_t)row - group * (uint32_t)heads) {}
+};
 struct RowsOf {
   const void* p;
   int64_t outer, inner;
-  __device__ __forceinline__ int64_t at(int64_t row, int heads) const {
-    if (heads == 1) return row * outer;
-    const int64_t o = row / heads;
-    return o * outer + (row - o * heads) * inner;
-  }
+  __device__ __forceinline__ int64_t at(Row r) const { return r.group * outer + r.head * inner; }
 };
 
 struct NormArgs {
@@ -66,7 +67,7 @@ __device__ __forceinline__ float row_sum(float a, float* red) {
   return a;
 }
 
-template <class TT, int V, int LPR, int NI, bool AFTER>
+template <class TT, int V, int LPR, int NI, bool AFTER, bool SCALE>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_fwd_kernel(NormArgs a) {
   using S = typename TT::S;
   constexpr int THREADS = LPR > 256 ? LPR : 256, RPB = THREADS / LPR;
@@ -78,16 +79,17 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_fwd_kernel(NormArg
     const int e = (lane + LPR * c) * V;
     if (e < a.N) {
       load_weights<V>(a.w, a.w_dtype, e, 1.0f, w[c]);
-      load_weights<V>(a.s, a.s_dtype, e, 1.0f, s[c]);
+      if (SCALE) load_weights<V>(a.s, a.s_dtype, e, 1.0f, s[c]);
 #pragma unroll
-      for (int i = 0; i < V; ++i) s[c][i] *= a.alpha;
+      for (int i = 0; i < V; ++i) s[c][i] = SCALE ? s[c][i] * a.alpha : a.alpha;
     }
   }
   for (int64_t base = (int64_t)blockIdx.x * RPB; base < a.rows; base += (int64_t)gridDim.x * RPB) {
     const bool live = base + slot < a.rows;
     const int64_t row = live ? base + slot : a.rows - 1;
-    const S* x = static_cast<const S*>(a.x.p) + a.x.at(row, a.heads);
-    const int64_t r0 = a.r.p ? a.r.at(row, a.heads) : 0, z0 = a.z.p ? a.z.at(row, a.heads) : 0;
+    const Row at(row, a.heads);
+    const S* x = static_cast<const S*>(a.x.p) + a.x.at(at);
+    const int64_t r0 = a.r.p ? a.r.at(at) : 0, z0 = a.z.p ? a.z.at(at) : 0;
     float v[NI][V], o[NI][V];   // what is normed; the residual
     float sq = 0.0f;
 #pragma unroll
@@ -122,7 +124,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_fwd_kernel(NormArg
           float z[V];
           load_piece<TT, V>(static_cast<const S*>(a.z.p) + z0 + e, z);
 #pragma unroll
-          for (int i = 0; i < V; ++i) v[c][i] *= z[i] * sigmoid(z[i]);
+          for (int i = 0; i < V; ++i) v[c][i] *= z[i] * sigmoid_for<TT>(z[i]);
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) v[c][i] = __builtin_fmaf(v[c][i], s[c][i], o[c][i]);
@@ -132,7 +134,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_fwd_kernel(NormArg
   }
 }
 
-template <class TT, int V, int LPR, int NI, bool AFTER>
+template <class TT, int V, int LPR, int NI, bool AFTER, bool SCALE>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_bwd_kernel(NormArgs a) {
   using S = typename TT::S;
   constexpr int THREADS = LPR > 256 ? LPR : 256, RPB = THREADS / LPR;
@@ -147,17 +149,18 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_bwd_kernel(NormArg
     for (int i = 0; i < V; ++i) dw[c][i] = ds[c][i] = 0.0f;
     if (e < a.N) {
       load_weights<V>(a.w, a.w_dtype, e, 1.0f, w[c]);
-      load_weights<V>(a.s, a.s_dtype, e, 1.0f, s[c]);
+      if (SCALE) load_weights<V>(a.s, a.s_dtype, e, 1.0f, s[c]);
 #pragma unroll
-      for (int i = 0; i < V; ++i) s[c][i] *= a.alpha;
+      for (int i = 0; i < V; ++i) s[c][i] = SCALE ? s[c][i] * a.alpha : a.alpha;
     }
   }
   const float inv_n = 1.0f / (float)a.N;
   for (int64_t base = (int64_t)blockIdx.x * RPB; base < a.rows; base += (int64_t)gridDim.x * RPB) {
     const bool live = base + slot < a.rows;
     const int64_t row = live ? base + slot : a.rows - 1;
-    const S* x = static_cast<const S*>(a.x.p) + a.x.at(row, a.heads);
-    const int64_t g0 = a.dy.p ? a.dy.at(row, a.heads) : 0;
+    const Row at(row, a.heads);
+    const S* x = static_cast<const S*>(a.x.p) + a.x.at(at);
+    const int64_t g0 = a.dy.p ? a.dy.at(at) : 0;
     const float rstd = a.rstd[row];
     float n[NI][V], m[NI][V];
     float sum = 0.0f;
@@ -170,10 +173,10 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_bwd_kernel(NormArg
       if constexpr (AFTER) {
         float z[V], f[V], df[V];
         if (a.z.p) {
-          load_piece<TT, V>(static_cast<const S*>(a.z.p) + a.z.at(row, a.heads) + e, z);
+          load_piece<TT, V>(static_cast<const S*>(a.z.p) + a.z.at(at) + e, z);
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const float q = sigmoid(z[i]);
+            const float q = sigmoid_for<TT>(z[i]);
             f[i] = z[i] * q;
             df[i] = q * __builtin_fmaf(z[i], 1.0f - q, 1.0f);
           }
@@ -185,7 +188,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_bwd_kernel(NormArg
         for (int i = 0; i < V; ++i) {
           n[c][i] *= rstd;
           const float o = m[c][i] * s[c][i], nf = n[c][i] * f[i];
-          ds[c][i] = __builtin_fmaf(m[c][i], nf * w[c][i], ds[c][i]);
+          if (SCALE) ds[c][i] = __builtin_fmaf(m[c][i], nf * w[c][i], ds[c][i]);
           dw[c][i] = __builtin_fmaf(o, nf, dw[c][i]);
           if (a.z.p) z[i] = o * n[c][i] * w[c][i] * df[i];
           m[c][i] = o * w[c][i] * f[i];
@@ -194,7 +197,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_bwd_kernel(NormArg
         if (a.z.p) store_piece<TT, V>(static_cast<S*>(a.dz) + row * a.N + e, z);
       } else {
         float r[V];
-        load_weights<V>(a.r.p, a.r_dtype, a.r.at(row, a.heads) + e, 0.0f, r);
+        load_weights<V>(a.r.p, a.r_dtype, a.r.at(at) + e, 0.0f, r);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           n[c][i] = __builtin_fmaf(n[c][i], s[c][i], r[i]) * rstd;
@@ -215,12 +218,12 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_bwd_kernel(NormArg
       if constexpr (!AFTER) {
         float v[V];
         if (a.dh.p) {
-          load_weights<V>(a.dh.p, a.r_dtype, a.dh.at(row, a.heads) + e, 0.0f, v);
+          load_weights<V>(a.dh.p, a.r_dtype, a.dh.at(at) + e, 0.0f, v);
 #pragma unroll
           for (int i = 0; i < V; ++i) m[c][i] += v[i];
         }
         store_piece_as<V>(a.dr, a.r_dtype, row * a.N + e, m[c]);
-        if (a.part_s) {
+        if (SCALE) {
           load_piece<TT, V>(x + e, v);
 #pragma unroll
           for (int i = 0; i < V; ++i) ds[c][i] = __builtin_fmaf(v[i], m[c][i], ds[c][i]);
@@ -260,23 +263,32 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_bwd_kernel(NormArg
   }
 }
 
-// Workgroups of the backward, each with 8 rows or more to walk over: a function
-// of the sizes alone, so that its sums come out the same on every run.
+// Workgroups of the backward, each with 8 rows or more to walk over and no more
+// than the card holds at once, five, three or two a CU by their registers
+// (32 768 rows of 768 with a scale: 1024 of them 128 us, 768 99): a function of
+// the sizes alone, so that its sums come out the same on every run.
 int64_t bwd_blocks(int64_t rows, int N) {
-  const int64_t per = N <= 64 ? 32 : 8, n = (rows + per - 1) / per;
-  return n < 1024 ? n : 1024;
+  const int64_t per = N <= 64 ? 32 : 8, n = (rows + per - 1) / per, most = N <= 512 ? 1280 : N <= 2048 ? 768 : 512;
+  return n < most ? n : most;
 }
 
-template <class TT, int V, int LPR, int NI, bool AFTER>
-void norm_launch(const NormArgs& a, bool bwd, hipStream_t st) {
+template <class TT, int V, int LPR, int NI, bool AFTER, bool SCALE>
+void launch_fwd(const NormArgs& a, hipStream_t st) {
   constexpr int THREADS = LPR > 256 ? LPR : 256, RPB = THREADS / LPR;
   int64_t blocks = (a.rows + RPB - 1) / RPB;
   if (blocks > 2048) blocks = 2048;   // 8 workgroups a CU: the weights are read once for many rows
-  if (bwd)
-    hipLaunchKernelGGL((norm_bwd_kernel<TT, V, LPR, NI, AFTER>), dim3((unsigned)bwd_blocks(a.rows, a.N)), dim3(THREADS),
-                       0, st, a);
-  else
-    hipLaunchKernelGGL((norm_fwd_kernel<TT, V, LPR, NI, AFTER>), dim3((unsigned)blocks), dim3(THREADS), 0, st, a);
+  hipLaunchKernelGGL((norm_fwd_kernel<TT, V, LPR, NI, AFTER, SCALE>), dim3((unsigned)blocks), dim3(THREADS), 0, st, a);
+}
+template <class TT, int V, int LPR, int NI, bool AFTER, bool SCALE>
+void launch_bwd(const NormArgs& a, hipStream_t st) {
+  constexpr int THREADS = LPR > 256 ? LPR : 256;
+  hipLaunchKernelGGL((norm_bwd_kernel<TT, V, LPR, NI, AFTER, SCALE>), dim3((unsigned)bwd_blocks(a.rows, a.N)),
+                     dim3(THREADS), 0, st, a);
+}
+template <class TT, int V, int LPR, int NI, bool AFTER, bool SCALE>
+void norm_launch(const NormArgs& a, bool bwd, hipStream_t st) {
+  if (bwd) launch_bwd<TT, V, LPR, NI, AFTER, SCALE>(a, st);
+  else launch_fwd<TT, V, LPR, NI, AFTER, SCALE>(a, st);
 }
 
 bool whole_pieces(const NormArgs& a, int size) {
@@ -289,33 +301,38 @@ bool whole_pieces(const NormArgs& a, int size) {
   return ((all | (uintptr_t)((int64_t)a.N * size)) & 15u) == 0;
 }
 
-template <class TT, bool AFTER>
+template <class TT, bool AFTER, bool SCALE>
 int norm_rows(const NormArgs& a, bool bwd, hipStream_t st) {
   constexpr int V = 16 / sizeof(typename TT::S);
   // V elements of another type are 8 bytes or two pieces of 16; with all strides
   // and N multiples of 8 elements each lies right
   if (whole_pieces(a, 2)) {
     const int pieces = (a.N + V - 1) / V;
-    if (pieces <= 16) norm_launch<TT, V, 16, 1, AFTER>(a, bwd, st);
-    else if (pieces <= 32) norm_launch<TT, V, 32, 1, AFTER>(a, bwd, st);
-    else if (pieces <= 64) norm_launch<TT, V, 64, 1, AFTER>(a, bwd, st);
-    else if (pieces <= 128) norm_launch<TT, V, 64, 2, AFTER>(a, bwd, st);
-    else if (pieces <= 256) norm_launch<TT, V, 256, 1, AFTER>(a, bwd, st);
-    else if (pieces <= 512) norm_launch<TT, V, 256, 2, AFTER>(a, bwd, st);
-    else if (pieces <= 1024) norm_launch<TT, V, 1024, 1, AFTER>(a, bwd, st);
-    else norm_launch<TT, V, 1024, 2, AFTER>(a, bwd, st);
+    // 24 pieces (heads of 192 in 16 bits): forward all of 8 lanes three times and
+    // not 24 of 32 (70 us against 98 for 262 144 rows), backward that is more
+    // registers than it gains (173 against 142)
+    if (pieces <= 8) norm_launch<TT, V, 8, 1, AFTER, SCALE>(a, bwd, st);
+    else if (pieces <= 16) norm_launch<TT, V, 16, 1, AFTER, SCALE>(a, bwd, st);
+    else if (pieces <= 24 && !bwd) launch_fwd<TT, V, 8, 3, AFTER, SCALE>(a, st);
+    else if (pieces <= 32) norm_launch<TT, V, 32, 1, AFTER, SCALE>(a, bwd, st);
+    else if (pieces <= 64) norm_launch<TT, V, 64, 1, AFTER, SCALE>(a, bwd, st);
+    else if (pieces <= 128) norm_launch<TT, V, 64, 2, AFTER, SCALE>(a, bwd, st);
+    else if (pieces <= 256) norm_launch<TT, V, 256, 1, AFTER, SCALE>(a, bwd, st);
+    else if (pieces <= 512) norm_launch<TT, V, 256, 2, AFTER, SCALE>(a, bwd, st);
+    else if (pieces <= 1024) norm_launch<TT, V, 1024, 1, AFTER, SCALE>(a, bwd, st);
+    else norm_launch<TT, V, 1024, 2, AFTER, SCALE>(a, bwd, st);
   } else {
-    if (a.N <= 64) norm_launch<TT, 1, 16, 4, AFTER>(a, bwd, st);
-    else if (a.N <= 256) norm_launch<TT, 1, 64, 4, AFTER>(a, bwd, st);
-    else if (a.N <= 1024) norm_launch<TT, 1, 256, 4, AFTER>(a, bwd, st);
-    else if (a.N <= 2048) norm_launch<TT, 1, 256, 8, AFTER>(a, bwd, st);
-    else norm_launch<TT, 1, 1024, 8, AFTER>(a, bwd, st);
+    if (a.N <= 64) norm_launch<TT, 1, 16, 4, AFTER, SCALE>(a, bwd, st);
+    else if (a.N <= 256) norm_launch<TT, 1, 64, 4, AFTER, SCALE>(a, bwd, st);
+    else if (a.N <= 1024) norm_launch<TT, 1, 256, 4, AFTER, SCALE>(a, bwd, st);
+    else if (a.N <= 2048) norm_launch<TT, 1, 256, 8, AFTER, SCALE>(a, bwd, st);
+    else norm_launch<TT, 1, 1024, 8, AFTER, SCALE>(a, bwd, st);
   }
   return check_launch(AFTER ? "norm_after_block" : "norm_before_block");
 }
 
 int norm_check(const NormArgs& a, int dtype, const char* what) {
-  UTTT_REQUIRE(a.rows >= 0 && a.rows < (1LL << 40) && a.heads >= 1 && a.N >= 1 && a.N <= kMaxRow,
+  UTTT_REQUIRE(a.rows >= 0 && a.rows < (1LL << 31) && a.heads >= 1 && a.N >= 1 && a.N <= kMaxRow,
                "%s: bad sizes rows=%lld heads=%d N=%d", what, (long long)a.rows, a.heads, a.N);
   UTTT_REQUIRE(dtype_bytes(dtype) && dtype_bytes(a.r_dtype) && dtype_bytes(a.y_dtype) && dtype_bytes(a.w_dtype) &&
                    dtype_bytes(a.s_dtype),
@@ -349,9 +366,9 @@ int norm_run(const NormArgs& a, int dtype, bool bwd, void* workspace, size_t wor
   }
   int rc = UTTT_OK;
   switch (dtype) {
-    case UTTT_F32: rc = norm_rows<F32T, AFTER>(b, bwd, st); break;
-    case UTTT_BF16: rc = norm_rows<BF16T, AFTER>(b, bwd, st); break;
-    default: rc = norm_rows<F16T, AFTER>(b, bwd, st); break;
+    case UTTT_F32: rc = a.s ? norm_rows<F32T, AFTER, true>(b, bwd, st) : norm_rows<F32T, AFTER, false>(b, bwd, st); break;
+    case UTTT_BF16: rc = a.s ? norm_rows<BF16T, AFTER, true>(b, bwd, st) : norm_rows<BF16T, AFTER, false>(b, bwd, st); break;
+    default: rc = a.s ? norm_rows<F16T, AFTER, true>(b, bwd, st) : norm_rows<F16T, AFTER, false>(b, bwd, st); break;
   }
   if (!rc && dweight) rc = launch_sums(b.part_w, blocks, a.N, dweight, b.w_dtype, st, what);
   if (!rc && dscale) rc = launch_sums(b.part_s, blocks, a.N, dscale, b.s_dtype, st, what);

@@ -7,8 +7,8 @@
 // first token.
 //
 // Bound by memory: the forward reads x and writes y, the backward reads x and
-// dy and writes dx.  A thread walks over a run of tokens with V channels (16
-// bytes where rows allow it), its window of W inputs in registers, the loads of
+// dy and writes dx.  A thread walks over a run of tokens with V channels (four
+// where rows allow it), its window of W inputs in registers, the loads of
 // several tokens ahead of their use; the W - 1 tokens around a run are read
 // twice, from cache.  The backward computes p again and keeps the W unfinished
 // dx in registers too.
@@ -103,7 +103,7 @@ __device__ __forceinline__ void push(float (&win)[W][V]) {
 template <class TT, int W, int V>
 __global__ __launch_bounds__(kConvThreads) void conv_fwd_kernel(ConvArgs a) {
   using S = typename TT::S;
-  constexpr int U = V > 1 ? 8 : 16;   // tokens loaded ahead
+  constexpr int U = 8;   // tokens that are loaded ahead
   const uint32_t id = blockIdx.x * kConvThreads + threadIdx.x;
   const int at = id / (uint32_t)a.nvec, d = (int)(id % (uint32_t)a.nvec) * V;
   if (at >= a.nruns) {
@@ -114,30 +114,52 @@ __global__ __launch_bounds__(kConvThreads) void conv_fwd_kernel(ConvArgs a) {
   if (r.seq < 0) return;
   const int t0 = r.c * a.R, n = min(a.R, r.len - t0);
   const S* xp = static_cast<const S*>(a.x) + r.b * a.x_sb + r.tok0 * a.x_st + d;
-  S* yp = static_cast<S*>(a.y) + ((int64_t)r.b * a.seqs.T + r.tok0) * a.D + d;
+  S* yp = static_cast<S*>(a.y) + ((int64_t)r.b * a.seqs.T + r.tok0 + t0) * a.D + d;
   float w[W][V], b[V], win[W][V];
   load_weights<W, V>(a, d, w, b);
   load_window<TT, W, V>(a, r, t0, xp, d, win);
-  for (int tt = t0; tt < t0 + n; tt += U) {
-    Piece<TT, V> x[U];
+  xp += (int64_t)t0 * a.x_st;
+  auto token = [&](const Piece<TT, V>& x) {
+    float p[V];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (tt + u < t0 + n) x[u].load(xp + (int64_t)(tt + u) * a.x_st);
+    for (int i = 0; i < V; ++i) {
+      win[W - 1][i] = x.get(i);
+      p[i] = b[i];
+#pragma unroll
+      for (int k = 0; k < W; ++k) p[i] = __builtin_fmaf(w[k][i], win[k][i], p[i]);
+    }
+    if (a.act)
+#pragma unroll
+      for (int i = 0; i < V; ++i) p[i] *= sigmoid_for<TT>(p[i]);
+    store_piece<TT, V>(yp, p);
+    yp += a.D;
+    push<W, V>(win);
+  };
+  Piece<TT, V> next[U];
+  auto load = [&]() {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (tt + u >= t0 + n) break;
-      float p[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        win[W - 1][i] = x[u].get(i);
-        p[i] = b[i];
-#pragma unroll
-        for (int k = 0; k < W; ++k) p[i] = __builtin_fmaf(w[k][i], win[k][i], p[i]);
-        if (a.act) p[i] *= sigmoid(p[i]);
-      }
-      store_piece<TT, V>(yp + (int64_t)(tt + u) * a.D, p);
-      push<W, V>(win);
+      next[u].load(xp);
+      xp += a.x_st;
     }
+  };
+  if (n >= U) load();
+  int t = 0;
+#pragma unroll 1
+  for (; t + U <= n; t += U) {
+    Piece<TT, V> x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = next[u];
+    if (t + 2 * U <= n) load();
+#pragma unroll
+    for (int u = 0; u < U; ++u) token(x[u]);
+  }
+#pragma unroll 1
+  for (; t < n; ++t) {
+    Piece<TT, V> x;
+    x.load(xp);
+    xp += a.x_st;
+    token(x);
   }
   if (a.hT && t0 + n >= r.len)
 #pragma unroll
@@ -152,7 +174,7 @@ constexpr int kBwdPieces = 32, kBwdRuns = kConvThreads / kBwdPieces;
 template <class TT, int W, int V>
 __global__ __launch_bounds__(kConvThreads) void conv_bwd_kernel(ConvArgs a) {
   using S = typename TT::S;
-  constexpr int U = V > 1 ? 4 : 8;
+  constexpr int U = 4;   // tokens that are loaded ahead
   __shared__ float red[kBwdRuns][kBwdPieces * V];
   const int nvb = (a.nvec + kBwdPieces - 1) / kBwdPieces;
   const int blk = blockIdx.x / nvb;
@@ -183,60 +205,89 @@ __global__ __launch_bounds__(kConvThreads) void conv_bwd_kernel(ConvArgs a) {
     for (int k = 0; k < W; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[k][i] = 0.0f;
+    // Token t: of the run itself (own) or behind it, in which case it only ends
+    // the dx of the run's last tokens; behind the sequence's end there is none.
+    auto token = [&](const Piece<TT, V>& x, const Piece<TT, V>& g, bool own) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        win[W - 1][i] = x.get(i);
+        float dp = g.get(i);
+        if (a.act) {
+          float p = b[i];
+#pragma unroll
+          for (int k = 0; k < W; ++k) p = __builtin_fmaf(w[k][i], win[k][i], p);
+          const float s = sigmoid_for<TT>(p);
+          dp *= s * __builtin_fmaf(p, 1.0f - s, 1.0f);
+        }
+#pragma unroll
+        for (int k = 0; k < W; ++k) acc[k][i] = __builtin_fmaf(w[k][i], dp, acc[k][i]);
+        if (own) {
+          db[i] += dp;
+#pragma unroll
+          for (int k = 0; k < W; ++k) dw[k][i] = __builtin_fmaf(dp, win[k][i], dw[k][i]);
+        }
+      }
+    };
+    auto step = [&]() {
+      push<W, V>(win);
+      push<W, V>(acc);
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[W - 1][i] = 0.0f;
+    };
+    // with what the final state adds, and positions before the first token
+    auto checked = [&](int t) {
+      if (t < r.len) {
+        Piece<TT, V> x, g;
+        x.load(xp + (int64_t)t * a.x_st);
+        g.load(gp + (int64_t)t * a.dy_st);
+        token(x, g, t < t1);
+      }
+      const int done = t - (W - 1), kept = done - (r.len - (W - 1));   // whose dx ends here; its place in the final state
+      if (done >= t0 || (done < 0 && t0 == 0)) {
+        if (a.dhT && kept >= 0) {
+          Piece<TT, V> e;
+          e.load(static_cast<const S*>(a.dhT) + ((int64_t)r.seq * (W - 1) + kept) * a.D + d);
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[0][i] += e.get(i);
+        }
+        if (done >= 0) store_piece<TT, V>(op + (int64_t)done * a.D, acc[0]);
+        else if (a.dh0)
+          store_piece<TT, V>(static_cast<S*>(a.dh0) + ((int64_t)r.seq * (W - 1) + done + W - 1) * a.D + d, acc[0]);
+      }
+      step();
+    };
     const int end = t1 + W - 1;   // the last token of the run is done with the W - 1 behind it
-    for (int tt = t0; tt < end; tt += U) {
+    int t = t0;
+#pragma unroll 1
+    for (; t < end && t < t0 + W - 1; ++t) checked(t);
+    // from here to the run's last token one position ends with each, before the final state
+    Piece<TT, V> nx[U], ng[U];
+    auto load = [&](int t) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        nx[u].load(xp + (int64_t)(t + u) * a.x_st);
+        ng[u].load(gp + (int64_t)(t + u) * a.dy_st);
+      }
+    };
+    if (t + U <= t1) load(t);
+#pragma unroll 1
+    for (; t + U <= t1; t += U) {
       Piece<TT, V> x[U], g[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        x[u].zero();
-        g[u].zero();
-        if (tt + u < end && tt + u < r.len) {
-          x[u].load(xp + (int64_t)(tt + u) * a.x_st);
-          g[u].load(gp + (int64_t)(tt + u) * a.dy_st);
-        }
+        x[u] = nx[u];
+        g[u] = ng[u];
       }
+      if (t + 2 * U <= t1) load(t + U);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int t = tt + u, done = t - (W - 1);   // the position whose dx ends here
-        if (t >= end) break;
-        if (t < r.len)   // behind the sequence's end nothing is added
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            win[W - 1][i] = x[u].get(i);
-            float dp = g[u].get(i);
-            if (a.act) {
-              float p = b[i];
-#pragma unroll
-              for (int k = 0; k < W; ++k) p = __builtin_fmaf(w[k][i], win[k][i], p);
-              const float s = sigmoid(p);
-              dp *= s * __builtin_fmaf(p, 1.0f - s, 1.0f);
-            }
-#pragma unroll
-            for (int k = 0; k < W; ++k) acc[k][i] = __builtin_fmaf(w[k][i], dp, acc[k][i]);
-            if (t < t1) {
-              db[i] += dp;
-#pragma unroll
-              for (int k = 0; k < W; ++k) dw[k][i] = __builtin_fmaf(dp, win[k][i], dw[k][i]);
-            }
-          }
-        if (done >= t0 || (done < 0 && t0 == 0)) {
-          const int kept = done - (r.len - (W - 1));   // its place in the final state
-          if (a.dhT && kept >= 0) {
-            Piece<TT, V> e;
-            e.load(static_cast<const S*>(a.dhT) + ((int64_t)r.seq * (W - 1) + kept) * a.D + d);
-#pragma unroll
-            for (int i = 0; i < V; ++i) acc[0][i] += e.get(i);
-          }
-          if (done >= 0) store_piece<TT, V>(op + (int64_t)done * a.D, acc[0]);
-          else if (a.dh0)
-            store_piece<TT, V>(static_cast<S*>(a.dh0) + ((int64_t)r.seq * (W - 1) + done + W - 1) * a.D + d, acc[0]);
-        }
-        push<W, V>(win);
-        push<W, V>(acc);
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[W - 1][i] = 0.0f;
+        token(x[u], g[u], true);
+        store_piece<TT, V>(op + (int64_t)(t + u - (W - 1)) * a.D, acc[0]);
+        step();
       }
     }
+#pragma unroll 1
+    for (; t < end; ++t) checked(t);
   }
   if (!a.part_w && !a.part_b) return;
 #pragma unroll
@@ -328,14 +379,13 @@ __global__ __launch_bounds__(kConvThreads) void conv_step_kernel(ConvStepArgs a)
     default: { constexpr int WW = 8; __VA_ARGS__; } break;  \
   }
 
-bool on16(std::initializer_list<const void*> ps) {
-  uintptr_t all = 0;
-  for (const void* p : ps) all |= reinterpret_cast<uintptr_t>(p);
-  return (all & 15u) == 0;
-}
+// Whether rows hold whole pieces of four elements.
 bool whole_pieces(const ConvArgs& a, int size) {
+  uintptr_t all = 0;
+  for (const void* p : {a.x, (const void*)a.y, a.h0, (const void*)a.hT, a.dy, (const void*)a.dx, a.dhT, (const void*)a.dh0})
+    all |= reinterpret_cast<uintptr_t>(p);
   const int64_t rows = a.D | a.x_sb | a.x_st | a.dy_sb | a.dy_st;
-  return (rows * size) % 16 == 0 && on16({a.x, a.y, a.h0, a.hT, a.dy, a.dx, a.dhT, a.dh0});
+  return ((all | (uintptr_t)(rows * size)) & (uintptr_t)(4 * size - 1)) == 0;
 }
 
 int64_t fwd_threads(const ConvArgs& a) {
@@ -372,8 +422,7 @@ int launch_conv(ConvArgs a, int W, bool bwd, hipStream_t st) {
 
 template <class TT>
 int conv_any(const ConvArgs& a, int W, bool bwd, hipStream_t st) {
-  constexpr int V = 16 / sizeof(typename TT::S);
-  return whole_pieces(a, sizeof(typename TT::S)) ? launch_conv<TT, V>(a, W, bwd, st) : launch_conv<TT, 1>(a, W, bwd, st);
+  return whole_pieces(a, sizeof(typename TT::S)) ? launch_conv<TT, 4>(a, W, bwd, st) : launch_conv<TT, 1>(a, W, bwd, st);
 }
 
 int conv_check(const ConvArgs& a, int W, int dtype, const char* what) {

@@ -81,7 +81,7 @@ __global__ __launch_bounds__(kScanThreads, fwd_waves(NP)) void scan_fwd_kernel(S
     float v = __builtin_fmaf(skip, x, (y[0] + y[1]) + (y[2] + y[3]));
     if (GATE) {
       const float z = TT::load(zbits);
-      v *= z * sigmoid(z);
+      v *= z * sigmoid_for<TT>(z);
     }
     y0[c] = TT::store(v);
   };

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(ScanStepArgs a)
         y = __builtin_fmaf(cm[j], h[j], y);
       }
       y = __builtin_fmaf(skip, x, sum_lanes<LN>(y));
-      if (a.z) y *= z * sigmoid(z);
+      if (a.z) y *= z * sigmoid_for<TT>(z);
       if (live && ln == 0) static_cast<S*>(a.out)[((int64_t)b * a.T + t) * a.D + d] = TT::store(y);
     }
     b = rows.next_of<kScanThreads>(b, slot);

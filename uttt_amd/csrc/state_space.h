@@ -99,6 +99,14 @@ __device__ __forceinline__ float sigmoid(float x) {
   const float e = exp_neg_abs(x), r = __builtin_amdgcn_rcpf(1.0f + e);
   return x < 0.0f ? e * r : r;
 }
+// The same where it goes into results of TT.  For 16-bit ones without the
+// correction: off by |x| 2^-24 and an ulp or two of it, a third of their 2^-24
+// in absolute terms.
+template <class TT>
+__device__ __forceinline__ float sigmoid_for(float x) {
+  if constexpr (sizeof(typename TT::S) == 4) return sigmoid(x);
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * x));
+}
 // ln(1 + e^x) and its slope 1 / (1 + e^-x), with s = 1 + e^-|x| and what its
 // rounding left out: ln(1 + e) = ln(s) + (e - (s - 1)) / s to the first order.
 __device__ __forceinline__ float softplus(float x, float& slope) {
