@@ -346,7 +346,8 @@ __global__ __launch_bounds__(kConvThreads) void conv_step_kernel(ConvStepArgs a)
     for (int k = 0; k < W; ++k) w[k] = load_any(a.w, a.w_dtype, (int64_t)d * W + k);
     if (a.b) bias = load_any(a.b, a.b_dtype, d);
   }
-  if (rows.taken_up_before<kConvThreads>(b, slot)) return;
+  const int others = rows.others<kConvThreads>(b, slot);
+  if (others & 1) return;   // an earlier row's workgroup takes this one up
   for (;;) {
     if (live)
       for (int t = 0; t < a.T; ++t) {
@@ -359,6 +360,7 @@ __global__ __launch_bounds__(kConvThreads) void conv_step_kernel(ConvStepArgs a)
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) win[k] = win[k + 1];
       }
+    if (!(others & 2)) break;
     b = rows.next_of<kConvThreads>(b, slot);
     if (b >= a.B) break;
   }

@@ -131,18 +131,26 @@ struct Rows {
                                      : static_cast<const int32_t*>(idx)[b];
     return s >= 0 && s < slots ? s : -1;
   }
-  // Whether an earlier row has row b's slot; for whole workgroups.
+  // Whether rows before and behind row b have its slot (bits 0 and 1); for whole
+  // workgroups.
   template <int THREADS>
-  __device__ __forceinline__ bool taken_up_before(int b, int64_t slot) const {
-    if (!idx) return false;
-    bool before = false;
-    for (int j = threadIdx.x; j < b; j += THREADS) before |= slot_of(j) == slot;
-    return __syncthreads_or(before);
+  __device__ __forceinline__ int others(int b, int64_t slot) const {
+    if (!idx) return 0;
+    __shared__ int found[THREADS / kWave];
+    int mine = 0;
+    for (int j = threadIdx.x; j < B; j += THREADS)
+      if (j != b && slot_of(j) == slot) mine |= j < b ? 1 : 2;
+    const int wave = (__ballot(mine & 1) ? 1 : 0) | (__ballot(mine & 2) ? 2 : 0);
+    if ((threadIdx.x & (kWave - 1)) == 0) found[threadIdx.x / kWave] = wave;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int i = 0; i < THREADS / kWave; ++i) all |= found[i];
+    return all;
   }
   // The next row behind b of its slot, B if there is none; for whole workgroups.
   template <int THREADS>
   __device__ __forceinline__ int next_of(int b, int64_t slot) const {
-    if (!idx) return B;
     __shared__ int next;
     __syncthreads();   // the last answer is read
     if (threadIdx.x == 0) next = B;
