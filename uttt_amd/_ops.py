@@ -119,9 +119,17 @@ def _int64s(*values):
 
 
 def strides_of(t, axes):
-    """Element strides of t's first `axes` axes as the C ABI takes them, 0 along an
-    axis of one, whose stride says nothing."""
-    return _int64s(*(s if n > 1 else 0 for s, n in zip(t.stride()[:axes], t.shape)))
+    """Element strides of t's first two or three axes as the C ABI takes them, 0
+    along an axis of one, whose stride says nothing."""
+    n, s = t.shape, t.stride()
+    if axes == 2:
+        return _int64s(s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0)
+    return _int64s(s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
+
+
+def evenly(step):
+    """The strides of rows `step` elements apart, in one group."""
+    return _int64s(step, 0)
 
 
 def none_if_empty(t):

@@ -370,9 +370,8 @@ int norm_run(const NormArgs& a, int dtype, bool bwd, void* workspace, size_t wor
     case UTTT_BF16: rc = a.s ? norm_rows<BF16T, AFTER, true>(b, bwd, st) : norm_rows<BF16T, AFTER, false>(b, bwd, st); break;
     default: rc = a.s ? norm_rows<F16T, AFTER, true>(b, bwd, st) : norm_rows<F16T, AFTER, false>(b, bwd, st); break;
   }
-  if (!rc && dweight) rc = launch_sums(b.part_w, blocks, a.N, dweight, b.w_dtype, st, what);
-  if (!rc && dscale) rc = launch_sums(b.part_s, blocks, a.N, dscale, b.s_dtype, st, what);
-  return rc;
+  if (rc) return rc;
+  return launch_sums(blocks, {{b.part_w, a.N, dweight, b.w_dtype}, {b.part_s, a.N, dscale, b.s_dtype}}, st, what);
 }
 
 }  // namespace

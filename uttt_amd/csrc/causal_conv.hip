@@ -498,9 +498,8 @@ extern "C" int uttt_causal_conv_bwd(const void* x, const int64_t* x_strides, int
     case UTTT_BF16: rc = conv_any<BF16T>(a, W, true, st); break;
     default: rc = conv_any<F16T>(a, W, true, st); break;
   }
-  if (!rc && dweight) rc = launch_sums(a.part_w, blocks, (int64_t)D * W, dweight, weight_dtype, st, what);
-  if (!rc && dbias) rc = launch_sums(a.part_b, blocks, D, dbias, bias_dtype, st, what);
-  return rc;
+  if (rc) return rc;
+  return launch_sums(blocks, {{a.part_w, (int64_t)D * W, dweight, weight_dtype}, {a.part_b, D, dbias, bias_dtype}}, st, what);
 }
 
 extern "C" int uttt_causal_conv_step(const void* x, const int64_t* x_strides, int dtype, const void* weight,

@@ -488,14 +488,19 @@ __global__ __launch_bounds__(256) void scan_bc_kernel(const float* __restrict__ 
   }
 }
 
-constexpr int kSumSlices = 16;
+constexpr int kSumSlices = 16, kMostSums = 3;
+struct SumArgs {
+  Sum sum[kMostSums];
+  int64_t first[kMostSums + 1];   // workgroups' numbers: 16 columns each
+};
 // 16 columns by 16 slices of the rows.
-__global__ __launch_bounds__(256) void sums_kernel(const float* __restrict__ part, int64_t n, int64_t M, void* out,
-                                                   int dtype) {
+__global__ __launch_bounds__(256) void sums_kernel(int64_t n, SumArgs a) {
   __shared__ double red[kSumSlices][17];
   const int c = threadIdx.x & 15, s = threadIdx.x >> 4;
-  for (int64_t base = (int64_t)blockIdx.x * 16; base < M; base += (int64_t)gridDim.x * 16) {
-    const int64_t e = base + c;
+  for (int64_t blk = blockIdx.x; blk < a.first[kMostSums]; blk += gridDim.x) {
+    const int k = blk < a.first[1] ? 0 : blk < a.first[2] ? 1 : 2;
+    const int64_t M = a.sum[k].M, e = (blk - a.first[k]) * 16 + c;
+    const float* part = a.sum[k].part;
     double v = 0.0;
     if (e < M)
 #pragma unroll 8
@@ -506,7 +511,7 @@ __global__ __launch_bounds__(256) void sums_kernel(const float* __restrict__ par
     if (s == 0 && e < M) {
 #pragma unroll
       for (int i = 1; i < kSumSlices; ++i) v += red[i][c];
-      store_any(out, dtype, e, (float)v);
+      store_any(a.sum[k].out, a.sum[k].dtype, e, (float)v);
     }
   }
 }
@@ -564,10 +569,18 @@ Parts bwd_parts(const ScanArgs& a) {
 
 }  // namespace
 
-int launch_sums(const float* part, int64_t n, int64_t M, void* out, int dtype, hipStream_t st, const char* what) {
-  const int64_t blocks = (M + 15) / 16;
-  hipLaunchKernelGGL(sums_kernel, dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, st, part, n, M,
-                     out, dtype);
+int launch_sums(int64_t n, std::initializer_list<Sum> sums, hipStream_t st, const char* what) {
+  SumArgs a{};
+  int k = 0;
+  for (const Sum& s : sums) {
+    a.sum[k] = s;
+    a.first[k + 1] = a.first[k] + (s.part ? (s.M + 15) / 16 : 0);
+    ++k;
+  }
+  for (; k < kMostSums; ++k) a.first[k + 1] = a.first[k];
+  const int64_t blocks = a.first[kMostSums];
+  if (blocks == 0) return UTTT_OK;
+  hipLaunchKernelGGL(sums_kernel, dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, st, n, a);
   return check_launch(what);
 }
 
@@ -648,8 +661,6 @@ extern "C" int uttt_selective_scan_bwd(const void* x, const int64_t* x_strides, 
     hipLaunchKernelGGL(scan_bc_kernel, dim3((unsigned)(n < 4096 ? n : 4096)), dim3(256), 0, st, a.part_bc, a.ncb, rows,
                        G * N, dtype, dB, dC);
   }
-  rc = launch_sums(a.part_A, a.nruns, (int64_t)D * N, dA, UTTT_F32, st, what);
-  if (!rc && dskip) rc = launch_sums(a.part_D, a.nruns, D, dskip, UTTT_F32, st, what);
-  if (!rc && ddt_bias) rc = launch_sums(a.part_bias, a.nruns, D, ddt_bias, UTTT_F32, st, what);
-  return rc;
+  return launch_sums(a.nruns, {{a.part_A, (int64_t)D * N, dA, UTTT_F32}, {a.part_D, D, dskip, UTTT_F32},
+                               {a.part_bias, D, ddt_bias, UTTT_F32}}, st, what);
 }

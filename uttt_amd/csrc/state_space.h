@@ -167,8 +167,13 @@ struct Rows {
 
 // out[e] = the sum of part[i][e] over i < n, for e < M, stored as dtype: in 64
 // bits and an order that n alone decides.
-int launch_sums(const float* part, int64_t n, int64_t M, void* out, int dtype, hipStream_t st,
-                const char* what);
+struct Sum {
+  const float* part;   // null: none
+  int64_t M;
+  void* out;
+  int dtype;
+};
+int launch_sums(int64_t n, std::initializer_list<Sum> sums, hipStream_t st, const char* what);
 
 }  // namespace ssm
 }  // namespace uttt

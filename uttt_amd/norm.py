@@ -10,7 +10,7 @@ import torch
 from torch import Tensor
 
 from . import _lib as L
-from ._ops import first_order_only, new_like, none_if_empty, run_function, strides_of, traced_op
+from ._ops import evenly, first_order_only, new_like, none_if_empty, run_function, strides_of, traced_op
 
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -123,31 +123,22 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
 MAX_BLOCK_ROW = 8192
 
 
-def _heads(t: Tensor) -> int:
-    """Rows come in groups of the second to last axis."""
-    return t.shape[-2] if t.dim() > 2 else 1
-
-
-def _grouped(t: Optional[Tensor]) -> Optional[Tensor]:
-    """t as [groups, rows of a group, N] with contiguous rows, a view wherever it can be."""
-    if t is None:
-        return None
+def _grouped(t: Tensor):
+    """t as [groups, rows of a group, N] with contiguous rows, a view wherever it can
+    be: groups of the second to last axis."""
     N = t.shape[-1]
     if t.stride(-1) != 1 and N > 1:
         t = t.contiguous()
-    return t.reshape(-1, _heads(t), N)   # -1: of no elements there are no rows, and no launch
-
-
-def _step2(t: Optional[Tensor]):
-    return None if t is None else strides_of(t, 2)
+    return t.reshape(-1, t.shape[-2] if t.dim() > 2 else 1, N)
 
 
 def _block_args(x: Tensor, *others: Optional[Tensor]):
-    """x and the others grouped, the rows, and the rows of a group."""
-    if x.numel() == 0:
-        return (x, *others), 0, 1
-    heads = _heads(x)
-    return tuple(_grouped(t) for t in (x, *others)), x.numel() // x.shape[-1], heads
+    """([(tensor, its row strides), ...] of x and the others, rows, rows of a group)."""
+    N, tensors = x.shape[-1], (x, *others)
+    if x.numel() == 0 or all(t is None or t.is_contiguous() for t in tensors):
+        return [(t, evenly(N)) for t in tensors], x.numel() // N, 1
+    tensors = [None if t is None else _grouped(t) for t in tensors]
+    return [(t, None if t is None else strides_of(t, 2)) for t in tensors], x.numel() // N, tensors[0].shape[1]
 
 
 def _rstd(x):
@@ -163,9 +154,9 @@ def _after_fwd(x: Tensor, weight: Optional[Tensor], gate: Optional[Tensor], resi
                scale: Optional[Tensor], alpha: float, eps: float, keep: bool) -> Tuple[Tensor, Tensor]:
     """(y, 1 / rms of each row for the backward, empty where nobody keeps it)."""
     y, rstd = _after_fake(x, weight, gate, residual, scale, alpha, eps, keep)
-    (x, gate, residual), rows, heads = _block_args(x, gate, residual)
-    L.call_on(x, "uttt_norm_after_fwd", L.ptr(x), _step2(x), _code(x), L.ptr(weight), _code(weight), L.ptr(gate),
-              _step2(gate), L.ptr(residual), _step2(residual), _code(y), L.ptr(scale), _code(scale), alpha, rows,
+    ((x, xs), (gate, gs), (residual, rs)), rows, heads = _block_args(x, gate, residual)
+    L.call_on(x, "uttt_norm_after_fwd", L.ptr(x), xs, _code(x), L.ptr(weight), _code(weight), L.ptr(gate),
+              gs, L.ptr(residual), rs, _code(y), L.ptr(scale), _code(scale), alpha, rows,
               heads, x.shape[-1], eps, L.ptr(y), L.ptr(rstd) if keep else None, L.stream_of(x))
     return y, rstd
 
@@ -189,11 +180,11 @@ def _after_bwd(x: Tensor, weight: Optional[Tensor], gate: Optional[Tensor], scal
                rstd: Tensor, dy: Tensor, want_dw: bool, want_ds: bool) -> List[Tensor]:
     grads = _after_bwd_fake(x, weight, gate, scale, alpha, rstd, dy, want_dw, want_ds)
     dx, dgate, dw, ds = grads
-    (x, gate, dy), rows, heads = _block_args(x, gate, dy)
+    ((x, xs), (gate, gs), (dy, ys)), rows, heads = _block_args(x, gate, dy)
     ws, size = _sums_workspace(x, rows, want_dw or want_ds)
-    L.call_on(x, "uttt_norm_after_bwd", L.ptr(x), _step2(x), _code(x), L.ptr(weight), _code(weight), L.ptr(gate),
-              _step2(gate), L.ptr(scale), _code(scale), alpha, rows, heads, x.shape[-1], L.ptr(rstd), L.ptr(dy),
-              _step2(dy), _code(dy), L.ptr(dx), None if gate is None else L.ptr(dgate), L.ptr(dw) if want_dw else None,
+    L.call_on(x, "uttt_norm_after_bwd", L.ptr(x), xs, _code(x), L.ptr(weight), _code(weight), L.ptr(gate),
+              gs, L.ptr(scale), _code(scale), alpha, rows, heads, x.shape[-1], L.ptr(rstd), L.ptr(dy),
+              ys, _code(dy), L.ptr(dx), None if gate is None else L.ptr(dgate), L.ptr(dw) if want_dw else None,
               L.ptr(ds) if want_ds else None, L.ptr(ws), size, L.stream_of(x))
     return grads
 
@@ -225,8 +216,8 @@ def _before_fwd(x: Tensor, residual: Tensor, weight: Optional[Tensor], scale: Op
                 eps: float, keep: bool) -> Tuple[Tensor, Tensor, Tensor]:
     """(y, the sum, 1 / rms of each row for the backward, empty where nobody keeps it)."""
     y, total, rstd = _before_fake(x, residual, weight, scale, alpha, eps, keep)
-    (x, residual), rows, heads = _block_args(x, residual)
-    L.call_on(x, "uttt_norm_before_fwd", L.ptr(x), _step2(x), _code(x), L.ptr(residual), _step2(residual),
+    ((x, xs), (residual, rs)), rows, heads = _block_args(x, residual)
+    L.call_on(x, "uttt_norm_before_fwd", L.ptr(x), xs, _code(x), L.ptr(residual), rs,
               _code(residual), L.ptr(weight), _code(weight), L.ptr(scale), _code(scale), alpha, rows, heads,
               x.shape[-1], eps, L.ptr(y), L.ptr(total), L.ptr(rstd) if keep else None, L.stream_of(x))
     return y, total, rstd
@@ -242,11 +233,11 @@ def _before_bwd(x: Tensor, residual: Tensor, weight: Optional[Tensor], scale: Op
                 want_ds: bool) -> List[Tensor]:
     grads = _before_bwd_fake(x, residual, weight, scale, alpha, rstd, dy, dtotal, want_dw, want_ds)
     dx, dr, dw, ds = grads
-    (x, residual, dy, dtotal), rows, heads = _block_args(x, residual, dy, dtotal)
+    ((x, xs), (residual, rs), (dy, ys), (dtotal, ts)), rows, heads = _block_args(x, residual, dy, dtotal)
     ws, size = _sums_workspace(x, rows, want_dw or want_ds)
-    L.call_on(x, "uttt_norm_before_bwd", L.ptr(x), _step2(x), _code(x), L.ptr(residual), _step2(residual),
+    L.call_on(x, "uttt_norm_before_bwd", L.ptr(x), xs, _code(x), L.ptr(residual), rs,
               _code(residual), L.ptr(weight), _code(weight), L.ptr(scale), _code(scale), alpha, rows, heads,
-              x.shape[-1], L.ptr(rstd), L.ptr(dy), _step2(dy), L.ptr(dtotal), _step2(dtotal), L.ptr(dx), L.ptr(dr),
+              x.shape[-1], L.ptr(rstd), L.ptr(dy), ys, L.ptr(dtotal), ts, L.ptr(dx), L.ptr(dr),
               L.ptr(dw) if want_dw else None, L.ptr(ds) if want_ds else None, L.ptr(ws), size, L.stream_of(x))
     return grads
 

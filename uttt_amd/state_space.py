@@ -387,14 +387,15 @@ def _check_scan(what, x, dt, A, B, C, D, gate, dt_bias):
     assert C.shape == B.shape, f"{what}: C {tuple(C.shape)} must have B's shape {tuple(B.shape)}"
     assert B.shape[2] >= 1 and Dm % B.shape[2] == 0, f"{what}: {Dm} channels must be a multiple of {B.shape[2]} groups"
     assert gate is None or gate.shape == x.shape, f"{what}: gate must have x's shape {tuple(x.shape)}"
+    dtype, dev = x.dtype, x.get_device()
     for name, t in (("B", B), ("C", C), ("gate", gate)):
-        assert t is None or t.dtype is x.dtype, f"{what}: {name} must have x's dtype {x.dtype}, got {t.dtype}"
+        assert t is None or t.dtype is dtype, f"{what}: {name} must have x's dtype {dtype}, got {t.dtype}"
     for name, t in (("D", D), ("dt_bias", dt_bias)):
         assert t is None or t.shape == (Dm,), f"{what}: {name} must be [{Dm}], got {tuple(t.shape)}"
     for name, t in (("A", A), ("D", D), ("dt_bias", dt_bias)):
         assert t is None or t.dtype is torch.float32, f"{what}: {name} must be fp32, got {t.dtype}"
     for name, t in (("dt", dt), ("A", A), ("B", B), ("C", C), ("D", D), ("gate", gate), ("dt_bias", dt_bias)):
-        assert t is None or t.device == x.device, f"{what}: {name} is on {t.device}, x on {x.device}"
+        assert t is None or t.get_device() == dev, f"{what}: {name} is on {t.device}, x on {x.device}"
 
 
 def selective_scan(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, *, D: Tensor | None = None,
