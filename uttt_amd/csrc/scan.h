@@ -76,6 +76,7 @@ __device__ __forceinline__ float sum_lanes(float x) {
   if constexpr (LN > 2) x = dpp_add<0x4e>(x);    // lane ^ 2
   if constexpr (LN > 4) x = dpp_add<0x141>(x);   // 7 - lane % 8
   if constexpr (LN > 8) x = dpp_add<0x140>(x);   // 15 - lane % 16
+  asm volatile("" : "+v"(x));   // the last addition stays here, in one instruction with its permutation
   return x;
 }
 
@@ -195,8 +196,7 @@ struct Place {
 };
 
 int scan_check(const ScanArgs& a, int dtype, const char* what);
-// Runs of the tokens: enough that `want` workgroups of `width` channels have work.
-void scan_runs(ScanArgs& a, int width, int want);
+void scan_runs(ScanArgs& a, int width, double chain, double busy, double extra);
 bool scan_fits(const ScanArgs& a);
 
 }  // namespace ssm

@@ -180,6 +180,7 @@ __device__ __forceinline__ float sum_apart(float x) {
   if constexpr (LN < 8) x = dpp_add<0x124>(x);
   if constexpr (LN < 4) x = dpp_add<0x122>(x);
   if constexpr (LN < 2) x = dpp_add<0x121>(x);
+  asm volatile("" : "+v"(x));   // as in sum_lanes
   return x;
 }
 
@@ -349,15 +350,13 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = halves_add(db[j], dc[j]);
     const float v0 = sum_apart<LN>(rows_add(v[0], v[2])), v1 = sum_apart<LN>(rows_add(v[1], v[3]));
-    if (ln == 0)
 #pragma unroll
-      for (int s = 0; s < CS; ++s) {
+      for (int s = 0; s < CS; ++s) {   // lanes of a channel the same
         lds.u[t][ch + s] = du[s];
         lds.aw[t][ch + s] = aw[s];
         if (GATE) lds.y[t][ch + s] = y[s];
       }
-    if ((lane & 15) < LN)
-      *reinterpret_cast<float2*>(&lds.sum[wave][t][lane >> 5][4 * ln + (lane >> 3 & 2)]) = make_float2(v0, v1);
+    *reinterpret_cast<float2*>(&lds.sum[wave][t][lane >> 5][4 * ln + (lane >> 3 & 2)]) = make_float2(v0, v1);
   };
 
   if (p.n > 0) load_tile((p.n - 1) / kTile * kTile);
@@ -548,7 +547,7 @@ int launch_bwd(const ScanArgs& a, hipStream_t st) {
   }
 }
 
-constexpr int kBwdBlocks = 3072;   // workgroups that are wanted at once
+void bwd_runs(ScanArgs& a) { scan_runs(a, scan_width(a.N), 0.8, 0.5, 0.3); }
 
 // Floats of the workspace's parts.
 struct Parts {
@@ -595,7 +594,7 @@ extern "C" size_t uttt_selective_scan_bwd_workspace_bytes(int B, int T, int nseq
   a.seqs = Seqs{packed ? &a : nullptr, 0, B, T, nseq};
   a.D = D; a.N = N; a.G = G;
   if (!seqs_ok(a.seqs) || D < 1 || G < 1 || D % G || N < 1 || N > kMaxStates) return 0;
-  scan_runs(a, scan_width(N), kBwdBlocks);
+  bwd_runs(a);
   return bwd_parts(a).bytes();
 }
 
@@ -630,7 +629,7 @@ extern "C" int uttt_selective_scan_bwd(const void* x, const int64_t* x_strides, 
   a.do_sb = dout_strides[0]; a.do_st = dout_strides[1];
   if (gate) { a.z_sb = gate_strides[0]; a.z_st = gate_strides[1]; }
   if (const int rc = scan_check(a, dtype, what)) return rc;
-  scan_runs(a, scan_width(N), kBwdBlocks);
+  bwd_runs(a);
   UTTT_REQUIRE(scan_fits(a), "%s: too many sequences, channels or states", what);
   const Parts parts = bwd_parts(a);
   UTTT_REQUIRE(workspace && workspace_bytes >= parts.bytes() && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0,

@@ -5,6 +5,8 @@
 // that are worked on side by side: what a run adds to a state of zeros and the
 // sum of its steps (local pass), the runs joined, h' = e^{A sum dt} h + end
 // (one thread a state), and the runs again from the states they start with.
+#include <math.h>
+
 #include "scan.h"
 
 namespace uttt {
@@ -58,12 +60,15 @@ __global__ __launch_bounds__(kScanThreads, fwd_waves(NP)) void scan_fwd_kernel(S
     else if (a.h0) load_row<NP>(a.h0 + ((int64_t)p.run.seq * a.D + d) * a.N, a.N, h);
   }
   float sum_dt = 0.0f;
-  // one token with B and C at q
-  auto token = [&](const float4* qB, const float4* qC, S* y0, S xbits, SD dtbits, S zbits) {
-    const float x = TT::load(xbits);
-    const float raw = DT::load(dtbits) + bias, grown = softplus(raw), dt = soft ? grown : raw;
-    const float u = dt * x;
+  // A token's step and what it writes; the states through a token with B and C at
+  // q, and the sum over them; what comes of it.
+  auto grow = [&](S xbits, SD dtbits, float& x, float& dt) {
+    const float raw = DT::load(dtbits) + bias, grown = softplus(raw);
+    x = TT::load(xbits);
+    dt = soft ? grown : raw;
     if (LOCAL) sum_dt += dt;
+  };
+  auto states = [&](const float4* qB, const float4* qC, float dt, float u) {
     float y[4] = {};
 #pragma unroll
     for (int q = 0; q < NP / 4; ++q) {
@@ -77,13 +82,15 @@ __global__ __launch_bounds__(kScanThreads, fwd_waves(NP)) void scan_fwd_kernel(S
         if (!LOCAL) y[j] = __builtin_fmaf(cc[j], hj, y[j]);
       }
     }
-    if (LOCAL) return;
-    float v = __builtin_fmaf(skip, x, (y[0] + y[1]) + (y[2] + y[3]));
+    return (y[0] + y[1]) + (y[2] + y[3]);
+  };
+  auto finish = [&](float sum, float x, S zbits) {
+    float v = __builtin_fmaf(skip, x, sum);
     if (GATE) {
       const float z = TT::load(zbits);
       v *= z * sigmoid_for<TT>(z);
     }
-    y0[c] = TT::store(v);
+    return v;
   };
 
   constexpr int U = 4;   // tokens whose x, dt and z are loaded ahead
@@ -130,29 +137,39 @@ __global__ __launch_bounds__(kScanThreads, fwd_waves(NP)) void scan_fwd_kernel(S
       int t = tt;
 #pragma unroll 1
       for (; t < min(tt + kTile, whole); t += U) {
-        S x[U], z[U];
-        SD dt[U];
+        // the steps of all U tokens, the states through one after another, the outputs
+        // of all U: chains of one token stand beside those of the others
+        S z[U];
+        float x[U], dt[U], y[U];
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-          x[i] = rx[i];
-          dt[i] = rdt[i];
+          grow(rx[i], rdt[i], x[i], dt[i]);
           z[i] = rz[i];
         }
         if (t + 2 * U <= p.n) load();
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-          token(qB, qC, yp, x[i], dt[i], z[i]);
+          y[i] = states(qB, qC, dt[i], dt[i] * x[i]);
           qB += NP / 4;
           qC += NP / 4;
-          yp += a.D;
           // without it decays of many tokens ahead are computed and spilled
           __builtin_amdgcn_sched_barrier(0);
         }
+        if (!LOCAL)
+#pragma unroll
+          for (int i = 0; i < U; ++i) {
+            yp[c] = TT::store(finish(y[i], x[i], z[i]));
+            yp += a.D;
+          }
       }
       if (left <= 0)   // the last few
 #pragma unroll 1
         for (; t < p.n; ++t) {
-          token(qB, qC, yp, xp[c], tp[c], GATE ? zp[c] : S(0));
+          float x, dt;
+          grow(xp[c], tp[c], x, dt);
+          const float y = states(qB, qC, dt, dt * x);
+          if (!LOCAL) yp[c] = TT::store(finish(y, x, GATE ? zp[c] : S(0)));
           xp += a.x_st;
           tp += a.dt_st;
           if (GATE) zp += a.z_st;
@@ -222,28 +239,42 @@ int launch_fwd(const ScanArgs& a, hipStream_t st) {
   return launch_fwd_as<TT, DT, 64>(a, st);
 }
 
-constexpr int kFwdBlocks = 1536;   // workgroups that are wanted at once
-
-void fwd_runs(ScanArgs& a) { scan_runs(a, kScanThreads, kFwdBlocks); }
+void fwd_runs(ScanArgs& a) { scan_runs(a, kScanThreads, 0.48, 0.3, 0.65); }
 
 }  // namespace
 
-// Runs that a wave of workgroups holds at once: one workgroup more would take
-// as long again (16 x 2048 tokens of 1536 channels: 1056 workgroups where 1024
-// fit 447 us, 960 of them TODO).
-void scan_runs(ScanArgs& a, int width, int want) {
+// Runs: as many as make kWanted workgroups, three rounds of them backward and one
+// and a half forward (16 x 2048 tokens of 1536 channels, both directions: 1024
+// 1540 us, 1536 1460, 3072 1515: shorter runs are evener, but more to join); where
+// there are fewer, a call is a chain of R tokens twice, half a microsecond each,
+// and of T / R joins, a tenth each, so that runs are no shorter than sqrt(T / 10)
+// tokens (300 tokens of 1536 channels of 16 states: runs of 64 65 us, of 16 36).
+// Whole sequences where that takes less: a token's workgroup `chain` us alone and
+// `busy` / 256 on a full card, runs a second pass of `extra` of the first, a launch,
+// the joins, and what is kept of each written and read (256 sequences of 64 tokens
+// of 256 channels: whole 39 us, 16-token runs 77).
+constexpr int kWanted = 1536;
+void scan_runs(ScanArgs& a, int width, double chain, double busy, double extra) {
+  const Seqs& s = a.seqs;
   a.Dg = a.D / a.G;
   a.ncb = (a.Dg + width - 1) / width;
-  const int64_t per = (int64_t)a.G * a.ncb, T = a.seqs.T;
-  const int64_t seqs = a.seqs.cu ? 1 : a.seqs.nseq;     // that share the workgroups
-  int64_t runs = want / (per * seqs);                   // of a sequence, of all packed tokens
-  if (a.seqs.cu && runs > a.seqs.nseq + 1) runs -= a.seqs.nseq;   // a sequence has one run more than whole ones
-  const int64_t most = T / (4 * kTile);                 // shorter ones would be mostly beginnings
-  if (runs > most) runs = most;
+  const int64_t T = s.T, per = (int64_t)a.G * a.ncb, seqs = s.cu ? 1 : s.nseq;   // that share the workgroups
+  int64_t runs = kWanted / (per * seqs);                          // of a sequence, of all packed tokens
+  if (s.cu && runs > s.nseq + 1) runs -= s.nseq;                  // a sequence has one run more than whole ones
+  const int64_t least = (int64_t)(sqrt((double)T / 10) / kTile + 1) * kTile;
+  if (runs > (T + least - 1) / least) runs = (T + least - 1) / least;
   if (runs < 1) runs = 1;
-  const int64_t R = ((T + runs - 1) / runs + kTile - 1) / kTile * kTile;
-  a.R = (int)(R < kTile ? kTile : R);
-  a.nruns = (int)run_count(a.seqs, a.R);
+  const auto tiles = [](int64_t n) { return n < kTile ? kTile : (n + kTile - 1) / kTile * kTile; };
+  const int64_t whole = tiles(T);
+  a.R = (int)tiles((T + runs - 1) / runs);
+  if (a.R < whole) {
+    const double work = (double)s.B * T * per * busy / 256, kept = (double)a.D * kept_states(a.N) * 16 / 4e6;
+    const double len = s.cu && s.nseq > 3 ? 3.0 * T / s.nseq : T;   // the longest packed one is a guess
+    const auto pass = [&](double R) { return work > R * chain ? work : R * chain; };
+    const double split = (1 + extra) * pass(a.R) + 12 + 0.1 * len / a.R + ((double)s.B * T / a.R + s.nseq) * kept;
+    if (pass(len) < split && len * 1.01 > T) a.R = (int)whole;
+  }
+  a.nruns = (int)run_count(s, a.R);
 }
 
 int scan_check(const ScanArgs& a, int dtype, const char* what) {
