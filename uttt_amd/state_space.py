@@ -27,6 +27,7 @@ from ._ops import (first_order_only, new_like, no_gradient, none_if_empty, run_f
                    traced_op)
 
 MAX_STATES = 64
+MAX_CHANNELS = 1 << 24
 MIN_WIDTH, MAX_WIDTH = 2, 8
 TILE = 16   # tokens between the states that a backward keeps
 
@@ -294,7 +295,7 @@ def _scan_infer(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optio
 
 def _kept_states(N):
     """N up to the next power of two of 4 or more, as the kernels keep states."""
-    return max(4, 1 << (N - 1).bit_length())
+    return 4 if N <= 4 else 8 if N <= 8 else 16 if N <= 16 else 32 if N <= 32 else 64
 
 
 def _scan_fwd_fake(x, dt, A, B, C, D, gate, dt_bias, softplus, initial_state, cu_seqlens, want_state):
@@ -380,6 +381,7 @@ def _check_scan(what, x, dt, A, B, C, D, gate, dt_bias):
     n, T, Dm = x.shape
     assert dt.shape == x.shape, f"{what}: dt {tuple(dt.shape)} must have x's shape {tuple(x.shape)}"
     assert dt.dtype in (torch.float32, x.dtype), f"{what}: dt must be fp32 or of x's dtype {x.dtype}, got {dt.dtype}"
+    assert Dm <= MAX_CHANNELS, f"{what}: {Dm} channels, at most {MAX_CHANNELS} are taken"
     assert A.dim() == 2 and A.shape[0] == Dm and 1 <= A.shape[1] <= MAX_STATES, (
         f"{what}: A must be [{Dm}, N] with N of 1 to {MAX_STATES}, got {tuple(A.shape)}")
     assert B.dim() == 4 and B.shape[:2] == (n, T) and B.shape[3] == A.shape[1], (
@@ -405,7 +407,7 @@ def selective_scan(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, *, D:
     """The selective scan over whole sequences.  Returns (y [B, T, D] in x's dtype,
     final states [N_seqs, D, N] fp32 or None).
 
-    x              [B, T, D] in fp32, bf16 or fp16.
+    x              [B, T, D] in fp32, bf16 or fp16; fewer than 2^30 tokens in all.
     dt             [B, T, D] steps in fp32 or x's dtype, to which dt_bias [D] is added and, with
                    dt_softplus, ln(1 + e^x) applied.
     A              [D, N] fp32, N up to 64: the states' rates, below zero where they decay.
