@@ -16,7 +16,11 @@ Contents (each function cites the reference file:line it restates):
                 shared state, with momentum and the Newton-Schulz5 (Muon) step;
   moe_read    - the routed read (permute, grouped apply, gate-weighted
                 unpermute) composed from the pieces above;
-  dense       - the uTTT-Dense / LaCT single-layer chunk loop.
+  dense       - the uTTT-Dense / LaCT single-layer chunk loop;
+  delta       - the gated delta rule in 64 bits, token by token;
+  state_space - the causal convolution, the selective scan and the norms around a
+                block in 64 bits, with bounds on what fp32 and the results'
+                roundings may differ.
 
 Every function is pinned by a check that a plausible mistake would fail
 (golden vectors, invariants, autograd, closed forms, brute force, planted

@@ -88,6 +88,15 @@ def test_empty_batches_and_too_many_tokens_are_refused():
         causal_conv(m(1 << 15, 1 << 15, 1), m(1, 4))
 
 
+def test_too_many_channels_are_refused():
+    wide = m(1, 1, (1 << 24) + 1)
+    rates, one = m((1 << 24) + 1, 1, dtype=F32), m(1, 1, 1, 1)
+    with pytest.raises(AssertionError, match="channels"):
+        selective_scan(wide, wide, rates, one, one)
+    with pytest.raises(AssertionError, match="channels"):
+        selective_scan_step(wide, wide, rates, one, one, m(1, (1 << 24) + 1, 1, dtype=F32))
+
+
 @pytest.mark.parametrize("kw,message", [
     (dict(state=m(4, 16, 12, dtype=F32)), "state must be"), (dict(state=m(4, 12, 16)), "state must be"),
     (dict(state=m(1, 12, 16, dtype=F32)), "2 rows, 1 states"), (dict(state=m(4, 16, 12, dtype=F32).transpose(1, 2)), "contiguous"),
@@ -333,7 +342,8 @@ def test_the_c_abi_refuses():
                                            None, p, p, p, p, p, None, None, None, None, ws, size, None)
 
     for fn in (scan_fwd, scan_bwd):
-        for kw, message in ((dict(N=65), "N=65"), (dict(N=0), "N=0"), (dict(D=7, G=2), "multiple"), (dict(dtype=7), "dtype"),
+        for kw, message in ((dict(N=65), "N=65"), (dict(N=0), "N=0"), (dict(D=7, G=2), "multiple"), (dict(D=(1 << 24) + 1), "2^24"),
+                            (dict(dtype=7), "dtype"),
                             (dict(dtype=1, dt=2), "dtype"), (dict(dtype=0, dt=1), "dtype"), (dict(n=2), "bad sizes"),
                             (dict(B=2, n=2, cu=p), "bad sizes"), (dict(x=None), "null"), (dict(A=p + 4), "16-byte"),
                             (dict(step=1 << 24), "between tokens"), (dict(T=5000, size=16), "workspace"),

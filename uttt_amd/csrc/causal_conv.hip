@@ -12,8 +12,8 @@
 // several tokens ahead of their use; the W - 1 tokens around a run are read
 // twice, from cache.  The backward computes p again and keeps the W unfinished
 // dx in registers too.  16 x 2048 tokens of 1536 channels, W = 4, bf16, silu:
-// forward 36 to 45 us (200 MB), backward 78 (300 MB, 3.9 TB/s) and the sums over
-// the workgroups 5; with eight channels a thread, half the waves, 87 and 142.
+// forward 36 to 50 us (200 MB), backward 79 (300 MB, 3.8 TB/s) and the sums over
+// the workgroups 4; with eight channels a thread, half the waves, 87 and 142.
 #include "state_space.h"
 
 namespace uttt {

@@ -20,8 +20,8 @@
 // Bound by vector instructions, about 3500 for 16 tokens of 32 channels of 16
 // states (11 a state backward, 6 forward), at two waves a SIMD, whose 256 registers
 // the states of half a tile, a tile's loads ahead and the sums fill.  16 x 2048
-// tokens of 1536 channels, 16 states, bf16, gated: local pass 212 us, joins 9,
-// gradients 800 (1.3 GB), dB and dC 12, the other sums 7.  All 16 tokens' states in
+// tokens of 1536 channels, 16 states, bf16, gated: local pass 208 us, joins 9,
+// gradients 780 (1.3 GB), dB and dC 12, the other sums 7.  All 16 tokens' states in
 // registers (spilled) and sums through LDS: 2284; one channel a lane at three waves
 // a SIMD: 803; writes of sums by one lane of a channel only, under masks: 860.
 #include "scan.h"

@@ -13,8 +13,8 @@
 // per state a product, an exponential (as long as four others), three more; some
 // 50 for a token's step, gate and conversions, at 16 states 145 in all.  Four
 // waves a SIMD issue them nearly without a gap; one alone takes 7 cycles each.
-// 16 x 2048 tokens of 1536 channels, 16 states, bf16, gated: local pass 170 us,
-// joins 13, outputs with the kept states 240 (600 MB, 2.5 TB/s).  With four lanes
+// 16 x 2048 tokens of 1536 channels, 16 states, bf16, gated: local pass 167 us,
+// joins 13, outputs with the kept states 233 (600 MB, 2.6 TB/s).  With four lanes
 // to a channel and two channels a lane, everything through LDS: 262 and 560 us.
 #include <math.h>
 
@@ -256,7 +256,8 @@ void fwd_runs(ScanArgs& a) { scan_runs(a, kScanThreads, 0.48, 0.3, 0.65); }
 
 // Runs: as many as make kWanted workgroups, three rounds of them backward and one
 // and a half forward (16 x 2048 tokens of 1536 channels, both directions: 1024
-// 1540 us, 1536 1460, 3072 1515: shorter runs are evener, but more to join); where
+// 1540 us, 1536 1460, twice as many 1515: shorter runs are evener, but more to
+// join, and the kernels were a tenth slower when this was measured); where
 // there are fewer, a call is a chain of R tokens twice, half a microsecond each,
 // and of T / R joins, a tenth each, so that runs are no shorter than sqrt(T / 10)
 // tokens (300 tokens of 1536 channels of 16 states: runs of 64 65 us, of 16 36).
