@@ -52,18 +52,20 @@ struct ScanArgs {
 template <int LN>
 struct Geo {
   static constexpr int NP = 4 * LN;               // states with those that only fill up
-  static constexpr int CS = LN >= 4 ? 2 : 1;      // channels of a lane
+  static constexpr int CS = LN == 4 || LN == 8 ? 2 : 1;   // channels of a lane
   static constexpr int WC = CS * 64 / LN;         // of a wave
   static constexpr int CB = 4 * WC;               // of a workgroup
+  static constexpr int HT = LN == 16 ? kTile : kTile / 2;   // tokens whose states are in registers
   static constexpr int TPP = kScanThreads / CB;   // tokens that the threads cover at a time
   static constexpr int EPT = kTile / TPP;         // elements of a tile per thread
   static constexpr int BPT = (kTile * NP + kScanThreads - 1) / kScanThreads;   // of B or C
 };
 
+constexpr int kWanted = 1536;   // workgroups of a split call (scan_runs)
 inline int scan_lanes(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 inline int scan_width(int N) {   // Geo<scan_lanes(N)>::CB
   const int ln = scan_lanes(N);
-  return (ln >= 4 ? 512 : 256) / ln;
+  return (ln == 4 || ln == 8 ? 512 : 256) / ln;
 }
 
 // Sum over the LN lanes of a channel, in all of them.
@@ -188,7 +190,7 @@ struct Place {
 };
 
 int scan_check(const ScanArgs& a, int dtype, const char* what);
-void scan_runs(ScanArgs& a, int width, double chain, double busy, double extra);
+void scan_runs(ScanArgs& a, int width, int wanted, double chain, double busy, double extra);
 bool scan_fits(const ScanArgs& a);
 
 }  // namespace ssm

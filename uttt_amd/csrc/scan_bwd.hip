@@ -24,6 +24,11 @@
 // gradients 780 (1.3 GB), dB and dC 12, the other sums 7.  All 16 tokens' states in
 // registers (spilled) and sums through LDS: 2284; one channel a lane at three waves
 // a SIMD: 803; writes of sums by one lane of a channel only, under masks: 860.
+// Beyond 32 states a channel takes 16 lanes, and a lane one channel with the
+// states of a whole tile, three waves a SIMD (8 x 1024 tokens of 1536 channels, 64
+// states, bf16, gated, both directions: 1153 us, with two channels and half tiles
+// 1321; 8 x 2048 tokens of 32 states: 1295 and 1214), for twice as many partial
+// sums of dB and dC.
 #include "scan.h"
 
 namespace uttt {
@@ -195,12 +200,12 @@ __device__ __forceinline__ float sum_apart(float x) {
 }
 
 template <class TT, class DT, int LN, bool GATE>
-__global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanArgs a) {
+__global__ __launch_bounds__(kScanThreads, LN < 16 ? 2 : 3) void scan_bwd_kernel(ScanArgs a) {
   using S = typename TT::S;
   using SD = typename DT::S;
   using M = Geo<LN>;
   using L = BwdLds<LN>;
-  constexpr int CS = M::CS, CB = M::CB, NP = M::NP, EPT = M::EPT, BPT = M::BPT;
+  constexpr int CS = M::CS, CB = M::CB, NP = M::NP, EPT = M::EPT, BPT = M::BPT, HT = M::HT;
   __shared__ L lds;
   const int tid = threadIdx.x, c = tid % CB, tq = tid / CB;
   Place p;
@@ -407,26 +412,26 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanArgs a) {
       for (int j = 0; j < 4; ++j) h0[s][j] = ch + s < p.nc ? rh[s][j] : 0.0f;
     __syncthreads();
     if (tt > 0) load_tile(tt - kTile);
-    // the tile's second half from the state in its middle, then the first: the
-    // states of half a tile stay in registers
+    // the tile's second half from the state in its middle, then the first, or the
+    // tile as a whole: the states of HT tokens stay in registers
     if (busy) {
 #pragma unroll
     for (int s = 0; s < CS; ++s)
 #pragma unroll
       for (int j = 0; j < 4; ++j) h8[s][j] = h0[s][j];
 #pragma unroll
-    for (int t = 0; t < kTile / 2; ++t) forward(t, h8, h8);
+    for (int t = 0; t < kTile - HT; ++t) forward(t, h8, h8);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int half = 1; half >= 0; --half) {
-      const int t0 = half * (kTile / 2);
-      float h[kTile / 2][CS][4];
+    for (int half = kTile / HT - 1; half >= 0; --half) {
+      const int t0 = half * HT;
+      float h[HT][CS][4];
 #pragma unroll
-      for (int t = 0; t < kTile / 2; ++t) forward(t0 + t, t ? h[t ? t - 1 : 0] : half ? h8 : h0, h[t]);
+      for (int t = 0; t < HT; ++t) forward(t0 + t, t ? h[t ? t - 1 : 0] : half ? h8 : h0, h[t]);
       Token now, next;
-      read(t0 + kTile / 2 - 1, now);
+      read(t0 + HT - 1, now);
 #pragma unroll
-      for (int t = kTile / 2 - 1; t >= 0; --t) {
+      for (int t = HT - 1; t >= 0; --t) {
         if (t) read(t0 + t - 1, next);
         if (t0 + t < nt) backward(t0 + t, now, t ? h[t ? t - 1 : 0] : half ? h8 : h0, h[t]);
         now = next;
@@ -557,7 +562,10 @@ int launch_bwd(const ScanArgs& a, hipStream_t st) {
   }
 }
 
-void bwd_runs(ScanArgs& a) { scan_runs(a, scan_width(a.N), 0.8, 0.5, 0.3); }
+void bwd_runs(ScanArgs& a) {
+  const int narrow = scan_lanes(a.N) == 16 ? 2 : 1;   // half the channels, and the time, of a workgroup
+  scan_runs(a, scan_width(a.N), kWanted * narrow, 0.8, 0.5 / narrow, 0.3);
+}
 
 // Floats of the workspace's parts.
 struct Parts {

@@ -250,12 +250,12 @@ int launch_fwd(const ScanArgs& a, hipStream_t st) {
   return launch_fwd_as<TT, DT, 64>(a, st);
 }
 
-void fwd_runs(ScanArgs& a) { scan_runs(a, kScanThreads, 0.48, 0.3, 0.65); }
+void fwd_runs(ScanArgs& a) { scan_runs(a, kScanThreads, kWanted, 0.48, 0.3, 0.65); }
 
 }  // namespace
 
-// Runs: as many as make kWanted workgroups, three rounds of them backward and one
-// and a half forward (16 x 2048 tokens of 1536 channels, both directions: 1024
+// Runs: as many as make `wanted` workgroups, kWanted or, of half the width, twice
+// that: three or four rounds of them backward and one and a half forward (16 x 2048 tokens of 1536 channels, both directions: 1024
 // 1540 us, 1536 1460, twice as many 1515: shorter runs are evener, but more to
 // join, and the kernels were a tenth slower when this was measured); where
 // there are fewer, a call is a chain of R tokens twice, half a microsecond each,
@@ -265,13 +265,12 @@ void fwd_runs(ScanArgs& a) { scan_runs(a, kScanThreads, 0.48, 0.3, 0.65); }
 // `busy` / 256 on a full card, runs a second pass of `extra` of the first, a launch,
 // the joins, and what is kept of each written and read (256 sequences of 64 tokens
 // of 256 channels: whole 39 us, 16-token runs 77).
-constexpr int kWanted = 1536;
-void scan_runs(ScanArgs& a, int width, double chain, double busy, double extra) {
+void scan_runs(ScanArgs& a, int width, int wanted, double chain, double busy, double extra) {
   const Seqs& s = a.seqs;
   a.Dg = a.D / a.G;
   a.ncb = (a.Dg + width - 1) / width;
   const int64_t T = s.T, per = (int64_t)a.G * a.ncb, seqs = s.cu ? 1 : s.nseq;   // that share the workgroups
-  int64_t runs = kWanted / (per * seqs);                          // of a sequence, of all packed tokens
+  int64_t runs = wanted / (per * seqs);                          // of a sequence, of all packed tokens
   if (s.cu && runs > s.nseq + 1) runs -= s.nseq;                  // a sequence has one run more than whole ones
   const int64_t least = (int64_t)(sqrt((double)T / 10) / kTile + 1) * kTile;
   if (runs > (T + least - 1) / least) runs = (T + least - 1) / least;
