@@ -92,6 +92,18 @@ __device__ __forceinline__ float log2_rate(float A) {
   return v < -FLT_MAX ? -FLT_MAX : v > FLT_MAX ? FLT_MAX : v;
 }
 
+// A state h, or an adjoint, through a run whose decay is 2^t, and what the run adds to it.  A
+// state of zero takes nothing through, also where 2^t is infinite (rates above
+// zero, or steps below it), and one that is in range before and behind the run
+// arrives where 2^t is not: then h takes it in four equal parts.
+__device__ __forceinline__ float through_run(float t, float h, float end) {
+  const bool far = !(fabsf(t) <= 126.0f);
+  const float f = exp2_hw(far ? 0.25f * t : t);
+  float v = h;
+  if (far) v = v * f * f * f;
+  return h == 0.0f ? end : __builtin_fmaf(f, v, end);
+}
+
 // Four states from index n of a row of N.
 __device__ __forceinline__ float4 load_states(const float* p, int n, int N) {
   if ((N & 3) == 0) return n < N ? *reinterpret_cast<const float4*>(p + n) : make_float4(0, 0, 0, 0);

@@ -163,7 +163,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_join_back_kernel(ScanArgs a
 #pragma unroll 8
   for (int c = runs - 1; c > 0; --c) {
     const int64_t i = r.base + c;
-    q = __builtin_fmaf(exp2_hw(decay[i * a.D + d] * A2), q, ends[i * K + in]);
+    q = through_run(decay[i * a.D + d] * A2, q, ends[i * K + in]);
     starts[(i - 1) * K + in] = q;
   }
 }

@@ -221,7 +221,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_join_kernel(ScanArgs a, int
 #pragma unroll 8
   for (int c = 1; c < runs; ++c) {
     const int64_t i = r.base + c - 1;
-    h = __builtin_fmaf(exp2_hw(decay[i * a.D + d] * A2), h, ends[i * K + in]);
+    h = through_run(decay[i * a.D + d] * A2, h, ends[i * K + in]);
     starts[(i + 1) * K + in] = h;
   }
 }
