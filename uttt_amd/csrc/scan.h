@@ -45,7 +45,7 @@ struct ScanArgs {
   const float* dhT;        // or null
   void *dx, *ddt, *dz;     // [B, T, D] in x's, dt's and x's type
   float* dh0;              // or null
-  float *part_A, *part_D, *part_bias;   // [nruns, D, N], [nruns, D], [nruns, D] or null
+  float *part_A, *part_D, *part_bias;   // [rows, D, N], [rows, D], [rows, D] or null; a row a run, or two
   float* part_bc;          // [ncb, B, T, 2, G, N]
 };
 

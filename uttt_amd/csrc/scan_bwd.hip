@@ -15,7 +15,7 @@
 // permutations (halves, rows of 16 and lanes of a row exchange what the other
 // needs: 16 instructions for 8 sums of 64), over its workgroup's waves in LDS, and
 // over the workgroups of a token by a launch of its own; sums over tokens (dA,
-// dDskip, d bias) by run and then by a launch.  All in a fixed order.
+// dDskip, d bias) by 256 tokens, by run and then by a launch.  All in a fixed order.
 //
 // Bound by vector instructions, about 3500 for 16 tokens of 32 channels of 16
 // states (11 a state backward, 6 forward), at two waves a SIMD, whose 256 registers
@@ -168,6 +168,26 @@ __global__ __launch_bounds__(kScanThreads) void scan_join_back_kernel(ScanArgs a
   }
 }
 
+// Sums over the tokens of a run longer than kFold (LONG) are added up every kFold
+// tokens into two floats, a sum and what its rounding left out, so that the errors
+// of dA, dDskip and d bias do not grow with the run: 16384 steps of 0.1 added one
+// by one were off by 2770 half ulps.  A kernel of its own, as the others' registers
+// leave no room for it: with folds everywhere 16 x 2048 tokens of 1536 channels, 16
+// states, both directions, take 1292 us, not 1267; runs of 1024 tokens with them
+// 1205 us, without 1168 (8 x 1024, 1536 channels, 64 states), and 5450, without
+// 5330 (64 x 4096, 768 channels, 16 states).
+constexpr int kFold = 256;
+__device__ __host__ __forceinline__ int64_t part_rows(const ScanArgs& a) {
+  return (int64_t)a.nruns * (a.R > kFold ? 2 : 1);
+}
+// had += v; returns what its rounding left out.
+__device__ __forceinline__ float add_exactly(float& had, float v) {
+  const float sum = had + v, back = sum - had;
+  const float rest = (had - (sum - back)) + (v - back);
+  had = sum;
+  return rest;
+}
+
 template <int LN>
 struct BwdLds {
   using M = Geo<LN>;
@@ -199,7 +219,7 @@ __device__ __forceinline__ float sum_apart(float x) {
   return x;
 }
 
-template <class TT, class DT, int LN, bool GATE>
+template <class TT, class DT, int LN, bool GATE, bool LONG>
 __global__ __launch_bounds__(kScanThreads, LN < 16 ? 2 : 3) void scan_bwd_kernel(ScanArgs a) {
   using S = typename TT::S;
   using SD = typename DT::S;
@@ -223,6 +243,17 @@ __global__ __launch_bounds__(kScanThreads, LN < 16 ? 2 : 3) void scan_bwd_kernel
       if (live && tq == 0) {
         if (a.part_D) a.part_D[(int64_t)num * a.D + p.d0 + c] = 0.0f;
         if (a.part_bias) a.part_bias[(int64_t)num * a.D + p.d0 + c] = 0.0f;
+      }
+      if (LONG) {   // the rest of its sums
+        const int64_t low = (int64_t)a.nruns * a.D;
+#pragma unroll
+        for (int s = 0; s < CS; ++s)
+          if (ch + s < p.nc)
+            store_states(a.part_A + (low + (int64_t)num * a.D + p.d0 + ch + s) * a.N, 4 * ln, a.N, make_float4(0, 0, 0, 0));
+        if (live && tq == 0) {
+          if (a.part_D) a.part_D[low + (int64_t)num * a.D + p.d0 + c] = 0.0f;
+          if (a.part_bias) a.part_bias[low + (int64_t)num * a.D + p.d0 + c] = 0.0f;
+        }
       }
     } else {   // the tokens of no sequence
       for (int i = num - a.nruns;; i += kLooseRuns) {
@@ -374,6 +405,51 @@ __global__ __launch_bounds__(kScanThreads, LN < 16 ? 2 : 3) void scan_bwd_kernel
     *reinterpret_cast<float2*>(&lds.sum[wave][t][lane >> 5][4 * ln + (lane >> 3 & 2)]) = make_float2(v0, v1);
   };
 
+  // The sums of up to kFold tokens into a long run's.
+  auto fold = [&](bool first) {
+    int id = tid;
+    asm volatile("" : "+v"(id));   // addresses are computed here and hold no registers before
+    const int fc = id % CB, fq = id / CB, fn = (id & 63) % LN, f0 = (id >> 6) * M::WC + (id & 63) / LN * CS;
+    const int64_t low = (int64_t)a.nruns * a.D;   // what rounding left out stands so far behind
+#pragma unroll
+    for (int s = 0; s < CS; ++s) {
+      if (f0 + s < p.nc) {
+        float* to = a.part_A + ((int64_t)num * a.D + p.d0 + f0 + s) * a.N;
+        float had[4] = {}, rest[4] = {};
+        if (!first) {
+          unpack(load_states(to, 4 * fn, a.N), had);
+          unpack(load_states(to + low * a.N, 4 * fn, a.N), rest);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) rest[j] += add_exactly(had[j], dA[s][j]);
+        store_states(to, 4 * fn, a.N, make_float4(had[0], had[1], had[2], had[3]));
+        store_states(to + low * a.N, 4 * fn, a.N, make_float4(rest[0], rest[1], rest[2], rest[3]));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) dA[s][j] = 0.0f;
+    }
+    float* red = &lds.u[0][0];
+    red[id] = sum_D;
+    red[kScanThreads + id] = sum_bias;
+    sum_D = sum_bias = 0.0f;
+    __syncthreads();
+    if (fq == 0 && fc < p.nc)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float* to = k ? a.part_bias : a.part_D;
+        if (!to) continue;
+        to += (int64_t)num * a.D + p.d0 + fc;
+        float v = red[k * kScanThreads + fc];
+#pragma unroll
+        for (int i = 1; i < M::TPP; ++i) v += red[k * kScanThreads + fc + i * CB];
+        float had = first ? 0.0f : *to, rest = first ? 0.0f : to[low];
+        rest += add_exactly(had, v);
+        *to = had;
+        to[low] = rest;
+      }
+    __syncthreads();
+  };
+
   if (p.n > 0) load_tile((p.n - 1) / kTile * kTile);
   for (int tt = p.n > 0 ? (p.n - 1) / kTile * kTile : -1; tt >= 0; tt -= kTile) {
     const int nt = min(kTile, p.n - tt);
@@ -462,16 +538,22 @@ __global__ __launch_bounds__(kScanThreads, LN < 16 ? 2 : 3) void scan_bwd_kernel
       a.part_bc[(((row0 + tl) * 2 + k) * a.G + p.g) * a.N + n] = (s[0] + s[W]) + (s[2 * W] + s[3 * W]);
     }
     __syncthreads();   // the next tile takes its place
+    if (LONG && tt > 0 && tt % kFold == 0) fold(tt + kFold >= p.n);
   }
 #pragma unroll
   for (int s = 0; s < CS; ++s) {
     if (ch + s >= p.nc) continue;
     const int64_t row = p.d0 + ch + s;
-    store_states(a.part_A + ((int64_t)num * a.D + row) * a.N, 4 * ln, a.N,
-                 make_float4(dA[s][0], dA[s][1], dA[s][2], dA[s][3]));
+    if (!LONG)
+      store_states(a.part_A + ((int64_t)num * a.D + row) * a.N, 4 * ln, a.N,
+                   make_float4(dA[s][0], dA[s][1], dA[s][2], dA[s][3]));
     if (a.dh0 && p.run.c == 0)
       store_states(a.dh0 + ((int64_t)p.run.seq * a.D + row) * a.N, 4 * ln, a.N,
                    make_float4(q[s][0], q[s][1], q[s][2], q[s][3]));
+  }
+  if (LONG) {
+    fold(p.n <= kFold);
+    return;
   }
   float* red = &lds.u[0][0];
   red[tid] = sum_D;
@@ -542,8 +624,9 @@ int launch_bwd_gated(const ScanArgs& a, hipStream_t st) {
     hipLaunchKernelGGL(scan_join_back_kernel, dim3((unsigned)((states + kScanThreads - 1) / kScanThreads)),
                        dim3(kScanThreads), 0, st, a, 4 * LN, a.ends, a.decay, a.starts);
   }
-  hipLaunchKernelGGL((scan_bwd_kernel<TT, DT, LN, GATE>), dim3(blocks + (a.seqs.cu ? kLooseRuns * per : 0)),
-                     dim3(kScanThreads), 0, st, a);
+  const dim3 all(blocks + (a.seqs.cu ? kLooseRuns * per : 0));
+  if (a.R > kFold) hipLaunchKernelGGL((scan_bwd_kernel<TT, DT, LN, GATE, true>), all, dim3(kScanThreads), 0, st, a);
+  else hipLaunchKernelGGL((scan_bwd_kernel<TT, DT, LN, GATE, false>), all, dim3(kScanThreads), 0, st, a);
   return check_launch("selective_scan_bwd");
 }
 template <class TT, class DT, int LN>
@@ -573,11 +656,11 @@ struct Parts {
   size_t bytes() const { return (joins + A + D + bias + bc) * 4; }
 };
 Parts bwd_parts(const ScanArgs& a) {
-  const size_t states = (size_t)a.nruns * a.D * a.N, chans = (size_t)a.nruns * a.D;
+  const size_t sums = (size_t)part_rows(a) * a.D;
   Parts p{};
-  p.joins = a.R >= a.seqs.T ? 0 : (2 * (size_t)kept_states(a.N) + 1) * chans;
-  p.A = states;
-  p.D = p.bias = chans;
+  p.joins = a.R >= a.seqs.T ? 0 : (2 * (size_t)kept_states(a.N) + 1) * a.nruns * a.D;
+  p.A = sums * a.N;
+  p.D = p.bias = sums;
   p.bc = (size_t)a.ncb * a.seqs.B * a.seqs.T * 2 * a.G * a.N;
   const auto whole = [](size_t& n) { n = (n + 3) / 4 * 4; };   // each starts on 16 bytes
   whole(p.joins); whole(p.A); whole(p.D); whole(p.bias); whole(p.bc);
@@ -678,6 +761,6 @@ extern "C" int uttt_selective_scan_bwd(const void* x, const int64_t* x_strides, 
     hipLaunchKernelGGL(scan_bc_kernel, dim3((unsigned)(n < 4096 ? n : 4096)), dim3(256), 0, st, a.part_bc, a.ncb, rows,
                        G * N, dtype, dB, dC);
   }
-  return launch_sums(a.nruns, {{a.part_A, (int64_t)D * N, dA, UTTT_F32}, {a.part_D, D, dskip, UTTT_F32},
+  return launch_sums(part_rows(a), {{a.part_A, (int64_t)D * N, dA, UTTT_F32}, {a.part_D, D, dskip, UTTT_F32},
                                {a.part_bias, D, ddt_bias, UTTT_F32}}, st, what);
 }
