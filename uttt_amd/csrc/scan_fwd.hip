@@ -264,7 +264,9 @@ void fwd_runs(ScanArgs& a) { scan_runs(a, kScanThreads, kWanted, 0.48, 0.3, 0.65
 // Whole sequences where that takes less: a token's workgroup `chain` us alone and
 // `busy` / 256 on a full card, runs a second pass of `extra` of the first, a launch,
 // the joins, and what is kept of each written and read (256 sequences of 64 tokens
-// of 256 channels: whole 39 us, 16-token runs 77).
+// of 256 channels: whole 39 us, 16-token runs 77).  Up to three packed sequences
+// count as long as all tokens; more always go by runs, as the host knows no length
+// (64 of 64 tokens, 1536 channels, 16 states: packed 87 us, as a batch 51).
 void scan_runs(ScanArgs& a, int width, int wanted, double chain, double busy, double extra) {
   const Seqs& s = a.seqs;
   a.Dg = a.D / a.G;
@@ -278,12 +280,11 @@ void scan_runs(ScanArgs& a, int width, int wanted, double chain, double busy, do
   const auto tiles = [](int64_t n) { return n < kTile ? kTile : (n + kTile - 1) / kTile * kTile; };
   const int64_t whole = tiles(T);
   a.R = (int)tiles((T + runs - 1) / runs);
-  if (a.R < whole) {
+  if (a.R < whole && (!s.cu || s.nseq <= 3)) {
     const double work = (double)s.B * T * per * busy / 256, kept = (double)a.D * kept_states(a.N) * 16 / 4e6;
-    const double len = s.cu && s.nseq > 3 ? 3.0 * T / s.nseq : T;   // the longest packed one is a guess
     const auto pass = [&](double R) { return work > R * chain ? work : R * chain; };
-    const double split = (1 + extra) * pass(a.R) + 12 + 0.1 * len / a.R + ((double)s.B * T / a.R + s.nseq) * kept;
-    if (pass(len) < split && len * 1.01 > T) a.R = (int)whole;
+    const double split = (1 + extra) * pass(a.R) + 12 + 0.1 * T / a.R + ((double)s.B * T / a.R + s.nseq) * kept;
+    if (pass((double)T) < split) a.R = (int)whole;
   }
   a.nruns = (int)run_count(s, a.R);
 }
