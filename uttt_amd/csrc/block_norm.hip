@@ -319,8 +319,8 @@ int norm_rows(const NormArgs& a, bool bwd, hipStream_t st) {
     else if (pieces <= 128) norm_launch<TT, V, 64, 2, AFTER, SCALE>(a, bwd, st);
     else if (pieces <= 256) norm_launch<TT, V, 256, 1, AFTER, SCALE>(a, bwd, st);
     else if (pieces <= 512) norm_launch<TT, V, 256, 2, AFTER, SCALE>(a, bwd, st);
-    else if (pieces <= 1024) norm_launch<TT, V, 1024, 1, AFTER, SCALE>(a, bwd, st);
-    else norm_launch<TT, V, 1024, 2, AFTER, SCALE>(a, bwd, st);
+    else if (V == 8 || pieces <= 1024) norm_launch<TT, V, 1024, 1, AFTER, SCALE>(a, bwd, st);   // 8192 elements at most
+    else if constexpr (V == 4) norm_launch<TT, V, 1024, 2, AFTER, SCALE>(a, bwd, st);
   } else {
     if (a.N <= 64) norm_launch<TT, 1, 16, 4, AFTER, SCALE>(a, bwd, st);
     else if (a.N <= 256) norm_launch<TT, 1, 64, 4, AFTER, SCALE>(a, bwd, st);
