@@ -14,6 +14,7 @@
 // dx in registers too.  16 x 2048 tokens of 1536 channels, W = 4, bf16, silu:
 // forward 36 to 50 us (200 MB), backward 79 (300 MB, 3.8 TB/s) and the sums over
 // the workgroups 4; with eight channels a thread, half the waves, 87 and 142.
+#include "rows.h"
 #include "state_space.h"
 
 namespace uttt {
@@ -22,7 +23,6 @@ namespace {
 
 constexpr int kConvThreads = 256;
 constexpr int kMinWidth = 2, kMaxWidth = 8;
-
 
 struct ConvArgs {
   Seqs seqs;
@@ -51,13 +51,6 @@ struct Piece {
   }
   __device__ __forceinline__ float get(int i) const { return TT::load(v[i]); }
 };
-template <class TT, int V>
-__device__ __forceinline__ void store_piece(typename TT::S* p, const float (&x)[V]) {
-  typename TT::S w[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) w[i] = TT::store(x[i]);
-  __builtin_memcpy(__builtin_assume_aligned(p, sizeof w), w, sizeof w);
-}
 
 // Zeros for the tokens of no sequence, `first` of kLooseRuns places.
 template <class TT, int V>
