@@ -263,13 +263,20 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_bwd_kernel(NormArg
   }
 }
 
-// Workgroups of the backward, each with 8 rows or more to walk over and no more
-// than the card holds at once, five, three or two a CU by their registers
-// (32 768 rows of 768 with a scale: 1024 of them 128 us, 768 99): a function of
-// the sizes alone, so that its sums come out the same on every run.
+// Workgroups of the backward, each with 8 rows or more to walk over: 1280, 768 or
+// 512, five, three or two a CU (32 768 rows of 768 before a block with a scale,
+// three a CU by registers: 1024 of them 128 us, 768 99; 262 144 rows of 192 after a
+// block without one: five.  Not every form fits so: with a scale after a block four
+// of up to 512 elements stand on a CU, and one of 1024 threads, beyond 4096).  More
+// where a thread would add more than 256 rows in a chain of fp32: rounding then
+// leaves the same of a sum however many rows there are, and the sum over the
+// workgroups is in 64 bits.  A function of the sizes alone, so that sums come out the
+// same on every run.
 int64_t bwd_blocks(int64_t rows, int N) {
-  const int64_t per = N <= 64 ? 32 : 8, n = (rows + per - 1) / per, most = N <= 512 ? 1280 : N <= 2048 ? 768 : 512;
-  return n < most ? n : most;
+  const int64_t per = N <= 64 ? 32 : 8, n = (rows + per - 1) / per;
+  const int64_t once = N <= 64 ? 16 : N <= 256 ? 4 : 1;   // rows of a workgroup at a time, in any form
+  const int64_t fill = N <= 512 ? 1280 : N <= 2048 ? 768 : 512, most = (rows + 256 * once - 1) / (256 * once);
+  return n < fill ? n : fill > most ? fill : most;
 }
 
 template <class TT, int V, int LPR, int NI, bool AFTER, bool SCALE>
