@@ -11,7 +11,10 @@
 // s is `alpha` times a learned [N], or alpha alone.
 //
 // Bound by memory: every tensor is read or written once.  A row stays in
-// registers between its two passes (LPR lanes, NI pieces of V elements each).
+// registers between its two passes (LPR lanes, NI pieces of V elements each).  Rows
+// that no 16 bytes divide (N, strides or addresses off 8 elements, in fp32 too) are
+// read by single elements: 32 768 rows of 772 before a block with a scale, both
+// directions, 460 us in bf16 and 433 in fp32, of 768 161 and 204.
 // The sums over rows for dw and ds stay in registers while a workgroup walks
 // over its rows, and are added by a second launch; what a backward needs of a
 // row again it reads again from its inputs, so that nothing is rounded twice.

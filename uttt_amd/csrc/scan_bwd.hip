@@ -19,16 +19,22 @@
 //
 // Bound by vector instructions, about 3500 for 16 tokens of 32 channels of 16
 // states (11 a state backward, 6 forward), at two waves a SIMD, whose 256 registers
-// the states of half a tile, a tile's loads ahead and the sums fill.  16 x 2048
+// the states of half a tile, a tile's loads ahead and the sums fill (15 or 16 are
+// spilled with a gate at 9 to 16 states, 19 to 24 in long runs, none in the others
+// of up to 32).  Up to 4
+// states a workgroup has 256 channels, whose tile takes 117 KB of LDS: one stands on
+// a CU, one wave a SIMD (16 x 2048 tokens of 1536 channels, both directions: 4
+// states 780 us, 8 states 862, 16 states 1267).  16 x 2048
 // tokens of 1536 channels, 16 states, bf16, gated: local pass 208 us, joins 9,
 // gradients 780 (1.3 GB), dB and dC 12, the other sums 7.  All 16 tokens' states in
 // registers (spilled) and sums through LDS: 2284; one channel a lane at three waves
 // a SIMD: 803; writes of sums by one lane of a channel only, under masks: 860.
 // Beyond 32 states a channel takes 16 lanes, and a lane one channel with the
 // states of a whole tile, three waves a SIMD (8 x 1024 tokens of 1536 channels, 64
-// states, bf16, gated, both directions: 1153 us, with two channels and half tiles
-// 1321; 8 x 2048 tokens of 32 states: 1295 and 1214), for twice as many partial
-// sums of dB and dC.
+// states, bf16, gated, both directions, without the folds of long runs below: 1153
+// us, with two channels and half tiles 1321; 8 x 2048 tokens of 32 states: 1295 and
+// 1214), for twice as many partial
+// sums of dB and dC: 16 channels a workgroup make 96 of them there, 403 MB.
 #include "scan.h"
 
 namespace uttt {

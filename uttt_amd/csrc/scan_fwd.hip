@@ -10,9 +10,10 @@
 // go from memory to the lane and back without a detour, steps and gates are
 // computed once, and no sum crosses lanes; B and C of 16 tokens are widened into
 // LDS a tile ahead and read by all lanes at once.  Bound by vector instructions:
-// per state a product, an exponential (as long as four others), three more; some
+// per state a product, an exponential (as long as two others), three more; some
 // 50 for a token's step, gate and conversions, at 16 states 145 in all.  Four
-// waves a SIMD issue them nearly without a gap; one alone takes 7 cycles each.
+// waves a SIMD issue them nearly without a gap (7 registers are spilled with a gate
+// at 9 to 16 states); one alone takes 7 cycles each.
 // 16 x 2048 tokens of 1536 channels, 16 states, bf16, gated: local pass 167 us,
 // joins 13, outputs with the kept states 233 (600 MB, 2.6 TB/s).  With four lanes
 // to a channel and two channels a lane, everything through LDS: 262 and 560 us.

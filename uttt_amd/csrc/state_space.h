@@ -62,7 +62,9 @@ __device__ __forceinline__ Run run_of(const Seqs& s, int at, int R) {
   return r;
 }
 
-constexpr int kLooseRuns = 8;   // places behind the last run for the tokens of no sequence
+// Places behind the last run for the tokens of no sequence, which are few where
+// buffers are filled: each writes its share in turn.
+constexpr int kLooseRuns = 8;
 // Token i of the tokens of no sequence of a packed call, -1 past the last one.
 __device__ __forceinline__ int loose_token(const Seqs& s, int i) {
   const int head = s.offset(0), tail = s.offset(s.nseq);

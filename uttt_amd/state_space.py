@@ -9,8 +9,9 @@ by its C, with a step dt that the token chooses:
 
 The reference ships models of this layer beside uTTT
 (uttt_llm/flame/custom_models/mamba2_swa/) on kernels that are not uTTT's own,
-with decays shared by a head, which are an A with equal entries here; the
-convolution also stands before its gated delta layers.
+with decays shared by a head, which are an A with equal entries here, and more
+states than the 64 that are taken here in their usual size; the convolution also
+stands before its gated delta layers.
 
 `causal_conv` and `selective_scan` are differentiable once in all their tensors
 (gradients of their gradients are refused).  There is no CPU path.
@@ -204,6 +205,8 @@ def causal_conv(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, activa
 
     Products and sums are fp32, each result rounded once to its type; gradients of weight and
     bias are summed in an order that the sizes and the 16-byte alignment of rows decide.
+    Tokens of no sequence are cleared by few threads: a buffer that is mostly padding takes
+    longer than a full one.
     Differentiable once in x, weight, bias and initial_state."""
     what = "causal_conv"
     shape = _check_conv(what, x, weight, bias, activation)
@@ -423,9 +426,14 @@ def selective_scan(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, *, D:
     others are copied.  All of it is computed in fp32, each result rounded once to its type;
     every sum has an order that the sizes decide.  A value that is not finite reaches the
     results of its token and later ones of its sequence (of x, dt and gate: in its channel), as
-    in the recurrence, and no others.  An A of -inf counts as fp32's lowest value.
-    Differentiable once in all tensors; the backward keeps the states at every 16th token, N / 4
-    bytes an element of x."""
+    in the recurrence, and no others.  An A of -inf counts as fp32's lowest value.  States may
+    grow (dt A above zero): what is in fp32's range at every token stays right and zeros stay
+    zero, but e^{dt A} of a single token is infinite past e^88, as in fp32.
+    Differentiable once in all tensors; the backward keeps the states at every 16th token: N up
+    to the next power of two of 4 or more, by 4 bytes, for each channel and 16 tokens (at 16
+    states 4 bytes an element of x), and of a packed sequence once more at most.  Tokens of no
+    sequence are cleared by few threads: a buffer that is mostly padding takes longer than a
+    full one."""
     what = "selective_scan"
     _check_scan(what, x, dt, A, B, C, D, gate, dt_bias)
     cu_seqlens = _check_sequences(what, x, cu_seqlens)
